@@ -3,7 +3,7 @@ block of 128 x 128, as a dense projection and as a mixture's experts, and the ro
 
   product  y = x W^T.  W holds OCP E4M3 codes and an f32 scale for every 128 rows x 128 columns; every 128 columns of an
            activation row are quantized to E4M3 within the call, under the smallest power of two that brings their largest
-           magnitude to 448 or less (not below 2^-126).  f32 in, f32 out.
+           magnitude to 448 or less (not below 2^-100).  f32 in, f32 out.
   experts  the same over groups of rows: pair p of group g (off[g] <= p < off[g + 1]) is row gather[p] of x times matrix g
            of a stack.
   route    every token's k best experts: scores softmax(l) or sigmoid(l) in 64 bits; with a bias, score + bias decides the
@@ -156,7 +156,7 @@ def _quantized(x):
     rows, cols = x.shape
     v = torch.nn.functional.pad(x, (0, -cols % BLOCK)).view(rows, -1, BLOCK)
     mantissa, exponent = torch.frexp(v.abs().amax(-1, keepdim=True))  # amax = mantissa 2^exponent; 448 = 0.875 x 2^9
-    e = torch.where(mantissa <= 0.875, exponent - 9, exponent - 8).clamp(min=-126)
+    e = torch.where(mantissa <= 0.875, exponent - 9, exponent - 8).clamp(min=-100)
     up, down = ((127 - e) << 23).view(torch.float32), ((127 + e) << 23).view(torch.float32)
     return ((v * up).to(torch.float8_e4m3fn).to(torch.float32) * down).view(rows, -1)[:, :cols]
 
@@ -256,7 +256,7 @@ def _quantized64(x):
         e = torch.ceil(torch.log2(torch.where(top > 0, top, 1.0) / 448.0))
         for d in (-1.0, 1.0):  # (the logarithm's own rounding)
             e = torch.where((top <= 448.0 * 2.0 ** (e - 1)) if d < 0 else (top > 448.0 * 2.0 ** e), e + d, e)
-        e = e.clamp(min=-126.0)
+        e = e.clamp(min=-100.0)
         z = v * 2.0 ** -e
         # E4M3: three bits behind the leading one, its exponent at least -6; halves to the even neighbour
         step = 2.0 ** (torch.floor(torch.log2(z.abs().clamp(min=2.0 ** -6))) - 3.0)
