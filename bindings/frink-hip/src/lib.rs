@@ -41,6 +41,22 @@ pub struct FrkMatvecLaunch {
     pub row_bytes: usize,
 }
 
+/// How `dev::route` scores and chooses experts (`frk_route_rule`).
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct FrkRouteRule {
+    pub score: i32,
+    pub norm: i32,
+    pub groups: i32,
+    pub top_groups: i32,
+    pub group_best: i32,
+    pub scale: f32,
+    /// `[n_experts]` on the device, or null
+    pub bias: *const f32,
+}
+pub const SCORE_SOFTMAX: i32 = 0;
+pub const SCORE_SIGMOID: i32 = 1;
+
 pub const ACT_F32: c_int = 0;
 pub const ACT_INT8: c_int = 1;
 /// K-quants on dequantized weights and the f32 activation (the reference's default x86 decode numerics).
@@ -48,6 +64,7 @@ pub const ACT_F32_DOT: c_int = 2;
 
 pub const ERR_NO_DEVICE: c_int = -1;
 pub const ERR_UNSUPPORTED: c_int = -2;
+pub const ERR_SHAPE: c_int = -3;
 
 extern "C" {
     fn frk_hip_probe(out: *mut FrkDeviceInfo) -> c_int;
@@ -76,6 +93,10 @@ extern "C" {
                                 out: *mut *mut FrkWeights) -> c_int;
     fn frk_hip_weights_from_device(kind: c_int, dev_bytes: *const c_void, len: usize, rows: usize, cols: usize,
                                    stream: *mut c_void, out: *mut *mut FrkWeights) -> c_int;
+    fn frk_hip_weights_register_fp8(codes: *const u8, scales: *const f32, rows: usize, cols: usize, matrices: usize,
+                                    out: *mut *mut FrkWeights) -> c_int;
+    fn frk_hip_weights_from_device_fp8(dev_codes: *const u8, dev_scales: *const f32, rows: usize, cols: usize, matrices: usize,
+                                       stream: *mut c_void, out: *mut *mut FrkWeights) -> c_int;
     fn frk_hip_weights_release(w: *mut FrkWeights) -> c_int;
     fn frk_hip_weights_keep_decoded(w: *mut FrkWeights, stream: *mut c_void) -> c_int;
     fn frk_hip_weights_rows(w: *const FrkWeights) -> usize;
@@ -105,6 +126,8 @@ extern "C" {
                                 x: *const f32, x_rows: usize, pairs: usize, y: *mut f32, stream: *mut c_void) -> c_int;
     fn frk_hip_route_top_k_softmax_dev(logits: *const f32, batch: usize, n_experts: usize, k: usize, norm: c_int,
                                        ids: *mut i32, weights: *mut f32, stream: *mut c_void) -> c_int;
+    fn frk_hip_route_dev(logits: *const f32, batch: usize, n_experts: usize, k: usize, rule: *const FrkRouteRule, ids: *mut i32,
+                         weights: *mut f32, stream: *mut c_void) -> c_int;
     fn frk_hip_moe_ffn_dev(gate: *const FrkWeights, up: *const FrkWeights, down: *const FrkWeights, n_experts: usize,
                            x: *const f32, batch: usize, ids: *const i32, weights: *const f32, k: usize,
                            out: *mut f32, stream: *mut c_void) -> c_int;
@@ -264,6 +287,26 @@ impl Weights {
         check(frk_hip_weights_from_device(kind, dev_bytes, len, rows, cols, stream, &mut w))?;
         Ok(Weights(w))
     }
+    /// E4M3 codes `[rows][cols]` with an f32 scale for every block of 128 x 128, `matrices` of them stacked.
+    pub fn register_fp8(codes: &[u8], scales: &[f32], rows: usize, cols: usize, matrices: usize) -> Result<Self, HipError> {
+        let blocks = |n: usize| (n + 127) / 128;
+        if matrices == 0 || codes.len() != rows * cols || scales.len() != matrices * blocks(rows / matrices) * blocks(cols) {
+            return Err(HipError { status: ERR_SHAPE, message: format!("{} codes, {} scales for {rows} x {cols} in {matrices} matrices", codes.len(), scales.len()) });
+        }
+        let mut w = std::ptr::null_mut();
+        check(unsafe { frk_hip_weights_register_fp8(codes.as_ptr(), scales.as_ptr(), rows, cols, matrices, &mut w) })?;
+        Ok(Weights(w))
+    }
+    /// The same from device memory, copied on `stream`.
+    ///
+    /// # Safety
+    /// `dev_codes` holds `rows * cols` bytes, `dev_scales` a float for every block of every matrix.
+    pub unsafe fn from_device_fp8(dev_codes: *const u8, dev_scales: *const f32, rows: usize, cols: usize, matrices: usize,
+                                  stream: *mut c_void) -> Result<Self, HipError> {
+        let mut w = std::ptr::null_mut();
+        check(frk_hip_weights_from_device_fp8(dev_codes, dev_scales, rows, cols, matrices, stream, &mut w))?;
+        Ok(Weights(w))
+    }
     pub fn rows(&self) -> usize { unsafe { frk_hip_weights_rows(self.0) } }
     pub fn cols(&self) -> usize { unsafe { frk_hip_weights_cols(self.0) } }
     pub fn kind(&self) -> c_int { unsafe { frk_hip_weights_kind(self.0) } }
@@ -393,6 +436,13 @@ pub mod dev {
     pub unsafe fn route_top_k_softmax(logits: *const f32, batch: usize, n_experts: usize, k: usize, norm: bool,
                                       ids: *mut i32, weights: *mut f32, stream: *mut c_void) -> Result<(), HipError> {
         check(frk_hip_route_top_k_softmax_dev(logits, batch, n_experts, k, norm as c_int, ids, weights, stream))
+    }
+    /// Routing by a rule: softmax or sigmoid scores, a bias for the choice, groups of experts.
+    /// # Safety
+    /// `logits[batch][n_experts]`, `ids[batch][k]`, `weights[batch][k]` and the rule's bias on the device.
+    pub unsafe fn route(logits: *const f32, batch: usize, n_experts: usize, k: usize, rule: &FrkRouteRule, ids: *mut i32,
+                        weights: *mut f32, stream: *mut c_void) -> Result<(), HipError> {
+        check(frk_hip_route_dev(logits, batch, n_experts, k, rule, ids, weights, stream))
     }
     /// `Decoder::moe_ffn_batch` (crates/frink-models/src/decoder/ffn_batch.rs:343-434) in one call.
     /// # Safety

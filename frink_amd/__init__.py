@@ -16,6 +16,9 @@ LIB_PATH = os.path.join(_HERE, "lib", "libfrink_hip.so")
 # quant kinds (ggml type ids) and their QuantKind::name()
 Q4_0, Q8_0, Q4_K, Q5_K, Q6_K = 2, 8, 12, 13, 14
 Q5_0, IQ4_XS, MXFP4 = 6, 23, 39
+# 8-bit floating point (OCP E4M3) with an f32 scale for every block of 128 x 128: no GGUF kind (Weights.from_device_fp8)
+FP8_BLOCK = 256
+SCORES = {"softmax": 0, "sigmoid": 1}
 KIND_NAME = {Q4_0: "Q4_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q5_K: "Q5_K", Q6_K: "Q6_K", Q5_0: "Q5_0", IQ4_XS: "IQ4_XS", MXFP4: "MXFP4"}
 BLOCK = {Q4_0: (18, 32), Q8_0: (34, 32), Q4_K: (144, 256), Q5_K: (176, 256), Q6_K: (210, 256),
          Q5_0: (22, 32), IQ4_XS: (136, 256), MXFP4: (17, 32)}  # (block_bytes, block_elems)
@@ -36,6 +39,7 @@ EXPORTS = [
     "frk_hip_quantize_q8_k_dev", "frk_hip_quantize_q8_0_dev", "frk_hip_dequant_dev",
     "frk_hip_get_rows_dev", "frk_hip_get_rows",
     "frk_hip_copy_dev", "frk_hip_read_dev", "frk_hip_issue_probe", "frk_hip_read_shape_dev", "frk_hip_gemm_grouped_dev",
+    "frk_hip_weights_register_fp8", "frk_hip_weights_from_device_fp8", "frk_hip_route_dev",
 ]
 
 
@@ -52,6 +56,12 @@ class BackendError(RuntimeError):
 class DeviceInfo(C.Structure):
     _fields_ = [("device_count", C.c_int32), ("compute_units", C.c_int32), ("name", C.c_char * 128),
                 ("gcn_arch", C.c_char * 64), ("total_vram_bytes", C.c_uint64), ("free_vram_bytes", C.c_uint64)]
+
+
+class RouteRule(C.Structure):
+    """frk_route_rule: how frk_hip_route_dev scores and chooses experts."""
+    _fields_ = [("score", C.c_int32), ("norm", C.c_int32), ("groups", C.c_int32), ("top_groups", C.c_int32),
+                ("group_best", C.c_int32), ("scale", C.c_float), ("bias_dev", C.c_void_p)]
 
 
 _lib = None
@@ -110,6 +120,9 @@ def lib():
             "frk_hip_read_dev": (i, [vp, sz, vp, vp]),
             "frk_hip_issue_probe": (i, [vp]),
             "frk_hip_gemm_grouped_dev": (i, [vp, sz, vp, vp, vp, sz, sz, vp, vp]),
+            "frk_hip_weights_register_fp8": (i, [vp, vp, sz, sz, sz, C.POINTER(vp)]),
+            "frk_hip_weights_from_device_fp8": (i, [vp, vp, sz, sz, sz, vp, C.POINTER(vp)]),
+            "frk_hip_route_dev": (i, [vp, sz, sz, sz, C.POINTER(RouteRule), vp, vp, vp]),
             "frk_hip_read_shape_dev": (i, [vp, sz, vp, i, i, i, i, vp]),
         }
         for name, (res, args) in sig.items():
@@ -184,6 +197,36 @@ class Weights:
         check(lib().frk_hip_weights_from_device(kind, C.c_void_p(data_dev.data_ptr()), data_dev.numel(), rows, cols,
                                                 _stream(), C.byref(h)))
         return cls(h, kind, rows, cols)
+
+    @staticmethod
+    def _check_fp8(codes, scales, rows, cols, matrices):
+        if rows <= 0 or cols <= 0 or matrices <= 0 or rows % matrices:
+            raise ValueError("%d rows of %d columns do not make %d matrices" % (rows, cols, matrices))
+        blocks = matrices * -(-(rows // matrices) // 128) * -(-cols // 128)
+        if codes != rows * cols or scales != blocks:
+            raise ValueError("%d codes and %d scales: %d matrices of %d x %d need %d and %d"
+                             % (codes, scales, matrices, rows // matrices, cols, rows * cols, blocks))
+
+    @classmethod
+    def from_host_fp8(cls, codes, scales, rows, cols, matrices=1):
+        """E4M3 codes [rows][cols] (numpy uint8) with f32 scales [matrices][ceil(rows / matrices / 128)][ceil(cols / 128)]."""
+        codes, scales = np.ascontiguousarray(codes, np.uint8), np.ascontiguousarray(scales, np.float32)
+        cls._check_fp8(codes.size, scales.size, rows, cols, matrices)
+        h = C.c_void_p()
+        check(lib().frk_hip_weights_register_fp8(_np_ptr(codes), _np_ptr(scales), rows, cols, matrices, C.byref(h)))
+        return cls(h, FP8_BLOCK, rows, cols)
+
+    @classmethod
+    def from_device_fp8(cls, codes, scales, rows, cols, matrices=1):
+        """The same from tensors on the GPU: codes float8_e4m3fn or uint8, scales float32, both contiguous."""
+        import torch
+        assert codes.dtype in (torch.float8_e4m3fn, torch.uint8) and codes.is_cuda and codes.is_contiguous()
+        assert scales.dtype == torch.float32 and scales.device == codes.device and scales.is_contiguous()
+        cls._check_fp8(codes.numel(), scales.numel(), rows, cols, matrices)
+        h = C.c_void_p()
+        check(lib().frk_hip_weights_from_device_fp8(C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), rows, cols,
+                                                    matrices, _stream(), C.byref(h)))
+        return cls(h, FP8_BLOCK, rows, cols)
 
     def keep_decoded(self):
         """Q5_0 / IQ4_XS / MXFP4: keep the rows decoded for the matrix cores beside the resident copy."""
@@ -354,6 +397,27 @@ def route_top_k_softmax(logits, k, norm):
     w = torch.empty((batch, k), dtype=torch.float32, device=logits.device)
     check(lib().frk_hip_route_top_k_softmax_dev(C.c_void_p(logits.data_ptr()), batch, n_experts, k, int(bool(norm)),
                                                 C.c_void_p(ids.data_ptr()), C.c_void_p(w.data_ptr()), _stream()))
+    return ids, w
+
+
+def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_best=1, norm=True, scale=1.0):
+    """frk_hip_route_dev: the k best experts of every row of logits[batch][n_experts] and their weights, (ids int32[batch][k],
+    weights f32[batch][k]).  score: "softmax" or "sigmoid"; bias (f32[n_experts]) takes part in the choice only; of `groups`
+    equal groups of experts the `top_groups` with the largest sums of their `group_best` best are used; the chosen scores are divided by
+    their sum (norm) and multiplied by `scale`.  Slots for which no expert is left (logits of -inf mask) hold id -1, weight 0."""
+    import torch
+    assert logits.dtype == torch.float32 and logits.is_cuda and logits.dim() == 2
+    logits = logits.contiguous()
+    batch, n_experts = logits.shape
+    if bias is not None:
+        assert bias.dtype == torch.float32 and bias.device == logits.device and bias.is_contiguous() and bias.numel() == n_experts
+    if score not in SCORES:
+        raise ValueError("score %r: one of %s" % (score, ", ".join(SCORES)))
+    rule = RouteRule(SCORES[score], int(bool(norm)), groups, top_groups, group_best, scale, None if bias is None else bias.data_ptr())
+    ids = torch.empty((batch, k), dtype=torch.int32, device=logits.device)
+    w = torch.empty((batch, k), dtype=torch.float32, device=logits.device)
+    check(lib().frk_hip_route_dev(C.c_void_p(logits.data_ptr()), batch, n_experts, k, C.byref(rule), C.c_void_p(ids.data_ptr()),
+                                  C.c_void_p(w.data_ptr()), _stream()))
     return ids, w
 
 

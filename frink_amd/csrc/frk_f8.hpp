@@ -1,0 +1,167 @@
+// Weights in 8-bit floating point with a scale for each block (FRK_KIND_FP8_BLOCK): what its kernels and the runtime share.
+//
+//   y[t][r] = sum over the 128-wide blocks b of  S[r / 128][b] * 2^e[t][b] * sum_i W[r][128 b + i] * q[t][128 b + i]
+//
+// W: OCP E4M3 codes, S: an f32 scale for every 128 rows x 128 columns of a matrix, q and e: the activations, quantized here
+// block by block.  e is the least exponent, -100 or more, with amax <= 448 * 2^e, so x * 2^-e is exact and q is x rounded
+// ONCE, to the nearest E4M3 (halves to even): an f32 scale amax / 448 would round the quotient first, and the two roundings
+// together miss the nearest value now and then.  A power of two costs no accuracy where E4M3 is normal.  (From -100 on q * 2^e
+// is a normal bf16 number, all of its four bits kept; below, 448 * 2^-100 = 3.5e-28, a block's values go towards zero.)
+// Infinities and NaN take no part in amax and become E4M3's NaN.
+//
+// The products run on the bf16 matrix cores: a code and q * 2^e are bf16 numbers, and their sums come out as f32 sums do.  The
+// 8-bit ones, twice as fast, add every eight products within 14 bits of the largest (measured on v_mfma_f32_16x16x32_fp8_fp8
+// and v_mfma_scale_f32_16x16x128_f8f6f4 alike: a product 2^-14 of its neighbour is lost, from the ninth on 2^-23 counts):
+// against 64-bit sums of 128 products of normal values 1.5e-5 in the 2-norm, of codes drawn evenly 5.1e-5; bf16 9e-9, 8e-8.
+#pragma once
+
+#include "frk_device.hpp"
+
+namespace frk {
+
+constexpr int F8_BLOCK = 128;
+constexpr int F8_STRIP = 16;              // weight rows that lie together
+constexpr int F8_PIECE = F8_STRIP * F8_BLOCK;  // bytes of a strip's block: what a wavefront's two loads bring
+
+// A resident stack of `matrices` matrices of rows x cols: every 16 rows a strip, a strip's blocks one after the other, and a
+// block as [2 halves][64 lanes][16 bytes] -- lane l row l % 16, half h columns 32 (l / 16) + 16 h .. + 15 -- so that a wavefront's
+// load is 1 KB in one piece and brings the operands of 16x16x32 products, eight codes each.  (A product's k runs over a lane
+// group's own columns, in any order, as long as the activations have the same.)  Rows past a matrix's last and columns past the
+// last are zeros.  Behind the strips the scales, [matrices][row blocks][blocks].
+struct F8Mat {
+    const uint8_t *q;
+    const float *s;
+    int rows, strips, blocks, row_blocks;  // of one matrix
+};
+static inline size_t f8_blocks(size_t n) { return (n + F8_BLOCK - 1) / F8_BLOCK; }
+static inline size_t f8_strips(size_t rows) { return (rows + F8_STRIP - 1) / F8_STRIP; }
+static inline F8Mat f8_mat(const frk_weights *w) {
+    const size_t rows = w->rows / w->matrices;
+    F8Mat m;
+    m.q = w->dev;
+    m.s = reinterpret_cast<const float *>(w->dev + w->layout.off_a);
+    m.rows = (int)rows;
+    m.strips = (int)f8_strips(rows);
+    m.blocks = (int)f8_blocks(w->cols);
+    m.row_blocks = (int)f8_blocks(rows);
+    return m;
+}
+
+// Activations: q * 2^e as bf16, [rows][blocks][128], zeros past cols.
+struct F8Acts {
+    uint16_t *v;
+    int rows;
+};
+static inline size_t f8_acts_bytes(size_t rows, size_t cols) { return round_up(rows * f8_blocks(cols) * F8_BLOCK * 2, 256); }
+static inline F8Acts f8_acts_carve(void *base, size_t rows) {
+    F8Acts a;
+    a.v = (uint16_t *)base;
+    a.rows = (int)rows;
+    return a;
+}
+
+// ---- quantization: sixteen lanes a block, eight neighbouring values each ----
+__device__ __forceinline__ uint32_t f8_row_max(uint32_t v) {  // over a row of 16 lanes
+    v = max(v, (uint32_t)dpp_i<DPP_QUAD_XOR1>((int)v));
+    v = max(v, (uint32_t)dpp_i<DPP_QUAD_XOR2>((int)v));
+    v = max(v, (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)v));
+    return max(v, (uint32_t)dpp_i<DPP_ROW_MIRROR>((int)v));
+}
+// the eight values' codes; `scale` = 2^e of the block
+__device__ __forceinline__ uint2 f8_quantize8(const float (&v)[8], float &scale) {
+    uint32_t top = 0;  // magnitudes compare as their bits
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu;
+        top = max(top, m < 0x7f800000u ? m : 0u);
+    }
+    top = f8_row_max(top);
+    // 448 = 1.75 * 2^8: e is the exponent less 8, one more where the mantissa is above 1.75
+    const int b = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    const uint32_t biased = (uint32_t)max(b, 127 - 100);
+    scale = __uint_as_float(biased << 23);
+    const float up = __uint_as_float((254u - biased) << 23);  // 2^-e
+    // (256 * 2^120 is no float any more: there the largest code is 240's)
+    const float most = biased == 127 + 120 ? 240.0f : 448.0f;
+    float z[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) z[i] = fminf(fmaxf(v[i] * up, -most), most);
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i], z[4 * i + 1], 0, false);
+        p = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i + 2], z[4 * i + 3], p, true);
+        w[i] = (uint32_t)p;
+#else
+        w[i] = 0;
+#endif
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if ((__float_as_uint(v[4 * i + j]) & 0x7f800000u) == 0x7f800000u) w[i] = (w[i] & ~(0xffu << (8 * j))) | (0x7fu << (8 * j));
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// eight values of a row from column k on, zeros past `cols`; WIDE: rows whose 16-byte pieces are aligned and whole
+template <bool WIDE>
+__device__ __forceinline__ void f8_load8(const float *__restrict__ row, int k, int cols, float (&v)[8]) {
+    if (WIDE) {
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 a = k < cols ? *reinterpret_cast<const float4 *>(row + k) : zero;
+        const float4 b = k + 4 < cols ? *reinterpret_cast<const float4 *>(row + k + 4) : zero;
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = k + i < cols ? row[k + i] : 0.0f;
+    }
+}
+static inline bool f8_wide_rows(const float *x, size_t cols) { return cols % 4 == 0 && (uintptr_t)x % 16 == 0; }
+
+typedef __bf16 f8_v2bf __attribute__((ext_vector_type(2)));
+// four codes as bf16 times `scale` (a power of two)
+__device__ __forceinline__ uint2 f8_to_bf16(uint32_t codes, float scale) {
+    uint2 out = make_uint2(0, 0);
+#if defined(__HIP_DEVICE_COMPILE__)
+    const f8_v2bf lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false), hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true);
+    __builtin_memcpy(&out.x, &lo, 4);
+    __builtin_memcpy(&out.y, &hi, 4);
+#endif
+    return out;
+}
+
+// four blocks of a row by a wavefront; with `up` of silu(x) * up, element by element
+template <bool WIDE>
+__device__ __forceinline__ void f8_quantize_quad(const float *__restrict__ x, const float *__restrict__ up, size_t row, int quad, int cols, int blocks,
+                                                 int lane, const F8Acts &out) {
+    float v[8], scale;
+    f8_load8<WIDE>(x + row * (size_t)cols, quad * 4 * F8_BLOCK + lane * 8, cols, v);
+    if (up) {
+        float u[8];
+        f8_load8<WIDE>(up + row * (size_t)cols, quad * 4 * F8_BLOCK + lane * 8, cols, u);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = silu_as_host(v[i]) * u[i];
+    }
+    const uint2 codes = f8_quantize8(v, scale);
+    const uint2 a = f8_to_bf16(codes.x, scale), b = f8_to_bf16(codes.y, scale);
+    if (quad * 4 + (lane >> 4) < blocks)
+        *reinterpret_cast<uint4 *>(out.v + row * (size_t)blocks * F8_BLOCK + (size_t)quad * 4 * F8_BLOCK + lane * 8) = make_uint4(a.x, a.y, b.x, b.y);
+}
+
+// ---- entry points for the runtime and the expert layers ----
+Layout f8_layout(size_t rows, size_t cols, size_t matrices, size_t *bytes);
+int launch_f8_repack(const uint8_t *src, const float *scales, const frk_weights *w, hipStream_t s);
+size_t f8_gemm_workspace_bytes(const frk_weights *w, size_t batch);
+int launch_f8_gemm(const frk_weights *w, const float *x, size_t batch, float *y, void *ws, hipStream_t s);
+size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs);
+int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
+                      float *y, void *ws, hipStream_t s);
+// rows of x (of silu(x) * up) quantized; `used`: a row whose entry is negative is left as it is
+int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols, const int *used, const F8Acts &out, hipStream_t s);
+// the products of the tiles {matrix, first row of the order, rows in use (up to F8_MAX_TOKENS), first row of y}; row i of the order is
+// activation row src[i], or i
+constexpr int F8_MAX_TOKENS = 64;
+int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, const int *src, const int4 *tiles, const int *n_tiles, size_t max_tiles, float *y,
+                    hipStream_t s);
+
+}  // namespace frk

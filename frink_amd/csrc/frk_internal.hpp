@@ -100,6 +100,7 @@ inline Layout layout_for(int kind, size_t cols) {
 struct frk_weights {
     int kind = 0;
     size_t rows = 0, cols = 0;
+    size_t matrices = 1;       // FP8_BLOCK: how many matrices of rows / matrices rows, each with its own blocks of scales
     size_t src_row_bytes = 0;  // GGUF bytes per row
     frk::Layout layout;
     uint8_t *dev = nullptr;    // resident copy (library-owned)
@@ -120,6 +121,8 @@ struct frk_weights {
 };
 
 namespace frk {
+
+inline bool is_f8_kind(int kind) { return kind == FRK_KIND_FP8_BLOCK; }
 
 // ---- scratch the library owns (quantized activations, intermediates) ----
 // One buffer per caller stream.  A lease holds the stream's buffer for as long as one entry point is
@@ -153,6 +156,7 @@ int launch_quantize_q8_k(const float *x, size_t n, int8_t *q, float *d, int16_t 
 int launch_swiglu_quantize_q8_k(const float *gate, const float *up, size_t n, int8_t *q, float *d, int16_t *bsums, hipStream_t s);
 int launch_swiglu_quantize_q8_0(const float *gate, const float *up, size_t n, int8_t *q, float *d, hipStream_t s);
 int launch_quantize_q8_0(const float *x, size_t n, int8_t *q, float *d, hipStream_t s);
+int launch_f8_dequant_rows(const frk_weights *w, const int32_t *ids, size_t n_out, float *out, hipStream_t s);
 int launch_dequant(const frk_weights *w, float *out, hipStream_t s);
 int launch_dequant_rows(const frk_weights *w, const int32_t *ids, size_t n_out, float *out, hipStream_t s);
 int launch_repack(int kind, const uint8_t *src, uint8_t *dst, size_t rows, size_t cols, const Layout &l,
@@ -353,7 +357,12 @@ int launch_moe_ffn(const frk_weights *gate, const frk_weights *up, const frk_wei
                    void *ws, hipStream_t s);
 int moe_copy_intermediates(void *ws, size_t batch, int k, int n_experts, int hidden, int ffn, float *gate_out,
                            float *up_out, int8_t *act_q, float *act_d, int32_t *pos_of, hipStream_t s);
+// experts in 8-bit floating point with a scale for each block
+size_t f8_moe_workspace_bytes(size_t batch, int k, int n_experts, size_t hidden, size_t ffn);
+int launch_moe_ffn_f8(const frk_weights *gate, const frk_weights *up, const frk_weights *down, int n_experts, const float *x, size_t batch,
+                      const int32_t *ids, const float *weights, int k, float *out, void *ws, hipStream_t s);
 int launch_swiglu(const float *gate, const float *up, size_t n, float *act, hipStream_t s);
+int launch_route(const float *logits, size_t batch, int n_experts, int k, const frk_route_rule &rule, int32_t *ids, float *weights, hipStream_t s);
 int launch_route_top_k_softmax(const float *logits, int batch, int n_experts, int k, int norm, int32_t *ids,
                                float *weights, hipStream_t s);
 // prefetch-all GEMVs (one wavefront per row, no LDS) for rows of 33..256 units

@@ -3,6 +3,7 @@
 //   bucket (token, slot) pairs by expert  ->  gate/up grouped GEMM over gathered token rows
 //   ->  silu(gate)*up, quantized to Q8_K  ->  down grouped GEMM  ->  out[tok] = sum_e w * down
 // with each token's experts added in the order the reference adds them (moe_combine_kernel).
+#include "frk_f8.hpp"
 #include "frk_mx_quant.hpp"
 
 #include <cmath>
@@ -1177,6 +1178,74 @@ int launch_moe_ffn_units_grouped(const frk_weights *gate, const frk_weights *up,
     if (rc) return rc;
     hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)batch, (unsigned)((hidden + 1023) / 1024)), dim3(256), 0, s, m.down_out, ids,
                        weights, m.pos_of, k, hidden, n_experts, (int)(batch >= MOE_BUCKET_ORDER_FROM), out);
+    FRK_LAUNCH_CHECK("moe_combine");
+    return FRK_OK;
+}
+
+// ---- experts in 8-bit floating point with a scale for each block (frk_f8.hip): bucketed, gate and up over the token rows
+// quantized once, silu(gate) * up quantized, down, the weighted sum ----
+struct F8MoeScratch {
+    void *x_acts, *a_acts;
+    float *gate_out, *up_out, *down_out;
+    int *group_off, *gather, *pos_of, *cpos_of, *n_tiles;
+    int4 *tiles;
+};
+static F8MoeScratch f8_moe_carve(void *base, size_t batch, int k, int n_experts, size_t hidden, size_t ffn, size_t *end) {
+    const size_t pairs = batch * (size_t)k, rows = moe_max_rows(pairs, n_experts);
+    char *p = (char *)base;
+    auto take = [&](size_t bytes) {
+        char *r = p;
+        p += round_up(bytes, 256);
+        return r;
+    };
+    F8MoeScratch m;
+    m.x_acts = take(f8_acts_bytes(batch, hidden));
+    m.a_acts = take(f8_acts_bytes(rows, ffn));
+    m.gate_out = (float *)take(rows * ffn * 4);
+    m.up_out = (float *)take(rows * ffn * 4);
+    m.down_out = (float *)take(rows * hidden * 4);
+    m.group_off = (int *)take((n_experts + 1) * 4);
+    m.gather = (int *)take(rows * 4);
+    m.pos_of = (int *)take(pairs * 4);
+    m.cpos_of = (int *)take(pairs * 4);
+    m.n_tiles = (int *)take(256);
+    m.tiles = (int4 *)take((rows / MOE_TILE + 1) * 16);
+    if (end) *end = (size_t)(p - (char *)base);
+    return m;
+}
+size_t f8_moe_workspace_bytes(size_t batch, int k, int n_experts, size_t hidden, size_t ffn) {
+    size_t end = 0;
+    (void)f8_moe_carve(nullptr, batch, k, n_experts, hidden, ffn, &end);
+    return end;
+}
+int launch_moe_ffn_f8(const frk_weights *gate, const frk_weights *up, const frk_weights *down, int n_experts, const float *x, size_t batch,
+                      const int32_t *ids, const float *weights, int k, float *out, void *ws, hipStream_t s) {
+    const size_t hidden = gate->cols, ffn = down->cols, pairs = batch * (size_t)k, rows = moe_max_rows(pairs, n_experts), max_tiles = rows / MOE_TILE;
+    static_assert(MOE_TILE == F8_MAX_TOKENS, "the kernel's tiles");
+    const F8MoeScratch m = f8_moe_carve(ws, batch, k, n_experts, hidden, ffn, nullptr);
+    static bool sized = false;  // a benign race: every thread sets the same attribute
+    if (!sized) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&moe_group_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)sizeof(GroupLds));
+        if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFuncSetAttribute(moe_group): %s", hipGetErrorString(e));
+        sized = true;
+    }
+    const GroupArgs ga{ids, (int)pairs, k, n_experts, m.group_off, m.gather, m.pos_of, m.cpos_of, m.tiles, m.n_tiles, (int)rows};
+    hipLaunchKernelGGL(moe_group_kernel, dim3(1), dim3(1024), sizeof(GroupLds), s, ga);
+    FRK_LAUNCH_CHECK("moe_group");
+    const F8Acts xa = f8_acts_carve(m.x_acts, batch), aa = f8_acts_carve(m.a_acts, rows);
+    int rc = launch_f8_quantize(x, nullptr, batch, hidden, nullptr, xa, s);
+    if (rc) return rc;
+    rc = launch_f8_tiles(gate, xa, m.gather, m.tiles, m.n_tiles, max_tiles, m.gate_out, s);
+    if (rc) return rc;
+    rc = launch_f8_tiles(up, xa, m.gather, m.tiles, m.n_tiles, max_tiles, m.up_out, s);
+    if (rc) return rc;
+    rc = launch_f8_quantize(m.gate_out, m.up_out, rows, ffn, m.gather, aa, s);
+    if (rc) return rc;
+    rc = launch_f8_tiles(down, aa, nullptr, m.tiles, m.n_tiles, max_tiles, m.down_out, s);
+    if (rc) return rc;
+    hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)batch, (unsigned)((hidden + 1023) / 1024)), dim3(256), 0, s, m.down_out, ids, weights,
+                       m.pos_of, k, (int)hidden, n_experts, (int)(batch >= MOE_BUCKET_ORDER_FROM), out);
     FRK_LAUNCH_CHECK("moe_combine");
     return FRK_OK;
 }

@@ -7,11 +7,13 @@
 #include <iterator>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <utility>
 #include <vector>
 
 #include "frk_internal.hpp"
+#include "frk_f8.hpp"
 #include "frk_stage.hpp"
 
 namespace frk {
@@ -372,6 +374,84 @@ int frk_hip_weights_from_device(int kind, const void *dev_bytes, size_t len, siz
     return make_resident(kind, (const uint8_t *)dev_bytes, rows, cols, (hipStream_t)stream, out);
 }
 
+static int check_f8_shape(size_t rows, size_t cols, size_t matrices) {
+    if (rows == 0 || cols == 0 || matrices == 0) return set_error(FRK_ERR_SHAPE, "empty shape: rows=%zu cols=%zu matrices=%zu", rows, cols, matrices);
+    if (rows % matrices) return set_error(FRK_ERR_SHAPE, "%zu rows do not divide into %zu matrices", rows, matrices);
+    if (rows > 0x7fffff00u || cols > 0x7fffff00u) return set_error(FRK_ERR_SHAPE, "shape too large");
+    if (matrices > 65535) return set_error(FRK_ERR_SHAPE, "%zu matrices (at most 65535)", matrices);
+    return FRK_OK;
+}
+static int make_f8_resident(const uint8_t *codes_dev, const float *scales_dev, size_t rows, size_t cols, size_t matrices, hipStream_t s,
+                            frk_weights **out) {
+    auto *w = new (std::nothrow) frk_weights();
+    if (!w) return set_error(FRK_ERR_OOM, "no host memory for a weights handle");
+    w->kind = FRK_KIND_FP8_BLOCK;
+    w->rows = rows;
+    w->cols = cols;
+    w->matrices = matrices;
+    w->src_row_bytes = cols;
+    w->layout = f8_layout(rows, cols, matrices, &w->dev_bytes);
+    int rc = FRK_OK;
+    hipError_t e = hipGetDevice(&w->device);
+    if (e != hipSuccess) rc = set_error(FRK_ERR_HIP, "hipGetDevice: %s", hipGetErrorString(e));
+    if (!rc) {
+        e = hipMalloc((void **)&w->dev, w->dev_bytes);
+        if (e != hipSuccess) rc = set_error(FRK_ERR_OOM, "hipMalloc(%zu) for resident weights: %s", w->dev_bytes, hipGetErrorString(e));
+    }
+    if (!rc) rc = launch_f8_repack(codes_dev, scales_dev, w, s);
+    if (rc) {
+        if (w->dev) (void)hipFree(w->dev);
+        delete w;
+        return rc;
+    }
+    *out = w;
+    return FRK_OK;
+}
+
+int frk_hip_weights_register_fp8(const uint8_t *host_codes, const float *host_scales, size_t rows, size_t cols, size_t matrices,
+                                 frk_weights **out) {
+    clear_error();
+    if (!host_codes || !host_scales || !out) return set_error(FRK_ERR_ARG, "frk_hip_weights_register_fp8: null argument");
+    *out = nullptr;
+    int rc = check_f8_shape(rows, cols, matrices);
+    if (rc) return rc;
+    std::lock_guard<std::mutex> lk(g_dev.mu);
+    rc = ensure_device_locked();
+    if (rc) return rc;
+    const size_t codes = rows * cols, scales = matrices * f8_blocks(rows / matrices) * f8_blocks(cols) * sizeof(float), at = round_up(codes, 256);
+    uint8_t *staging = nullptr;
+    FRK_HIP_TRY(hipMalloc((void **)&staging, at + scales));
+    hipError_t e = hipMemcpyAsync(staging, host_codes, codes, hipMemcpyHostToDevice, g_dev.stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(staging + at, host_scales, scales, hipMemcpyHostToDevice, g_dev.stream);
+    frk_weights *w = nullptr;
+    if (e != hipSuccess) rc = set_error(FRK_ERR_HIP, "hipMemcpyAsync(weights): %s", hipGetErrorString(e));
+    if (!rc) rc = make_f8_resident(staging, reinterpret_cast<const float *>(staging + at), rows, cols, matrices, g_dev.stream, &w);
+    e = hipStreamSynchronize(g_dev.stream);
+    (void)hipFree(staging);
+    if (!rc && e != hipSuccess) {
+        rc = set_error(FRK_ERR_HIP, "hipStreamSynchronize: %s", hipGetErrorString(e));
+        (void)hipFree(w->dev);
+        delete w;
+    }
+    if (!rc) *out = w;
+    return rc;
+}
+
+int frk_hip_weights_from_device_fp8(const uint8_t *dev_codes, const float *dev_scales, size_t rows, size_t cols, size_t matrices,
+                                    void *stream, frk_weights **out) {
+    clear_error();
+    if (!dev_codes || !dev_scales || !out) return set_error(FRK_ERR_ARG, "frk_hip_weights_from_device_fp8: null argument");
+    *out = nullptr;
+    int rc = check_f8_shape(rows, cols, matrices);
+    if (rc) return rc;
+    {
+        std::lock_guard<std::mutex> lk(g_dev.mu);
+        rc = ensure_device_locked();
+        if (rc) return rc;
+    }
+    return make_f8_resident(dev_codes, dev_scales, rows, cols, matrices, (hipStream_t)stream, out);
+}
+
 int frk_hip_weights_release(frk_weights *w) {
     clear_error();
     if (!w) return FRK_OK;
@@ -550,7 +630,28 @@ static int gemv_units_int(const frk_weights *w, const float *x, float *y, hipStr
     return launch_gemv_units_int(w, q, d, y, s);
 }
 
+// FP8_BLOCK: one path at every batch size, so a row's result does not depend on the batch it is in.
+static int f8_on_current_device(const frk_weights *w) {
+    int dev = -1;
+    FRK_HIP_TRY(hipGetDevice(&dev));
+    if (dev != w->device) return set_error(FRK_ERR_ARG, "the matrix is on device %d, the current device is %d", w->device, dev);
+    return FRK_OK;
+}
+static int gemm_f8(const frk_weights *w, const float *x, size_t batch, float *y, hipStream_t s, Scratch &scratch) {
+    if (batch > (size_t)1 << 30) return set_error(FRK_ERR_SHAPE, "a batch of %zu rows is too large", batch);
+    void *ws = nullptr;
+    int rc = f8_on_current_device(w);
+    if (!rc) rc = scratch.get(f8_gemm_workspace_bytes(w, batch), s, &ws);
+    if (rc) return rc;
+    return launch_f8_gemm(w, x, batch, y, ws, s);
+}
+
 static int gemv_impl(const frk_weights *w, const float *x, float *y, int act_mode, hipStream_t s, Scratch &scratch) {
+    if (is_f8_kind(w->kind)) {
+        if (act_mode != FRK_ACT_F32 && act_mode != FRK_ACT_INT8)
+            return set_error(FRK_ERR_UNSUPPORTED, "FP8_BLOCK weights multiply quantized activations only (mode %d)", act_mode);
+        return gemm_f8(w, x, 1, y, s, scratch);
+    }
     if (act_mode == FRK_ACT_F32_DOT && (w->kind == FRK_KIND_Q4_K || w->kind == FRK_KIND_Q5_K || w->kind == FRK_KIND_Q6_K)) {
         if (!kquant_f32_gemv_fits(w))
             return set_error(FRK_ERR_UNSUPPORTED, "the f32-dot GEMV of the K-quants takes rows of at most 16384 columns (%zu)", w->cols);
@@ -910,6 +1011,7 @@ static int gemm_units_int(const frk_weights *w, const float *x, size_t batch, fl
 }
 
 static int gemm_impl(const frk_weights *w, const float *x, size_t batch, float *y, void *stream, Scratch &scratch) {
+    if (is_f8_kind(w->kind)) return gemm_f8(w, x, batch, y, (hipStream_t)stream, scratch);
     // one row is the decode path, whatever the kind
     if (batch == 1) return gemv_impl(w, x, y, FRK_ACT_F32, (hipStream_t)stream, scratch);
     if (takes_tiles(w, batch)) {  // (frk_hip_gemm_pair_dev: the same test)
@@ -1244,7 +1346,7 @@ int frk_hip_gemv_multi_dev(const frk_weights *const *ws, size_t n, const float *
     }
     for (size_t i = 0; i < n; i++) {
         int rc;
-        if (ws[i]->kind == FRK_KIND_Q8_0 || ws[i]->kind == FRK_KIND_Q4_0 || is_unit_kind(ws[i]->kind))
+        if (ws[i]->kind == FRK_KIND_Q8_0 || ws[i]->kind == FRK_KIND_Q4_0 || is_unit_kind(ws[i]->kind) || is_f8_kind(ws[i]->kind))
             rc = frk_hip_gemv_dev(ws[i], x, ys[i], FRK_ACT_F32, stream);  // (these kinds multiply the f32 activation itself)
         else rc = frk_hip_gemv_q8k_dev(ws[i], a.q, a.d, a.bsums, ys[i], stream);
         if (rc) return rc;
@@ -1263,7 +1365,9 @@ int frk_hip_ffn_swiglu_dev(const frk_weights *gate, const frk_weights *up, const
     const size_t ffn = gate->rows;
     // scratch for gate(x), up(x) and silu(gate)*up behind the quantized activation
     const size_t q_cols = std::max(gate->cols, down->cols);  // either projection may quantize its input here
-    const size_t q_area = round_up(q_cols, 256) + round_up(q_cols / 32 * 4, 256) + round_up(q_cols / 8, 256);
+    size_t q_area = round_up(q_cols, 256) + round_up(q_cols / 32 * 4, 256) + round_up(q_cols / 8, 256);
+    for (const frk_weights *w : {gate, up, down})
+        if (is_f8_kind(w->kind)) q_area = std::max(q_area, f8_gemm_workspace_bytes(w, 1));
     WorkspaceLease lease;
     int rc = workspace(q_area + 3 * round_up(ffn * 4, 256), s, lease);
     if (rc) return rc;
@@ -1310,6 +1414,24 @@ int frk_hip_route_top_k_softmax_dev(const float *logits, size_t batch, size_t n_
                                       (hipStream_t)stream);
 }
 
+int frk_hip_route_dev(const float *logits, size_t batch, size_t n_experts, size_t k, const frk_route_rule *rule, int32_t *ids, float *weights,
+                      void *stream) {
+    clear_error();
+    if (!logits || !rule || !ids || !weights) return set_error(FRK_ERR_ARG, "frk_hip_route_dev: null argument");
+    if (batch == 0 || n_experts == 0) return set_error(FRK_ERR_SHAPE, "empty shape: batch=%zu experts=%zu", batch, n_experts);
+    if (k == 0 || k > n_experts) return set_error(FRK_ERR_SHAPE, "top-k %zu must be between 1 and the %zu experts", k, n_experts);
+    if (n_experts > 1024 || k > 64 || batch > (size_t)1 << 30)
+        return set_error(FRK_ERR_SHAPE, "experts=%zu (max 1024), k=%zu (max 64), batch=%zu (max 2^30)", n_experts, k, batch);
+    if (rule->score != FRK_SCORE_SOFTMAX && rule->score != FRK_SCORE_SIGMOID) return set_error(FRK_ERR_UNSUPPORTED, "no score function %d", rule->score);
+    if (rule->groups < 1 || rule->groups > 64 || n_experts % (size_t)rule->groups)
+        return set_error(FRK_ERR_SHAPE, "%zu experts in %d groups (1 .. 64, equal ones)", n_experts, rule->groups);
+    if (rule->top_groups < 1 || rule->top_groups > rule->groups || rule->group_best < 1 || rule->group_best > 2)
+        return set_error(FRK_ERR_SHAPE, "%d of %d groups by their %d best experts (1 or 2)", rule->top_groups, rule->groups, rule->group_best);
+    if ((size_t)rule->top_groups * (n_experts / (size_t)rule->groups) < k)
+        return set_error(FRK_ERR_SHAPE, "%d groups of %zu experts hold fewer than top-k %zu", rule->top_groups, n_experts / (size_t)rule->groups, k);
+    return launch_route(logits, batch, (int)n_experts, (int)k, *rule, ids, weights, (hipStream_t)stream);
+}
+
 int frk_hip_moe_ffn_dev(const frk_weights *gate, const frk_weights *up, const frk_weights *down, size_t n_experts,
                         const float *x, size_t batch, const int32_t *ids, const float *weights, size_t k, float *out,
                         void *stream) {
@@ -1321,11 +1443,12 @@ int frk_hip_moe_ffn_dev(const frk_weights *gate, const frk_weights *up, const fr
     if (n_experts > 1024 || k > 64 || k > n_experts)
         return set_error(FRK_ERR_SHAPE, "experts=%zu (max 1024), k=%zu (max 64, at most the expert count)", n_experts, k);
     const bool unit_experts = is_unit_kind(gate->kind) && up->kind == gate->kind && is_unit_kind(down->kind);
-    if (!unit_experts &&
+    const bool f8_experts = is_f8_kind(gate->kind) && is_f8_kind(up->kind) && is_f8_kind(down->kind);
+    if (!unit_experts && !f8_experts &&
         (gate->kind != FRK_KIND_Q4_K || up->kind != FRK_KIND_Q4_K || (down->kind != FRK_KIND_Q4_K && down->kind != FRK_KIND_Q6_K)))
         return set_error(FRK_ERR_UNSUPPORTED,
-                         "the expert GEMMs take Q4_K gate and up and Q4_K or Q6_K down experts, or Q5_0 / IQ4_XS / MXFP4 experts "
-                         "with gate and up of one kind (got kinds %d/%d/%d)",
+                         "the expert GEMMs take Q4_K gate and up and Q4_K or Q6_K down experts, Q5_0 / IQ4_XS / MXFP4 experts "
+                         "with gate and up of one kind, or FP8_BLOCK experts (got kinds %d/%d/%d)",
                          gate->kind, up->kind, down->kind);
     if (gate->rows % n_experts || down->rows % n_experts)
         return set_error(FRK_ERR_SHAPE, "stacked rows %zu/%zu do not divide into %zu experts", gate->rows, down->rows,
@@ -1337,6 +1460,16 @@ int frk_hip_moe_ffn_dev(const frk_weights *gate, const frk_weights *up, const fr
                          gate->rows, gate->cols, up->rows, up->cols, down->rows, down->cols, n_experts, hidden, ffn);
     if (batch * k > (size_t)1 << 30) return set_error(FRK_ERR_SHAPE, "batch*k = %zu pairs is too many", batch * k);
     WorkspaceLease lease;
+    if (f8_experts) {
+        if (hidden % 4) return set_error(FRK_ERR_SHAPE, "FP8_BLOCK experts over %zu columns: a multiple of four", hidden);
+        for (const frk_weights *w : {gate, up, down})
+            if (w->matrices != n_experts)
+                return set_error(FRK_ERR_SHAPE, "an FP8_BLOCK stack holds %zu matrices, the call names %zu experts", w->matrices, n_experts);
+        int rc = f8_on_current_device(gate);
+        if (!rc) rc = workspace(f8_moe_workspace_bytes(batch, (int)k, (int)n_experts, hidden, ffn), (hipStream_t)stream, lease);
+        if (rc) return rc;
+        return launch_moe_ffn_f8(gate, up, down, (int)n_experts, x, batch, ids, weights, (int)k, out, lease.ptr, (hipStream_t)stream);
+    }
     if (unit_experts && moe_units_takes_grouped_path(gate, up, down, (int)n_experts, batch, (int)k)) {
         int rc = workspace(moe_units_grouped_workspace_bytes(gate->kind, down->kind, batch, (int)k, (int)n_experts, (int)hidden, (int)ffn), (hipStream_t)stream, lease);
         if (rc) return rc;
@@ -1361,10 +1494,10 @@ int frk_hip_gemm_grouped_dev(const frk_weights *stacked, size_t n_groups, const 
     clear_error();
     if (!stacked || !group_off || (pairs && (!x || !y))) return set_error(FRK_ERR_ARG, "frk_hip_gemm_grouped_dev: null argument");
     if (n_groups == 0 || n_groups > 1024) return set_error(FRK_ERR_SHAPE, "groups=%zu (1 .. 1024)", n_groups);
-    const bool units = is_unit_kind(stacked->kind) && units_have_planar_form(stacked);
-    if (stacked->kind != FRK_KIND_Q4_K && stacked->kind != FRK_KIND_Q6_K && !units)
+    const bool units = is_unit_kind(stacked->kind) && units_have_planar_form(stacked), f8 = is_f8_kind(stacked->kind);
+    if (!f8 && stacked->kind != FRK_KIND_Q4_K && stacked->kind != FRK_KIND_Q6_K && !units)
         return set_error(FRK_ERR_UNSUPPORTED,
-                         "the grouped GEMM takes Q4_K, Q6_K, Q5_0, IQ4_XS or MXFP4 (scale bytes within 104..143) weights (got kind %d)",
+                         "the grouped GEMM takes Q4_K, Q6_K, Q5_0, IQ4_XS, MXFP4 (scale bytes within 104..143) or FP8_BLOCK weights (got kind %d)",
                          stacked->kind);
     if (stacked->rows % n_groups)
         return set_error(FRK_ERR_SHAPE, "stacked rows %zu do not divide into %zu groups", stacked->rows, n_groups);
@@ -1373,6 +1506,14 @@ int frk_hip_gemm_grouped_dev(const frk_weights *stacked, size_t n_groups, const 
     if (pairs == 0) return FRK_OK;
     if (x_rows == 0) return set_error(FRK_ERR_SHAPE, "%zu pairs over no activation rows", pairs);
     WorkspaceLease lease;
+    if (f8) {
+        if (stacked->matrices != n_groups)
+            return set_error(FRK_ERR_SHAPE, "the FP8_BLOCK stack holds %zu matrices, the call names %zu groups", stacked->matrices, n_groups);
+        int rc = f8_on_current_device(stacked);
+        if (!rc) rc = workspace(f8_grouped_workspace_bytes(stacked, x_rows, pairs), (hipStream_t)stream, lease);
+        if (rc) return rc;
+        return launch_f8_grouped(stacked, group_off, gather, x, x_rows, pairs, y, lease.ptr, (hipStream_t)stream);
+    }
     if (units) {
         int rc = workspace(grouped_units_workspace_bytes(stacked->kind, n_groups, stacked->rows, x_rows, pairs, stacked->cols), (hipStream_t)stream, lease);
         if (rc) return rc;

@@ -48,6 +48,12 @@ enum {
  * Names are QuantKind::name() (crates/frink-core/src/weight_matrix.rs:264-290). */
 enum { FRK_KIND_Q4_0 = 2, FRK_KIND_Q5_0 = 6, FRK_KIND_Q8_0 = 8, FRK_KIND_Q4_K = 12, FRK_KIND_Q5_K = 13, FRK_KIND_Q6_K = 14,
        FRK_KIND_IQ4_XS = 23, FRK_KIND_MXFP4 = 39 };
+/* FRK_KIND_FP8_BLOCK, outside ggml's numbers: OCP E4M3 codes with an f32 scale for every block of 128 x 128, which no
+ * GGUF file holds and the reference has no counterpart of.  Its matrices come through frk_hip_weights_register_fp8 /
+ * frk_hip_weights_from_device_fp8 (codes and scales are two buffers), so the seam's answers about it
+ * (frk_hip_matvec_kernel, _has_launch, _gemm_supported, _block_*) are "no kernel" and the host-buffer launch functions
+ * refuse it; the device-pointer entry points take its handles as they say there. */
+enum { FRK_KIND_FP8_BLOCK = 256 };
 /* Q5_0, IQ4_XS and MXFP4 (the 17-byte GGUF block form) have the dequantizer / row gather and the
  * decode GEMV on the f32 activation (dot_q5_0_f32, dot_iq4_xs_f32, dot_mxfp4_gguf_f32,
  * crates/frink-quant/src/lib.rs:4380-4418, 4894-4934, 5506); a batch is one such GEMV per row, the
@@ -115,6 +121,27 @@ int frk_hip_weights_register(int kind, const void *host_bytes, size_t len, size_
  * into the library's own allocation; the source may be freed afterwards). */
 int frk_hip_weights_from_device(int kind, const void *dev_bytes, size_t len, size_t rows,
                                 size_t cols, void *stream, frk_weights **out);
+/* A matrix, or a stack of `matrices` matrices of one shape, in 8-bit floating point with a scale for each block:
+ * codes[rows][cols] in OCP E4M3 (0x7f and 0xff are NaN; there is no infinity), scales[matrices][ceil(R / 128)][ceil(cols / 128)]
+ * f32 with R = rows / matrices; weight (r, k) of matrix m is its code times scales[m][r / 128][k / 128].  Any R and cols: the
+ * last blocks may be partly used.  register takes host buffers (borrowed for the call; synchronous; unlike
+ * frk_hip_weights_register it keeps no cache), from_device buffers on the current device (copied on `stream`; they may be
+ * freed once the stream has passed the call).  The resident copy pads rows to 16 and columns to 128.
+ *
+ * What takes such a handle, f32 in and f32 out as for the other kinds: frk_hip_gemv_dev (FRK_ACT_F32 and FRK_ACT_INT8 are the
+ * same here), frk_hip_gemv_multi_dev, frk_hip_ffn_swiglu_dev, frk_hip_gemm_dev, frk_hip_gemm_pair_dev,
+ * frk_hip_gemm_noalloc_dev, frk_hip_gemm_grouped_dev and frk_hip_moe_ffn_dev (n_groups, n_experts = matrices; three such stacks
+ * and a hidden size that is a multiple of four), frk_hip_dequant_dev, frk_hip_get_rows(_dev); the others return
+ * FRK_ERR_UNSUPPORTED.  Every 128 columns of an activation row are quantized within the call to E4M3, to the nearest and
+ * halves to even, under 2^e, e the least exponent of -100 or more that brings the largest finite magnitude to 448 or less
+ * (magnitudes above 240 * 2^120, where the next code's value is no float, become that); an infinity or a NaN becomes a NaN and
+ * takes no part in that: its output row is NaN.  So
+ *   y[t][r] = sum over blocks b of scales[r / 128][b] * 2^e[t][b] * (sum over the block of code * quantized activation),
+ * the products exact, the sums in f32. */
+int frk_hip_weights_register_fp8(const uint8_t *host_codes, const float *host_scales, size_t rows, size_t cols, size_t matrices,
+                                 frk_weights **out);
+int frk_hip_weights_from_device_fp8(const uint8_t *dev_codes, const float *dev_scales, size_t rows, size_t cols, size_t matrices,
+                                    void *stream, frk_weights **out);
 int frk_hip_weights_release(frk_weights *w);
 /* Q5_0 / IQ4_XS / MXFP4 (scale bytes within 104..143) reach the matrix cores decoded to signed bytes; a batched call
  * (frk_hip_gemm_dev from four rows on, frk_hip_gemm_grouped_dev, frk_hip_moe_ffn_dev from 32 tokens on) decodes
@@ -277,6 +304,32 @@ int frk_hip_gemm_noalloc_dev(const frk_weights *w, const float *x_dev, size_t ba
 int frk_hip_route_top_k_softmax_dev(const float *logits_dev, size_t batch, size_t n_experts, size_t k,
                                     int norm, int32_t *ids_dev, float *weights_dev, void *stream);
 
+/* Routing by a rule, for a batch of tokens: logits[batch][n_experts] -> ids[batch][k], weights[batch][k].
+ *   score    p = softmax(l) over a token's experts, or sigmoid(l) each
+ *   bias     f32 [n_experts] on the device, or null: c = p + bias decides which experts are chosen (a bias for balance);
+ *            without it c = p
+ *   groups   expert i belongs to group i / (n_experts / groups).  A group's value is the sum of its `group_best` (1 or 2)
+ *            largest c; only experts of the `top_groups` groups of the largest values can be chosen.  1, 1, 1: no groups
+ *   the k largest c are chosen, in descending order
+ *   weights  the chosen experts' p, divided by their sum when norm != 0, times scale
+ * Scores, their sums and comparisons are in 64 bits, so that no rounding of theirs decides between two experts; a weight is rounded to
+ * f32 once.  Equal values go to the lower index, of groups too.  An expert whose logit is -inf or NaN has p = 0 and cannot be chosen
+ * (a mask; nor can one whose bias is -inf or NaN be chosen), nor counts in its group's value; a group of such experts only is chosen last.  Where fewer than k experts are
+ * left, the remaining slots get id -1 and weight 0, which frk_hip_moe_ffn_dev skips.  Logits of +inf share a softmax evenly.
+ * The reference's routers with sigmoid scores, a bias and groups live in crates/frink-moe; the plain softmax one, whose f32
+ * arithmetic a caller may depend on, is frk_hip_route_top_k_softmax_dev.
+ * n_experts <= 1024, k <= 64, groups <= 64 and a divisor of n_experts, top_groups * (n_experts / groups) >= k. */
+enum { FRK_SCORE_SOFTMAX = 0, FRK_SCORE_SIGMOID = 1 };
+typedef struct {
+    int32_t score;      /* FRK_SCORE_* */
+    int32_t norm;
+    int32_t groups, top_groups, group_best;
+    float scale;
+    const float *bias_dev;
+} frk_route_rule;
+int frk_hip_route_dev(const float *logits_dev, size_t batch, size_t n_experts, size_t k, const frk_route_rule *rule,
+                      int32_t *ids_dev, float *weights_dev, void *stream);
+
 /* Decoder::moe_ffn_batch (crates/frink-models/src/decoder/ffn_batch.rs:343-434) with SwiGLU experts
  * (frink_moe::run_expert, crates/frink-moe/src/lib.rs:1068-1165): out[batch][hidden] =
  * sum over each token's k routed experts of weights * down_e(silu(gate_e x) * up_e x), added in the
@@ -284,7 +337,7 @@ int frk_hip_route_top_k_softmax_dev(const float *logits_dev, size_t batch, size_
  * ffn_batch.rs:355), routing order below (the per-position path's combine_expert_outputs,
  * crates/frink-moe/src/lib.rs:1246-1263).  gate/up/down hold the experts stacked row-wise
  * (expert e = rows [e*ffn, (e+1)*ffn) of gate and up, [e*hidden, (e+1)*hidden) of down); gate and up
- * are Q4_K, down is Q4_K or Q6_K; or all three of Q5_0 / IQ4_XS / MXFP4 (gate and up of one kind): below 32 tokens
+ * are Q4_K, down is Q4_K or Q6_K; or all three FP8_BLOCK; or all three of Q5_0 / IQ4_XS / MXFP4 (gate and up of one kind): below 32 tokens
  * every (token, slot) pair runs on the integer decode kernel of its kind (MXFP4: while that is estimated to be the
  * faster one), from there on the pairs are bucketed by expert and the experts run on a grouped matrix-core kernel,
  * decoded to signed bytes in scratch memory or (MXFP4 rows of 384 columns and more) as they are stored; an MXFP4
