@@ -8,7 +8,7 @@ fn main() {
     let hipcc = std::env::var("HIPCC").unwrap_or_else(|_| "/opt/rocm/bin/hipcc".into());
     let srcs = [
         "frk_runtime.cpp", "frk_quant.hip", "frk_gemv.hip", "frk_gemv_fused.hip", "frk_gemm.hip", "frk_gemm_q6.hip", "frk_gemm_rows.hip",
-        "frk_gemm_q8.hip", "frk_gemm_q8_pipe.hip", "frk_gemm_mx.hip", "frk_mx_experts.hip", "frk_f8.hip", "frk_moe.hip", "frk_route.hip", "frk_thin.hip", "frk_gemv_direct.hip", "frk_gemv_f32dot.hip", "frk_kinds.hip", "frk_probe.hip",
+        "frk_gemm_q8.hip", "frk_gemm_q8_pipe.hip", "frk_gemm_mx.hip", "frk_mx_experts.hip", "frk_f8.hip", "frk_f8_tile.hip", "frk_moe.hip", "frk_route.hip", "frk_thin.hip", "frk_gemv_direct.hip", "frk_gemv_f32dot.hip", "frk_kinds.hip", "frk_probe.hip",
     ];
     let mut objs = vec![];
     for s in srcs {
@@ -16,6 +16,7 @@ fn main() {
         let ok = std::process::Command::new(&hipcc)
             .args(["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Iinclude",
                    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-x", "hip", "-c"])
+            .args(if s == "frk_f8_tile.hip" { &["-mllvm", "-amdgpu-mfma-vgpr-form"][..] } else { &[][..] })
             .arg(format!("csrc/{s}"))
             .arg("-o")
             .arg(&o)

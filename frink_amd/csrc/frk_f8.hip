@@ -125,18 +125,7 @@ int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols
 }
 
 // ---- the GEMM.  A workgroup of eight wavefronts has one strip of sixteen weight rows and up to 16 TT tokens; its wavefronts
-// share the columns, in order, and their sums meet in LDS.  A tile is {matrix, first row of the order, rows in use, first row
-// of y}; row i of the order reads activation row src[i] (i itself without a list). ----
-struct F8Gemm {
-    F8Mat w;
-    F8Acts a;
-    const int *src;
-    const int4 *tiles;  // null: dense, matrix blockIdx.y
-    const int *n_tiles;
-    int M;  // dense: rows of x
-    size_t ldy;
-    float *y;
-};
+// share the columns, in order, and their sums meet in LDS. ----
 constexpr int F8_WAVES = 8;
 template <int TT>
 __global__ __launch_bounds__(64 * F8_WAVES) void f8_gemm_kernel(F8Gemm g) {
@@ -224,6 +213,7 @@ int launch_f8_gemm(const frk_weights *w, const float *x, size_t batch, float *y,
     const size_t jobs = g.w.strips * tok_tiles;
     if (jobs > 0x7fffffffu || w->matrices > 65535) return set_error(FRK_ERR_SHAPE, "%zu rows over %zu matrices of %d: too many", batch, w->matrices, g.w.rows);
     const dim3 grid((unsigned)jobs, (unsigned)w->matrices);
+    if (batch > 64) return launch_f8_tile(g, (batch + 127) / 128, w->matrices, s);
     if (batch <= 16) hipLaunchKernelGGL(f8_gemm_kernel<1>, grid, dim3(64 * F8_WAVES), 0, s, g);
     else if (batch <= 32) hipLaunchKernelGGL(f8_gemm_kernel<2>, grid, dim3(64 * F8_WAVES), 0, s, g);
     else hipLaunchKernelGGL(f8_gemm_kernel<4>, grid, dim3(64 * F8_WAVES), 0, s, g);

@@ -148,6 +148,20 @@ __device__ __forceinline__ void f8_quantize_quad(const float *__restrict__ x, co
         *reinterpret_cast<uint4 *>(out.v + row * (size_t)blocks * F8_BLOCK + (size_t)quad * 4 * F8_BLOCK + lane * 8) = make_uint4(a.x, a.y, b.x, b.y);
 }
 
+// A product: of dense batches, or of tiles {matrix, first row of the order, rows in use, first row of y}, where row i of the order
+// reads activation row src[i] (i itself without a list).
+struct F8Gemm {
+    F8Mat w;
+    F8Acts a;
+    const int *src;
+    const int4 *tiles;  // null: dense, matrix blockIdx.y
+    const int *n_tiles;
+    int M;  // dense: rows of x
+    size_t ldy;
+    float *y;
+};
+int launch_f8_tile(const F8Gemm &g, size_t tok_tiles, size_t matrices, hipStream_t s);
+
 // ---- entry points for the runtime and the expert layers ----
 Layout f8_layout(size_t rows, size_t cols, size_t matrices, size_t *bytes);
 int launch_f8_repack(const uint8_t *src, const float *scales, const frk_weights *w, hipStream_t s);
