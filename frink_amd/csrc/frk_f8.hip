@@ -101,25 +101,25 @@ int launch_f8_dequant_rows(const frk_weights *w, const int32_t *ids, size_t n_ou
     return FRK_OK;
 }
 
-// ---- quantization of a batch: a wavefront four blocks of a row ----
+// ---- quantization of a batch: a wavefront eight blocks of a row ----
 template <bool WIDE>
-__global__ __launch_bounds__(256) void f8_quantize_kernel(const float *__restrict__ x, const float *__restrict__ up, size_t jobs, int quads, int cols,
+__global__ __launch_bounds__(256) void f8_quantize_kernel(const float *__restrict__ x, const float *__restrict__ up, size_t jobs, int parts, int cols,
                                                           int blocks, const int *__restrict__ used, F8Acts out) {
     const int lane = threadIdx.x & 63;
     for (size_t j = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); j < jobs; j += (size_t)gridDim.x * 4) {
-        const size_t row = j / quads;
+        const size_t row = j / parts;
         if (used && used[row] < 0) continue;
-        f8_quantize_quad<WIDE>(x, up, row, (int)(j % quads), cols, blocks, lane, out);
+        f8_quantize_blocks<WIDE>(x, up, row, (int)(j % parts) * F8_QUANTIZE_BLOCKS, cols, blocks, lane, out);
     }
 }
 int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols, const int *used, const F8Acts &out, hipStream_t s) {
-    const int blocks = (int)f8_blocks(cols), quads = (blocks + 3) / 4;
-    const size_t jobs = rows * quads;
+    const int blocks = (int)f8_blocks(cols), parts = (blocks + F8_QUANTIZE_BLOCKS - 1) / F8_QUANTIZE_BLOCKS;
+    const size_t jobs = rows * parts;
     if (jobs == 0) return FRK_OK;
     const dim3 grid((unsigned)std::min<size_t>((jobs + 3) / 4, 1 << 16));
     const bool wide = f8_wide_rows(x, cols) && (!up || f8_wide_rows(up, cols));
-    if (wide) hipLaunchKernelGGL(f8_quantize_kernel<true>, grid, dim3(256), 0, s, x, up, jobs, quads, (int)cols, blocks, used, out);
-    else hipLaunchKernelGGL(f8_quantize_kernel<false>, grid, dim3(256), 0, s, x, up, jobs, quads, (int)cols, blocks, used, out);
+    if (wide) hipLaunchKernelGGL(f8_quantize_kernel<true>, grid, dim3(256), 0, s, x, up, jobs, parts, (int)cols, blocks, used, out);
+    else hipLaunchKernelGGL(f8_quantize_kernel<false>, grid, dim3(256), 0, s, x, up, jobs, parts, (int)cols, blocks, used, out);
     FRK_LAUNCH_CHECK("f8_quantize");
     return FRK_OK;
 }
@@ -127,6 +127,7 @@ int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols
 // ---- the GEMM.  A workgroup of eight wavefronts has one strip of sixteen weight rows and up to 16 TT tokens; its wavefronts
 // share the columns, in order, and their sums meet in LDS. ----
 constexpr int F8_WAVES = 8;
+constexpr int F8_MAX_TOKENS = 64;  // of a workgroup
 template <int TT>
 __global__ __launch_bounds__(64 * F8_WAVES) void f8_gemm_kernel(F8Gemm g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -213,7 +214,7 @@ int launch_f8_gemm(const frk_weights *w, const float *x, size_t batch, float *y,
     const size_t jobs = g.w.strips * tok_tiles;
     if (jobs > 0x7fffffffu || w->matrices > 65535) return set_error(FRK_ERR_SHAPE, "%zu rows over %zu matrices of %d: too many", batch, w->matrices, g.w.rows);
     const dim3 grid((unsigned)jobs, (unsigned)w->matrices);
-    if (batch > 64) return launch_f8_tile(g, (batch + 127) / 128, w->matrices, s);
+    if (batch > 64) return launch_f8_tile(g, 128, (batch + 127) / 128, w->matrices, 1, 0, s);
     if (batch <= 16) hipLaunchKernelGGL(f8_gemm_kernel<1>, grid, dim3(64 * F8_WAVES), 0, s, g);
     else if (batch <= 32) hipLaunchKernelGGL(f8_gemm_kernel<2>, grid, dim3(64 * F8_WAVES), 0, s, g);
     else hipLaunchKernelGGL(f8_gemm_kernel<4>, grid, dim3(64 * F8_WAVES), 0, s, g);
@@ -222,8 +223,8 @@ int launch_f8_gemm(const frk_weights *w, const float *x, size_t batch, float *y,
 }
 
 // ---- grouped: the tile list of the groups given.  Offsets are clamped to 0 .. pairs and made non-decreasing (each the largest
-// so far), so the tiles are at most pairs / 64 + groups whatever the list holds.  One workgroup of 1024 threads, a group each. ----
-__global__ __launch_bounds__(1024) void f8_tiles_kernel(const int32_t *__restrict__ group_off, int n_groups, int pairs, int4 *__restrict__ tiles,
+// so far), so the tiles are at most pairs / tokens + groups whatever the list holds.  One workgroup of 1024 threads, a group each. ----
+__global__ __launch_bounds__(1024) void f8_tiles_kernel(const int32_t *__restrict__ group_off, int n_groups, int pairs, int tokens, int4 *__restrict__ tiles,
                                                         int *__restrict__ n_tiles) {
     __shared__ int off[1025], at[1025];
     const int tid = threadIdx.x;
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(1024) void f8_tiles_kernel(const int32_t *__restric
             top = max(top, off[g]);
             if (g) {
                 at[g - 1] = n;
-                n += (top - from + F8_MAX_TOKENS - 1) / F8_MAX_TOKENS;
+                n += (top - from + tokens - 1) / tokens;
             }
             off[g] = top;
         }
@@ -245,15 +246,19 @@ __global__ __launch_bounds__(1024) void f8_tiles_kernel(const int32_t *__restric
     __syncthreads();
     if (tid < n_groups) {
         const int n = off[tid + 1] - off[tid];
-        for (int i = 0; i * F8_MAX_TOKENS < n; i++)
-            tiles[at[tid] + i] = make_int4(tid, off[tid] + i * F8_MAX_TOKENS, min(F8_MAX_TOKENS, n - i * F8_MAX_TOKENS), off[tid] + i * F8_MAX_TOKENS);
+        for (int i = 0; i * tokens < n; i++)
+            tiles[at[tid] + i] = make_int4(tid, off[tid] + i * tokens, min(tokens, n - i * tokens), off[tid] + i * tokens);
     }
 }
-static size_t f8_max_tiles(size_t pairs, size_t groups) { return pairs / F8_MAX_TOKENS + std::min(groups, pairs); }
-size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs) {
-    return f8_acts_bytes(x_rows, w->cols) + 256 + f8_max_tiles(pairs, w->matrices) * 16;
+static size_t f8_max_tiles(size_t pairs, size_t groups, int tokens) { return pairs / (size_t)tokens + std::min(groups, pairs); }
+static int f8_tile_tokens(size_t pairs, size_t groups) {
+    const size_t mean = pairs / groups;
+    return mean >= 96 ? 128 : mean >= 16 ? 64 : 32;
 }
-int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, const int *src, const int4 *tiles, const int *n_tiles, size_t max_tiles, float *y,
+size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs) {
+    return f8_acts_bytes(x_rows, w->cols) + 256 + f8_max_tiles(pairs, w->matrices, 32) * 16;
+}
+int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, int tokens, const int *src, const int4 *tiles, const int *n_tiles, size_t max_tiles, float *y,
                     hipStream_t s) {
     F8Gemm g{};
     g.w = f8_mat(w);
@@ -263,23 +268,19 @@ int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, const int *src, co
     g.n_tiles = n_tiles;
     g.ldy = g.w.rows;
     g.y = y;
-    const size_t jobs = g.w.strips * max_tiles;
-    if (jobs == 0) return FRK_OK;
-    if (jobs > 0x7fffffffu) return set_error(FRK_ERR_SHAPE, "%zu tiles over matrices of %d rows: too many", max_tiles, g.w.rows);
-    hipLaunchKernelGGL(f8_gemm_kernel<4>, dim3((unsigned)jobs), dim3(64 * F8_WAVES), 0, s, g);
-    FRK_LAUNCH_CHECK("f8_tiles");
-    return FRK_OK;
+    return launch_f8_tile(g, tokens, max_tiles, 1, 1, 0, s);
 }
 int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
                       float *y, void *ws, hipStream_t s) {
     const F8Acts acts = f8_acts_carve(ws, x_rows);
+    const int tokens = f8_tile_tokens(pairs, w->matrices);
     int *n_tiles = (int *)((char *)ws + f8_acts_bytes(x_rows, w->cols));
     int4 *tiles = (int4 *)(n_tiles + 64);
     int rc = launch_f8_quantize(x, nullptr, x_rows, w->cols, nullptr, acts, s);
     if (rc) return rc;
-    hipLaunchKernelGGL(f8_tiles_kernel, dim3(1), dim3(1024), 0, s, group_off, (int)w->matrices, (int)pairs, tiles, n_tiles);
+    hipLaunchKernelGGL(f8_tiles_kernel, dim3(1), dim3(1024), 0, s, group_off, (int)w->matrices, (int)pairs, tokens, tiles, n_tiles);
     FRK_LAUNCH_CHECK("f8_tile_list");
-    return launch_f8_tiles(w, acts, gather, tiles, n_tiles, f8_max_tiles(pairs, w->matrices), y, s);
+    return launch_f8_tiles(w, acts, tokens, gather, tiles, n_tiles, f8_max_tiles(pairs, w->matrices, tokens), y, s);
 }
 
 }  // namespace frk

@@ -60,22 +60,27 @@ static inline F8Acts f8_acts_carve(void *base, size_t rows) {
     return a;
 }
 
-// ---- quantization: sixteen lanes a block, eight neighbouring values each ----
-__device__ __forceinline__ uint32_t f8_row_max(uint32_t v) {  // over a row of 16 lanes
+// ---- quantization: 32 lanes a block, four neighbouring values each (whole lines a load, and a store of eight bytes a lane) ----
+__device__ __forceinline__ uint32_t f8_half_max(uint32_t v) {  // over 32 lanes
     v = max(v, (uint32_t)dpp_i<DPP_QUAD_XOR1>((int)v));
     v = max(v, (uint32_t)dpp_i<DPP_QUAD_XOR2>((int)v));
     v = max(v, (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)v));
-    return max(v, (uint32_t)dpp_i<DPP_ROW_MIRROR>((int)v));
+    v = max(v, (uint32_t)dpp_i<DPP_ROW_MIRROR>((int)v));
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto rows = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // rows 0, 0, 2, 2 and 1, 1, 3, 3
+    v = max((uint32_t)rows[0], (uint32_t)rows[1]);
+#endif
+    return v;
 }
-// the eight values' codes; `scale` = 2^e of the block
-__device__ __forceinline__ uint2 f8_quantize8(const float (&v)[8], float &scale) {
+// the four values' codes; `scale` = 2^e of the block
+__device__ __forceinline__ uint32_t f8_quantize4(const float (&v)[4], float &scale) {
     uint32_t top = 0;  // magnitudes compare as their bits
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < 4; i++) {
         const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu;
         top = max(top, m < 0x7f800000u ? m : 0u);
     }
-    top = f8_row_max(top);
+    top = f8_half_max(top);
     // 448 = 1.75 * 2^8: e is the exponent less 8, one more where the mantissa is above 1.75
     const int b = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
     const uint32_t biased = (uint32_t)max(b, 127 - 100);
@@ -83,37 +88,30 @@ __device__ __forceinline__ uint2 f8_quantize8(const float (&v)[8], float &scale)
     const float up = __uint_as_float((254u - biased) << 23);  // 2^-e
     // (256 * 2^120 is no float any more: there the largest code is 240's)
     const float most = biased == 127 + 120 ? 240.0f : 448.0f;
-    float z[8];
+    float z[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) z[i] = fminf(fmaxf(v[i] * up, -most), most);
-    uint32_t w[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < 4; i++) z[i] = fminf(fmaxf(v[i] * up, -most), most);
+    uint32_t codes = 0;
 #if defined(__HIP_DEVICE_COMPILE__)
-        int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i], z[4 * i + 1], 0, false);
-        p = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i + 2], z[4 * i + 3], p, true);
-        w[i] = (uint32_t)p;
-#else
-        w[i] = 0;
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+    codes = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], p, true);
 #endif
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if ((__float_as_uint(v[4 * i + j]) & 0x7f800000u) == 0x7f800000u) w[i] = (w[i] & ~(0xffu << (8 * j))) | (0x7fu << (8 * j));
-    }
-    return make_uint2(w[0], w[1]);
+    for (int j = 0; j < 4; j++)
+        if ((__float_as_uint(v[j]) & 0x7f800000u) == 0x7f800000u) codes = (codes & ~(0xffu << (8 * j))) | (0x7fu << (8 * j));
+    return codes;
 }
 
-// eight values of a row from column k on, zeros past `cols`; WIDE: rows whose 16-byte pieces are aligned and whole
+// four values of a row from column k on, zeros past `cols`; WIDE: rows whose 16-byte pieces are aligned and whole
 template <bool WIDE>
-__device__ __forceinline__ void f8_load8(const float *__restrict__ row, int k, int cols, float (&v)[8]) {
+__device__ __forceinline__ void f8_load4(const float *__restrict__ row, int k, int cols, float (&v)[4]) {
     if (WIDE) {
-        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 a = k < cols ? *reinterpret_cast<const float4 *>(row + k) : zero;
-        const float4 b = k + 4 < cols ? *reinterpret_cast<const float4 *>(row + k + 4) : zero;
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k < cols) a = *reinterpret_cast<const float4 *>(row + k);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = k + i < cols ? row[k + i] : 0.0f;
+        for (int i = 0; i < 4; i++) v[i] = k + i < cols ? row[k + i] : 0.0f;
     }
 }
 static inline bool f8_wide_rows(const float *x, size_t cols) { return cols % 4 == 0 && (uintptr_t)x % 16 == 0; }
@@ -130,22 +128,32 @@ __device__ __forceinline__ uint2 f8_to_bf16(uint32_t codes, float scale) {
     return out;
 }
 
-// four blocks of a row by a wavefront; with `up` of silu(x) * up, element by element
+// eight blocks of a row by a wavefront, all their loads ahead; with `up` of silu(x) * up, element by element
+constexpr int F8_QUANTIZE_BLOCKS = 8;
 template <bool WIDE>
-__device__ __forceinline__ void f8_quantize_quad(const float *__restrict__ x, const float *__restrict__ up, size_t row, int quad, int cols, int blocks,
-                                                 int lane, const F8Acts &out) {
-    float v[8], scale;
-    f8_load8<WIDE>(x + row * (size_t)cols, quad * 4 * F8_BLOCK + lane * 8, cols, v);
-    if (up) {
-        float u[8];
-        f8_load8<WIDE>(up + row * (size_t)cols, quad * 4 * F8_BLOCK + lane * 8, cols, u);
+__device__ __forceinline__ void f8_quantize_blocks(const float *__restrict__ x, const float *__restrict__ up, size_t row, int first, int cols, int blocks,
+                                                   int lane, const F8Acts &out) {
+    constexpr int N = F8_QUANTIZE_BLOCKS / 2;
+    const int k = first * F8_BLOCK + lane * 4;
+    float v[N][4], u[N][4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = silu_as_host(v[i]) * u[i];
+    for (int i = 0; i < N; i++) f8_load4<WIDE>(x + row * (size_t)cols, k + i * 2 * F8_BLOCK, cols, v[i]);
+    if (up) {
+#pragma unroll
+        for (int i = 0; i < N; i++) f8_load4<WIDE>(up + row * (size_t)cols, k + i * 2 * F8_BLOCK, cols, u[i]);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[i][j] = silu_as_host(v[i][j]) * u[i][j];
     }
-    const uint2 codes = f8_quantize8(v, scale);
-    const uint2 a = f8_to_bf16(codes.x, scale), b = f8_to_bf16(codes.y, scale);
-    if (quad * 4 + (lane >> 4) < blocks)
-        *reinterpret_cast<uint4 *>(out.v + row * (size_t)blocks * F8_BLOCK + (size_t)quad * 4 * F8_BLOCK + lane * 8) = make_uint4(a.x, a.y, b.x, b.y);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (first + 2 * i >= blocks) break;  // (uniform)
+        float scale;
+        const uint32_t codes = f8_quantize4(v[i], scale);
+        if (first + 2 * i + (lane >> 5) < blocks)
+            *reinterpret_cast<uint2 *>(out.v + row * (size_t)blocks * F8_BLOCK + k + i * 2 * F8_BLOCK) = f8_to_bf16(codes, scale);
+    }
 }
 
 // A product: of dense batches, or of tiles {matrix, first row of the order, rows in use, first row of y}, where row i of the order
@@ -160,7 +168,8 @@ struct F8Gemm {
     size_t ldy;
     float *y;
 };
-int launch_f8_tile(const F8Gemm &g, size_t tok_tiles, size_t matrices, hipStream_t s);
+// over tiles of `tokens` tokens (32, 64 or 128); parts > 1 (dense): shares of the columns, each its own copy of y, part_stride floats apart
+int launch_f8_tile(const F8Gemm &g, int tokens, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s);
 
 // ---- entry points for the runtime and the expert layers ----
 Layout f8_layout(size_t rows, size_t cols, size_t matrices, size_t *bytes);
@@ -172,10 +181,9 @@ int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int3
                       float *y, void *ws, hipStream_t s);
 // rows of x (of silu(x) * up) quantized; `used`: a row whose entry is negative is left as it is
 int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols, const int *used, const F8Acts &out, hipStream_t s);
-// the products of the tiles {matrix, first row of the order, rows in use (up to F8_MAX_TOKENS), first row of y}; row i of the order is
+// the products of the tiles {matrix, first row of the order, rows in use (up to `tokens`), first row of y}; row i of the order is
 // activation row src[i], or i
-constexpr int F8_MAX_TOKENS = 64;
-int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, const int *src, const int4 *tiles, const int *n_tiles, size_t max_tiles, float *y,
+int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, int tokens, const int *src, const int4 *tiles, const int *n_tiles, size_t max_tiles, float *y,
                     hipStream_t s);
 
 }  // namespace frk

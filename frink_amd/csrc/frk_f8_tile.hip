@@ -16,40 +16,46 @@ typedef float f8_v16f __attribute__((ext_vector_type(16)));
     } while (0)
 
 // RW x TW wavefronts of MR tiles of 32 weight rows x MT tiles of 32 tokens each
-template <int RW, int TW, int MR, int MT>
+template <int RW, int TW, int MR, int MT, int STAGES>
 struct F8TileShape {
     static constexpr int WAVES = RW * TW, ROWS = RW * MR * 32, TOKENS = TW * MT * 32;
     static constexpr int W_BYTES = ROWS * F8_BLOCK, X_BYTES = TOKENS * F8_BLOCK * 2, STAGE = W_BYTES + X_BYTES;
     static constexpr int W_REQ = W_BYTES / 1024 / WAVES, X_REQ = X_BYTES / 1024 / WAVES;
     static_assert(W_REQ * WAVES * 1024 == W_BYTES && X_REQ * WAVES * 1024 == X_BYTES, "whole requests");
-    static constexpr size_t LDS = 2 * STAGE;
+    static constexpr int REQUESTS = W_REQ + X_REQ;  // of a wavefront and block
+    static_assert(STAGES >= 2 && REQUESTS * (STAGES - 1) < 64, "requests that a wait can count");
+    static constexpr size_t LDS = STAGES * STAGE;
     static_assert(LDS <= 160 * 1024 && F8_BLOCK % (MR * 32) == 0, "LDS of a CU; a wavefront's rows in one block of scales");
 };
 
-template <int RW, int TW, int MR, int MT>
-__global__ __launch_bounds__(64 * RW * TW, 1) void f8_tile_kernel(F8Gemm g, int row_tiles, int tok_tiles) {
+template <int RW, int TW, int MR, int MT, int STAGES>
+__global__ __launch_bounds__(64 * RW * TW, 2) void f8_tile_kernel(F8Gemm g, int row_tiles, int tok_tiles, int matrices, int parts, size_t part_stride) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    using T = F8TileShape<RW, TW, MR, MT>;
+    using T = F8TileShape<RW, TW, MR, MT, STAGES>;
     extern __shared__ __align__(16) uint8_t f8_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int li = lane & 31, lh = lane >> 5;
     const int rw = wave % RW, tw = wave / RW;
-    // an XCD (workgroup id mod 8) takes a run of the list, row tiles of a token tile after one another
+    // An XCD (workgroup id mod 8) takes a run of the list, which goes through panels of eight token tiles row tile by row tile: its 32
+    // CUs then work on 4 row tiles x 8 token tiles, whose blocks its L2 holds once.
+    if (g.tiles) tok_tiles = min(*g.n_tiles, tok_tiles);
     const int total = row_tiles * tok_tiles, per_xcd = (total + 7) / 8;
     const int index = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
     if (((int)blockIdx.x >> 3) >= per_xcd || index >= total) return;
-    const int row_tile = index / tok_tiles, tok_tile = index % tok_tiles;
+    const int panel = index / (8 * row_tiles), wide_panel = min(8, tok_tiles - 8 * panel), in_panel = index - panel * 8 * row_tiles;
+    const int row_tile = in_panel / wide_panel, tok_tile = 8 * panel + in_panel % wide_panel;
     int4 tile;
     size_t y_col = 0;
     if (g.tiles) {
-        if (tok_tile >= *g.n_tiles) return;
         tile = g.tiles[tok_tile];
     } else {
         const int first = tok_tile * T::TOKENS;
-        tile = make_int4((int)blockIdx.y, first, min(T::TOKENS, g.M - first), first);
-        y_col = (size_t)blockIdx.y * g.w.rows;
+        tile = make_int4((int)blockIdx.y % matrices, first, min(T::TOKENS, g.M - first), first);
+        y_col = (size_t)tile.x * g.w.rows;
     }
-    const int blocks = g.w.blocks;
+    // this part's columns
+    const int part = (int)blockIdx.y / matrices, blocks = g.w.blocks;
+    const int from = (int)((long long)blocks * part / parts), until = (int)((long long)blocks * (part + 1) / parts);
     const uint32_t lds0 = lds_address(f8_lds);
     const int strip0 = row_tile * (T::ROWS / F8_STRIP);
 
@@ -72,9 +78,8 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void f8_tile_kernel(F8Gemm g, int 
         w_off[c] = (uint32_t)strip * (uint32_t)blocks * F8_PIECE + (uint32_t)((n & 1) * 1024 + lane * 16);
     }
     const uint8_t *const w_base = g.w.q + ((size_t)tile.x * g.w.strips + strip0) * blocks * F8_PIECE;
-    constexpr int REQUESTS = T::W_REQ + T::X_REQ;  // of a wavefront and block
     auto request = [&](int slot, int b, int c) {
-        const uint32_t to = lds0 + (uint32_t)(slot & 1) * T::STAGE;
+        const uint32_t to = lds0 + (uint32_t)slot * T::STAGE;
         if (c < T::W_REQ) dma16(to + (wave * T::W_REQ + c) * 1024, w_base + (size_t)b * F8_PIECE, w_off[c]);
         else dma16(to + T::W_BYTES + (wave * T::X_REQ + c - T::W_REQ) * 1024, x_base + (size_t)b * (F8_BLOCK * 2), x_off[c - T::W_REQ]);
     };
@@ -110,35 +115,38 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void f8_tile_kernel(F8Gemm g, int 
     // ---- A block is MR * MT steps of one tile's eight products.  Beside a step's products the wavefront adds the step before's sums, scaled,
     // converts the next row tile's codes (in a row tile's last step), and in a block's last row tile reads the next block's
     // tokens and first codes: that block is waited for in front of it, behind which nobody reads the present one any more.
-    for (int c = 0; c < REQUESTS; c++) request(0, 0, c);
-    for (int c = 0; c < REQUESTS; c++) request(1, min(1, blocks - 1), c);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(REQUESTS) : "memory");
+    for (int a = 0; a < STAGES; a++)
+        for (int c = 0; c < T::REQUESTS; c++) request(a, min(from + a, until - 1), c);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::REQUESTS * (STAGES - 1)) : "memory");
     lds_barrier();
-    f8_v8bf x0[MT][8], x1[MT][8], w[8];
+    f8_v8bf x[MT][8], w[8];
     uint4 raw[4];
 #pragma unroll
     for (int j = 0; j < MT; j++)
 #pragma unroll
-        for (int k = 0; k < 8; k++) x0[j][k] = read_x(f8_lds, j, k);
+        for (int k = 0; k < 8; k++) x[j][k] = read_x(f8_lds, j, k);
 #pragma unroll
     for (int k = 0; k < 4; k++) raw[k] = read_w(f8_lds, 0, k);
 #pragma unroll
     for (int k = 0; k < 8; k++) w[k] = convert(raw, k);
     f8_v16f p[2] = {f8_v16f{0.0f}, f8_v16f{0.0f}};
-    float s_before = 0.0f, s = scales[0];
+    float s_before = 0.0f, s = scales[from];
+    int slot = 0, next_slot = 1;
     constexpr int STEPS = MR * MT;
     static_assert(STEPS % 2 == 0, "the two sums");
-    auto block = [&](int b, f8_v8bf (&x)[MT][8], f8_v8bf (&xn)[MT][8]) {
-        const uint8_t *const st = f8_lds + (size_t)(b & 1) * T::STAGE, *const next = f8_lds + (size_t)((b + 1) & 1) * T::STAGE;
-        const float s_next = scales[min(b + 1, blocks - 1)];
+    for (int b = from; b < until; b++) {
+        const uint8_t *const st = f8_lds + (size_t)slot * T::STAGE, *const next = f8_lds + (size_t)next_slot * T::STAGE;
+        const float s_next = scales[min(b + 1, until - 1)];
 #pragma unroll
         for (int n = 0; n < STEPS; n++) {
             const int i = n / MT, j = n % MT;
             const bool last = i == MR - 1;  // the block's last row tile
             if (last && j == 0) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::REQUESTS * (STAGES - 2)) : "memory");
                 lds_barrier();
+                __builtin_amdgcn_s_setprio(1);
             }
+            if (n == 0) __builtin_amdgcn_s_setprio(0);
             f8_v16f &sum = p[n & 1], &before = p[(n + 1) & 1];
             f8_v16f &to = n == 0 ? acc[MR - 1][MT - 1] : acc[(n - 1) / MT][(n - 1) % MT];
             const float by = n == 0 ? s_before : s;
@@ -147,13 +155,13 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void f8_tile_kernel(F8Gemm g, int 
                 if (k == 0) sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[k], x[j][k], (f8_v16f{0.0f}), 0, 0, 0);
                 else sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[k], x[j][k], sum, 0, 0, 0);
                 if (j == 0 && k < 4) raw[k] = last ? read_w(next, 0, k) : read_w(st, i + 1, k);
-                if (last) xn[j][k] = read_x(next, j, k);
+                if (last) x[j][k] = read_x(next, j, k);
                 to[2 * k] = __builtin_fmaf(before[2 * k], by, to[2 * k]);
                 to[2 * k + 1] = __builtin_fmaf(before[2 * k + 1], by, to[2 * k + 1]);
                 if (j == MT - 1) w[k] = convert(raw, k);
-                if (last) {  // (past the end the last block again, which nobody reads)
+                if (last && j == 0) {  // (past the end the last block again, which nobody reads)
 #pragma unroll
-                    for (int c = (j * 8 + k) * REQUESTS / (8 * MT); c < (j * 8 + k + 1) * REQUESTS / (8 * MT); c++) request(b, min(b + 2, blocks - 1), c);
+                    for (int c = k * T::REQUESTS / 8; c < (k + 1) * T::REQUESTS / 8; c++) request(slot, min(b + STAGES, until - 1), c);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -161,23 +169,19 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void f8_tile_kernel(F8Gemm g, int 
         }
         s_before = s;
         s = s_next;
-    };
-    int b = 0;
-    for (; b + 1 < blocks; b += 2) {
-        block(b, x0, x1);
-        block(b + 1, x1, x0);
+        slot = next_slot;
+        next_slot = next_slot == STAGES - 1 ? 0 : next_slot + 1;
     }
-    if (b < blocks) block(b, x0, x1);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing comes into LDS that is no longer this workgroup's)
 #pragma unroll
     for (int r = 0; r < 16; r++) acc[MR - 1][MT - 1][r] = __builtin_fmaf(p[1][r], s_before, acc[MR - 1][MT - 1][r]);
     // register r of a lane: row 8 (r / 4) + 4 (lane / 32) + r % 4 of a tile, token lane % 32
-    const bool wide = g.ldy % 4 == 0 && (g.w.rows & 3) == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
+    const bool wide = g.ldy % 4 == 0 && (g.w.rows & 3) == 0 && part_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
 #pragma unroll
     for (int j = 0; j < MT; j++) {
         const int t = (tw * MT + j) * 32 + li;
         if (t >= tile.z) continue;
-        float *const dst = g.y + (size_t)(tile.w + t) * g.ldy + y_col;
+        float *const dst = g.y + part * part_stride + (size_t)(tile.w + t) * g.ldy + y_col;
 #pragma unroll
         for (int i = 0; i < MR; i++)
 #pragma unroll
@@ -195,20 +199,31 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void f8_tile_kernel(F8Gemm g, int 
 #endif
 }
 
-int launch_f8_tile(const F8Gemm &g, size_t tok_tiles, size_t matrices, hipStream_t s) {
-    using T = F8TileShape<2, 2, 4, 2>;
+template <int RW, int TW, int MR, int MT, int STAGES>
+static int go_f8_tile(const F8Gemm &g, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s) {
+    using T = F8TileShape<RW, TW, MR, MT, STAGES>;
     const size_t row_tiles = ((size_t)g.w.rows + T::ROWS - 1) / T::ROWS, total = row_tiles * tok_tiles;
-    if (total > 0x7ffffff8u) return set_error(FRK_ERR_SHAPE, "%zu x %zu tiles: too many", row_tiles, tok_tiles);
+    if (total > 0x7ffffff8u || matrices * parts > 65535) return set_error(FRK_ERR_SHAPE, "%zu x %zu tiles of %zu matrices: too many", row_tiles, tok_tiles, matrices);
+    if (total == 0) return FRK_OK;
+    // (a request's offset of a lane is 32 bits wide: a gathered row's from the first, others' from their tile's)
+    if (g.src && (size_t)g.a.rows * g.w.blocks * (F8_BLOCK * 2) > 0xffffffffu)
+        return set_error(FRK_ERR_SHAPE, "%d gathered rows of %d blocks: more than 4 GiB of quantized activations", g.a.rows, g.w.blocks);
     static bool sized = false;  // a benign race: every thread sets the same attribute
     if (!sized) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tile_kernel<2, 2, 4, 2>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::LDS);
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tile_kernel<RW, TW, MR, MT, STAGES>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)T::LDS);
         if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFuncSetAttribute(f8_tile): %s", hipGetErrorString(e));
         sized = true;
     }
-    hipLaunchKernelGGL((f8_tile_kernel<2, 2, 4, 2>), dim3((unsigned)((total + 7) / 8 * 8), (unsigned)matrices), dim3(64 * T::WAVES), T::LDS, s, g, (int)row_tiles,
-                       (int)tok_tiles);
+    hipLaunchKernelGGL((f8_tile_kernel<RW, TW, MR, MT, STAGES>), dim3((unsigned)((total + 7) / 8 * 8), (unsigned)(matrices * parts)), dim3(64 * T::WAVES), T::LDS, s,
+                       g, (int)row_tiles, (int)tok_tiles, (int)matrices, parts, part_stride);
     FRK_LAUNCH_CHECK("f8_tile");
     return FRK_OK;
+}
+int launch_f8_tile(const F8Gemm &g, int tokens, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s) {
+    if (tokens == 128) return go_f8_tile<4, 2, 2, 2, 2>(g, tok_tiles, matrices, parts, part_stride, s);
+    if (tokens == 64) return go_f8_tile<2, 2, 2, 1, 2>(g, tok_tiles, matrices, parts, part_stride, s);
+    return go_f8_tile<4, 1, 2, 1, 2>(g, tok_tiles, matrices, parts, part_stride, s);
 }
 
 }  // namespace frk
