@@ -124,137 +124,289 @@ int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols
     return FRK_OK;
 }
 
-// ---- the GEMM.  A workgroup of eight wavefronts has one strip of sixteen weight rows and up to 16 TT tokens; its wavefronts
-// share the columns, in order, and their sums meet in LDS. ----
-constexpr int F8_WAVES = 8;
-constexpr int F8_MAX_TOKENS = 64;  // of a workgroup
-template <int TT>
-__global__ __launch_bounds__(64 * F8_WAVES) void f8_gemm_kernel(F8Gemm g) {
+// ---- A few tokens: the weights' bytes and the launch's own chain of steps bound it.  A workgroup of NW wavefronts has one strip of sixteen
+// weight rows and up to 16 TT tokens; its wavefronts share the columns, in order, straight from memory into registers, D blocks
+// ahead, and their sums meet in LDS.
+//   DENSE  strip blockIdx.x, matrix blockIdx.y, token tile blockIdx.z
+//   PAIRS  strip blockIdx.x, pair blockIdx.y of a grouped product: every sixteenth (FUSED: fourth) pair of its group takes the
+//          group's next sixteen (four), the others end at once.  No list is made in front of it: each wavefront looks the group up itself
+// FUSED: up to F8_FUSED tokens are quantized by the workgroup itself (a wavefront its own columns', while its first codes
+// are on their way), not by a launch in front. ----
+struct F8Rows {
+    F8Mat w;
+    F8Acts a;           // not FUSED
+    const float *x;     // FUSED
+    int cols, x_rows;
+    int M;                          // DENSE
+    const int *group_off, *gather;  // PAIRS
+    int n_groups, pairs;
+    size_t ldy;
+    float *y;
+};
+constexpr size_t F8_FUSED = 4;
+constexpr size_t F8_FUSED_LDS = 64 * 1024;
+
+// the range of up to `most` pairs that pair `p` leads, by the offsets clamped and made non-decreasing (each the largest so far): {group, first, number};
+// a number of 0: it leads none
+__device__ __forceinline__ int4 f8_lead(const int *__restrict__ off, int n_groups, int pairs, int p, int most, int lane) {
+    int after = n_groups + 1;  // the first offset above p
+    for (int i = lane; i <= n_groups; i += 64)
+        if (min(max(off[i], 0), pairs) > p) {
+            after = i;
+            break;
+        }
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) after = min(after, __shfl_xor(after, m));
+    if (after == 0 || after > n_groups) return make_int4(0, 0, 0, 0);
+    int begin = 0;
+    for (int i = lane; i < after; i += 64) begin = max(begin, min(max(off[i], 0), pairs));
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) begin = max(begin, __shfl_xor(begin, m));
+    const int end = min(max(off[after], 0), pairs);
+    if ((p - begin) % most) return make_int4(0, 0, 0, 0);
+    return make_int4(after - 1, p, min(most, end - p), 0);
+}
+
+template <int NW, int TT, int D, bool FUSED, bool PAIRS, bool WIDE>
+__global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ float4 sums[F8_WAVES][TT][64];
+    static_assert(!PAIRS || TT == 1, "sixteen pairs");
+    extern __shared__ __align__(16) uint8_t f8_rows_lds[];  // FUSED: [blocks][tokens][128] bf16
+    __shared__ float4 sums[NW][TT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int strip = (int)(blockIdx.x % (unsigned)g.w.strips), t_index = (int)(blockIdx.x / (unsigned)g.w.strips);
-    int4 tile;
-    size_t y_col;  // of the matrix's first row
-    if (g.tiles) {
-        if (t_index >= *g.n_tiles) return;
-        tile = g.tiles[t_index];
-        y_col = 0;
+    const int strip = blockIdx.x, blocks = g.w.blocks;
+    int matrix, first, used;
+    size_t y_col = 0;
+    if (PAIRS) {
+        const int4 lead = f8_lead(g.group_off, g.n_groups, g.pairs, (int)blockIdx.y, FUSED ? (int)F8_FUSED : 16, lane);
+        matrix = __builtin_amdgcn_readfirstlane(lead.x), first = __builtin_amdgcn_readfirstlane(lead.y), used = __builtin_amdgcn_readfirstlane(lead.z);
+        if (used == 0) return;
     } else {
-        const int first = t_index * 16 * TT;
-        tile = make_int4((int)blockIdx.y, first, min(16 * TT, g.M - first), first);
-        y_col = (size_t)blockIdx.y * g.w.rows;
+        matrix = blockIdx.y, first = (int)blockIdx.z * 16 * TT, used = min(16 * TT, g.M - first);
+        y_col = (size_t)matrix * g.w.rows;
     }
-    const int b0 = g.w.blocks * wave / F8_WAVES, b1 = g.w.blocks * (wave + 1) / F8_WAVES;
-    const uint8_t *wq = g.w.q + (((size_t)tile.x * g.w.strips + strip) * g.w.blocks) * F8_PIECE + lane * 16;
-    const float *ws = g.w.s + ((size_t)tile.x * g.w.row_blocks + strip * F8_STRIP / F8_BLOCK) * g.w.blocks;
-    int row[TT];
+    const int b0 = (int)((long long)blocks * wave / NW), b1 = (int)((long long)blocks * (wave + 1) / NW);
+    const uint8_t *const wq = g.w.q + (((size_t)matrix * g.w.strips + strip) * blocks) * F8_PIECE + lane * 16;
+    const float *const ws = g.w.s + ((size_t)matrix * g.w.row_blocks + strip * F8_STRIP / F8_BLOCK) * blocks;
+    int row[TT];  // this lane's activation rows
 #pragma unroll
     for (int t = 0; t < TT; t++) {
-        const int i = tile.y + min(16 * t + (lane & 15), tile.z - 1);
-        row[t] = min(max(g.src ? g.src[i] : i, 0), g.a.rows - 1);
+        const int i = first + min(16 * t + (lane & 15), used - 1);
+        row[t] = min(max(PAIRS && g.gather ? g.gather[i] : i, 0), g.x_rows - 1);
     }
     f8_v4f acc[TT];
 #pragma unroll
     for (int t = 0; t < TT; t++) acc[t] = f8_v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    auto operand = [](uint32_t lo, uint32_t hi) {
-        const uint2 a = f8_to_bf16(lo, 1.0f), b = f8_to_bf16(hi, 1.0f);
-        const uint4 v = make_uint4(a.x, a.y, b.x, b.y);
-        f8_v8bf o;
-        __builtin_memcpy(&o, &v, 16);
-        return o;
-    };
-    for (int b = b0; b < b1; b++) {
-        const uint4 w0 = *reinterpret_cast<const uint4 *>(wq + (size_t)b * F8_PIECE), w1 = *reinterpret_cast<const uint4 *>(wq + (size_t)b * F8_PIECE + 1024);
-        const f8_v8bf w[4] = {operand(w0.x, w0.y), operand(w0.z, w0.w), operand(w1.x, w1.y), operand(w1.z, w1.w)};
-        const float s = ws[b];
+    if (b0 < b1) {
+        uint4 w[D][2], x[FUSED ? 1 : D][TT][4];
+        float s[D];
+        auto fetch_w = [&](int u, int b) {
+            const uint8_t *const at = wq + (size_t)min(b, b1 - 1) * F8_PIECE;
+            w[u][0] = stream_load16(at);
+            w[u][1] = stream_load16(at + 1024);
+            s[u] = ws[min(b, b1 - 1)];
+        };
+        auto fetch_x = [&](int u, int b) {
 #pragma unroll
-        for (int t = 0; t < TT; t++) {
-            const f8_v8bf *x = reinterpret_cast<const f8_v8bf *>(g.a.v + ((size_t)row[t] * g.w.blocks + b) * F8_BLOCK + (lane >> 4) * 32);
-            f8_v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < TT; t++) {
+                const size_t piece = PAIRS ? (size_t)row[t] * blocks + min(b, b1 - 1) : ((size_t)min((first >> 4) + t, (g.x_rows - 1) >> 4) * blocks + min(b, b1 - 1)) * F8_STRIP;
+                const uint4 *const at = reinterpret_cast<const uint4 *>(g.a.v + piece * F8_BLOCK) + (PAIRS ? (lane >> 4) * 4 : lane);
 #pragma unroll
-            for (int k = 0; k < 4; k++) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[k], x[k], p, 0, 0, 0);
+                for (int k = 0; k < 4; k++) x[u][t][k] = at[PAIRS ? k : k * 64];
+            }
+        };
+        uint16_t *const own = reinterpret_cast<uint16_t *>(f8_rows_lds) + (size_t)b0 * used * F8_BLOCK;  // FUSED: [block - b0][token][128]
+        if (FUSED) {
+            constexpr int N = 4;  // pairs of blocks a pass
+            float v[N][4];
+            auto load = [&](int t, int at) {
+                const float *const xr = g.x + (size_t)__builtin_amdgcn_readlane(row[0], t) * g.cols;
 #pragma unroll
-            for (int r = 0; r < 4; r++) acc[t][r] = __builtin_fmaf(p[r], s, acc[t][r]);
+                for (int i = 0; i < N; i++) f8_load4<WIDE>(xr, (at + 2 * i) * F8_BLOCK + lane * 4, min(g.cols, b1 * F8_BLOCK), v[i]);
+            };
+            auto store = [&](int t, int at) {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    if (at + 2 * i >= b1) break;  // (uniform)
+                    float scale;
+                    const uint32_t codes = f8_quantize4(v[i], scale);
+                    const int b = at + 2 * i + (lane >> 5);
+                    if (b < b1) *reinterpret_cast<uint2 *>(own + ((size_t)(b - b0) * used + t) * F8_BLOCK + (lane & 31) * 4) = f8_to_bf16(codes, scale);
+                }
+            };
+            load(0, b0);
+#pragma unroll
+            for (int u = 0; u < D; u++) fetch_w(u, b0 + u);
+            store(0, b0);
+            for (int t = 0, at = b0 + 2 * N; t < used; t++, at = b0)
+                for (; at < b1; at += 2 * N) {
+                    load(t, at);
+                    store(t, at);
+                }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wavefront reads its own stores only)
+        } else {
+#pragma unroll
+            for (int u = 0; u < D; u++) fetch_w(u, b0 + u), fetch_x(u, b0 + u);
+        }
+        const uint16_t *const own_lane = own + min(lane & 15, used - 1) * F8_BLOCK + (lane >> 4) * 32;
+        for (int b = b0; b < b1; b += D) {
+#pragma unroll
+            for (int u = 0; u < D; u++) {
+                if (b + u < b1) {  // (uniform)
+                    f8_v8bf wv[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint4 &raw = w[u][k >> 1];
+                        const uint2 lo = f8_to_bf16(k & 1 ? raw.z : raw.x, 1.0f), hi = f8_to_bf16(k & 1 ? raw.w : raw.y, 1.0f);
+                        const uint4 both = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                        __builtin_memcpy(&wv[k], &both, 16);
+                    }
+#pragma unroll
+                    for (int t = 0; t < TT; t++) {
+                        f8_v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            f8_v8bf xv;
+                            if (FUSED) xv = *reinterpret_cast<const f8_v8bf *>(own_lane + (size_t)(b + u - b0) * used * F8_BLOCK + k * 8);
+                            else __builtin_memcpy(&xv, &x[u][t][k], 16);
+                            p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[k], xv, p, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; r++) acc[t][r] = __builtin_fmaf(p[r], s[u], acc[t][r]);
+                    }
+                    if (b + u + D < b1) {
+                        fetch_w(u, b + u + D);
+                        if (!FUSED) fetch_x(u, b + u + D);
+                    }
+                }
+            }
         }
     }
 #pragma unroll
     for (int t = 0; t < TT; t++) sums[wave][t][lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
     __syncthreads();
-    for (int i = threadIdx.x; i < TT * 64; i += 64 * F8_WAVES) {
-        const int t = i >> 6, l = i & 63, tok = 16 * t + (l & 15);
-        float4 v = sums[0][t][l];
+    const int last_wave = min(NW, TT);  // a wavefront a tile of tokens
+    if (wave >= last_wave) return;
+    const int t = wave, tok = 16 * t + (lane & 15);
+    float4 v = sums[0][t][lane];
 #pragma unroll
-        for (int k = 1; k < F8_WAVES; k++) {
-            const float4 o = sums[k][t][l];
-            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-        }
-        if (tok >= tile.z) continue;
-        const int r0 = strip * F8_STRIP + 4 * (l >> 4);
-        float *dst = g.y + (size_t)(tile.w + tok) * g.ldy + y_col;
-        const float out[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (r0 + r < g.w.rows) dst[r0 + r] = out[r];
+    for (int k = 1; k < NW; k++) {
+        const float4 o = sums[k][t][lane];
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
     }
+    if (tok >= used) return;
+    const int r0 = strip * F8_STRIP + 4 * (lane >> 4);
+    float *const dst = g.y + (size_t)(first + tok) * g.ldy + y_col;
+    const float out[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (r0 + r < g.w.rows) dst[r0 + r] = out[r];
 #endif
 }
 
-size_t f8_gemm_workspace_bytes(const frk_weights *w, size_t batch) { return f8_acts_bytes(batch, w->cols); }
-int launch_f8_gemm(const frk_weights *w, const float *x, size_t batch, float *y, void *ws, hipStream_t s) {
-    F8Gemm g{};
-    g.w = f8_mat(w);
-    g.a = f8_acts_carve(ws, batch);
-    g.M = (int)batch;
-    g.ldy = w->rows;
-    g.y = y;
-    int rc = launch_f8_quantize(x, nullptr, batch, w->cols, nullptr, g.a, s);
-    if (rc) return rc;
-    const size_t tok_tiles = (batch + F8_MAX_TOKENS - 1) / F8_MAX_TOKENS;
-    const size_t jobs = g.w.strips * tok_tiles;
-    if (jobs > 0x7fffffffu || w->matrices > 65535) return set_error(FRK_ERR_SHAPE, "%zu rows over %zu matrices of %d: too many", batch, w->matrices, g.w.rows);
-    const dim3 grid((unsigned)jobs, (unsigned)w->matrices);
-    if (batch > 64) return launch_f8_tile(g, 128, (batch + 127) / 128, w->matrices, 1, 0, s);
-    if (batch <= 16) hipLaunchKernelGGL(f8_gemm_kernel<1>, grid, dim3(64 * F8_WAVES), 0, s, g);
-    else if (batch <= 32) hipLaunchKernelGGL(f8_gemm_kernel<2>, grid, dim3(64 * F8_WAVES), 0, s, g);
-    else hipLaunchKernelGGL(f8_gemm_kernel<4>, grid, dim3(64 * F8_WAVES), 0, s, g);
-    FRK_LAUNCH_CHECK("f8_gemm");
+template <int NW, int TT, int D, bool FUSED, bool PAIRS>
+static int go_f8_rows(const F8Rows &g, const dim3 &grid, size_t lds, hipStream_t s) {
+    if (f8_wide_rows(g.x, (size_t)g.cols)) hipLaunchKernelGGL((f8_rows_kernel<NW, TT, D, FUSED, PAIRS, true>), grid, dim3(64 * NW), lds, s, g);
+    else hipLaunchKernelGGL((f8_rows_kernel<NW, TT, D, FUSED, PAIRS, false>), grid, dim3(64 * NW), lds, s, g);
+    FRK_LAUNCH_CHECK("f8_rows");
     return FRK_OK;
 }
 
+constexpr size_t F8_ROWS_TOKENS = 64;  // batches of up to so many rows
+static bool f8_fused(size_t tokens, size_t cols) { return tokens <= F8_FUSED && tokens * f8_blocks(cols) * F8_BLOCK * 2 <= F8_FUSED_LDS; }
+
+size_t f8_gemm_workspace_bytes(const frk_weights *w, size_t batch) { return f8_fused(batch, w->cols) ? 0 : f8_acts_bytes(batch, w->cols); }
+int launch_f8_gemm(const frk_weights *w, const float *x, size_t batch, float *y, void *ws, hipStream_t s) {
+    const F8Mat m = f8_mat(w);
+    const F8Acts acts = f8_acts_carve(ws, batch, batch <= F8_ROWS_TOKENS);
+    const bool fused = f8_fused(batch, w->cols);
+    if (!fused) {
+        int rc = launch_f8_quantize(x, nullptr, batch, w->cols, nullptr, acts, s);
+        if (rc) return rc;
+    }
+    if (batch > F8_ROWS_TOKENS) {
+        F8Gemm g{};
+        g.w = m;
+        g.a = acts;
+        g.M = (int)batch;
+        g.ldy = w->rows;
+        g.y = y;
+        return launch_f8_tile(g, 128, (batch + 127) / 128, w->matrices, 1, 0, s);
+    }
+    F8Rows g{};
+    g.w = m;
+    g.a = acts;
+    g.x = x;
+    g.cols = (int)w->cols;
+    g.x_rows = g.M = (int)batch;
+    g.ldy = w->rows;
+    g.y = y;
+    const dim3 grid((unsigned)m.strips, (unsigned)w->matrices);
+    if (fused) return go_f8_rows<8, 1, 4, true, false>(g, grid, batch * m.blocks * F8_BLOCK * 2, s);
+    if (batch <= 16) return go_f8_rows<8, 1, 4, false, false>(g, grid, 0, s);
+    if (batch <= 32) return go_f8_rows<8, 2, 2, false, false>(g, grid, 0, s);
+    return go_f8_rows<8, 4, 1, false, false>(g, grid, 0, s);
+}
+
 // ---- grouped: the tile list of the groups given.  Offsets are clamped to 0 .. pairs and made non-decreasing (each the largest
-// so far), so the tiles are at most pairs / tokens + groups whatever the list holds.  One workgroup of 1024 threads, a group each. ----
-__global__ __launch_bounds__(1024) void f8_tiles_kernel(const int32_t *__restrict__ group_off, int n_groups, int pairs, int tokens, int4 *__restrict__ tiles,
-                                                        int *__restrict__ n_tiles) {
-    __shared__ int off[1025], at[1025];
-    const int tid = threadIdx.x;
-    for (int g = tid; g <= n_groups; g += 1024) off[g] = min(max(group_off[g], 0), pairs);
-    __syncthreads();
-    if (tid == 0) {
-        int top = 0, n = 0;
-        for (int g = 0; g <= n_groups; g++) {
-            const int from = top;
-            top = max(top, off[g]);
-            if (g) {
-                at[g - 1] = n;
-                n += (top - from + tokens - 1) / tokens;
-            }
-            off[g] = top;
-        }
-        *n_tiles = n;
+// so far), so the tiles are at most pairs / tokens + groups whatever the list holds.  1024 threads, a group each. ----
+struct F8TilesArgs {
+    const int32_t *group_off;
+    int n_groups, pairs, tokens;
+    int4 *tiles;
+    int *n_tiles;
+};
+__device__ __forceinline__ void f8_tile_list(const F8TilesArgs &a) {
+    __shared__ int wave_top[16], wave_sum[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // the largest offset up to and with this group's first, and with its end
+    const int mine = tid < a.n_groups ? min(max(a.group_off[tid], 0), a.pairs) : 0;
+    const int end = tid < a.n_groups ? min(max(a.group_off[tid + 1], 0), a.pairs) : 0;
+    int top = mine;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int o = __shfl_up(top, m);
+        if (lane >= m) top = max(top, o);
     }
+    if (lane == 63) wave_top[wave] = top;
     __syncthreads();
-    if (tid < n_groups) {
-        const int n = off[tid + 1] - off[tid];
-        for (int i = 0; i * tokens < n; i++)
-            tiles[at[tid] + i] = make_int4(tid, off[tid] + i * tokens, min(tokens, n - i * tokens), off[tid] + i * tokens);
+    for (int w = 0; w < wave; w++) top = max(top, wave_top[w]);
+    const int n = tid < a.n_groups ? max(end - top, 0) : 0, tiles = (n + a.tokens - 1) / a.tokens;
+    int sum = tiles;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int o = __shfl_up(sum, m);
+        if (lane >= m) sum += o;
     }
+    if (lane == 63) wave_sum[wave] = sum;
+    __syncthreads();
+    int at = sum - tiles, total = 0;
+    for (int w = 0; w < 16; w++) {
+        if (w < wave) at += wave_sum[w];
+        total += wave_sum[w];
+    }
+    for (int i = 0; i < tiles; i++) a.tiles[at + i] = make_int4(tid, top + i * a.tokens, min(a.tokens, n - i * a.tokens), top + i * a.tokens);
+    if (tid == 0) *a.n_tiles = total;
+}
+// beside the quantization, which does not depend on it: workgroup 0 makes the list
+template <bool WIDE>
+__global__ __launch_bounds__(1024) void f8_tiles_quantize_kernel(F8TilesArgs a, const float *__restrict__ x, size_t jobs, int parts, int cols, int blocks,
+                                                                 F8Acts out) {
+    if (blockIdx.x == 0) {
+        f8_tile_list(a);
+        return;
+    }
+    const int lane = threadIdx.x & 63;
+    for (size_t j = (size_t)(blockIdx.x - 1) * 16 + (threadIdx.x >> 6); j < jobs; j += (size_t)(gridDim.x - 1) * 16)
+        f8_quantize_blocks<WIDE>(x, nullptr, j / parts, (int)(j % parts) * F8_QUANTIZE_BLOCKS, cols, blocks, lane, out);
 }
 static size_t f8_max_tiles(size_t pairs, size_t groups, int tokens) { return pairs / (size_t)tokens + std::min(groups, pairs); }
 static int f8_tile_tokens(size_t pairs, size_t groups) {
     const size_t mean = pairs / groups;
     return mean >= 96 ? 128 : mean >= 16 ? 64 : 32;
 }
+// a few pairs: a launch that looks the groups up itself
+static bool f8_few_pairs(size_t pairs, size_t groups) { return pairs <= 64 && groups >= pairs / 2; }
 size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs) {
     return f8_acts_bytes(x_rows, w->cols) + 256 + f8_max_tiles(pairs, w->matrices, 32) * 16;
 }
@@ -273,13 +425,37 @@ int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, int tokens, const 
 int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
                       float *y, void *ws, hipStream_t s) {
     const F8Acts acts = f8_acts_carve(ws, x_rows);
+    const bool few = f8_few_pairs(pairs, w->matrices), fused = few && f8_fused(F8_FUSED, w->cols);
+    if (few && !fused) {
+        int rc = launch_f8_quantize(x, nullptr, x_rows, w->cols, nullptr, acts, s);
+        if (rc) return rc;
+    }
+    if (few) {
+        F8Rows g{};
+        g.w = f8_mat(w);
+        g.a = acts;
+        g.x = x;
+        g.cols = (int)w->cols;
+        g.x_rows = (int)x_rows;
+        g.group_off = group_off;
+        g.gather = gather;
+        g.n_groups = (int)w->matrices;
+        g.pairs = (int)pairs;
+        g.ldy = g.w.rows;
+        g.y = y;
+        const dim3 grid((unsigned)g.w.strips, (unsigned)pairs);
+        return fused ? go_f8_rows<8, 1, 4, true, true>(g, grid, F8_FUSED * g.w.blocks * F8_BLOCK * 2, s) : go_f8_rows<8, 1, 4, false, true>(g, grid, 0, s);
+    }
     const int tokens = f8_tile_tokens(pairs, w->matrices);
     int *n_tiles = (int *)((char *)ws + f8_acts_bytes(x_rows, w->cols));
     int4 *tiles = (int4 *)(n_tiles + 64);
-    int rc = launch_f8_quantize(x, nullptr, x_rows, w->cols, nullptr, acts, s);
-    if (rc) return rc;
-    hipLaunchKernelGGL(f8_tiles_kernel, dim3(1), dim3(1024), 0, s, group_off, (int)w->matrices, (int)pairs, tokens, tiles, n_tiles);
-    FRK_LAUNCH_CHECK("f8_tile_list");
+    const F8TilesArgs list{group_off, (int)w->matrices, (int)pairs, tokens, tiles, n_tiles};
+    const int blocks = (int)f8_blocks(w->cols), parts = (blocks + F8_QUANTIZE_BLOCKS - 1) / F8_QUANTIZE_BLOCKS;
+    const size_t jobs = x_rows * parts;
+    const dim3 grid((unsigned)std::min<size_t>(1 + (jobs + 15) / 16, 1 << 14));
+    if (f8_wide_rows(x, w->cols)) hipLaunchKernelGGL(f8_tiles_quantize_kernel<true>, grid, dim3(1024), 0, s, list, x, jobs, parts, (int)w->cols, blocks, acts);
+    else hipLaunchKernelGGL(f8_tiles_quantize_kernel<false>, grid, dim3(1024), 0, s, list, x, jobs, parts, (int)w->cols, blocks, acts);
+    FRK_LAUNCH_CHECK("f8_tiles_quantize");
     return launch_f8_tiles(w, acts, tokens, gather, tiles, n_tiles, f8_max_tiles(pairs, w->matrices, tokens), y, s);
 }
 

@@ -47,14 +47,18 @@ static inline F8Mat f8_mat(const frk_weights *w) {
     return m;
 }
 
-// Activations: q * 2^e as bf16, [rows][blocks][128], zeros past cols.
+// Activations: q * 2^e as bf16, zeros past cols; [rows][blocks][128], or (`strips`) every sixteen rows a strip, a strip's blocks one after
+// the other, a block as [4 products][64 lanes][8], lane l row l % 16, product k columns 32 (l / 16) + 8 k .. + 7: a wavefront's
+// load of a product's operand is then 1 KB in one piece (rows past the last hold whatever the memory did).
 struct F8Acts {
     uint16_t *v;
     int rows;
+    bool strips;
 };
-static inline size_t f8_acts_bytes(size_t rows, size_t cols) { return round_up(rows * f8_blocks(cols) * F8_BLOCK * 2, 256); }
-static inline F8Acts f8_acts_carve(void *base, size_t rows) {
+static inline size_t f8_acts_bytes(size_t rows, size_t cols) { return round_up((rows + 15) / 16 * 16 * f8_blocks(cols) * F8_BLOCK * 2, 256); }
+static inline F8Acts f8_acts_carve(void *base, size_t rows, bool strips = false) {
     F8Acts a;
+    a.strips = strips;
     a.v = (uint16_t *)base;
     a.rows = (int)rows;
     return a;
@@ -74,31 +78,47 @@ __device__ __forceinline__ uint32_t f8_half_max(uint32_t v) {  // over 32 lanes
 }
 // the four values' codes; `scale` = 2^e of the block
 __device__ __forceinline__ uint32_t f8_quantize4(const float (&v)[4], float &scale) {
-    uint32_t top = 0;  // magnitudes compare as their bits
+    // magnitudes compare as their bits
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu;
-        top = max(top, m < 0x7f800000u ? m : 0u);
-    }
+    for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     top = f8_half_max(top);
+    // hardly ever: infinities and NaN, which take no part, or a largest magnitude above 240 * 2^120, from which on the next code's
+    // value is no float
+    constexpr uint32_t PLAIN = 0x7f700000u;
+    const bool special = __any(top > PLAIN);  // (uniform)
+    if (special) {
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu;
+            top = max(top, m < 0x7f800000u ? min(m, PLAIN) : 0u);
+        }
+        top = f8_half_max(top);
+    }
     // 448 = 1.75 * 2^8: e is the exponent less 8, one more where the mantissa is above 1.75
-    const int b = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    const int b = (int)((top + 0x1fffffu) >> 23) - 8;
     const uint32_t biased = (uint32_t)max(b, 127 - 100);
     scale = __uint_as_float(biased << 23);
     const float up = __uint_as_float((254u - biased) << 23);  // 2^-e
-    // (256 * 2^120 is no float any more: there the largest code is 240's)
-    const float most = biased == 127 + 120 ? 240.0f : 448.0f;
     float z[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) z[i] = fminf(fmaxf(v[i] * up, -most), most);
+    for (int i = 0; i < 4; i++) z[i] = v[i] * up;
+    if (special) {
+        const float most = biased == 127 + 120 ? 240.0f : 448.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) z[i] = fminf(fmaxf(z[i], -most), most);
+    }
     uint32_t codes = 0;
 #if defined(__HIP_DEVICE_COMPILE__)
     int p = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
     codes = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], p, true);
 #endif
+    if (special) {
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if ((__float_as_uint(v[j]) & 0x7f800000u) == 0x7f800000u) codes = (codes & ~(0xffu << (8 * j))) | (0x7fu << (8 * j));
+        for (int j = 0; j < 4; j++)
+            if ((__float_as_uint(v[j]) & 0x7f800000u) == 0x7f800000u) codes = (codes & ~(0xffu << (8 * j))) | (0x7fu << (8 * j));
+    }
     return codes;
 }
 
@@ -151,8 +171,10 @@ __device__ __forceinline__ void f8_quantize_blocks(const float *__restrict__ x, 
         if (first + 2 * i >= blocks) break;  // (uniform)
         float scale;
         const uint32_t codes = f8_quantize4(v[i], scale);
-        if (first + 2 * i + (lane >> 5) < blocks)
-            *reinterpret_cast<uint2 *>(out.v + row * (size_t)blocks * F8_BLOCK + k + i * 2 * F8_BLOCK) = f8_to_bf16(codes, scale);
+        const int b = first + 2 * i + (lane >> 5), in = (lane & 31) * 4;
+        const size_t at = out.strips ? ((row >> 4) * blocks + b) * (F8_STRIP * F8_BLOCK) + (size_t)((in >> 3 & 3) * 512 + ((in >> 5) * 16 + (row & 15)) * 8 + (in & 7))
+                                     : (row * blocks + b) * F8_BLOCK + in;
+        if (b < blocks) *reinterpret_cast<uint2 *>(out.v + at) = f8_to_bf16(codes, scale);
     }
 }
 
