@@ -312,26 +312,69 @@ static int go_f8_rows(const F8Rows &g, const dim3 &grid, size_t lds, hipStream_t
     return FRK_OK;
 }
 
-constexpr size_t F8_ROWS_TOKENS = 64;  // batches of up to so many rows
+constexpr size_t F8_ROWS_TOKENS = 64;  // most of the rows kernel
 static bool f8_fused(size_t tokens, size_t cols) { return tokens <= F8_FUSED && tokens * f8_blocks(cols) * F8_BLOCK * 2 <= F8_FUSED_LDS; }
 
-size_t f8_gemm_workspace_bytes(const frk_weights *w, size_t batch) { return f8_fused(batch, w->cols) ? 0 : f8_acts_bytes(batch, w->cols); }
-int launch_f8_gemm(const frk_weights *w, const float *x, size_t batch, float *y, void *ws, hipStream_t s) {
+// By estimated time.  Both kernels are a chain of steps a wavefront until the chip is full: a block of 128 columns takes a tile's wavefronts
+// as long alone on a CU as beside the CU's other workgroups, up to how many fit; a strip of the rows kernel likewise.  Shares of the
+// columns cost a second launch, 3.3 us, and the traffic of the parts.  In us, measured / by these lines (rows x columns, tokens):
+// 4096 x 4096 at 64 128x64 tiles 27.7 / 29.5, two shares 20.7 / 21.7, the rows kernel 14.1 / 14.0; 14336 x 4096 at 64 two shares
+// 23.3 / 24.1, the rows kernel 37.6 / 36.5; at 512 256x128 59.7 / 55.7, 256x64 62.1 / 53.7, 128x64 73.3 / 75.6; 4096 x 4096 at 512
+// 256x64 36.2 / 33.3, in two shares 30.9 / 30.3.
+F8Plan f8_plan(const frk_weights *w, size_t batch) {
     const F8Mat m = f8_mat(w);
-    const F8Acts acts = f8_acts_carve(ws, batch, batch <= F8_ROWS_TOKENS);
-    const bool fused = f8_fused(batch, w->cols);
-    if (!fused) {
+    F8Plan best{-1, 1, f8_fused(batch, w->cols), 0, 0};
+    if (best.fused) return best;
+    best.acts_bytes = f8_acts_bytes(batch, w->cols);
+    if (batch <= 16) return best;  // (the tiles hold 32 tokens and more)
+    double least = 1e30;
+    if (batch <= F8_ROWS_TOKENS) {
+        const double rounds = std::max(1.0, (double)(m.strips * w->matrices) / 256.0);
+        least = 5.0 + rounds * std::max(0.5, m.blocks / 32.0) * (batch <= 32 ? 5.5 : 9.0);
+    }
+    static constexpr struct {
+        double slots, alone, full;  // workgroups of the chip; us a block
+    } COST[F8_TILE_SHAPES] = {{256, 1.36, 1.60}, {512, 0.87, 1.72}, {512, 0.75, 1.08}, {1024, 0.68, 1.30}};
+    static constexpr int SHARES[] = {1, 2, 3, 4, 6, 8, 12, 16};
+    const size_t n = batch * w->rows;
+    for (int shape = 0; shape < F8_TILE_SHAPES; shape++)
+        for (int parts : SHARES) {
+            if (parts > 1 && (parts > m.blocks / 2 || parts * n * 4 > SPLIT_PARTS_BYTES)) break;
+            const F8TileSize t = F8_TILE_SIZE[shape];
+            const double groups = (double)((m.rows + t.rows - 1) / t.rows) * (double)((batch + t.tokens - 1) / t.tokens) * (double)w->matrices * parts;
+            const double fill = groups / COST[shape].slots, half = shape == F8_TILE_256x128 ? 0.0 : 0.5;  // up to `half` a workgroup is alone on its CU
+            const double chain = (double)((m.blocks + parts - 1) / parts);
+            double us = 4.5;
+            if (fill <= 1.0) us += chain * (COST[shape].alone + (COST[shape].full - COST[shape].alone) * std::max(0.0, fill - half) / (1.0 - half)) + 1.0;
+            else us += (fill < 3.0 ? std::ceil(fill - 0.02) : fill) * (chain * COST[shape].full + 1.0);
+            if (parts > 1) us += 3.3 + 0.45e-6 * 4.0 * (double)n * parts;
+            if (us < least) {
+                least = us;
+                best.shape = shape;
+                best.parts = parts;
+            }
+        }
+    if (best.parts > 1) best.parts_bytes = best.parts * n * 4;
+    return best;
+}
+int launch_f8_gemm(const frk_weights *w, const F8Plan &plan, const float *x, size_t batch, float *y, void *ws, void *parts, hipStream_t s) {
+    const F8Mat m = f8_mat(w);
+    const F8Acts acts = f8_acts_carve(ws, batch, plan.shape < 0);
+    if (!plan.fused) {
         int rc = launch_f8_quantize(x, nullptr, batch, w->cols, nullptr, acts, s);
         if (rc) return rc;
     }
-    if (batch > F8_ROWS_TOKENS) {
+    if (plan.shape >= 0) {
         F8Gemm g{};
         g.w = m;
         g.a = acts;
         g.M = (int)batch;
         g.ldy = w->rows;
-        g.y = y;
-        return launch_f8_tile(g, 128, (batch + 127) / 128, w->matrices, 1, 0, s);
+        const size_t n = batch * w->rows, tokens = (size_t)F8_TILE_SIZE[plan.shape].tokens;
+        g.y = plan.parts > 1 ? (float *)parts : y;
+        int rc = launch_f8_tile(g, plan.shape, (batch + tokens - 1) / tokens, w->matrices, plan.parts, n, s);
+        if (rc || plan.parts == 1) return rc;
+        return launch_sum_parts((const float *)parts, plan.parts, n, y, s);
     }
     F8Rows g{};
     g.w = m;
@@ -342,7 +385,7 @@ int launch_f8_gemm(const frk_weights *w, const float *x, size_t batch, float *y,
     g.ldy = w->rows;
     g.y = y;
     const dim3 grid((unsigned)m.strips, (unsigned)w->matrices);
-    if (fused) return go_f8_rows<8, 1, 4, true, false>(g, grid, batch * m.blocks * F8_BLOCK * 2, s);
+    if (plan.fused) return go_f8_rows<8, 1, 4, true, false>(g, grid, batch * m.blocks * F8_BLOCK * 2, s);
     if (batch <= 16) return go_f8_rows<8, 1, 4, false, false>(g, grid, 0, s);
     if (batch <= 32) return go_f8_rows<8, 2, 2, false, false>(g, grid, 0, s);
     return go_f8_rows<8, 4, 1, false, false>(g, grid, 0, s);
@@ -401,16 +444,16 @@ __global__ __launch_bounds__(1024) void f8_tiles_quantize_kernel(F8TilesArgs a, 
         f8_quantize_blocks<WIDE>(x, nullptr, j / parts, (int)(j % parts) * F8_QUANTIZE_BLOCKS, cols, blocks, lane, out);
 }
 static size_t f8_max_tiles(size_t pairs, size_t groups, int tokens) { return pairs / (size_t)tokens + std::min(groups, pairs); }
-static int f8_tile_tokens(size_t pairs, size_t groups) {
+static int f8_grouped_shape(size_t pairs, size_t groups) {
     const size_t mean = pairs / groups;
-    return mean >= 96 ? 128 : mean >= 16 ? 64 : 32;
+    return mean >= 96 ? F8_TILE_256x128 : mean >= 16 ? F8_TILE_128x64 : F8_TILE_128x32;
 }
 // a few pairs: a launch that looks the groups up itself
 static bool f8_few_pairs(size_t pairs, size_t groups) { return pairs <= 64 && groups >= pairs / 2; }
 size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs) {
     return f8_acts_bytes(x_rows, w->cols) + 256 + f8_max_tiles(pairs, w->matrices, 32) * 16;
 }
-int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, int tokens, const int *src, const int4 *tiles, const int *n_tiles, size_t max_tiles, float *y,
+int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, int shape, const int *src, const int4 *tiles, const int *n_tiles, size_t max_tiles, float *y,
                     hipStream_t s) {
     F8Gemm g{};
     g.w = f8_mat(w);
@@ -420,7 +463,7 @@ int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, int tokens, const 
     g.n_tiles = n_tiles;
     g.ldy = g.w.rows;
     g.y = y;
-    return launch_f8_tile(g, tokens, max_tiles, 1, 1, 0, s);
+    return launch_f8_tile(g, shape, max_tiles, 1, 1, 0, s);
 }
 int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
                       float *y, void *ws, hipStream_t s) {
@@ -446,7 +489,7 @@ int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int3
         const dim3 grid((unsigned)g.w.strips, (unsigned)pairs);
         return fused ? go_f8_rows<8, 1, 4, true, true>(g, grid, F8_FUSED * g.w.blocks * F8_BLOCK * 2, s) : go_f8_rows<8, 1, 4, false, true>(g, grid, 0, s);
     }
-    const int tokens = f8_tile_tokens(pairs, w->matrices);
+    const int shape = f8_grouped_shape(pairs, w->matrices), tokens = F8_TILE_SIZE[shape].tokens;
     int *n_tiles = (int *)((char *)ws + f8_acts_bytes(x_rows, w->cols));
     int4 *tiles = (int4 *)(n_tiles + 64);
     const F8TilesArgs list{group_off, (int)w->matrices, (int)pairs, tokens, tiles, n_tiles};
@@ -456,7 +499,7 @@ int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int3
     if (f8_wide_rows(x, w->cols)) hipLaunchKernelGGL(f8_tiles_quantize_kernel<true>, grid, dim3(1024), 0, s, list, x, jobs, parts, (int)w->cols, blocks, acts);
     else hipLaunchKernelGGL(f8_tiles_quantize_kernel<false>, grid, dim3(1024), 0, s, list, x, jobs, parts, (int)w->cols, blocks, acts);
     FRK_LAUNCH_CHECK("f8_tiles_quantize");
-    return launch_f8_tiles(w, acts, tokens, gather, tiles, n_tiles, f8_max_tiles(pairs, w->matrices, tokens), y, s);
+    return launch_f8_tiles(w, acts, shape, gather, tiles, n_tiles, f8_max_tiles(pairs, w->matrices, tokens), y, s);
 }
 
 }  // namespace frk

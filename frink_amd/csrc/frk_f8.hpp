@@ -190,22 +190,33 @@ struct F8Gemm {
     size_t ldy;
     float *y;
 };
-// over tiles of `tokens` tokens (32, 64 or 128); parts > 1 (dense): shares of the columns, each its own copy of y, part_stride floats apart
-int launch_f8_tile(const F8Gemm &g, int tokens, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s);
+// over tiles of a shape (weight rows x tokens); parts > 1 (dense): shares of the columns, each its own copy of y, part_stride floats apart
+enum { F8_TILE_256x128, F8_TILE_256x64, F8_TILE_128x64, F8_TILE_128x32, F8_TILE_SHAPES };
+struct F8TileSize {
+    int rows, tokens;
+};
+constexpr F8TileSize F8_TILE_SIZE[F8_TILE_SHAPES] = {{256, 128}, {256, 64}, {128, 64}, {128, 32}};
+int launch_f8_tile(const F8Gemm &g, int shape, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s);
+// How a dense batch is multiplied: by the rows kernel (shape -1; `fused`: its own quantization), or over tiles in `parts` shares
+struct F8Plan {
+    int shape, parts;
+    bool fused;
+    size_t acts_bytes, parts_bytes;  // of scratch memory
+};
+F8Plan f8_plan(const frk_weights *w, size_t batch);
 
 // ---- entry points for the runtime and the expert layers ----
 Layout f8_layout(size_t rows, size_t cols, size_t matrices, size_t *bytes);
 int launch_f8_repack(const uint8_t *src, const float *scales, const frk_weights *w, hipStream_t s);
-size_t f8_gemm_workspace_bytes(const frk_weights *w, size_t batch);
-int launch_f8_gemm(const frk_weights *w, const float *x, size_t batch, float *y, void *ws, hipStream_t s);
+int launch_f8_gemm(const frk_weights *w, const F8Plan &plan, const float *x, size_t batch, float *y, void *ws, void *parts, hipStream_t s);
 size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs);
 int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
                       float *y, void *ws, hipStream_t s);
 // rows of x (of silu(x) * up) quantized; `used`: a row whose entry is negative is left as it is
 int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols, const int *used, const F8Acts &out, hipStream_t s);
-// the products of the tiles {matrix, first row of the order, rows in use (up to `tokens`), first row of y}; row i of the order is
-// activation row src[i], or i
-int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, int tokens, const int *src, const int4 *tiles, const int *n_tiles, size_t max_tiles, float *y,
+// the products of the tiles {matrix, first row of the order, rows in use (up to the shape's tokens), first row of y}; row i of the order
+// is activation row src[i], or i
+int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, int shape, const int *src, const int4 *tiles, const int *n_tiles, size_t max_tiles, float *y,
                     hipStream_t s);
 
 }  // namespace frk

@@ -247,10 +247,13 @@ static int go_f8_tile(const F8Gemm &g, size_t tok_tiles, size_t matrices, int pa
     FRK_LAUNCH_CHECK("f8_tile");
     return FRK_OK;
 }
-int launch_f8_tile(const F8Gemm &g, int tokens, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s) {
-    if (tokens == 128) return go_f8_tile<4, 2, 4>(g, tok_tiles, matrices, parts, part_stride, s);
-    if (tokens == 64) return go_f8_tile<2, 2, 2>(g, tok_tiles, matrices, parts, part_stride, s);
-    return go_f8_tile<4, 1, 2>(g, tok_tiles, matrices, parts, part_stride, s);
+int launch_f8_tile(const F8Gemm &g, int shape, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s) {
+    switch (shape) {
+    case F8_TILE_256x128: return go_f8_tile<4, 2, 4>(g, tok_tiles, matrices, parts, part_stride, s);
+    case F8_TILE_256x64: return go_f8_tile<4, 1, 4>(g, tok_tiles, matrices, parts, part_stride, s);
+    case F8_TILE_128x64: return go_f8_tile<2, 2, 2>(g, tok_tiles, matrices, parts, part_stride, s);
+    default: return go_f8_tile<2, 1, 2>(g, tok_tiles, matrices, parts, part_stride, s);
+    }
 }
 
 }  // namespace frk

@@ -1221,6 +1221,7 @@ size_t f8_moe_workspace_bytes(size_t batch, int k, int n_experts, size_t hidden,
 int launch_moe_ffn_f8(const frk_weights *gate, const frk_weights *up, const frk_weights *down, int n_experts, const float *x, size_t batch,
                       const int32_t *ids, const float *weights, int k, float *out, void *ws, hipStream_t s) {
     const size_t hidden = gate->cols, ffn = down->cols, pairs = batch * (size_t)k, rows = moe_max_rows(pairs, n_experts), max_tiles = rows / MOE_TILE;
+    static_assert(MOE_TILE == F8_TILE_SIZE[F8_TILE_128x64].tokens, "the tiles' shape");
     const F8MoeScratch m = f8_moe_carve(ws, batch, k, n_experts, hidden, ffn, nullptr);
     static bool sized = false;  // a benign race: every thread sets the same attribute
     if (!sized) {
@@ -1235,13 +1236,13 @@ int launch_moe_ffn_f8(const frk_weights *gate, const frk_weights *up, const frk_
     const F8Acts xa = f8_acts_carve(m.x_acts, batch), aa = f8_acts_carve(m.a_acts, rows);
     int rc = launch_f8_quantize(x, nullptr, batch, hidden, nullptr, xa, s);
     if (rc) return rc;
-    rc = launch_f8_tiles(gate, xa, MOE_TILE, m.gather, m.tiles, m.n_tiles, max_tiles, m.gate_out, s);
+    rc = launch_f8_tiles(gate, xa, F8_TILE_128x64, m.gather, m.tiles, m.n_tiles, max_tiles, m.gate_out, s);
     if (rc) return rc;
-    rc = launch_f8_tiles(up, xa, MOE_TILE, m.gather, m.tiles, m.n_tiles, max_tiles, m.up_out, s);
+    rc = launch_f8_tiles(up, xa, F8_TILE_128x64, m.gather, m.tiles, m.n_tiles, max_tiles, m.up_out, s);
     if (rc) return rc;
     rc = launch_f8_quantize(m.gate_out, m.up_out, rows, ffn, m.gather, aa, s);
     if (rc) return rc;
-    rc = launch_f8_tiles(down, aa, MOE_TILE, nullptr, m.tiles, m.n_tiles, max_tiles, m.down_out, s);
+    rc = launch_f8_tiles(down, aa, F8_TILE_128x64, nullptr, m.tiles, m.n_tiles, max_tiles, m.down_out, s);
     if (rc) return rc;
     hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)batch, (unsigned)((hidden + 1023) / 1024)), dim3(256), 0, s, m.down_out, ids, weights,
                        m.pos_of, k, (int)hidden, n_experts, (int)(batch >= MOE_BUCKET_ORDER_FROM), out);

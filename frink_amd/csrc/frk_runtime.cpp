@@ -639,11 +639,12 @@ static int f8_on_current_device(const frk_weights *w) {
 }
 static int gemm_f8(const frk_weights *w, const float *x, size_t batch, float *y, hipStream_t s, Scratch &scratch) {
     if (batch > (size_t)1 << 30) return set_error(FRK_ERR_SHAPE, "a batch of %zu rows is too large", batch);
-    void *ws = nullptr;
+    void *ws = nullptr, *parts = nullptr;
+    const F8Plan plan = f8_plan(w, batch);
     int rc = f8_on_current_device(w);
-    if (!rc) rc = scratch.get(f8_gemm_workspace_bytes(w, batch), s, &ws);
+    if (!rc && plan.acts_bytes) rc = scratch.get(plan.acts_bytes, plan.parts_bytes, s, &ws, &parts);
     if (rc) return rc;
-    return launch_f8_gemm(w, x, batch, y, ws, s);
+    return launch_f8_gemm(w, plan, x, batch, y, ws, parts, s);
 }
 
 static int gemv_impl(const frk_weights *w, const float *x, float *y, int act_mode, hipStream_t s, Scratch &scratch) {
@@ -1367,7 +1368,7 @@ int frk_hip_ffn_swiglu_dev(const frk_weights *gate, const frk_weights *up, const
     const size_t q_cols = std::max(gate->cols, down->cols);  // either projection may quantize its input here
     size_t q_area = round_up(q_cols, 256) + round_up(q_cols / 32 * 4, 256) + round_up(q_cols / 8, 256);
     for (const frk_weights *w : {gate, up, down})
-        if (is_f8_kind(w->kind)) q_area = std::max(q_area, f8_gemm_workspace_bytes(w, 1));
+        if (is_f8_kind(w->kind)) q_area = std::max(q_area, f8_plan(w, 1).acts_bytes);
     WorkspaceLease lease;
     int rc = workspace(q_area + 3 * round_up(ffn * 4, 256), s, lease);
     if (rc) return rc;
