@@ -21,10 +21,6 @@ HIPCC_FLAGS = [
     "-Wall", "-Wno-unused-function", "-Wno-unused-command-line-argument",
 ]
 
-# A source's own flags.  frk_f8_tile.hip: a product's sums go through the vector ALU, which reads no accumulation registers: with
-# the matrix cores' results in those it is a copy for every sum.
-SOURCE_FLAGS = {"frk_f8_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
-
 
 def hipcc():
     for c in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", "hipcc"):
@@ -39,7 +35,7 @@ def build_lib(verbose=False):
     procs = []
     for src in SOURCES:
         obj = os.path.join(LIBDIR, os.path.splitext(src)[0] + ".o")
-        cmd = [hipcc()] + HIPCC_FLAGS + SOURCE_FLAGS.get(src, []) + ["-x", "hip", "-c", os.path.join(CSRC, src), "-o", obj]
+        cmd = [hipcc()] + HIPCC_FLAGS + ["-x", "hip", "-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))

@@ -144,7 +144,7 @@ struct F8Rows {
     float *y;
 };
 constexpr size_t F8_FUSED = 4;
-constexpr size_t F8_FUSED_LDS = 64 * 1024;
+constexpr size_t F8_FUSED_LDS = 56 * 1024;  // beside the 8 KB of sums: what a launch may have without more ado
 
 // the range of up to `most` pairs that pair `p` leads, by the offsets clamped and made non-decreasing (each the largest so far): {group, first, number};
 // a number of 0: it leads none
@@ -188,9 +188,11 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
     const int b0 = (int)((long long)blocks * wave / NW), b1 = (int)((long long)blocks * (wave + 1) / NW);
     const uint8_t *const wq = g.w.q + (((size_t)matrix * g.w.strips + strip) * blocks) * F8_PIECE + lane * 16;
     const float *const ws = g.w.s + ((size_t)matrix * g.w.row_blocks + strip * F8_STRIP / F8_BLOCK) * blocks;
-    int row[TT];  // this lane's activation rows
+    // this lane's activation rows; lanes past the last token read its (eight tokens of 14336 x 4096: 15.8 us, with sixteen's traffic 19.2)
+    int row[TT], token[TT];
 #pragma unroll
     for (int t = 0; t < TT; t++) {
+        token[t] = (lane & 48) + min(lane & 15, max(used - 1 - 16 * t, 0));
         const int i = first + min(16 * t + (lane & 15), used - 1);
         row[t] = min(max(PAIRS && g.gather ? g.gather[i] : i, 0), g.x_rows - 1);
     }
@@ -198,19 +200,26 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
 #pragma unroll
     for (int t = 0; t < TT; t++) acc[t] = f8_v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (b0 < b1) {
+        // the next 64 blocks' scales, one a lane (a scalar load a block is waited for with the one just asked for)
+        float scales = ws[min(b0 + lane, b1 - 1)];
+        __builtin_amdgcn_sched_barrier(0);  // (first, so that its wait is not one for the codes)
+        auto next_scales = [&](int b) {
+            if (b > b0 && ((b - b0) & 63) == 0)
+                asm volatile("global_load_dword %0, %1, %2\n\ts_waitcnt vmcnt(0)" : "=v"(scales) : "v"((uint32_t)min(b + lane, b1 - 1) * 4u), "s"(ws) : "memory");
+        };
+        static_assert(64 % D == 0, "whole rounds");
         uint4 w[D][2], x[FUSED ? 1 : D][TT][4];
-        float s[D];
         auto fetch_w = [&](int u, int b) {
             const uint8_t *const at = wq + (size_t)min(b, b1 - 1) * F8_PIECE;
+            // (past the last-level cache, as weights met once a step are: 3 to 7 % faster than plain loads on matrices that aren't in it)
             w[u][0] = stream_load16(at);
             w[u][1] = stream_load16(at + 1024);
-            s[u] = ws[min(b, b1 - 1)];
         };
         auto fetch_x = [&](int u, int b) {
 #pragma unroll
             for (int t = 0; t < TT; t++) {
                 const size_t piece = PAIRS ? (size_t)row[t] * blocks + min(b, b1 - 1) : ((size_t)min((first >> 4) + t, (g.x_rows - 1) >> 4) * blocks + min(b, b1 - 1)) * F8_STRIP;
-                const uint4 *const at = reinterpret_cast<const uint4 *>(g.a.v + piece * F8_BLOCK) + (PAIRS ? (lane >> 4) * 4 : lane);
+                const uint4 *const at = reinterpret_cast<const uint4 *>(g.a.v + piece * F8_BLOCK) + (PAIRS ? (lane >> 4) * 4 : token[t]);
 #pragma unroll
                 for (int k = 0; k < 4; k++) x[u][t][k] = at[PAIRS ? k : k * 64];
             }
@@ -249,35 +258,54 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
             for (int u = 0; u < D; u++) fetch_w(u, b0 + u), fetch_x(u, b0 + u);
         }
         const uint16_t *const own_lane = own + min(lane & 15, used - 1) * F8_BLOCK + (lane >> 4) * 32;
-        for (int b = b0; b < b1; b += D) {
+        auto consume = [&](int u, int b) {
+            const float by = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scales), (b - b0) & 63));
+            f8_v8bf wv[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint4 &raw = w[u][k >> 1];
+                const uint2 lo = f8_to_bf16(k & 1 ? raw.z : raw.x, 1.0f), hi = f8_to_bf16(k & 1 ? raw.w : raw.y, 1.0f);
+                const uint4 both = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                __builtin_memcpy(&wv[k], &both, 16);
+            }
+#pragma unroll
+            for (int t = 0; t < TT; t++) {
+                f8_v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    f8_v8bf xv;
+                    if (FUSED) xv = *reinterpret_cast<const f8_v8bf *>(own_lane + (size_t)(b - b0) * used * F8_BLOCK + k * 8);
+                    else __builtin_memcpy(&xv, &x[u][t][k], 16);
+                    p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[k], xv, p, 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[t][r] = __builtin_fmaf(p[r], by, acc[t][r]);
+            }
+        };
+        // Requests without a branch around them, so that the wait for a block counts those behind it; and no branch between a product
+        // and the reads of its sum: the compiler does not count its wait states across one that splits and joins.
+        int b = b0;
+        for (; b + 2 * D <= b1; b += D) {
+            next_scales(b);
 #pragma unroll
             for (int u = 0; u < D; u++) {
-                if (b + u < b1) {  // (uniform)
-                    f8_v8bf wv[4];
+                consume(u, b + u);
+                fetch_w(u, b + u + D);
+                if (!FUSED) fetch_x(u, b + u + D);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        for (; b < b1; b += D) {
+            next_scales(b);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint4 &raw = w[u][k >> 1];
-                        const uint2 lo = f8_to_bf16(k & 1 ? raw.z : raw.x, 1.0f), hi = f8_to_bf16(k & 1 ? raw.w : raw.y, 1.0f);
-                        const uint4 both = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                        __builtin_memcpy(&wv[k], &both, 16);
-                    }
+            for (int u = 0; u < D; u++) {
+                if (b + u >= b1) break;  // (uniform)
+                consume(u, b + u);
 #pragma unroll
-                    for (int t = 0; t < TT; t++) {
-                        f8_v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            f8_v8bf xv;
-                            if (FUSED) xv = *reinterpret_cast<const f8_v8bf *>(own_lane + (size_t)(b + u - b0) * used * F8_BLOCK + k * 8);
-                            else __builtin_memcpy(&xv, &x[u][t][k], 16);
-                            p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[k], xv, p, 0, 0, 0);
-                        }
-#pragma unroll
-                        for (int r = 0; r < 4; r++) acc[t][r] = __builtin_fmaf(p[r], s[u], acc[t][r]);
-                    }
-                    if (b + u + D < b1) {
-                        fetch_w(u, b + u + D);
-                        if (!FUSED) fetch_x(u, b + u + D);
-                    }
+                for (int t = 0; t < TT; t++) asm volatile("" : "+v"(acc[t]));
+                if (b + u + D < b1) {
+                    fetch_w(u, b + u + D);
+                    if (!FUSED) fetch_x(u, b + u + D);
                 }
             }
         }
@@ -444,10 +472,10 @@ __global__ __launch_bounds__(1024) void f8_tiles_quantize_kernel(F8TilesArgs a, 
         f8_quantize_blocks<WIDE>(x, nullptr, j / parts, (int)(j % parts) * F8_QUANTIZE_BLOCKS, cols, blocks, lane, out);
 }
 static size_t f8_max_tiles(size_t pairs, size_t groups, int tokens) { return pairs / (size_t)tokens + std::min(groups, pairs); }
-static int f8_grouped_shape(size_t pairs, size_t groups) {
-    const size_t mean = pairs / groups;
-    return mean >= 96 ? F8_TILE_256x128 : mean >= 16 ? F8_TILE_128x64 : F8_TILE_128x32;
-}
+// Measured in us with tiles of 256x128 / 256x64 / 128x64 / 128x32 (weight rows x pairs): 32 groups of 2880 x 2880 and 256 pairs each on average 188 /
+// 180 / 235 / 243, 64 95 / 98 / 112 / 96, 32 88 / 68 / 78 / 75, 16 85 / 64 / 73 / 60; 128 of 768 x 2048 and 128 pairs 108 / 85 / 102 / 105, 32 68 / 54 / 56 / 59,
+// 16 64 / 50 / 53 / 46, 4 63 / 47 / 51 / 42.
+static int f8_grouped_shape(size_t pairs, size_t groups) { return pairs >= 24 * groups ? F8_TILE_256x64 : F8_TILE_128x32; }
 // a few pairs: a launch that looks the groups up itself
 static bool f8_few_pairs(size_t pairs, size_t groups) { return pairs <= 64 && groups >= pairs / 2; }
 size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs) {

@@ -377,7 +377,8 @@ int frk_hip_weights_from_device(int kind, const void *dev_bytes, size_t len, siz
 static int check_f8_shape(size_t rows, size_t cols, size_t matrices) {
     if (rows == 0 || cols == 0 || matrices == 0) return set_error(FRK_ERR_SHAPE, "empty shape: rows=%zu cols=%zu matrices=%zu", rows, cols, matrices);
     if (rows % matrices) return set_error(FRK_ERR_SHAPE, "%zu rows do not divide into %zu matrices", rows, matrices);
-    if (rows > 0x7fffff00u || cols > 0x7fffff00u) return set_error(FRK_ERR_SHAPE, "shape too large");
+    // (a tile's 128 rows of activations lie within 32 bits of each other)
+    if (rows > 0x7fffff00u || cols > (1u << 23)) return set_error(FRK_ERR_SHAPE, "shape too large: rows=%zu cols=%zu", rows, cols);
     if (matrices > 65535) return set_error(FRK_ERR_SHAPE, "%zu matrices (at most 65535)", matrices);
     return FRK_OK;
 }
@@ -630,7 +631,7 @@ static int gemv_units_int(const frk_weights *w, const float *x, float *y, hipStr
     return launch_gemv_units_int(w, q, d, y, s);
 }
 
-// FP8_BLOCK: one path at every batch size, so a row's result does not depend on the batch it is in.
+// FP8_BLOCK: a row is quantized alike in every batch; its sums' order, and so their last bits, is the plan's for the batch.
 static int f8_on_current_device(const frk_weights *w) {
     int dev = -1;
     FRK_HIP_TRY(hipGetDevice(&dev));

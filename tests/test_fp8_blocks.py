@@ -24,7 +24,7 @@ def _activations(rng, rows, cols):
 
 SHAPES = [(1, 1, 1), (15, 127, 2), (16, 128, 1), (17, 129, 3), (129, 255, 16), (128, 640, 17), (300, 1000, 33), (64, 96, 64),
           (257, 2880, 65), (1000, 513, 130), (144, 14336, 5), (576, 2304, 9), (33, 1156, 200), (272, 384, 257), (512, 1152, 300),
-          (31, 4100, 1), (768, 2048, 31), (2880, 160, 97)]
+          (31, 4100, 1), (768, 2048, 31), (2880, 160, 97), (40, 28672, 1), (33, 32768, 1), (20, 7168, 4), (20, 7300, 4)]
 
 
 @pytest.mark.gpu
@@ -177,6 +177,7 @@ def _groups(rng, counts):
     (1, 1, [1], 1), (17, 129, [0, 3, 0, 1], 4), (130, 300, [16, 17, 1, 64, 65, 0, 130], 50), (64, 256, [1] * 40, 8),
     (768, 2048, [1, 0] * 8, 1), (200, 512, [300, 5], 77), (48, 96, [0] * 1000 + [2] + [0] * 23, 2), (2880, 160, [3, 90, 33], 126),
     (144, 640, [0, 0, 700], 700), (36, 260, [2, 1, 5, 0, 8] * 30, 19),
+    (24, 7168, [4, 1, 0, 5], 6), (24, 7296, [4, 1, 0, 17], 6), (270, 160, [24, 23, 25], 72), (270, 160, [24, 23, 24], 71),
 ])
 def test_grouped_against_64_bits(fa, rows, cols, counts, x_rows):
     print("fp8 grouped", rows, cols, len(counts), x_rows, flush=True)
@@ -299,7 +300,7 @@ def test_the_kind_is_outside_the_seam():
 
 
 @pytest.mark.parametrize("rows,cols,matrices,needle", [
-    (0, 128, 1, "empty"), (4, 0, 1, "empty"), (4, 128, 0, "empty"), (7, 128, 2, "divide"), (2 ** 31, 1, 1, "too large"), (1, 2 ** 31, 1, "too large"),
+    (0, 128, 1, "empty"), (4, 0, 1, "empty"), (4, 128, 0, "empty"), (7, 128, 2, "divide"), (2 ** 31, 1, 1, "too large"), (1, 2 ** 31, 1, "too large"), (1, 2 ** 23 + 1, 1, "too large"),
     (70000, 8, 70000, "65535"),
 ])
 def test_shapes_refused_before_any_device_call(rows, cols, matrices, needle):
@@ -309,6 +310,26 @@ def test_shapes_refused_before_any_device_call(rows, cols, matrices, needle):
     assert L.frk_hip_weights_from_device_fp8(p, p, rows, cols, matrices, None, C.byref(h)) == fa.ERR_SHAPE
     assert needle in fa.last_error() and not h.value
     assert L.frk_hip_weights_register_fp8(p, p, rows, cols, matrices, C.byref(h)) == fa.ERR_SHAPE
+
+
+@pytest.mark.parametrize("name", ["frk_f8.hip", "frk_f8_tile.hip"])
+def test_no_register_is_read_before_its_wait(tmp_path, name):
+    """The compiler does not count the wait states behind a matrix instruction across a branch that splits and joins: one such
+    branch in the loop over the blocks once left a sum's readers two instructions behind it."""
+    import os
+    import subprocess
+
+    import isa_mfma_lint
+    import isa_wait_lint
+    from frink_amd import build as fb
+    out = tmp_path / "kernels.s"
+    cmd = [fb.hipcc()] + fb.HIPCC_FLAGS + ["-x", "hip", "--cuda-device-only", "-S", os.path.join(fb.CSRC, name), "-o", str(out)]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+    asm = out.read_text()
+    assert "v_mfma" in asm and isa_mfma_lint.violations(asm) == []
+    for k in isa_wait_lint.kernels(asm):
+        assert isa_wait_lint.violations(asm, k) == [], k
 
 
 def test_null_arguments():
