@@ -16,7 +16,6 @@ fn main() {
         let ok = std::process::Command::new(&hipcc)
             .args(["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Iinclude",
                    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-x", "hip", "-c"])
-            .args(if s == "frk_f8_tile.hip" { &["-mllvm", "-amdgpu-mfma-vgpr-form"][..] } else { &[][..] })
             .arg(format!("csrc/{s}"))
             .arg("-o")
             .arg(&o)

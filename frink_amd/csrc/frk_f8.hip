@@ -130,16 +130,21 @@ int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols
 //   DENSE  strip blockIdx.x, matrix blockIdx.y, token tile blockIdx.z
 //   PAIRS  strip blockIdx.x, pair blockIdx.y of a grouped product: every sixteenth (FUSED: fourth) pair of its group takes the
 //          group's next sixteen (four), the others end at once.  No list is made in front of it: each wavefront looks the group up itself
+//   SLOTS  strip blockIdx.x, (token, slot) blockIdx.y of an expert layer: the matrix is the slot's expert (FUSED only).  With `up` the strip of
+//          both stacks, and y = silu(gate) * up
 // FUSED: up to F8_FUSED tokens are quantized by the workgroup itself (a wavefront its own columns', while its first codes
 // are on their way), not by a launch in front. ----
+enum { F8_DENSE = 0, F8_PAIRS = 1, F8_SLOTS = 2, F8_SLOTS_GLU = 3 };
 struct F8Rows {
-    F8Mat w;
+    F8Mat w, up;        // up: SLOTS_GLU
     F8Acts a;           // not FUSED
     const float *x;     // FUSED
     int cols, x_rows;
     int M;                          // DENSE
     const int *group_off, *gather;  // PAIRS
     int n_groups, pairs;
+    const int *ids;                 // SLOTS: experts, of n_groups; a slot's activation row is slot / slots_a_row
+    int slots_a_row;
     size_t ldy;
     float *y;
 };
@@ -167,12 +172,15 @@ __device__ __forceinline__ int4 f8_lead(const int *__restrict__ off, int n_group
     return make_int4(after - 1, p, min(most, end - p), 0);
 }
 
-template <int NW, int TT, int D, bool FUSED, bool PAIRS, bool WIDE>
+template <int NW, int TT, int D, bool FUSED, int MODE, bool WIDE>
 __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    static_assert(!PAIRS || TT == 1, "sixteen pairs");
+    constexpr bool PAIRS = MODE == F8_PAIRS, SLOTS = MODE == F8_SLOTS || MODE == F8_SLOTS_GLU;
+    constexpr int NM = MODE == F8_SLOTS_GLU ? 2 : 1;  // stacks
+    static_assert(MODE == F8_DENSE || TT == 1, "sixteen pairs");
+    static_assert(!SLOTS || FUSED, "a slot's row");
     extern __shared__ __align__(16) uint8_t f8_rows_lds[];  // FUSED: [blocks][tokens][128] bf16
-    __shared__ float4 sums[NW][TT][64];
+    __shared__ float4 sums[NW][NM * TT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int strip = blockIdx.x, blocks = g.w.blocks;
     int matrix, first, used;
@@ -181,39 +189,55 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
         const int4 lead = f8_lead(g.group_off, g.n_groups, g.pairs, (int)blockIdx.y, FUSED ? (int)F8_FUSED : 16, lane);
         matrix = __builtin_amdgcn_readfirstlane(lead.x), first = __builtin_amdgcn_readfirstlane(lead.y), used = __builtin_amdgcn_readfirstlane(lead.z);
         if (used == 0) return;
+    } else if (SLOTS) {
+        matrix = g.ids[blockIdx.y], first = blockIdx.y, used = 1;
+        if (matrix < 0 || matrix >= g.n_groups) return;  // (adds nothing to its token)
     } else {
         matrix = blockIdx.y, first = (int)blockIdx.z * 16 * TT, used = min(16 * TT, g.M - first);
         y_col = (size_t)matrix * g.w.rows;
     }
     const int b0 = (int)((long long)blocks * wave / NW), b1 = (int)((long long)blocks * (wave + 1) / NW);
-    const uint8_t *const wq = g.w.q + (((size_t)matrix * g.w.strips + strip) * blocks) * F8_PIECE + lane * 16;
-    const float *const ws = g.w.s + ((size_t)matrix * g.w.row_blocks + strip * F8_STRIP / F8_BLOCK) * blocks;
+    const uint8_t *wq[NM];
+    const float *ws[NM];
+#pragma unroll
+    for (int m = 0; m < NM; m++) {
+        const F8Mat &w = m ? g.up : g.w;
+        wq[m] = w.q + (((size_t)matrix * w.strips + strip) * blocks) * F8_PIECE + lane * 16;
+        ws[m] = w.s + ((size_t)matrix * w.row_blocks + strip * F8_STRIP / F8_BLOCK) * blocks;
+    }
     // this lane's activation rows; lanes past the last token read its (eight tokens of 14336 x 4096: 15.8 us, with sixteen's traffic 19.2)
     int row[TT], token[TT];
 #pragma unroll
     for (int t = 0; t < TT; t++) {
         token[t] = (lane & 48) + min(lane & 15, max(used - 1 - 16 * t, 0));
         const int i = first + min(16 * t + (lane & 15), used - 1);
-        row[t] = min(max(PAIRS && g.gather ? g.gather[i] : i, 0), g.x_rows - 1);
+        row[t] = SLOTS ? i / g.slots_a_row : min(max(PAIRS && g.gather ? g.gather[i] : i, 0), g.x_rows - 1);
     }
-    f8_v4f acc[TT];
+    f8_v4f acc[NM * TT];
 #pragma unroll
-    for (int t = 0; t < TT; t++) acc[t] = f8_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < NM * TT; t++) acc[t] = f8_v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (b0 < b1) {
         // the next 64 blocks' scales, one a lane (a scalar load a block is waited for with the one just asked for)
-        float scales = ws[min(b0 + lane, b1 - 1)];
+        float scales[NM];
+#pragma unroll
+        for (int m = 0; m < NM; m++) scales[m] = ws[m][min(b0 + lane, b1 - 1)];
         __builtin_amdgcn_sched_barrier(0);  // (first, so that its wait is not one for the codes)
         auto next_scales = [&](int b) {
-            if (b > b0 && ((b - b0) & 63) == 0)
-                asm volatile("global_load_dword %0, %1, %2\n\ts_waitcnt vmcnt(0)" : "=v"(scales) : "v"((uint32_t)min(b + lane, b1 - 1) * 4u), "s"(ws) : "memory");
+            if (b == b0 || ((b - b0) & 63)) return;
+#pragma unroll
+            for (int m = 0; m < NM; m++)
+                asm volatile("global_load_dword %0, %1, %2\n\ts_waitcnt vmcnt(0)" : "=v"(scales[m]) : "v"((uint32_t)min(b + lane, b1 - 1) * 4u), "s"(ws[m]) : "memory");
         };
         static_assert(64 % D == 0, "whole rounds");
-        uint4 w[D][2], x[FUSED ? 1 : D][TT][4];
+        uint4 w[D][NM][2], x[FUSED ? 1 : D][TT][4];
         auto fetch_w = [&](int u, int b) {
-            const uint8_t *const at = wq + (size_t)min(b, b1 - 1) * F8_PIECE;
             // (past the last-level cache, as weights met once a step are: 3 to 7 % faster than plain loads on matrices that aren't in it)
-            w[u][0] = stream_load16(at);
-            w[u][1] = stream_load16(at + 1024);
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                const uint8_t *const at = wq[m] + (size_t)min(b, b1 - 1) * F8_PIECE;
+                w[u][m][0] = stream_load16(at);
+                w[u][m][1] = stream_load16(at + 1024);
+            }
         };
         auto fetch_x = [&](int u, int b) {
 #pragma unroll
@@ -259,27 +283,30 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
         }
         const uint16_t *const own_lane = own + min(lane & 15, used - 1) * F8_BLOCK + (lane >> 4) * 32;
         auto consume = [&](int u, int b) {
-            const float by = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scales), (b - b0) & 63));
-            f8_v8bf wv[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint4 &raw = w[u][k >> 1];
-                const uint2 lo = f8_to_bf16(k & 1 ? raw.z : raw.x, 1.0f), hi = f8_to_bf16(k & 1 ? raw.w : raw.y, 1.0f);
-                const uint4 both = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                __builtin_memcpy(&wv[k], &both, 16);
-            }
-#pragma unroll
-            for (int t = 0; t < TT; t++) {
-                f8_v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int m = 0; m < NM; m++) {
+                const float by = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scales[m]), (b - b0) & 63));
+                f8_v8bf wv[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    f8_v8bf xv;
-                    if (FUSED) xv = *reinterpret_cast<const f8_v8bf *>(own_lane + (size_t)(b - b0) * used * F8_BLOCK + k * 8);
-                    else __builtin_memcpy(&xv, &x[u][t][k], 16);
-                    p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[k], xv, p, 0, 0, 0);
+                    const uint4 &raw = w[u][m][k >> 1];
+                    const uint2 lo = f8_to_bf16(k & 1 ? raw.z : raw.x, 1.0f), hi = f8_to_bf16(k & 1 ? raw.w : raw.y, 1.0f);
+                    const uint4 both = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    __builtin_memcpy(&wv[k], &both, 16);
                 }
 #pragma unroll
-                for (int r = 0; r < 4; r++) acc[t][r] = __builtin_fmaf(p[r], by, acc[t][r]);
+                for (int t = 0; t < TT; t++) {
+                    f8_v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        f8_v8bf xv;
+                        if (FUSED) xv = *reinterpret_cast<const f8_v8bf *>(own_lane + (size_t)(b - b0) * used * F8_BLOCK + k * 8);
+                        else __builtin_memcpy(&xv, &x[u][t][k], 16);
+                        p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[k], xv, p, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[m * TT + t][r] = __builtin_fmaf(p[r], by, acc[m * TT + t][r]);
+                }
             }
         };
         // Requests without a branch around them, so that the wait for a block counts those behind it; and no branch between a product
@@ -302,7 +329,7 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
                 if (b + u >= b1) break;  // (uniform)
                 consume(u, b + u);
 #pragma unroll
-                for (int t = 0; t < TT; t++) asm volatile("" : "+v"(acc[t]));
+                for (int t = 0; t < NM * TT; t++) asm volatile("" : "+v"(acc[t]));
                 if (b + u + D < b1) {
                     fetch_w(u, b + u + D);
                     if (!FUSED) fetch_x(u, b + u + D);
@@ -311,16 +338,24 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
         }
     }
 #pragma unroll
-    for (int t = 0; t < TT; t++) sums[wave][t][lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+    for (int t = 0; t < NM * TT; t++) sums[wave][t][lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
     __syncthreads();
     const int last_wave = min(NW, TT);  // a wavefront a tile of tokens
     if (wave >= last_wave) return;
     const int t = wave, tok = 16 * t + (lane & 15);
-    float4 v = sums[0][t][lane];
+    auto total = [&](int i) {
+        float4 v = sums[0][i][lane];
 #pragma unroll
-    for (int k = 1; k < NW; k++) {
-        const float4 o = sums[k][t][lane];
-        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+        for (int k = 1; k < NW; k++) {
+            const float4 o = sums[k][i][lane];
+            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+        }
+        return v;
+    };
+    float4 v = total(t);
+    if (NM == 2) {
+        const float4 u = total(TT);  // (TT is 1)
+        v = make_float4(silu_as_host(v.x) * u.x, silu_as_host(v.y) * u.y, silu_as_host(v.z) * u.z, silu_as_host(v.w) * u.w);
     }
     if (tok >= used) return;
     const int r0 = strip * F8_STRIP + 4 * (lane >> 4);
@@ -332,10 +367,10 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
 #endif
 }
 
-template <int NW, int TT, int D, bool FUSED, bool PAIRS>
+template <int NW, int TT, int D, bool FUSED, int MODE>
 static int go_f8_rows(const F8Rows &g, const dim3 &grid, size_t lds, hipStream_t s) {
-    if (f8_wide_rows(g.x, (size_t)g.cols)) hipLaunchKernelGGL((f8_rows_kernel<NW, TT, D, FUSED, PAIRS, true>), grid, dim3(64 * NW), lds, s, g);
-    else hipLaunchKernelGGL((f8_rows_kernel<NW, TT, D, FUSED, PAIRS, false>), grid, dim3(64 * NW), lds, s, g);
+    if (f8_wide_rows(g.x, (size_t)g.cols)) hipLaunchKernelGGL((f8_rows_kernel<NW, TT, D, FUSED, MODE, true>), grid, dim3(64 * NW), lds, s, g);
+    else hipLaunchKernelGGL((f8_rows_kernel<NW, TT, D, FUSED, MODE, false>), grid, dim3(64 * NW), lds, s, g);
     FRK_LAUNCH_CHECK("f8_rows");
     return FRK_OK;
 }
@@ -413,10 +448,10 @@ int launch_f8_gemm(const frk_weights *w, const F8Plan &plan, const float *x, siz
     g.ldy = w->rows;
     g.y = y;
     const dim3 grid((unsigned)m.strips, (unsigned)w->matrices);
-    if (plan.fused) return go_f8_rows<8, 1, 4, true, false>(g, grid, batch * m.blocks * F8_BLOCK * 2, s);
-    if (batch <= 16) return go_f8_rows<8, 1, 4, false, false>(g, grid, 0, s);
-    if (batch <= 32) return go_f8_rows<8, 2, 2, false, false>(g, grid, 0, s);
-    return go_f8_rows<8, 4, 1, false, false>(g, grid, 0, s);
+    if (plan.fused) return go_f8_rows<8, 1, 4, true, F8_DENSE>(g, grid, batch * m.blocks * F8_BLOCK * 2, s);
+    if (batch <= 16) return go_f8_rows<8, 1, 4, false, F8_DENSE>(g, grid, 0, s);
+    if (batch <= 32) return go_f8_rows<8, 2, 2, false, F8_DENSE>(g, grid, 0, s);
+    return go_f8_rows<8, 4, 1, false, F8_DENSE>(g, grid, 0, s);
 }
 
 // ---- grouped: the tile list of the groups given.  Offsets are clamped to 0 .. pairs and made non-decreasing (each the largest
@@ -475,9 +510,30 @@ static size_t f8_max_tiles(size_t pairs, size_t groups, int tokens) { return pai
 // Measured in us with tiles of 256x128 / 256x64 / 128x64 / 128x32 (weight rows x pairs): 32 groups of 2880 x 2880 and 256 pairs each on average 188 /
 // 180 / 235 / 243, 64 95 / 98 / 112 / 96, 32 88 / 68 / 78 / 75, 16 85 / 64 / 73 / 60; 128 of 768 x 2048 and 128 pairs 108 / 85 / 102 / 105, 32 68 / 54 / 56 / 59,
 // 16 64 / 50 / 53 / 46, 4 63 / 47 / 51 / 42.
-static int f8_grouped_shape(size_t pairs, size_t groups) { return pairs >= 24 * groups ? F8_TILE_256x64 : F8_TILE_128x32; }
-// a few pairs: a launch that looks the groups up itself
-static bool f8_few_pairs(size_t pairs, size_t groups) { return pairs <= 64 && groups >= pairs / 2; }
+int f8_grouped_shape(size_t pairs, size_t groups) { return pairs >= 24 * groups ? F8_TILE_256x64 : F8_TILE_128x32; }
+// A few pairs: a launch that looks the groups up itself.  In us, so / by tiles, a token's pairs over different groups: 128 groups of 768 x 2048, 16 pairs 9.7 /
+// 16.1, 32 15.9 / 16.8, 48 21.5 / 20.1; 32 of 2880 x 2880, 16 pairs 27.7 / 33.5, 32 44.9 / 39.7; 8 of 1792 x 4096, 16 pairs 16.9 / 25.2.
+static bool f8_few_pairs(size_t pairs, size_t groups) { return pairs <= 24 && groups >= pairs / 2; }
+// Of an expert layer: each slot by itself, its row quantized by the workgroups that read it.  The layer in us, so / bucketed: 32 experts of 2880 x 2880, 4
+// slots 26 / 65, 16 77 / 91, 24 108 / 106, 32 140 / 114; 128 of 768 x 2048, 8 slots 20 / 45, 24 39 / 48, 48 66 / 62; 8 of 1792 x 4096, 8 slots 38 / 69.
+bool f8_few_slots(size_t slots, size_t experts, size_t hidden, size_t ffn) {
+    return f8_few_pairs(slots, experts) && f8_blocks(std::max(hidden, ffn)) * F8_BLOCK * 2 <= F8_FUSED_LDS - 8 * 1024;  // (8 KB more of sums)
+}
+int launch_f8_slots(const frk_weights *w, const frk_weights *up, const int32_t *ids, size_t slots, int slots_a_row, const float *x, float *y, hipStream_t s) {
+    F8Rows g{};
+    g.w = f8_mat(w);
+    if (up) g.up = f8_mat(up);
+    g.x = x;
+    g.cols = (int)w->cols;
+    g.ids = ids;
+    g.n_groups = (int)w->matrices;
+    g.slots_a_row = slots_a_row;
+    g.ldy = g.w.rows;
+    g.y = y;
+    const dim3 grid((unsigned)g.w.strips, (unsigned)slots);
+    const size_t lds = (size_t)g.w.blocks * F8_BLOCK * 2;
+    return up ? go_f8_rows<8, 1, 4, true, F8_SLOTS_GLU>(g, grid, lds, s) : go_f8_rows<8, 1, 4, true, F8_SLOTS>(g, grid, lds, s);
+}
 size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs) {
     return f8_acts_bytes(x_rows, w->cols) + 256 + f8_max_tiles(pairs, w->matrices, 32) * 16;
 }
@@ -515,7 +571,7 @@ int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int3
         g.ldy = g.w.rows;
         g.y = y;
         const dim3 grid((unsigned)g.w.strips, (unsigned)pairs);
-        return fused ? go_f8_rows<8, 1, 4, true, true>(g, grid, F8_FUSED * g.w.blocks * F8_BLOCK * 2, s) : go_f8_rows<8, 1, 4, false, true>(g, grid, 0, s);
+        return fused ? go_f8_rows<8, 1, 4, true, F8_PAIRS>(g, grid, F8_FUSED * g.w.blocks * F8_BLOCK * 2, s) : go_f8_rows<8, 1, 4, false, F8_PAIRS>(g, grid, 0, s);
     }
     const int shape = f8_grouped_shape(pairs, w->matrices), tokens = F8_TILE_SIZE[shape].tokens;
     int *n_tiles = (int *)((char *)ws + f8_acts_bytes(x_rows, w->cols));

@@ -212,6 +212,11 @@ int launch_f8_gemm(const frk_weights *w, const F8Plan &plan, const float *x, siz
 size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs);
 int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
                       float *y, void *ws, hipStream_t s);
+// an expert layer's few slots: y[slot] = product of expert ids[slot] and row slot / slots_a_row of x; with `up` silu(w x) * (up x).  A slot
+// whose id is no expert is left as it was
+bool f8_few_slots(size_t slots, size_t experts, size_t hidden, size_t ffn);
+int launch_f8_slots(const frk_weights *w, const frk_weights *up, const int32_t *ids, size_t slots, int slots_a_row, const float *x, float *y, hipStream_t s);
+int f8_grouped_shape(size_t pairs, size_t groups);  // the tiles' shape
 // rows of x (of silu(x) * up) quantized; `used`: a row whose entry is negative is left as it is
 int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols, const int *used, const F8Acts &out, hipStream_t s);
 // the products of the tiles {matrix, first row of the order, rows in use (up to the shape's tokens), first row of y}; row i of the order

@@ -1182,34 +1182,71 @@ int launch_moe_ffn_units_grouped(const frk_weights *gate, const frk_weights *up,
     return FRK_OK;
 }
 
-// ---- experts in 8-bit floating point with a scale for each block (frk_f8.hip): bucketed, gate and up over the token rows
-// quantized once, silu(gate) * up quantized, down, the weighted sum ----
+// ---- experts in 8-bit floating point with a scale for each block (frk_f8.hip).  A few slots: gate, up and SwiGLU in one launch, down in
+// the next, each slot by itself.  More: bucketed, beside it the token rows quantized once; gate, up, silu(gate) * up quantized, down.
+// At the end the weighted sum. ----
+template <int TILE, bool WIDE>
+__global__ __launch_bounds__(1024) void moe_group_quantize_f8_kernel(GroupArgs a, const float *__restrict__ x, size_t jobs, int parts, int cols, int blocks,
+                                                                     F8Acts out) {
+    if (blockIdx.x == 0) {
+        moe_group<TILE>(a);
+        return;
+    }
+    const int lane = threadIdx.x & 63;
+    for (size_t j = (size_t)(blockIdx.x - 1) * 16 + (threadIdx.x >> 6); j < jobs; j += (size_t)(gridDim.x - 1) * 16)
+        f8_quantize_blocks<WIDE>(x, nullptr, j / parts, (int)(j % parts) * F8_QUANTIZE_BLOCKS, cols, blocks, lane, out);
+}
+template <int TILE, bool WIDE>
+static int launch_moe_group_quantize_f8(const GroupArgs &a, const float *x, size_t rows, size_t cols, const F8Acts &out, hipStream_t s) {
+    static bool sized = false;  // a benign race: every thread sets the same attribute
+    if (!sized) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&moe_group_quantize_f8_kernel<TILE, WIDE>),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(GroupLds));
+        if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFuncSetAttribute(moe_group_quantize_f8): %s", hipGetErrorString(e));
+        sized = true;
+    }
+    const int blocks = (int)f8_blocks(cols), parts = (blocks + F8_QUANTIZE_BLOCKS - 1) / F8_QUANTIZE_BLOCKS;
+    const size_t jobs = rows * parts;
+    hipLaunchKernelGGL((moe_group_quantize_f8_kernel<TILE, WIDE>), dim3((unsigned)std::min<size_t>(1 + (jobs + 15) / 16, 1 << 12)), dim3(1024), sizeof(GroupLds), s,
+                       a, x, jobs, parts, (int)cols, blocks, out);
+    FRK_LAUNCH_CHECK("moe_group_quantize_f8");
+    return FRK_OK;
+}
 struct F8MoeScratch {
+    bool few;
+    int shape, tile;
+    size_t rows;  // of the grouped order; few: slots
     void *x_acts, *a_acts;
-    float *gate_out, *up_out, *down_out;
+    float *gate_out, *up_out, *down_out;  // few: gate_out holds silu(gate) * up
     int *group_off, *gather, *pos_of, *cpos_of, *n_tiles;
     int4 *tiles;
 };
 static F8MoeScratch f8_moe_carve(void *base, size_t batch, int k, int n_experts, size_t hidden, size_t ffn, size_t *end) {
-    const size_t pairs = batch * (size_t)k, rows = moe_max_rows(pairs, n_experts);
+    const size_t pairs = batch * (size_t)k;
     char *p = (char *)base;
     auto take = [&](size_t bytes) {
         char *r = p;
         p += round_up(bytes, 256);
         return r;
     };
-    F8MoeScratch m;
-    m.x_acts = take(f8_acts_bytes(batch, hidden));
-    m.a_acts = take(f8_acts_bytes(rows, ffn));
-    m.gate_out = (float *)take(rows * ffn * 4);
-    m.up_out = (float *)take(rows * ffn * 4);
-    m.down_out = (float *)take(rows * hidden * 4);
-    m.group_off = (int *)take((n_experts + 1) * 4);
-    m.gather = (int *)take(rows * 4);
-    m.pos_of = (int *)take(pairs * 4);
-    m.cpos_of = (int *)take(pairs * 4);
-    m.n_tiles = (int *)take(256);
-    m.tiles = (int4 *)take((rows / MOE_TILE + 1) * 16);
+    F8MoeScratch m{};
+    m.few = f8_few_slots(pairs, n_experts, hidden, ffn);
+    m.shape = f8_grouped_shape(pairs, n_experts);
+    m.tile = F8_TILE_SIZE[m.shape].tokens;
+    m.rows = m.few ? pairs : moe_max_rows(pairs, n_experts, m.tile);
+    m.gate_out = (float *)take(m.rows * ffn * 4);
+    m.down_out = (float *)take(m.rows * hidden * 4);
+    if (!m.few) {
+        m.up_out = (float *)take(m.rows * ffn * 4);
+        m.x_acts = take(f8_acts_bytes(batch, hidden));
+        m.a_acts = take(f8_acts_bytes(m.rows, ffn));
+        m.group_off = (int *)take((n_experts + 1) * 4);
+        m.gather = (int *)take(m.rows * 4);
+        m.pos_of = (int *)take(pairs * 4);
+        m.cpos_of = (int *)take(pairs * 4);
+        m.n_tiles = (int *)take(256);
+        m.tiles = (int4 *)take((m.rows / m.tile + 1) * 16);
+    }
     if (end) *end = (size_t)(p - (char *)base);
     return m;
 }
@@ -1220,29 +1257,24 @@ size_t f8_moe_workspace_bytes(size_t batch, int k, int n_experts, size_t hidden,
 }
 int launch_moe_ffn_f8(const frk_weights *gate, const frk_weights *up, const frk_weights *down, int n_experts, const float *x, size_t batch,
                       const int32_t *ids, const float *weights, int k, float *out, void *ws, hipStream_t s) {
-    const size_t hidden = gate->cols, ffn = down->cols, pairs = batch * (size_t)k, rows = moe_max_rows(pairs, n_experts), max_tiles = rows / MOE_TILE;
-    static_assert(MOE_TILE == F8_TILE_SIZE[F8_TILE_128x64].tokens, "the tiles' shape");
+    const size_t hidden = gate->cols, ffn = down->cols, pairs = batch * (size_t)k;
     const F8MoeScratch m = f8_moe_carve(ws, batch, k, n_experts, hidden, ffn, nullptr);
-    static bool sized = false;  // a benign race: every thread sets the same attribute
-    if (!sized) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&moe_group_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)sizeof(GroupLds));
-        if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFuncSetAttribute(moe_group): %s", hipGetErrorString(e));
-        sized = true;
+    int rc = FRK_OK;
+    if (m.few) {
+        rc = launch_f8_slots(gate, up, ids, pairs, k, x, m.gate_out, s);
+        if (!rc) rc = launch_f8_slots(down, nullptr, ids, pairs, 1, m.gate_out, m.down_out, s);
+    } else {
+        const size_t max_tiles = m.rows / m.tile;
+        const GroupArgs ga{ids, (int)pairs, k, n_experts, m.group_off, m.gather, m.pos_of, m.cpos_of, m.tiles, m.n_tiles, (int)m.rows};
+        const F8Acts xa = f8_acts_carve(m.x_acts, batch), aa = f8_acts_carve(m.a_acts, m.rows);
+        const bool wide = f8_wide_rows(x, hidden);
+        if (m.tile == 64) rc = wide ? launch_moe_group_quantize_f8<64, true>(ga, x, batch, hidden, xa, s) : launch_moe_group_quantize_f8<64, false>(ga, x, batch, hidden, xa, s);
+        else rc = wide ? launch_moe_group_quantize_f8<32, true>(ga, x, batch, hidden, xa, s) : launch_moe_group_quantize_f8<32, false>(ga, x, batch, hidden, xa, s);
+        if (!rc) rc = launch_f8_tiles(gate, xa, m.shape, m.gather, m.tiles, m.n_tiles, max_tiles, m.gate_out, s);
+        if (!rc) rc = launch_f8_tiles(up, xa, m.shape, m.gather, m.tiles, m.n_tiles, max_tiles, m.up_out, s);
+        if (!rc) rc = launch_f8_quantize(m.gate_out, m.up_out, m.rows, ffn, m.gather, aa, s);
+        if (!rc) rc = launch_f8_tiles(down, aa, m.shape, nullptr, m.tiles, m.n_tiles, max_tiles, m.down_out, s);
     }
-    const GroupArgs ga{ids, (int)pairs, k, n_experts, m.group_off, m.gather, m.pos_of, m.cpos_of, m.tiles, m.n_tiles, (int)rows};
-    hipLaunchKernelGGL(moe_group_kernel, dim3(1), dim3(1024), sizeof(GroupLds), s, ga);
-    FRK_LAUNCH_CHECK("moe_group");
-    const F8Acts xa = f8_acts_carve(m.x_acts, batch), aa = f8_acts_carve(m.a_acts, rows);
-    int rc = launch_f8_quantize(x, nullptr, batch, hidden, nullptr, xa, s);
-    if (rc) return rc;
-    rc = launch_f8_tiles(gate, xa, F8_TILE_128x64, m.gather, m.tiles, m.n_tiles, max_tiles, m.gate_out, s);
-    if (rc) return rc;
-    rc = launch_f8_tiles(up, xa, F8_TILE_128x64, m.gather, m.tiles, m.n_tiles, max_tiles, m.up_out, s);
-    if (rc) return rc;
-    rc = launch_f8_quantize(m.gate_out, m.up_out, rows, ffn, m.gather, aa, s);
-    if (rc) return rc;
-    rc = launch_f8_tiles(down, aa, F8_TILE_128x64, nullptr, m.tiles, m.n_tiles, max_tiles, m.down_out, s);
     if (rc) return rc;
     hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)batch, (unsigned)((hidden + 1023) / 1024)), dim3(256), 0, s, m.down_out, ids, weights,
                        m.pos_of, k, (int)hidden, n_experts, (int)(batch >= MOE_BUCKET_ORDER_FROM), out);

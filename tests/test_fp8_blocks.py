@@ -395,7 +395,8 @@ def _plain_layer(parts, x, ids, weights):
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,experts,k,hidden,ffn", [
     (1, 4, 2, 260, 130), (3, 8, 8, 128, 384), (16, 6, 3, 384, 100), (33, 5, 2, 640, 256), (70, 3, 1, 132, 513), (200, 4, 2, 256, 128),
-    (1, 64, 8, 512, 192), (40, 128, 4, 256, 96)])
+    (1, 64, 8, 512, 192), (40, 128, 4, 256, 96), (4, 16, 3, 1028, 700), (8, 32, 8, 260, 1300), (1, 3, 1, 20480, 40), (1, 3, 1, 20608, 40),
+    (1, 2, 1, 16, 1)])
 def test_expert_layer_against_64_bits(fa, batch, experts, k, hidden, ffn):
     print("fp8 experts", batch, experts, k, hidden, ffn, flush=True)
     rng = np.random.default_rng(batch + experts * hidden)
