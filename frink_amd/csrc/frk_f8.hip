@@ -190,7 +190,7 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
         matrix = __builtin_amdgcn_readfirstlane(lead.x), first = __builtin_amdgcn_readfirstlane(lead.y), used = __builtin_amdgcn_readfirstlane(lead.z);
         if (used == 0) return;
     } else if (SLOTS) {
-        matrix = g.ids[blockIdx.y], first = blockIdx.y, used = 1;
+        matrix = g.ids ? g.ids[blockIdx.y] : 0, first = blockIdx.y, used = 1;
         if (matrix < 0 || matrix >= g.n_groups) return;  // (adds nothing to its token)
     } else {
         matrix = blockIdx.y, first = (int)blockIdx.z * 16 * TT, used = min(16 * TT, g.M - first);
@@ -516,9 +516,8 @@ int f8_grouped_shape(size_t pairs, size_t groups) { return pairs >= 24 * groups 
 static bool f8_few_pairs(size_t pairs, size_t groups) { return pairs <= 24 && groups >= pairs / 2; }
 // Of an expert layer: each slot by itself, its row quantized by the workgroups that read it.  The layer in us, so / bucketed: 32 experts of 2880 x 2880, 4
 // slots 26 / 65, 16 77 / 91, 24 108 / 106, 32 140 / 114; 128 of 768 x 2048, 8 slots 20 / 45, 24 39 / 48, 48 66 / 62; 8 of 1792 x 4096, 8 slots 38 / 69.
-bool f8_few_slots(size_t slots, size_t experts, size_t hidden, size_t ffn) {
-    return f8_few_pairs(slots, experts) && f8_blocks(std::max(hidden, ffn)) * F8_BLOCK * 2 <= F8_FUSED_LDS - 8 * 1024;  // (8 KB more of sums)
-}
+bool f8_slots_fit(size_t cols) { return f8_blocks(cols) * F8_BLOCK * 2 <= F8_FUSED_LDS - 8 * 1024; }  // (8 KB more of sums)
+bool f8_few_slots(size_t slots, size_t experts, size_t hidden, size_t ffn) { return f8_few_pairs(slots, experts) && f8_slots_fit(std::max(hidden, ffn)); }
 int launch_f8_slots(const frk_weights *w, const frk_weights *up, const int32_t *ids, size_t slots, int slots_a_row, const float *x, float *y, hipStream_t s) {
     F8Rows g{};
     g.w = f8_mat(w);

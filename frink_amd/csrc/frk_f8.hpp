@@ -213,7 +213,8 @@ size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pa
 int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
                       float *y, void *ws, hipStream_t s);
 // an expert layer's few slots: y[slot] = product of expert ids[slot] and row slot / slots_a_row of x; with `up` silu(w x) * (up x).  A slot
-// whose id is no expert is left as it was
+// whose id is no expert is left as it was; without ids every slot is matrix 0's
+bool f8_slots_fit(size_t cols);
 bool f8_few_slots(size_t slots, size_t experts, size_t hidden, size_t ffn);
 int launch_f8_slots(const frk_weights *w, const frk_weights *up, const int32_t *ids, size_t slots, int slots_a_row, const float *x, float *y, hipStream_t s);
 int f8_grouped_shape(size_t pairs, size_t groups);  // the tiles' shape

@@ -1392,6 +1392,11 @@ int frk_hip_ffn_swiglu_dev(const frk_weights *gate, const frk_weights *up, const
     } else if (up->kind == FRK_KIND_Q8_0 && q8_0_cols_form(gate)) {
         rc = launch_gemv_q8_0_f32_glu(gate, up, x, act, s);
         if (rc) return rc;
+    } else if (is_f8_kind(gate->kind) && is_f8_kind(up->kind) && gate->matrices == 1 && up->matrices == 1 && f8_slots_fit(gate->cols)) {
+        rc = f8_on_current_device(gate);
+        if (!rc) rc = f8_on_current_device(up);
+        if (!rc) rc = launch_f8_slots(gate, up, nullptr, 1, 1, x, act, s);
+        if (rc) return rc;
     } else {
         const frk_weights *pair[2] = {gate, up};
         float *outs[2] = {g_out, u_out};
@@ -1468,6 +1473,8 @@ int frk_hip_moe_ffn_dev(const frk_weights *gate, const frk_weights *up, const fr
             if (w->matrices != n_experts)
                 return set_error(FRK_ERR_SHAPE, "an FP8_BLOCK stack holds %zu matrices, the call names %zu experts", w->matrices, n_experts);
         int rc = f8_on_current_device(gate);
+        if (!rc) rc = f8_on_current_device(up);
+        if (!rc) rc = f8_on_current_device(down);
         if (!rc) rc = workspace(f8_moe_workspace_bytes(batch, (int)k, (int)n_experts, hidden, ffn), (hipStream_t)stream, lease);
         if (rc) return rc;
         return launch_moe_ffn_f8(gate, up, down, (int)n_experts, x, batch, ids, weights, (int)k, out, lease.ptr, (hipStream_t)stream);
