@@ -61,7 +61,8 @@ __global__ __launch_bounds__(64 * RW * TW, 2) void f8_tile_kernel(F8Gemm g, int 
     const uint32_t lds0 = lds_address(f8_lds);
     const int strip0 = row_tile * (T::ROWS / F8_STRIP) + rw * MR;  // of this wavefront
 
-    // ---- tokens: a stage holds them 256 bytes each, piece p of token t in place p ^ t % 16
+    // ---- tokens: a stage holds them 256 bytes each, piece p of token t in place (p / 4 + 4 (p % 4)) ^ t % 16.  (LDS serves lanes 0-3, 12-15 and
+    // 20-27 of a 16-byte read together, 4-11 with 16-19 and 28-31: in place p ^ t % 16 every two of those share their banks.)
     uint32_t x_off[T::REQUESTS];
     const uint8_t *x_base = reinterpret_cast<const uint8_t *>(g.a.v);
     const int first_row = g.src ? 0 : min(tile.y, g.a.rows - 1);
@@ -70,13 +71,14 @@ __global__ __launch_bounds__(64 * RW * TW, 2) void f8_tile_kernel(F8Gemm g, int 
     for (int c = 0; c < T::REQUESTS; c++) {
         const int t = (wave * T::REQUESTS + c) * 4 + (lane >> 4), i = min(t, tile.z - 1);
         const uint32_t row = (uint32_t)(min(max(g.src ? g.src[tile.y + i] : tile.y + i, 0), g.a.rows - 1) - first_row);
-        x_off[c] = row * (uint32_t)blocks * (F8_BLOCK * 2) + (uint32_t)((lane & 15) ^ (t & 15)) * 16;
+        const int place = (lane & 15) ^ (t & 15);
+        x_off[c] = row * (uint32_t)blocks * (F8_BLOCK * 2) + (uint32_t)(place >> 2 | (place & 3) << 2) * 16;
     }
     auto request = [&](int slot, int b, int c) {
         dma16(lds0 + (uint32_t)slot * T::STAGE + (wave * T::REQUESTS + c) * 1024, x_base + (size_t)b * (F8_BLOCK * 2), x_off[c]);
     };
-    const uint32_t x_lane = (uint32_t)((tw * MT * 16 + li) * 256 + (((4 * lg) ^ li) * 16));  // this lane's token's four pieces
-    auto read_x = [&](const uint8_t *st, int j, int k) { return *reinterpret_cast<const f8_v8bf *>(st + j * 16 * 256 + (x_lane ^ (uint32_t)(k * 16))); };
+    const uint32_t x_lane = (uint32_t)((tw * MT * 16 + li) * 256 + ((lg ^ li) * 16));  // this lane's token's four pieces
+    auto read_x = [&](const uint8_t *st, int j, int k) { return *reinterpret_cast<const f8_v8bf *>(st + j * 16 * 256 + (x_lane ^ (uint32_t)(k * 64))); };
     // ---- codes: straight into registers, a block ahead (LDS, at 128 bytes a cycle and CU, has enough to do with the tokens)
     const uint8_t *w_base[MR];
 #pragma unroll
