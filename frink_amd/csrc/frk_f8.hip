@@ -4,6 +4,7 @@
 #include "frk_f8.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace frk {
 
@@ -380,10 +381,9 @@ static bool f8_fused(size_t tokens, size_t cols) { return tokens <= F8_FUSED && 
 
 // By estimated time.  Both kernels are a chain of steps a wavefront until the chip is full: a block of 128 columns takes a tile's wavefronts
 // as long alone on a CU as beside the CU's other workgroups, up to how many fit; a strip of the rows kernel likewise.  Shares of the
-// columns cost a second launch, 3.3 us, and the traffic of the parts.  In us, measured / by these lines (rows x columns, tokens):
-// 4096 x 4096 at 64 128x64 tiles 27.7 / 29.5, two shares 20.7 / 21.7, the rows kernel 14.1 / 14.0; 14336 x 4096 at 64 two shares
-// 23.3 / 24.1, the rows kernel 37.6 / 36.5; at 512 256x128 59.7 / 55.7, 256x64 62.1 / 53.7, 128x64 73.3 / 75.6; 4096 x 4096 at 512
-// 256x64 36.2 / 33.3, in two shares 30.9 / 30.3.
+// columns cost a second launch, 3.3 us, and the traffic of the parts.  Every kernel, tile and number of shares timed at 26 sizes (24 to 4096 tokens, 576 x 7168 to
+// 14336 x 4096): the choice is within 4 % of the fastest at 23, 6 % behind at 512 tokens of 4096 x 4096 (33.0 against 31.1 us), 11 at 384, 14 at 128 of
+// 14336 x 4096 (33.0 against 29.0).
 F8Plan f8_plan(const frk_weights *w, size_t batch) {
     const F8Mat m = f8_mat(w);
     F8Plan best{-1, 1, f8_fused(batch, w->cols), 0, 0};
@@ -405,11 +405,13 @@ F8Plan f8_plan(const frk_weights *w, size_t batch) {
             if (parts > 1 && (parts > m.blocks / 2 || parts * n * 4 > SPLIT_PARTS_BYTES)) break;
             const F8TileSize t = F8_TILE_SIZE[shape];
             const double groups = (double)((m.rows + t.rows - 1) / t.rows) * (double)((batch + t.tokens - 1) / t.tokens) * (double)w->matrices * parts;
-            const double fill = groups / COST[shape].slots, half = shape == F8_TILE_256x128 ? 0.0 : 0.5;  // up to `half` a workgroup is alone on its CU
+            const double fill = groups / COST[shape].slots, whole = std::floor(fill + 0.02), rest = fill - whole;
+            // a round that isn't full: up to half of the slots (256 x 128: a CU has one) a workgroup is alone on its CU, then the fullest CU counts
+            const double alone = COST[shape].alone, full = COST[shape].full, half = shape == F8_TILE_256x128 ? 0.0 : 0.5;
+            const double jump = shape == F8_TILE_256x64 || shape == F8_TILE_128x64 ? 0.6 : 0.0;
+            const double partly = rest <= half ? alone : alone + (full - alone) * (jump + (1.0 - jump) * (rest - half) / (1.0 - half));
             const double chain = (double)((m.blocks + parts - 1) / parts);
-            double us = 4.5;
-            if (fill <= 1.0) us += chain * (COST[shape].alone + (COST[shape].full - COST[shape].alone) * std::max(0.0, fill - half) / (1.0 - half)) + 1.0;
-            else us += (fill < 3.0 ? std::ceil(fill - 0.02) : fill) * (chain * COST[shape].full + 1.0);
+            double us = 7.0 + whole * (chain * full + 1.0) + (rest > 0.0 ? chain * partly + 1.0 : 0.0);
             if (parts > 1) us += 3.3 + 0.45e-6 * 4.0 * (double)n * parts;
             if (us < least) {
                 least = us;

@@ -126,7 +126,8 @@ int frk_hip_weights_from_device(int kind, const void *dev_bytes, size_t len, siz
  * f32 with R = rows / matrices; weight (r, k) of matrix m is its code times scales[m][r / 128][k / 128].  Any R and cols: the
  * last blocks may be partly used.  register takes host buffers (borrowed for the call; synchronous; unlike
  * frk_hip_weights_register it keeps no cache), from_device buffers on the current device (copied on `stream`; they may be
- * freed once the stream has passed the call).  The resident copy pads rows to 16 and columns to 128.
+ * freed once the stream has passed the call).  The resident copy pads rows to 16 and columns to 128.  At most 2^23 columns and 65535
+ * matrices; a gathered product's activations, two bytes a value quantized, at most 4 GiB.
  *
  * What takes such a handle, f32 in and f32 out as for the other kinds: frk_hip_gemv_dev (FRK_ACT_F32 and FRK_ACT_INT8 are the
  * same here), frk_hip_gemv_multi_dev, frk_hip_ffn_swiglu_dev, frk_hip_gemm_dev, frk_hip_gemm_pair_dev,
@@ -314,8 +315,9 @@ int frk_hip_route_top_k_softmax_dev(const float *logits_dev, size_t batch, size_
  *   weights  the chosen experts' p, divided by their sum when norm != 0, times scale
  * Scores, their sums and comparisons are in 64 bits, so that no rounding of theirs decides between two experts; a weight is rounded to
  * f32 once.  Equal values go to the lower index, of groups too.  An expert whose logit is -inf or NaN has p = 0 and cannot be chosen
- * (a mask; nor can one whose bias is -inf or NaN be chosen), nor counts in its group's value; a group of such experts only is chosen last.  Where fewer than k experts are
- * left, the remaining slots get id -1 and weight 0, which frk_hip_moe_ffn_dev skips.  Logits of +inf share a softmax evenly.
+ * (a mask;
+ * nor can one whose bias is -inf or NaN be chosen), nor counts in its group's value; a group of such experts only is chosen last.
+ * Where fewer than k experts are left, the remaining slots get id -1 and weight 0, which frk_hip_moe_ffn_dev skips.  Logits of +inf share a softmax evenly.
  * The reference's routers with sigmoid scores, a bias and groups live in crates/frink-moe; the plain softmax one, whose f32
  * arithmetic a caller may depend on, is frk_hip_route_top_k_softmax_dev.
  * n_experts <= 1024, k <= 64, groups <= 64 and a divisor of n_experts, top_groups * (n_experts / groups) >= k. */
