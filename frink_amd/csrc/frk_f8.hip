@@ -381,9 +381,9 @@ static bool f8_fused(size_t tokens, size_t cols) { return tokens <= F8_FUSED && 
 
 // By estimated time.  Both kernels are a chain of steps a wavefront until the chip is full: a block of 128 columns takes a tile's wavefronts
 // as long alone on a CU as beside the CU's other workgroups, up to how many fit; a strip of the rows kernel likewise.  Shares of the
-// columns cost a second launch, 3.3 us, and the traffic of the parts.  Every kernel, tile and number of shares timed at 26 sizes (24 to 4096 tokens, 576 x 7168 to
-// 14336 x 4096): the choice is within 4 % of the fastest at 23, 6 % behind at 512 tokens of 4096 x 4096 (33.0 against 31.1 us), 11 at 384, 14 at 128 of
-// 14336 x 4096 (33.0 against 29.0).
+// columns cost a second launch, 3.3 us, and the traffic of the parts.  Every kernel, tile and number of shares timed at 35 sizes (24 to 4096
+// tokens, 576 x 7168 to 14336 x 4096): the choice is within 4 % of the fastest but for 512 tokens of 4096 x 14336 (74 against 71 us), 1500 of 2048 x 2048 (27.7
+// against 26.1) and 384 of 4096 x 4096 (32.2 against 28.8).
 F8Plan f8_plan(const frk_weights *w, size_t batch) {
     const F8Mat m = f8_mat(w);
     F8Plan best{-1, 1, f8_fused(batch, w->cols), 0, 0};
@@ -397,7 +397,7 @@ F8Plan f8_plan(const frk_weights *w, size_t batch) {
     }
     static constexpr struct {
         double slots, alone, full;  // workgroups of the chip; us a block
-    } COST[F8_TILE_SHAPES] = {{256, 1.36, 1.60}, {512, 0.87, 1.72}, {512, 0.75, 1.08}, {1024, 0.68, 1.30}};
+    } COST[F8_TILE_SHAPES] = {{256, 1.36, 1.60}, {512, 0.87, 1.72}, {1024, 0.68, 1.30}};
     static constexpr int SHARES[] = {1, 2, 3, 4, 6, 8, 12, 16};
     const size_t n = batch * w->rows;
     for (int shape = 0; shape < F8_TILE_SHAPES; shape++)
@@ -406,9 +406,9 @@ F8Plan f8_plan(const frk_weights *w, size_t batch) {
             const F8TileSize t = F8_TILE_SIZE[shape];
             const double groups = (double)((m.rows + t.rows - 1) / t.rows) * (double)((batch + t.tokens - 1) / t.tokens) * (double)w->matrices * parts;
             const double fill = groups / COST[shape].slots, whole = std::floor(fill + 0.02), rest = fill - whole;
-            // a round that isn't full: up to half of the slots (256 x 128: a CU has one) a workgroup is alone on its CU, then the fullest CU counts
-            const double alone = COST[shape].alone, full = COST[shape].full, half = shape == F8_TILE_256x128 ? 0.0 : 0.5;
-            const double jump = shape == F8_TILE_256x64 || shape == F8_TILE_128x64 ? 0.6 : 0.0;
+            // a round that isn't full: as long as the workgroups are (nearly) alone on their CUs, then the fullest CU counts
+            static constexpr double HALF[F8_TILE_SHAPES] = {0.0, 0.5, 0.35}, JUMP[F8_TILE_SHAPES] = {0.0, 0.6, 0.0};
+            const double alone = COST[shape].alone, full = COST[shape].full, half = HALF[shape], jump = JUMP[shape];
             const double partly = rest <= half ? alone : alone + (full - alone) * (jump + (1.0 - jump) * (rest - half) / (1.0 - half));
             const double chain = (double)((m.blocks + parts - 1) / parts);
             double us = 7.0 + whole * (chain * full + 1.0) + (rest > 0.0 ? chain * partly + 1.0 : 0.0);
@@ -509,9 +509,8 @@ __global__ __launch_bounds__(1024) void f8_tiles_quantize_kernel(F8TilesArgs a, 
         f8_quantize_blocks<WIDE>(x, nullptr, j / parts, (int)(j % parts) * F8_QUANTIZE_BLOCKS, cols, blocks, lane, out);
 }
 static size_t f8_max_tiles(size_t pairs, size_t groups, int tokens) { return pairs / (size_t)tokens + std::min(groups, pairs); }
-// Measured in us with tiles of 256x128 / 256x64 / 128x64 / 128x32 (weight rows x pairs): 32 groups of 2880 x 2880 and 256 pairs each on average 188 /
-// 180 / 235 / 243, 64 95 / 98 / 112 / 96, 32 88 / 68 / 78 / 75, 16 85 / 64 / 73 / 60; 128 of 768 x 2048 and 128 pairs 108 / 85 / 102 / 105, 32 68 / 54 / 56 / 59,
-// 16 64 / 50 / 53 / 46, 4 63 / 47 / 51 / 42.
+// Measured in us with tiles of 256x128 / 256x64 / 128x32 (weight rows x pairs): 32 groups of 2880 x 2880 and 256 pairs each on average 188 / 180 / 243, 64
+// 95 / 98 / 96, 32 88 / 68 / 75, 16 85 / 64 / 60; 128 of 768 x 2048 and 128 pairs 108 / 85 / 105, 32 68 / 54 / 59, 16 64 / 50 / 46, 4 63 / 47 / 42.
 int f8_grouped_shape(size_t pairs, size_t groups) { return pairs >= 24 * groups ? F8_TILE_256x64 : F8_TILE_128x32; }
 // A few pairs: a launch that looks the groups up itself.  In us, so / by tiles, a token's pairs over different groups: 128 groups of 768 x 2048, 16 pairs 9.7 /
 // 16.1, 32 15.9 / 16.8, 48 21.5 / 20.1; 32 of 2880 x 2880, 16 pairs 27.7 / 33.5, 32 44.9 / 39.7; 8 of 1792 x 4096, 16 pairs 16.9 / 25.2.

@@ -191,11 +191,11 @@ struct F8Gemm {
     float *y;
 };
 // over tiles of a shape (weight rows x tokens); parts > 1 (dense): shares of the columns, each its own copy of y, part_stride floats apart
-enum { F8_TILE_256x128, F8_TILE_256x64, F8_TILE_128x64, F8_TILE_128x32, F8_TILE_SHAPES };
+enum { F8_TILE_256x128, F8_TILE_256x64, F8_TILE_128x32, F8_TILE_SHAPES };
 struct F8TileSize {
     int rows, tokens;
 };
-constexpr F8TileSize F8_TILE_SIZE[F8_TILE_SHAPES] = {{256, 128}, {256, 64}, {128, 64}, {128, 32}};
+constexpr F8TileSize F8_TILE_SIZE[F8_TILE_SHAPES] = {{256, 128}, {256, 64}, {128, 32}};
 int launch_f8_tile(const F8Gemm &g, int shape, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s);
 // How a dense batch is multiplied: by the rows kernel (shape -1; `fused`: its own quantization), or over tiles in `parts` shares
 struct F8Plan {

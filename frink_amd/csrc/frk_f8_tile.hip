@@ -253,7 +253,6 @@ int launch_f8_tile(const F8Gemm &g, int shape, size_t tok_tiles, size_t matrices
     switch (shape) {
     case F8_TILE_256x128: return go_f8_tile<4, 2, 4>(g, tok_tiles, matrices, parts, part_stride, s);
     case F8_TILE_256x64: return go_f8_tile<4, 1, 4>(g, tok_tiles, matrices, parts, part_stride, s);
-    case F8_TILE_128x64: return go_f8_tile<2, 2, 2>(g, tok_tiles, matrices, parts, part_stride, s);
     default: return go_f8_tile<2, 1, 2>(g, tok_tiles, matrices, parts, part_stride, s);
     }
 }
