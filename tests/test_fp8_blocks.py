@@ -395,7 +395,7 @@ def _plain_layer(parts, x, ids, weights):
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,experts,k,hidden,ffn", [
     (1, 4, 2, 260, 130), (3, 8, 8, 128, 384), (16, 6, 3, 384, 100), (33, 5, 2, 640, 256), (70, 3, 1, 132, 513), (200, 4, 2, 256, 128),
-    (1, 64, 8, 512, 192), (40, 128, 4, 256, 96), (4, 16, 3, 1028, 700), (8, 32, 8, 260, 1300), (1, 3, 1, 20480, 40), (1, 3, 1, 20608, 40),
+    (1, 64, 8, 512, 192), (40, 128, 4, 256, 96), (4, 16, 3, 1028, 700), (8, 32, 8, 260, 1300), (1, 3, 1, 24576, 40), (1, 3, 1, 24704, 40),
     (1, 2, 1, 16, 1)])
 def test_expert_layer_against_64_bits(fa, batch, experts, k, hidden, ffn):
     print("fp8 experts", batch, experts, k, hidden, ffn, flush=True)
@@ -439,6 +439,53 @@ def test_router_and_experts_captured_together(fa):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(y, step())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden,ffn", [(640, 832), (256, 130), (24576, 48)])
+def test_a_layer_of_one_expert_is_the_ffn(fa, hidden, ffn):
+    import torch
+    rng = np.random.default_rng(hidden)
+    _, (gate, up, down) = _layer(fa, rng, 1, hidden, ffn)
+    x = to_dev(_activations(rng, 1, hidden))
+    y = fa.moe_ffn(gate, up, down, 1, x, torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.ones((1, 1), device="cuda"))
+    want = fa.ffn_swiglu(gate, up, down, x[0])
+    assert torch.equal(y[0], want)  # the same sums in the same order
+
+
+@pytest.mark.gpu
+def test_two_threads_on_two_streams(fa):
+    """Calls of one handle from two threads at once, each on its own stream: the results of calls one after the other."""
+    import threading
+
+    import torch
+    rng = np.random.default_rng(21)
+    w = _resident(fa, *plain.random_matrix(rng, 500, 1300))
+    stack = _resident(fa, *plain.random_matrix(rng, 96, 300, matrices=4))
+    jobs, want = [], []
+    for batch in (2, 9, 33, 150):
+        x, g = to_dev(_activations(rng, batch, 1300)), to_dev(_activations(rng, batch, 300))
+        off = to_dev(_groups(rng, [batch // 2, 0, batch - batch // 2, 0]))
+        jobs.append((x, g, off))
+        want.append((w.gemm(x), fa.gemm_grouped(stack, 4, off, g)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(order):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for i in order * 10:
+                got = w.gemm(jobs[i][0]), fa.gemm_grouped(stack, 4, jobs[i][2], jobs[i][1])
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+                stream.synchronize()
+    threads = [threading.Thread(target=work, args=(o,)) for o in ([0, 1, 2, 3], [3, 2, 1, 0])]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == []
 
 
 @pytest.mark.gpu

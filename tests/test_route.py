@@ -39,7 +39,8 @@ def test_number_of_experts(fa, n_experts, score):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("groups,size", [(2, 1), (2, 7), (8, 32), (4, 64), (8, 20), (3, 100), (16, 16), (64, 16), (64, 1), (12, 5), (33, 31)])
+@pytest.mark.parametrize("groups,size", [(2, 1), (2, 7), (8, 32), (4, 64), (8, 20), (3, 100), (16, 16), (64, 16), (64, 1), (12, 5), (33, 31),
+                                         (32, 8), (4, 32), (8, 64), (2, 128), (3, 64), (6, 8), (5, 4)])
 @pytest.mark.parametrize("group_best", [1, 2])
 def test_groups(fa, groups, size, group_best):
     rng = np.random.default_rng(groups * size)
@@ -77,6 +78,19 @@ def test_batches(fa, batch):
     rng = np.random.default_rng(batch)
     logits = rng.standard_normal((batch, 48)).astype(np.float32)
     _check(fa, logits, 6, bias=(rng.standard_normal(48) * 0.1).astype(np.float32), score="sigmoid", groups=4, top_groups=2, group_best=2, scale=2.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [64, 128, 256, 512, 1024])
+def test_logits_and_biases_of_any_alignment(fa, n):
+    rng = np.random.default_rng(n)
+    logits, bias = rng.standard_normal((5, n)).astype(np.float32), (rng.standard_normal(n) * 0.1).astype(np.float32)
+    rule = dict(score="sigmoid", groups=4, top_groups=2, group_best=2)
+    want_ids, want = plain.route(logits, 8, bias=bias, **rule)
+    for logits_at, bias_at in ((1, 0), (0, 1), (2, 3)):
+        x, b = (to_dev(np.concatenate([np.zeros(at, np.float32), v.ravel()]))[at:] for v, at in ((logits, logits_at), (bias, bias_at)))
+        ids, w = fa.route(x.view(5, n), 8, bias=b, **rule)
+        assert np.array_equal(ids.cpu().numpy(), want_ids) and np.allclose(w.cpu().numpy(), want, rtol=2.0 ** -23, atol=0)
 
 
 @pytest.mark.gpu
