@@ -170,6 +170,19 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _stream_at(x):
+    """_stream() for a call over x.  Kernels on the current device cannot read another's tensors: refused here."""
+    import torch
+    try:
+        here = torch._C._cuda_getDevice()
+        stream = torch._C._cuda_getCurrentRawStream(here)
+    except AttributeError:
+        here, stream = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+    if x.get_device() != here:
+        raise ValueError("the tensor is on device %d, the current device is %d" % (x.get_device(), here))
+    return stream
+
+
 def _np_ptr(a):
     return C.c_void_p(a.ctypes.data)
 
@@ -225,7 +238,7 @@ class Weights:
         cls._check_fp8(codes.numel(), scales.numel(), rows, cols, matrices)
         h = C.c_void_p()
         check(lib().frk_hip_weights_from_device_fp8(C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), rows, cols,
-                                                    matrices, _stream(), C.byref(h)))
+                                                    matrices, _stream_at(codes), C.byref(h)))
         return cls(h, FP8_BLOCK, rows, cols)
 
     def keep_decoded(self):
@@ -252,7 +265,7 @@ class Weights:
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.numel() == self.cols
         y = out if out is not None else torch.empty(self.rows, dtype=torch.float32, device=x.device)
         check(lib().frk_hip_gemv_dev(self.handle, C.c_void_p(x.data_ptr()), C.c_void_p(y.data_ptr()), act_mode,
-                                     _stream()))
+                                     _stream_at(x)))
         return y
 
     def gemv_q8k(self, acts, out=None):
@@ -279,7 +292,7 @@ class Weights:
         batch = x.numel() // self.cols
         # (a small product waits for its call: like its input 0.3 us ahead of torch.empty)
         y = out if out is not None else x.new_empty((batch, self.rows))
-        check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), _stream()))
+        check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), _stream_at(x)))
         return y
 
     def gemm_acts(self, acts, out=None):
@@ -296,7 +309,7 @@ class Weights:
         batch = x.numel() // self.cols
         assert out.dtype == torch.float32 and out.is_cuda and out.is_contiguous() and out.numel() == batch * self.rows
         check(lib().frk_hip_gemm_noalloc_dev(self.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(out.data_ptr()),
-                                             _stream()))
+                                             _stream_at(x)))
         return out
 
     def dequant(self):
@@ -359,7 +372,7 @@ def gemm_pair(w0, w1, x, outs=None):
     batch = x.numel() // w0.cols
     y0, y1 = outs if outs is not None else (torch.empty((batch, w.rows), dtype=torch.float32, device=x.device) for w in (w0, w1))
     check(lib().frk_hip_gemm_pair_dev(w0.handle, w1.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(y0.data_ptr()),
-                                      C.c_void_p(y1.data_ptr()), _stream()))
+                                      C.c_void_p(y1.data_ptr()), _stream_at(x)))
     return y0, y1
 
 
@@ -415,7 +428,7 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_b
         raise ValueError("score %r: one of %s" % (score, ", ".join(SCORES)))
     rule = RouteRule(SCORES[score], int(bool(norm)), groups, top_groups, group_best, scale, None if bias is None else bias.data_ptr())
     ids, w = logits.new_empty((batch, k), dtype=torch.int32), logits.new_empty((batch, k))
-    check(lib().frk_hip_route_dev(logits.data_ptr(), batch, n_experts, k, C.byref(rule), ids.data_ptr(), w.data_ptr(), _stream()))
+    check(lib().frk_hip_route_dev(logits.data_ptr(), batch, n_experts, k, C.byref(rule), ids.data_ptr(), w.data_ptr(), _stream_at(logits)))
     return ids, w
 
 
@@ -428,7 +441,7 @@ def moe_ffn(gate, up, down, n_experts, x, ids, weights, out=None):
     batch, k = ids.shape
     y = out if out is not None else x.new_empty((batch, down.rows // n_experts))
     check(lib().frk_hip_moe_ffn_dev(gate.handle, up.handle, down.handle, n_experts, x.data_ptr(), batch, ids.data_ptr(), weights.data_ptr(), k,
-                                    y.data_ptr(), _stream()))
+                                    y.data_ptr(), _stream_at(x)))
     return y
 
 
@@ -437,7 +450,7 @@ def gemm_grouped(stacked, n_groups, group_off, x, gather=None, out=None):
     (row p without a gather list) times group g's matrix, rows [g*R, (g+1)*R) of `stacked`; out[pairs][R]."""
     import torch
     assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.shape[-1] == stacked.cols
-    assert group_off.dtype == torch.int32 and group_off.is_cuda and group_off.numel() == n_groups + 1
+    assert group_off.dtype == torch.int32 and group_off.is_cuda and group_off.is_contiguous() and group_off.numel() == n_groups + 1
     x_rows = x.numel() // stacked.cols
     if gather is not None:
         assert gather.dtype == torch.int32 and gather.is_cuda and gather.is_contiguous()
@@ -446,7 +459,7 @@ def gemm_grouped(stacked, n_groups, group_off, x, gather=None, out=None):
         pairs = x_rows
     y = out if out is not None else x.new_empty((pairs, stacked.rows // n_groups))
     check(lib().frk_hip_gemm_grouped_dev(stacked.handle, n_groups, group_off.data_ptr(), gather.data_ptr() if gather is not None else None,
-                                         x.data_ptr(), x_rows, pairs, y.data_ptr(), _stream()))
+                                         x.data_ptr(), x_rows, pairs, y.data_ptr(), _stream_at(x)))
     return y
 
 
@@ -476,7 +489,7 @@ def gemv_multi(ws, x, outs=None):
     ys = outs if outs is not None else [torch.empty(w.rows, dtype=torch.float32, device=x.device) for w in ws]
     hs = (C.c_void_p * n)(*[w.handle for w in ws])
     ps = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
-    check(lib().frk_hip_gemv_multi_dev(hs, n, C.c_void_p(x.data_ptr()), ps, _stream()))
+    check(lib().frk_hip_gemv_multi_dev(hs, n, C.c_void_p(x.data_ptr()), ps, _stream_at(x)))
     return ys
 
 
@@ -485,7 +498,7 @@ def ffn_swiglu(gate, up, down, x, out=None):
     import torch
     y = out if out is not None else torch.empty(down.rows, dtype=torch.float32, device=x.device)
     check(lib().frk_hip_ffn_swiglu_dev(gate.handle, up.handle, down.handle, C.c_void_p(x.data_ptr()),
-                                       C.c_void_p(y.data_ptr()), _stream()))
+                                       C.c_void_p(y.data_ptr()), _stream_at(x)))
     return y
 
 

@@ -454,6 +454,31 @@ def test_a_layer_of_one_expert_is_the_ffn(fa, hidden, ffn):
 
 
 @pytest.mark.gpu
+def test_tensors_of_another_device_are_refused(fa):
+    import torch
+
+    class Elsewhere:  # (a tensor of a second device, which this one need not have)
+        def __init__(self, t):
+            self.t = t
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+        def get_device(self):
+            return self.t.get_device() + 1
+    rng = np.random.default_rng(2)
+    codes, scales = plain.random_matrix(rng, 16, 128)
+    w = _resident(fa, codes, scales)
+    x = Elsewhere(torch.zeros((1, 128), device="cuda"))
+    ids, weights = torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.ones((1, 1), device="cuda")
+    for call in (lambda: w.gemm(x), lambda: w.gemv(x), lambda: w.gemm_noalloc(x, torch.zeros((1, 16), device="cuda")), lambda: fa.gemm_pair(w, w, x),
+                 lambda: fa.gemv_multi([w, w], x), lambda: fa.gemm_grouped(w, 1, to_dev(np.array([0, 1], np.int32)), x),
+                 lambda: fa.moe_ffn(w, w, w, 1, x, ids, weights), lambda: fa.Weights.from_device_fp8(Elsewhere(to_dev(codes)), to_dev(scales), 16, 128)):
+        with pytest.raises(ValueError, match="current device"):
+            call()
+
+
+@pytest.mark.gpu
 def test_two_threads_on_two_streams(fa):
     """Calls of one handle from two threads at once, each on its own stream: the results of calls one after the other."""
     import threading
