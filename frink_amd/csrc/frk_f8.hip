@@ -155,22 +155,27 @@ constexpr size_t F8_FUSED_LDS = 56 * 1024;  // beside the 8 KB of sums: what a l
 // the range of up to `most` pairs that pair `p` leads, by the offsets clamped and made non-decreasing (each the largest so far): {group, first, number};
 // a number of 0: it leads none
 __device__ __forceinline__ int4 f8_lead(const int *__restrict__ off, int n_groups, int pairs, int p, int most, int lane) {
-    int after = n_groups + 1;  // the first offset above p
-    for (int i = lane; i <= n_groups; i += 64)
-        if (min(max(off[i], 0), pairs) > p) {
-            after = i;
-            break;
+    int begin = 0;  // a lane's part of the largest before
+    for (int i0 = 0; i0 <= n_groups; i0 += 256) {
+        // 256 at once: one trip to memory for most lists (eight pairs of 128 groups of 768 x 2048: the kernel 6.9 -> 6.6 us, sixteen 9.7 -> 8.0)
+        int v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = i0 + 64 * j + lane <= n_groups ? off[i0 + 64 * j + lane] : 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[j] = min(max(v[j], 0), pairs);
+            const uint64_t above = __ballot(v[j] > p);
+            if (above) {  // (uniform) the first offset above p ends the pair's group
+                const int first = __builtin_ctzll(above), after = i0 + 64 * j + first, end = __builtin_amdgcn_readlane(v[j], first);
+                const int half = (int)f8_half_max((uint32_t)max(begin, lane < first ? v[j] : 0));
+                begin = max(__builtin_amdgcn_readlane(half, 0), __builtin_amdgcn_readlane(half, 32));
+                if (after == 0 || (p - begin) % most) return make_int4(0, 0, 0, 0);
+                return make_int4(after - 1, p, min(most, end - p), 0);
+            }
+            begin = max(begin, v[j]);
         }
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) after = min(after, __shfl_xor(after, m));
-    if (after == 0 || after > n_groups) return make_int4(0, 0, 0, 0);
-    int begin = 0;
-    for (int i = lane; i < after; i += 64) begin = max(begin, min(max(off[i], 0), pairs));
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) begin = max(begin, __shfl_xor(begin, m));
-    const int end = min(max(off[after], 0), pairs);
-    if ((p - begin) % most) return make_int4(0, 0, 0, 0);
-    return make_int4(after - 1, p, min(most, end - p), 0);
+    }
+    return make_int4(0, 0, 0, 0);
 }
 
 template <int NW, int TT, int D, bool FUSED, int MODE, bool WIDE>
@@ -512,13 +517,13 @@ static size_t f8_max_tiles(size_t pairs, size_t groups, int tokens) { return pai
 // Measured in us with tiles of 256x128 / 256x64 / 128x32 (weight rows x pairs): 32 groups of 2880 x 2880 and 256 pairs each on average 188 / 180 / 243, 64
 // 95 / 98 / 96, 32 88 / 68 / 75, 16 85 / 64 / 60; 128 of 768 x 2048 and 128 pairs 108 / 85 / 105, 32 68 / 54 / 59, 16 64 / 50 / 46, 4 63 / 47 / 42.
 int f8_grouped_shape(size_t pairs, size_t groups) { return pairs >= 24 * groups ? F8_TILE_256x64 : F8_TILE_128x32; }
-// A few pairs: a launch that looks the groups up itself.  In us, so / by tiles, a token's pairs over different groups: 128 groups of 768 x 2048, 16 pairs 9.7 /
-// 16.1, 32 15.9 / 16.8, 48 21.5 / 20.1; 32 of 2880 x 2880, 16 pairs 27.7 / 33.5, 32 44.9 / 39.7; 8 of 1792 x 4096, 16 pairs 16.9 / 25.2.
-static bool f8_few_pairs(size_t pairs, size_t groups) { return pairs <= 24 && groups >= pairs / 2; }
+// A few pairs: a launch that looks the groups up itself.  In us, so / by tiles, a token's pairs over different groups: 128 groups of 768 x 2048, 16 pairs 8.0 /
+// 16.5, 32 14.5 / 16.9, 48 19.6 / 20.3, 64 24.2 / 23.0; 32 of 2880 x 2880, 16 pairs 25.0 / 33.2, 32 40.1 / 39.8, 48 53.4 / 49.8; 8 of 1792 x 4096, 16 15.0 / 26.0.
+static bool f8_few_pairs(size_t pairs, size_t groups) { return pairs <= 32 && groups >= pairs / 2; }
 // Of an expert layer: each slot by itself, its row quantized by the workgroups that read it.  The layer in us, so / bucketed: 32 experts of 2880 x 2880, 4
-// slots 26 / 65, 16 77 / 91, 24 108 / 106, 32 140 / 114; 128 of 768 x 2048, 8 slots 20 / 45, 24 39 / 48, 48 66 / 62; 8 of 1792 x 4096, 8 slots 38 / 69.
+// slots 25 / 65, 16 77 / 95, 24 108 / 99, 32 140 / 106; 128 of 768 x 2048, 8 slots 20 / 45, 24 39 / 49, 32 48 / 51, 48 66 / 58; 8 of 1792 x 4096, 8 slots 37 / 70.
 bool f8_slots_fit(size_t cols) { return f8_blocks(cols) * F8_BLOCK * 2 <= F8_FUSED_LDS - 8 * 1024; }  // (8 KB more of sums)
-bool f8_few_slots(size_t slots, size_t experts, size_t hidden, size_t ffn) { return f8_few_pairs(slots, experts) && f8_slots_fit(std::max(hidden, ffn)); }
+bool f8_few_slots(size_t slots, size_t experts, size_t hidden, size_t ffn) { return slots <= 24 && f8_few_pairs(slots, experts) && f8_slots_fit(std::max(hidden, ffn)); }
 int launch_f8_slots(const frk_weights *w, const frk_weights *up, const int32_t *ids, size_t slots, int slots_a_row, const float *x, float *y, hipStream_t s) {
     F8Rows g{};
     g.w = f8_mat(w);
