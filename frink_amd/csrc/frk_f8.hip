@@ -133,7 +133,7 @@ int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols
 //          group's next sixteen (four), the others end at once.  No list is made in front of it: each wavefront looks the group up itself
 //   SLOTS  strip blockIdx.x, (token, slot) blockIdx.y of an expert layer: the matrix is the slot's expert (FUSED only).  With `up` the strip of
 //          both stacks, and y = silu(gate) * up
-// FUSED: up to F8_FUSED tokens are quantized by the workgroup itself (a wavefront its own columns', while its first codes
+// FUSED: a few tokens (PAIRS: F8_FUSED) are quantized by the workgroup itself (a wavefront its own columns', while its first codes
 // are on their way), not by a launch in front. ----
 enum { F8_DENSE = 0, F8_PAIRS = 1, F8_SLOTS = 2, F8_SLOTS_GLU = 3 };
 struct F8Rows {
@@ -382,7 +382,14 @@ static int go_f8_rows(const F8Rows &g, const dim3 &grid, size_t lds, hipStream_t
 }
 
 constexpr size_t F8_ROWS_TOKENS = 64;  // most of the rows kernel
-static bool f8_fused(size_t tokens, size_t cols) { return tokens <= F8_FUSED && tokens * f8_blocks(cols) * F8_BLOCK * 2 <= F8_FUSED_LDS; }
+static bool f8_fused_fits(size_t tokens, size_t cols) { return tokens * f8_blocks(cols) * F8_BLOCK * 2 <= F8_FUSED_LDS; }
+// Of a dense batch: up to four tokens; up to eight where the strips are one round of the chip and a token's quantization, which every workgroup
+// does, is short.  In us, so / with a launch for it (rows x columns): 4096 x 4096 one token 5.6 / 8.7, four 7.6 / 9.1, six 9.0 / 9.2; 2880 x 2880 four 6.6 / 8.4, six
+// 8.0 / 8.6, eight 9.2 / 8.8; 768 x 2048 eight 6.8 / 7.9, twelve 8.5 / 8.2; 14336 x 4096 (3.5 rounds) one 11.5 / 15.9, four 15.8 / 16.2, six 20.8 / 16.3.
+static bool f8_fused(size_t tokens, const frk_weights *w, const F8Mat &m) {
+    if (!f8_fused_fits(tokens, w->cols)) return false;
+    return tokens <= F8_FUSED || (tokens <= 2 * F8_FUSED && (size_t)m.strips * w->matrices <= 256 && tokens * w->cols <= 20480);
+}
 
 // By estimated time.  Both kernels are a chain of steps a wavefront until the chip is full: a block of 128 columns takes a tile's wavefronts
 // as long alone on a CU as beside the CU's other workgroups, up to how many fit; a strip of the rows kernel likewise.  Shares of the
@@ -391,7 +398,7 @@ static bool f8_fused(size_t tokens, size_t cols) { return tokens <= F8_FUSED && 
 // against 26.1) and 384 of 4096 x 4096 (32.2 against 28.8).
 F8Plan f8_plan(const frk_weights *w, size_t batch) {
     const F8Mat m = f8_mat(w);
-    F8Plan best{-1, 1, f8_fused(batch, w->cols), 0, 0};
+    F8Plan best{-1, 1, f8_fused(batch, w, m), 0, 0};
     if (best.fused) return best;
     best.acts_bytes = f8_acts_bytes(batch, w->cols);
     if (batch <= 16) return best;  // (the tiles hold 32 tokens and more)
@@ -557,7 +564,7 @@ int launch_f8_tiles(const frk_weights *w, const F8Acts &acts, int shape, const i
 int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
                       float *y, void *ws, hipStream_t s) {
     const F8Acts acts = f8_acts_carve(ws, x_rows);
-    const bool few = f8_few_pairs(pairs, w->matrices), fused = few && f8_fused(F8_FUSED, w->cols);
+    const bool few = f8_few_pairs(pairs, w->matrices), fused = few && f8_fused_fits(F8_FUSED, w->cols);
     if (few && !fused) {
         int rc = launch_f8_quantize(x, nullptr, x_rows, w->cols, nullptr, acts, s);
         if (rc) return rc;

@@ -24,7 +24,8 @@ def _activations(rng, rows, cols):
 
 SHAPES = [(1, 1, 1), (15, 127, 2), (16, 128, 1), (17, 129, 3), (129, 255, 16), (128, 640, 17), (300, 1000, 33), (64, 96, 64),
           (257, 2880, 65), (1000, 513, 130), (144, 14336, 5), (576, 2304, 9), (33, 1156, 200), (272, 384, 257), (512, 1152, 300),
-          (31, 4100, 1), (768, 2048, 31), (2880, 160, 97), (40, 28672, 1), (33, 32768, 1), (20, 7168, 4), (20, 7300, 4)]
+          (31, 4100, 1), (768, 2048, 31), (2880, 160, 97), (40, 28672, 1), (33, 32768, 1), (20, 7168, 4), (20, 7300, 4),
+          (100, 2500, 8), (4096, 130, 7), (4112, 130, 7), (50, 4096, 5), (50, 4100, 5), (60, 96, 9)]
 
 
 @pytest.mark.gpu
@@ -43,7 +44,7 @@ def test_product_against_64_bits(fa, rows, cols, batch):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("batch", [1, 3, 16, 40, 70, 300])
+@pytest.mark.parametrize("batch", [1, 3, 7, 16, 40, 70, 300])
 def test_activations_are_rounded_once_to_the_nearest(fa, batch):
     """A weight row that picks one column returns that activation as quantized, bit for bit: halves between codes, the
     largest value just at and above 448 times a power of two, subnormal codes, the smallest and largest floats."""
