@@ -207,7 +207,9 @@ int frk_hip_launch_dense_ffn_swiglu(const frk_matvec_launch *gate, const frk_mat
  * capturing it (a call that would need to grow returns FRK_ERR_HIP and launches nothing) -- and a
  * buffer that was current during a capture belongs to that graph from then on: a later, larger call
  * on the stream gets a new buffer and the old one stays allocated and untouched until the process
- * ends, so replays of the graph stay valid (at the price of that memory).  One exception: a K-quant batch
+ * ends, so replays of the graph stay valid (at the price of that memory).  Graphs captured from one stream, and
+ * its calls of the same and smaller shapes, share the buffer: replays are ordered behind each other and behind those calls
+ * (on that stream, or by events).  One exception: a K-quant batch
  * that frk_hip_gemm_q8k_dev takes and that runs on the matrix cores (see there) grows the buffer during a
  * capture too -- in frk_hip_gemm_q8k_dev and frk_hip_gemm_acts_dev whatever it holds, in frk_hip_gemm_dev
  * and frk_hip_gemm_pair_dev if it holds the batch's rows in Q8_K -- so that what a call returns
