@@ -434,10 +434,10 @@ F8Plan f8_plan(const frk_weights *w, size_t batch) {
     if (best.parts > 1) best.parts_bytes = best.parts * n * 4;
     return best;
 }
-int launch_f8_gemm(const frk_weights *w, const F8Plan &plan, const float *x, size_t batch, float *y, void *ws, void *parts, hipStream_t s) {
+int launch_f8_gemm(const frk_weights *w, const F8Plan &plan, const float *x, size_t batch, float *y, void *ws, bool quantized, void *parts, hipStream_t s) {
     const F8Mat m = f8_mat(w);
     const F8Acts acts = f8_acts_carve(ws, batch, plan.shape < 0);
-    if (!plan.fused) {
+    if (!plan.fused && !quantized) {
         int rc = launch_f8_quantize(x, nullptr, batch, w->cols, nullptr, acts, s);
         if (rc) return rc;
     }

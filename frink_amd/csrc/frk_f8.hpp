@@ -208,7 +208,8 @@ F8Plan f8_plan(const frk_weights *w, size_t batch);
 // ---- entry points for the runtime and the expert layers ----
 Layout f8_layout(size_t rows, size_t cols, size_t matrices, size_t *bytes);
 int launch_f8_repack(const uint8_t *src, const float *scales, const frk_weights *w, hipStream_t s);
-int launch_f8_gemm(const frk_weights *w, const F8Plan &plan, const float *x, size_t batch, float *y, void *ws, void *parts, hipStream_t s);
+// `quantized`: ws holds the batch from a call before, of a plan with the same layout (both of the rows kernel or both over tiles)
+int launch_f8_gemm(const frk_weights *w, const F8Plan &plan, const float *x, size_t batch, float *y, void *ws, bool quantized, void *parts, hipStream_t s);
 size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs);
 int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
                       float *y, void *ws, hipStream_t s);

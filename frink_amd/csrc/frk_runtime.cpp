@@ -645,7 +645,23 @@ static int gemm_f8(const frk_weights *w, const float *x, size_t batch, float *y,
     int rc = f8_on_current_device(w);
     if (!rc && plan.acts_bytes) rc = scratch.get(plan.acts_bytes, plan.parts_bytes, s, &ws, &parts);
     if (rc) return rc;
-    return launch_f8_gemm(w, plan, x, batch, y, ws, parts, s);
+    return launch_f8_gemm(w, plan, x, batch, y, ws, false, parts, s);
+}
+// both over one quantization, where their plans read the same layout: 16 tokens of 14336 x 4096 twice 39.0 -> 35.8 us, 512 120 -> 116
+static int gemm_f8_pair(const frk_weights *w0, const frk_weights *w1, const float *x, size_t batch, float *y0, float *y1, hipStream_t s, Scratch &scratch) {
+    if (batch > (size_t)1 << 30) return set_error(FRK_ERR_SHAPE, "a batch of %zu rows is too large", batch);
+    const F8Plan plan0 = f8_plan(w0, batch), plan1 = f8_plan(w1, batch);
+    if (plan0.fused || plan1.fused || (plan0.shape < 0) != (plan1.shape < 0)) {
+        int rc = gemm_f8(w0, x, batch, y0, s, scratch);
+        return rc ? rc : gemm_f8(w1, x, batch, y1, s, scratch);
+    }
+    void *ws = nullptr, *parts = nullptr;
+    int rc = f8_on_current_device(w0);
+    if (!rc) rc = f8_on_current_device(w1);
+    if (!rc) rc = scratch.get(plan0.acts_bytes, std::max(plan0.parts_bytes, plan1.parts_bytes), s, &ws, &parts);
+    if (!rc) rc = launch_f8_gemm(w0, plan0, x, batch, y0, ws, false, parts, s);
+    if (!rc) rc = launch_f8_gemm(w1, plan1, x, batch, y1, ws, true, parts, s);  // (its parts behind the first one's sum)
+    return rc;
 }
 
 static int gemv_impl(const frk_weights *w, const float *x, float *y, int act_mode, hipStream_t s, Scratch &scratch) {
@@ -1120,6 +1136,7 @@ int frk_hip_gemm_pair_dev(const frk_weights *w0, const frk_weights *w1, const fl
         return set_error(FRK_ERR_SHAPE, "the matrices have %zu and %zu columns: they share one batch of activations", w0->cols, w1->cols);
     hipStream_t s = (hipStream_t)stream;
     Scratch scratch;
+    if (is_f8_kind(w0->kind) && is_f8_kind(w1->kind)) return gemm_f8_pair(w0, w1, x, batch, y0, y1, s, scratch);
     if (takes_tiles(w0, batch) && takes_tiles(w1, batch)) {
         // one quantization into the tiled form, then the two GEMMs (each with its own room for a split's parts)
         const size_t acts_bytes = round_up(q8k_tiled_bytes(batch, w0->cols), 256);

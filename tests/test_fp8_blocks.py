@@ -25,7 +25,7 @@ def _activations(rng, rows, cols):
 SHAPES = [(1, 1, 1), (15, 127, 2), (16, 128, 1), (17, 129, 3), (129, 255, 16), (128, 640, 17), (300, 1000, 33), (64, 96, 64),
           (257, 2880, 65), (1000, 513, 130), (144, 14336, 5), (576, 2304, 9), (33, 1156, 200), (272, 384, 257), (512, 1152, 300),
           (31, 4100, 1), (768, 2048, 31), (2880, 160, 97), (40, 28672, 1), (33, 32768, 1), (20, 7168, 4), (20, 7300, 4),
-          (100, 2500, 8), (4096, 130, 7), (4112, 130, 7), (50, 4096, 5), (50, 4100, 5), (60, 96, 9)]
+          (100, 2500, 8), (4096, 130, 7), (4112, 130, 7), (50, 4096, 5), (50, 4100, 5), (60, 96, 9), (17, 70000, 3), (9, 66000, 20), (9, 132000, 1)]
 
 
 @pytest.mark.gpu
@@ -178,7 +178,7 @@ def _groups(rng, counts):
     (1, 1, [1], 1), (17, 129, [0, 3, 0, 1], 4), (130, 300, [16, 17, 1, 64, 65, 0, 130], 50), (64, 256, [1] * 40, 8),
     (768, 2048, [1, 0] * 8, 1), (200, 512, [300, 5], 77), (48, 96, [0] * 1000 + [2] + [0] * 23, 2), (2880, 160, [3, 90, 33], 126),
     (144, 640, [0, 0, 700], 700), (36, 260, [2, 1, 5, 0, 8] * 30, 19),
-    (24, 7168, [4, 1, 0, 5], 6), (24, 7296, [4, 1, 0, 17], 6), (270, 160, [24, 23, 25], 72), (270, 160, [24, 23, 24], 71),
+    (24, 7168, [4, 1, 0, 5], 6), (5, 66000, [2, 0, 1], 3), (24, 7296, [4, 1, 0, 17], 6), (270, 160, [24, 23, 25], 72), (270, 160, [24, 23, 24], 71),
 ])
 def test_grouped_against_64_bits(fa, rows, cols, counts, x_rows):
     print("fp8 grouped", rows, cols, len(counts), x_rows, flush=True)
@@ -452,6 +452,33 @@ def test_a_layer_of_one_expert_is_the_ffn(fa, hidden, ffn):
     y = fa.moe_ffn(gate, up, down, 1, x, torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.ones((1, 1), device="cuda"))
     want = fa.ffn_swiglu(gate, up, down, x[0])
     assert torch.equal(y[0], want)  # the same sums in the same order
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [((512, 300), 1024), ((4096, 64), 640), ((40, 9000), 300), ((2880, 2880), 2880)])
+def test_a_pair_is_its_matrices(fa, rows, cols):
+    """Pairs of one quantization and of two, whichever kernels their plans name; captured and replayed."""
+    import torch
+    rng = np.random.default_rng(cols)
+    w0, w1 = (_resident(fa, *plain.random_matrix(rng, r, cols)) for r in rows)
+    for batch in (1, 4, 6, 8, 16, 17, 40, 64, 65, 130, 300):
+        x = to_dev(_activations(rng, batch, cols))
+        want = w0.gemm(x), w1.gemm(x)
+        got = fa.gemm_pair(w0, w1, x)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), batch
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        fa.gemm_pair(w0, w1, x, outs=got)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        fa.gemm_pair(w0, w1, x, outs=got)
+    for _ in range(3):
+        x.copy_(to_dev(_activations(rng, batch, cols)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], w0.gemm(x)) and torch.equal(got[1], w1.gemm(x))
 
 
 @pytest.mark.gpu
