@@ -1356,7 +1356,13 @@ int frk_hip_gemv_multi_dev(const frk_weights *const *ws, size_t n, const float *
         }
         return FRK_OK;
     }
-    // otherwise one Q8_K quantization for every K-quant matrix of the group
+    // Otherwise one Q8_K quantization for every K-quant matrix of the group, in the stream's scratch memory until the last of them.
+    // FP8_BLOCK rows too long to be quantized by their product's launch go through the same memory: they come first.
+    for (size_t i = 0; i < n; i++) {
+        if (!is_f8_kind(ws[i]->kind)) continue;
+        int rc = frk_hip_gemv_dev(ws[i], x, ys[i], FRK_ACT_F32, stream);
+        if (rc) return rc;
+    }
     Q8KActs a = {nullptr, nullptr, nullptr};
     Scratch scratch;
     if (any_k) {
@@ -1365,7 +1371,8 @@ int frk_hip_gemv_multi_dev(const frk_weights *const *ws, size_t n, const float *
     }
     for (size_t i = 0; i < n; i++) {
         int rc;
-        if (ws[i]->kind == FRK_KIND_Q8_0 || ws[i]->kind == FRK_KIND_Q4_0 || is_unit_kind(ws[i]->kind) || is_f8_kind(ws[i]->kind))
+        if (is_f8_kind(ws[i]->kind)) continue;
+        if (ws[i]->kind == FRK_KIND_Q8_0 || ws[i]->kind == FRK_KIND_Q4_0 || is_unit_kind(ws[i]->kind))
             rc = frk_hip_gemv_dev(ws[i], x, ys[i], FRK_ACT_F32, stream);  // (these kinds multiply the f32 activation itself)
         else rc = frk_hip_gemv_q8k_dev(ws[i], a.q, a.d, a.bsums, ys[i], stream);
         if (rc) return rc;

@@ -14,6 +14,9 @@
 struct HipStub {
     std::map<const void *, std::string> names;  // of the kernels' host handles
     std::vector<std::string> launched;
+    std::vector<std::pair<dim3, dim3>> shapes;  // of all launches: grid, workgroup
+    std::pair<dim3, dim3> next;
+    int device = 0;          // the current one
     bool capturing = false;  // what hipStreamIsCapturing says
     static HipStub &get() {
         static HipStub stub;
@@ -28,8 +31,10 @@ struct HipStub {
     }
 };
 extern "C" {
-hipError_t __hipPushCallConfiguration(dim3, dim3, size_t, hipStream_t) { return hipSuccess; }
-hipError_t __hipPopCallConfiguration(dim3 *g, dim3 *b, size_t *lds, hipStream_t *s) { return *g = *b = dim3(1), *lds = 0, *s = nullptr, hipSuccess; }
+hipError_t __hipPushCallConfiguration(dim3 g, dim3 b, size_t, hipStream_t) { return HipStub::get().next = {g, b}, hipSuccess; }
+hipError_t __hipPopCallConfiguration(dim3 *g, dim3 *b, size_t *lds, hipStream_t *s) {
+    return *g = HipStub::get().next.first, *b = HipStub::get().next.second, *lds = 0, *s = nullptr, hipSuccess;
+}
 void **__hipRegisterFatBinary(const void *) { static void *handle; return &handle; }
 void __hipRegisterVar(void **, void *, char *, char *, int, size_t, int, int) {}
 void __hipUnregisterFatBinary(void **) {}
@@ -47,7 +52,10 @@ void __hipRegisterFunction(void **, const void *host, char *, const char *mangle
     }
     HipStub::get().names[host] = out;
 }
-hipError_t hipLaunchKernel(const void *f, dim3, dim3, void **, size_t, hipStream_t) { return HipStub::get().launched.push_back(HipStub::get().names[f]), hipSuccess; }
+hipError_t hipLaunchKernel(const void *f, dim3 grid, dim3 group, void **, size_t, hipStream_t) {
+    HipStub::get().launched.push_back(HipStub::get().names[f]);
+    return HipStub::get().shapes.emplace_back(grid, group), hipSuccess;
+}
 hipError_t hipMalloc(void **p, size_t n) { return (*p = calloc(1, n)) ? hipSuccess : hipErrorOutOfMemory; }
 hipError_t hipHostMalloc(void **p, size_t n, unsigned) { return hipMalloc(p, n); }
 hipError_t hipFree(void *p) { return free(p), hipSuccess; }
@@ -55,7 +63,7 @@ hipError_t hipMemcpy(void *to, const void *from, size_t n, hipMemcpyKind) { retu
 hipError_t hipMemcpyAsync(void *to, const void *from, size_t n, hipMemcpyKind, hipStream_t) { return memcpy(to, from, n), hipSuccess; }
 hipError_t hipMemsetAsync(void *to, int v, size_t n, hipStream_t) { return memset(to, v, n), hipSuccess; }
 hipError_t hipMemGetInfo(size_t *f, size_t *t) { return *f = *t = (size_t)288 << 30, hipSuccess; }
-hipError_t hipGetDevice(int *dev) { return *dev = 0, hipSuccess; }
+hipError_t hipGetDevice(int *dev) { return *dev = HipStub::get().device, hipSuccess; }
 hipError_t hipGetDeviceCount(int *n) { return *n = 1, hipSuccess; }
 hipError_t hipDeviceGetAttribute(int *v, hipDeviceAttribute_t, int) { return *v = 256, hipSuccess; }
 hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600 *p, int) {

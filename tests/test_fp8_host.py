@@ -1,0 +1,69 @@
+"""What calls over weights in 8-bit floating point launch and refuse, on the CPU (host_library.py)."""
+import pytest
+
+import host_library
+import oracle as fo
+
+FP8 = 256
+PROGRAM = r"""
+#include <cstdio>
+#include "frink_amd/csrc/frk_f8.hpp"
+#include "include/frink_hip.h"
+static float room[64];  // (addresses only: nothing runs)
+static void fill(frk_weights &w, int kind, size_t rows, size_t cols, size_t matrices = 1) {
+    w.kind = kind, w.rows = rows, w.cols = cols, w.matrices = matrices, w.dev = (uint8_t *)room;
+    if (kind == FRK_KIND_FP8_BLOCK) w.layout = frk::f8_layout(rows, cols, matrices, &w.dev_bytes);
+    else w.layout = frk::layout_for(kind, cols);
+}
+static void tell(int rc) {
+    printf("%d %s | %s\n", rc, HipStub::get().take().c_str(), frk_hip_last_error());
+}
+int main() {  // a call a line; its status, the kernels it launched and its error
+    char call[32];
+    while (scanf("%31s", call) == 1) {
+        const std::string name = call;
+        if (name == "multi" || name == "ffn") {  // columns, number, kinds
+            size_t cols, n;
+            if (scanf("%zu %zu", &cols, &n) != 2) return 1;
+            std::vector<frk_weights> w(n);
+            std::vector<const frk_weights *> ws(n);
+            std::vector<float *> ys(n, room);
+            for (size_t i = 0; i < n; i++) {
+                int kind;
+                if (scanf("%d", &kind) != 1) return 1;
+                fill(w[i], kind, i < 2 ? 64 : 32, name == "ffn" && i == 2 ? 64 : cols), ws[i] = &w[i];
+            }
+            tell(name == "ffn" ? frk_hip_ffn_swiglu_dev(ws[0], ws[1], ws[2], room, room, nullptr) : frk_hip_gemv_multi_dev(ws.data(), n, room, ys.data(), nullptr));
+        } else {
+            return 1;
+        }
+    }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def said(tmp_path_factory):
+    binary = host_library.build(tmp_path_factory.mktemp("fp8"), PROGRAM)
+
+    def of(*calls):
+        lines = host_library.run(binary, "".join(c + "\n" for c in calls)).splitlines()
+        assert len(lines) == len(calls)
+        split = [(line.split(None, 1)[0], line.split(None, 1)[1].split(" | ") + [""]) for line in lines]
+        return [(int(rc), names.split(), error) for rc, (names, error, *_) in split]
+
+    return of
+
+
+@pytest.mark.parametrize("cols", [28672, 32768])
+def test_quantized_rows_of_one_kind_stay_until_their_products(said, cols):
+    """Scratch memory that holds Q8_K activations for several products is not written in between."""
+    kinds = [[FP8, fo.Q4_K], [fo.Q4_K, FP8, fo.Q6_K], [FP8, fo.Q5_K, fo.Q4_K, FP8], [fo.Q6_K, fo.Q4_K, FP8]]
+    calls = ["multi %d %d %s" % (cols, len(k), " ".join(map(str, k))) for k in kinds]
+    calls += ["ffn %d 3 %d %d %d" % (cols, a, b, FP8) for a, b in ((FP8, fo.Q4_K), (fo.Q4_K, FP8))]
+    for call, (rc, names, error) in zip(calls, said(*calls)):
+        assert rc == 0, error
+        first = [i for i, n in enumerate(names) if n.startswith("quantize_q8_k")]
+        last = max(i for i, n in enumerate(names) if n.startswith("gemv"))
+        assert len(first) == 1 and first[0] < last, names
+        assert not [n for n in names[first[0]:last] if n.startswith("f8_quantize")], (call, names)
