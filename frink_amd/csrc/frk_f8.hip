@@ -356,7 +356,7 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
             const float4 o = sums[k][i][lane];
             v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
         }
-        return v;
+        return make_float4(v.x * F8_UP, v.y * F8_UP, v.z * F8_UP, v.w * F8_UP);
     };
     float4 v = total(t);
     if (NM == 2) {

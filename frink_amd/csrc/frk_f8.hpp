@@ -5,12 +5,13 @@
 // W: OCP E4M3 codes, S: an f32 scale for every 128 rows x 128 columns of a matrix, q and e: the activations, quantized here
 // block by block.  e is the least exponent, -100 or more, with amax <= 448 * 2^e, so x * 2^-e is exact and q is x rounded
 // ONCE, to the nearest E4M3 (halves to even): an f32 scale amax / 448 would round the quotient first, and the two roundings
-// together miss the nearest value now and then.  A power of two costs no accuracy where E4M3 is normal.  (From -100 on q * 2^e
-// is a normal bf16 number, all of its four bits kept; below, 448 * 2^-100 = 3.5e-28, a block's values go towards zero.)
+// together miss the nearest value now and then.  A power of two costs no accuracy where E4M3 is normal.  (Below 448 * 2^-100 =
+// 3.5e-28 a block's values go towards zero.)
 // Infinities and NaN take no part in amax and become E4M3's NaN.
 //
-// The products run on the bf16 matrix cores: a code and q * 2^e are bf16 numbers, and their sums come out as f32 sums do.  The
-// 8-bit ones, twice as fast, add every eight products within 14 bits of the largest (measured on v_mfma_f32_16x16x32_fp8_fp8
+// The products run on the bf16 matrix cores: a code and q * 2^(e - 16) are bf16 numbers (normal ones: q * 2^e is 2^-109 or more), and their
+// sums come out as f32 sums do.  With the 16 no block's sum overflows before it meets its scale: 128 * 448 times the largest
+// activation, 240 * 2^120, is 2^142.8.  All sums are of 2^-16 of their value; the last one is multiplied back, exactly from 2^-126 on.  The 8-bit ones, twice as fast, add every eight products within 14 bits of the largest (measured on v_mfma_f32_16x16x32_fp8_fp8
 // and v_mfma_scale_f32_16x16x128_f8f6f4 alike: a product 2^-14 of its neighbour is lost, from the ninth on 2^-23 counts):
 // against 64-bit sums of 128 products of normal values 1.5e-5 in the 2-norm, of codes drawn evenly 5.1e-5; bf16 9e-9, 8e-8.
 #pragma once
@@ -47,9 +48,11 @@ static inline F8Mat f8_mat(const frk_weights *w) {
     return m;
 }
 
-// Activations: q * 2^e as bf16, zeros past cols; [rows][blocks][128], or (`strips`) every sixteen rows a strip, a strip's blocks one after
+// Activations: q * 2^(e - F8_DOWN) as bf16, zeros past cols; [rows][blocks][128], or (`strips`) every sixteen rows a strip, a strip's blocks one after
 // the other, a block as [4 products][64 lanes][8], lane l row l % 16, product k columns 32 (l / 16) + 8 k .. + 7: a wavefront's
 // load of a product's operand is then 1 KB in one piece (rows past the last hold whatever the memory did).
+constexpr int F8_DOWN = 16;
+constexpr float F8_UP = 65536.0f;  // what a result is multiplied by
 struct F8Acts {
     uint16_t *v;
     int rows;
@@ -76,7 +79,7 @@ __device__ __forceinline__ uint32_t f8_half_max(uint32_t v) {  // over 32 lanes
 #endif
     return v;
 }
-// the four values' codes; `scale` = 2^e of the block
+// the four values' codes; `scale` = 2^(e - F8_DOWN) of the block
 __device__ __forceinline__ uint32_t f8_quantize4(const float (&v)[4], float &scale) {
     // magnitudes compare as their bits
     uint32_t top = 0;
@@ -99,7 +102,7 @@ __device__ __forceinline__ uint32_t f8_quantize4(const float (&v)[4], float &sca
     // 448 = 1.75 * 2^8: e is the exponent less 8, one more where the mantissa is above 1.75
     const int b = (int)((top + 0x1fffffu) >> 23) - 8;
     const uint32_t biased = (uint32_t)max(b, 127 - 100);
-    scale = __uint_as_float(biased << 23);
+    scale = __uint_as_float((biased - F8_DOWN) << 23);
     const float up = __uint_as_float((254u - biased) << 23);  // 2^-e
     float z[4];
 #pragma unroll

@@ -216,12 +216,14 @@ __global__ __launch_bounds__(64 * RW * TW, 2) void f8_tile_kernel(F8Gemm g, int 
 #pragma unroll
         for (int i = 0; i < MR; i++) {
             const int r0 = (strip0 + i) * F8_STRIP + 4 * lg;
+            const float4 v = make_float4(acc[i][j][0] * F8_UP, acc[i][j][1] * F8_UP, acc[i][j][2] * F8_UP, acc[i][j][3] * F8_UP);
             if (wide) {
-                if (r0 < g.w.rows) *reinterpret_cast<float4 *>(dst + r0) = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+                if (r0 < g.w.rows) *reinterpret_cast<float4 *>(dst + r0) = v;
             } else {
+                const float out[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    if (r0 + r < g.w.rows) dst[r0 + r] = acc[i][j][r];
+                    if (r0 + r < g.w.rows) dst[r0 + r] = out[r];
             }
         }
     }

@@ -38,3 +38,61 @@ def test_several_kinds_over_one_activation(fa, cols):
         for _ in range(2):
             got = fa.ffn_swiglu(gate, up, down, x).cpu().numpy()
             assert (np.abs(got - d @ act) <= room).all()
+
+
+def _ends(rng, end, matrices, rows, cols, batch):
+    """Codes, scales and activations whose products are f32's largest (the results far below) or smallest (far above)."""
+    sign = rng.integers(0, 2, (matrices, rows, cols), dtype=np.uint8) << 7
+    blocks = (matrices, -(-rows // 128), -(-cols // 128))
+    if end == "largest":
+        codes, scales = sign | np.uint8(0x7e), np.full(blocks, 2.0 ** -30, np.float32)
+        x = rng.uniform(0.5, 1.0, (batch, cols)) * np.finfo(np.float32).max
+    else:
+        codes, scales = sign | rng.integers(0, 4, sign.shape, dtype=np.uint8), np.full(blocks, 2.0 ** 100, np.float32)
+        x = rng.integers(0, 20, (batch, cols)) * 2.0 ** -109
+    x *= rng.choice([-1, 1], x.shape)
+    x[batch // 2] = np.abs(x[batch // 2])
+    return codes, scales, x.astype(np.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("end", ["largest", "smallest"])
+@pytest.mark.parametrize("batch", [1, 4, 16, 30, 64, 100, 300])
+def test_products_at_the_ends_of_the_range(fa, end, batch):
+    """Sums of codes times activations that f32 does not hold, or holds as subnormal numbers only, under scales that bring them back."""
+    print("fp8 range", end, batch, flush=True)
+    rng = np.random.default_rng(batch)
+    codes, scales, x = _ends(rng, end, 2, 140, 1300, batch)
+    for m in range(2):  # one sign: the sums reach the end
+        codes[m, ::5] &= 0x7f
+    want, room = np.empty((batch, 280)), np.empty((batch, 280))
+    for m in range(2):
+        want[:, 140 * m:140 * (m + 1)], room[:, 140 * m:140 * (m + 1)] = plain.product(codes[m], scales[m], x)
+    w = _resident(fa, codes, scales)
+    got = w.gemm(to_dev(x)).cpu().numpy()
+    assert (np.abs(got - want) <= room).all()
+    off = np.array([0, batch // 3, batch], np.int32)
+    got = fa.gemm_grouped(w, 2, to_dev(off), to_dev(x)).cpu().numpy()
+    for m in range(2):
+        s, r = slice(off[m], off[m + 1]), slice(140 * m, 140 * (m + 1))
+        assert (np.abs(got[s] - want[s, r]) <= room[s, r]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 60])
+def test_expert_layer_over_the_largest_activations(fa, batch):
+    from test_fp8_blocks import _plain_layer
+    rng = np.random.default_rng(batch)
+    experts, hidden, ffn = 4, 260, 200
+    codes, _, x = _ends(rng, "largest", 2 * experts, ffn, hidden, batch)
+    scales = np.full((2 * experts, 2, 3), 2.0 ** -132, np.float32)
+    parts = [(codes[:experts], scales[:experts]), (codes[experts:], scales[experts:]), plain.random_matrix(rng, hidden, ffn, matrices=experts)]
+    gate, up, down = (_resident(fa, *p) for p in parts)
+    ids = rng.integers(0, experts, (batch, 2)).astype(np.int32)
+    weights = rng.uniform(0.2, 1, (batch, 2)).astype(np.float32)
+    got = fa.moe_ffn(gate, up, down, experts, to_dev(x), to_dev(ids), to_dev(weights)).cpu().numpy()
+    want, room = _plain_layer(parts, x, ids, weights)
+    assert (np.abs(got - want) <= room * 1.01).all()
+    y = fa.ffn_swiglu(_resident(fa, codes[:1], scales[:1]), _resident(fa, codes[4:5], scales[:1]), _resident(fa, *(p[:1] for p in parts[2])), to_dev(x[0]))
+    want, room = _plain_layer([(codes[:1], scales[:1]), (codes[4:5], scales[:1]), tuple(p[:1] for p in parts[2])], x[:1], [[0]], [[1.0]])
+    assert (np.abs(y.cpu().numpy() - want[0]) <= room[0] * 1.01).all()
