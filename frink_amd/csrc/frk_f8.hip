@@ -17,6 +17,14 @@ typedef float f8_v4f __attribute__((ext_vector_type(4)));
         if (e_ != hipSuccess) return set_error(FRK_ERR_HIP, what " launch: %s", hipGetErrorString(e_)); \
     } while (0)
 
+int f8_on_current_device(const frk_weights *w) {
+    int dev = -1;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipGetDevice: %s", hipGetErrorString(e));
+    if (dev != w->device) return set_error(FRK_ERR_ARG, "the matrix is on device %d, the current device is %d", w->device, dev);
+    return FRK_OK;
+}
+
 Layout f8_layout(size_t rows, size_t cols, size_t matrices, size_t *bytes) {
     const size_t m_rows = rows / matrices;
     Layout l;
@@ -95,6 +103,8 @@ __global__ __launch_bounds__(256) void f8_dequant_kernel(F8Mat w, size_t all_row
 }
 int launch_f8_dequant_rows(const frk_weights *w, const int32_t *ids, size_t n_out, float *out, hipStream_t s) {
     if (n_out == 0) return FRK_OK;
+    int rc = f8_on_current_device(w);
+    if (rc) return rc;
     const size_t n = n_out * w->cols;
     hipLaunchKernelGGL(f8_dequant_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, s, f8_mat(w), w->rows, ids,
                        n_out, (int)w->cols, out);

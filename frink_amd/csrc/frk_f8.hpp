@@ -11,8 +11,9 @@
 //
 // The products run on the bf16 matrix cores: a code and q * 2^(e - 16) are bf16 numbers (normal ones: q * 2^e is 2^-109 or more), and their
 // sums come out as f32 sums do.  With the 16 no block's sum overflows before it meets its scale: 128 * 448 times the largest
-// activation, 240 * 2^120, is 2^142.8.  All sums are of 2^-16 of their value; the last one is multiplied back, exactly from 2^-126 on.  The 8-bit ones, twice as fast, add every eight products within 14 bits of the largest (measured on v_mfma_f32_16x16x32_fp8_fp8
-// and v_mfma_scale_f32_16x16x128_f8f6f4 alike: a product 2^-14 of its neighbour is lost, from the ninth on 2^-23 counts):
+// activation, 240 * 2^120, is 2^143.7.  All sums are of 2^-16 of their value; the last one is multiplied back, exactly from 2^-126 on.
+// The 8-bit cores, twice as fast, add every eight products within 14 bits of the largest (measured on v_mfma_f32_16x16x32_fp8_fp8 and
+// v_mfma_scale_f32_16x16x128_f8f6f4 alike: a product 2^-14 of its neighbour is lost, from the ninth on 2^-23 counts):
 // against 64-bit sums of 128 products of normal values 1.5e-5 in the 2-norm, of codes drawn evenly 5.1e-5; bf16 9e-9, 8e-8.
 #pragma once
 
@@ -209,6 +210,7 @@ struct F8Plan {
 F8Plan f8_plan(const frk_weights *w, size_t batch);
 
 // ---- entry points for the runtime and the expert layers ----
+int f8_on_current_device(const frk_weights *w);  // a status: what every entry point refuses before it launches anything
 Layout f8_layout(size_t rows, size_t cols, size_t matrices, size_t *bytes);
 int launch_f8_repack(const uint8_t *src, const float *scales, const frk_weights *w, hipStream_t s);
 // `quantized`: ws holds the batch from a call before, of a plan with the same layout (both of the rows kernel or both over tiles)

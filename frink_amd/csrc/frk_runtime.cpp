@@ -37,6 +37,7 @@ struct DeviceState {
     bool probed = false;
     int device_count = 0;
     hipStream_t stream = nullptr;  // for host-buffer entry points
+    int stream_device = -1;        // its device
     // host staging for the host-buffer entry points
     void *x_dev = nullptr, *y_dev = nullptr;
     size_t x_bytes = 0, y_bytes = 0;
@@ -58,8 +59,17 @@ static int ensure_device_locked() {
     if (!g_dev.stream) {
         // default priority on purpose
         hipError_t e = hipStreamCreateWithFlags(&g_dev.stream, hipStreamNonBlocking);
+        if (e == hipSuccess) e = hipGetDevice(&g_dev.stream_device);
         if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipStreamCreateWithFlags: %s", hipGetErrorString(e));
     }
+    return FRK_OK;
+}
+// FP8_BLOCK: that stream's kernels read memory of its own device
+static int f8_on_stream_device() {
+    int dev = -1;
+    FRK_HIP_TRY(hipGetDevice(&dev));
+    if (dev != g_dev.stream_device)
+        return set_error(FRK_ERR_ARG, "host buffers go through device %d, the current device is %d", g_dev.stream_device, dev);
     return FRK_OK;
 }
 
@@ -418,6 +428,7 @@ int frk_hip_weights_register_fp8(const uint8_t *host_codes, const float *host_sc
     if (rc) return rc;
     std::lock_guard<std::mutex> lk(g_dev.mu);
     rc = ensure_device_locked();
+    if (!rc) rc = f8_on_stream_device();
     if (rc) return rc;
     const size_t codes = rows * cols, scales = matrices * f8_blocks(rows / matrices) * f8_blocks(cols) * sizeof(float), at = round_up(codes, 256);
     uint8_t *staging = nullptr;
@@ -632,12 +643,6 @@ static int gemv_units_int(const frk_weights *w, const float *x, float *y, hipStr
 }
 
 // FP8_BLOCK: a row is quantized alike in every batch; its sums' order, and so their last bits, is the plan's for the batch.
-static int f8_on_current_device(const frk_weights *w) {
-    int dev = -1;
-    FRK_HIP_TRY(hipGetDevice(&dev));
-    if (dev != w->device) return set_error(FRK_ERR_ARG, "the matrix is on device %d, the current device is %d", w->device, dev);
-    return FRK_OK;
-}
 static int gemm_f8(const frk_weights *w, const float *x, size_t batch, float *y, hipStream_t s, Scratch &scratch) {
     if (batch > (size_t)1 << 30) return set_error(FRK_ERR_SHAPE, "a batch of %zu rows is too large", batch);
     void *ws = nullptr, *parts = nullptr;
@@ -1710,6 +1715,8 @@ int frk_hip_get_rows(const frk_weights *w, const int32_t *ids, size_t n_ids, flo
     std::lock_guard<std::mutex> lk(g_launch_mu);
     const size_t ib = n_ids * sizeof(int32_t), ob = n_ids * w->cols * sizeof(float);
     int rc = stage_buffers(ib, ob);
+    if (!rc && is_f8_kind(w->kind)) rc = f8_on_stream_device();
+    if (!rc && is_f8_kind(w->kind)) rc = f8_on_current_device(w);
     if (!rc) rc = stage_in(ids, ib);
     if (!rc) rc = launch_dequant_rows(w, (const int32_t *)g_dev.x_dev, n_ids, (float *)g_dev.y_dev, g_dev.stream);
     const HostOut rows = {out, ob};

@@ -34,6 +34,34 @@ int main() {  // a call a line; its status, the kernels it launched and its erro
                 fill(w[i], kind, i < 2 ? 64 : 32, name == "ffn" && i == 2 ? 64 : cols), ws[i] = &w[i];
             }
             tell(name == "ffn" ? frk_hip_ffn_swiglu_dev(ws[0], ws[1], ws[2], room, room, nullptr) : frk_hip_gemv_multi_dev(ws.data(), n, room, ys.data(), nullptr));
+        } else if (name == "elsewhere") {  // a matrix of device 1, device 0 the current one: every entry point that takes it
+            static frk_weights w, q;
+            fill(w, FRK_KIND_FP8_BLOCK, 256, 256, 2), fill(q, FRK_KIND_Q4_K, 256, 256);
+            w.device = 1;
+            int32_t ids[4] = {0, 1, 0, 0};
+            float out[1024];
+            const frk_weights *const pair[2] = {&q, &w};
+            float *const ys[2] = {room, room};
+            frk_weights *fresh = nullptr;
+            tell(frk_hip_weights_register_fp8((const uint8_t *)out, out, 16, 16, 1, &fresh));
+            tell(frk_hip_gemv_dev(&w, room, room, FRK_ACT_F32, nullptr));
+            tell(frk_hip_gemm_dev(&w, room, 40, room, nullptr));
+            tell(frk_hip_gemm_noalloc_dev(&w, room, 40, room, nullptr));
+            tell(frk_hip_gemm_pair_dev(&w, &w, room, 40, room, room, nullptr));
+            tell(frk_hip_gemv_multi_dev(pair, 2, room, ys, nullptr));
+            tell(frk_hip_ffn_swiglu_dev(&w, &w, &w, room, room, nullptr));
+            tell(frk_hip_gemm_grouped_dev(&w, 2, ids, nullptr, room, 4, 4, room, nullptr));
+            static frk_weights e[3];
+            for (frk_weights &m : e) fill(m, FRK_KIND_FP8_BLOCK, 256, 128, 2);
+            e[2].device = 1;
+            tell(frk_hip_moe_ffn_dev(&e[0], &e[1], &e[2], 2, room, 2, ids, room, 1, room, nullptr));
+            tell(frk_hip_dequant_dev(&w, room, nullptr));
+            tell(frk_hip_get_rows_dev(&w, ids, 2, room, nullptr));
+            tell(frk_hip_get_rows(&w, ids, 2, out));
+            HipStub::get().device = 1;  // the host-buffer entry points' stream is device 0's
+            tell(frk_hip_get_rows(&w, ids, 2, out));
+            tell(frk_hip_weights_register_fp8((const uint8_t *)out, out, 16, 16, 1, &fresh));
+            HipStub::get().device = 0;
         } else {
             return 1;
         }
@@ -46,9 +74,9 @@ int main() {  // a call a line; its status, the kernels it launched and its erro
 def said(tmp_path_factory):
     binary = host_library.build(tmp_path_factory.mktemp("fp8"), PROGRAM)
 
-    def of(*calls):
-        lines = host_library.run(binary, "".join(c + "\n" for c in calls)).splitlines()
-        assert len(lines) == len(calls)
+    def of(*calls, lines=None):
+        count, lines = lines or len(calls), host_library.run(binary, "".join(c + "\n" for c in calls)).splitlines()
+        assert len(lines) == count
         split = [(line.split(None, 1)[0], line.split(None, 1)[1].split(" | ") + [""]) for line in lines]
         return [(int(rc), names.split(), error) for rc, (names, error, *_) in split]
 
@@ -67,3 +95,10 @@ def test_quantized_rows_of_one_kind_stay_until_their_products(said, cols):
         last = max(i for i, n in enumerate(names) if n.startswith("gemv"))
         assert len(first) == 1 and first[0] < last, names
         assert not [n for n in names[first[0]:last] if n.startswith("f8_quantize")], (call, names)
+
+
+def test_a_matrix_of_another_device_is_refused(said):
+    here, *elsewhere = said("elsewhere", lines=14)
+    assert here[0] == 0
+    for call, (rc, names, error) in enumerate(elsewhere):
+        assert rc == -4 and names == ["-"] and "device" in error, (call, rc, names, error)
