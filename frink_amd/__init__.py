@@ -170,17 +170,25 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _stream_at(x):
-    """_stream() for a call over x.  Kernels on the current device cannot read another's tensors: refused here."""
+def _stream_at(fp8, *tensors):
+    """_stream() for a call over tensors (or None).  fp8: with FP8_BLOCK weights, whose calls refuse tensors of another device than the
+    current one.  The other kinds' take a peer's memory as they always did."""
     import torch
     try:
         here = torch._C._cuda_getDevice()
         stream = torch._C._cuda_getCurrentRawStream(here)
     except AttributeError:
         here, stream = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
-    if x.get_device() != here:
-        raise ValueError("the tensor is on device %d, the current device is %d" % (x.get_device(), here))
+    for t in tensors:
+        if t is not None:
+            at = t.get_device()
+            if fp8 and at != here:
+                raise ValueError("the tensor is on device %d, the current device is %d" % (at, here))
     return stream
+
+
+def _any_fp8(*ws):
+    return any(w.kind == FP8_BLOCK for w in ws)
 
 
 def _np_ptr(a):
@@ -238,7 +246,7 @@ class Weights:
         cls._check_fp8(codes.numel(), scales.numel(), rows, cols, matrices)
         h = C.c_void_p()
         check(lib().frk_hip_weights_from_device_fp8(C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), rows, cols,
-                                                    matrices, _stream_at(codes), C.byref(h)))
+                                                    matrices, _stream_at(True, codes), C.byref(h)))
         return cls(h, FP8_BLOCK, rows, cols)
 
     def keep_decoded(self):
@@ -265,7 +273,7 @@ class Weights:
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.numel() == self.cols
         y = out if out is not None else torch.empty(self.rows, dtype=torch.float32, device=x.device)
         check(lib().frk_hip_gemv_dev(self.handle, C.c_void_p(x.data_ptr()), C.c_void_p(y.data_ptr()), act_mode,
-                                     _stream_at(x)))
+                                     _stream_at(self.kind == FP8_BLOCK, x)))
         return y
 
     def gemv_q8k(self, acts, out=None):
@@ -292,7 +300,7 @@ class Weights:
         batch = x.numel() // self.cols
         # (a small product waits for its call: like its input 0.3 us ahead of torch.empty)
         y = out if out is not None else x.new_empty((batch, self.rows))
-        check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), _stream_at(x)))
+        check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), _stream_at(self.kind == FP8_BLOCK, x)))
         return y
 
     def gemm_acts(self, acts, out=None):
@@ -309,7 +317,7 @@ class Weights:
         batch = x.numel() // self.cols
         assert out.dtype == torch.float32 and out.is_cuda and out.is_contiguous() and out.numel() == batch * self.rows
         check(lib().frk_hip_gemm_noalloc_dev(self.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(out.data_ptr()),
-                                             _stream_at(x)))
+                                             _stream_at(self.kind == FP8_BLOCK, x)))
         return out
 
     def dequant(self):
@@ -372,7 +380,7 @@ def gemm_pair(w0, w1, x, outs=None):
     batch = x.numel() // w0.cols
     y0, y1 = outs if outs is not None else (torch.empty((batch, w.rows), dtype=torch.float32, device=x.device) for w in (w0, w1))
     check(lib().frk_hip_gemm_pair_dev(w0.handle, w1.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(y0.data_ptr()),
-                                      C.c_void_p(y1.data_ptr()), _stream_at(x)))
+                                      C.c_void_p(y1.data_ptr()), _stream_at(_any_fp8(w0, w1), x)))
     return y0, y1
 
 
@@ -428,7 +436,7 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_b
         raise ValueError("score %r: one of %s" % (score, ", ".join(SCORES)))
     rule = RouteRule(SCORES[score], int(bool(norm)), groups, top_groups, group_best, scale, None if bias is None else bias.data_ptr())
     ids, w = logits.new_empty((batch, k), dtype=torch.int32), logits.new_empty((batch, k))
-    check(lib().frk_hip_route_dev(logits.data_ptr(), batch, n_experts, k, C.byref(rule), ids.data_ptr(), w.data_ptr(), _stream_at(logits)))
+    check(lib().frk_hip_route_dev(logits.data_ptr(), batch, n_experts, k, C.byref(rule), ids.data_ptr(), w.data_ptr(), _stream_at(True, logits)))
     return ids, w
 
 
@@ -441,7 +449,7 @@ def moe_ffn(gate, up, down, n_experts, x, ids, weights, out=None):
     batch, k = ids.shape
     y = out if out is not None else x.new_empty((batch, down.rows // n_experts))
     check(lib().frk_hip_moe_ffn_dev(gate.handle, up.handle, down.handle, n_experts, x.data_ptr(), batch, ids.data_ptr(), weights.data_ptr(), k,
-                                    y.data_ptr(), _stream_at(x)))
+                                    y.data_ptr(), _stream_at(_any_fp8(gate, up, down), x)))
     return y
 
 
@@ -459,7 +467,7 @@ def gemm_grouped(stacked, n_groups, group_off, x, gather=None, out=None):
         pairs = x_rows
     y = out if out is not None else x.new_empty((pairs, stacked.rows // n_groups))
     check(lib().frk_hip_gemm_grouped_dev(stacked.handle, n_groups, group_off.data_ptr(), gather.data_ptr() if gather is not None else None,
-                                         x.data_ptr(), x_rows, pairs, y.data_ptr(), _stream_at(x)))
+                                         x.data_ptr(), x_rows, pairs, y.data_ptr(), _stream_at(stacked.kind == FP8_BLOCK, x)))
     return y
 
 
@@ -489,7 +497,7 @@ def gemv_multi(ws, x, outs=None):
     ys = outs if outs is not None else [torch.empty(w.rows, dtype=torch.float32, device=x.device) for w in ws]
     hs = (C.c_void_p * n)(*[w.handle for w in ws])
     ps = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
-    check(lib().frk_hip_gemv_multi_dev(hs, n, C.c_void_p(x.data_ptr()), ps, _stream_at(x)))
+    check(lib().frk_hip_gemv_multi_dev(hs, n, C.c_void_p(x.data_ptr()), ps, _stream_at(_any_fp8(*ws), x)))
     return ys
 
 
@@ -498,7 +506,7 @@ def ffn_swiglu(gate, up, down, x, out=None):
     import torch
     y = out if out is not None else torch.empty(down.rows, dtype=torch.float32, device=x.device)
     check(lib().frk_hip_ffn_swiglu_dev(gate.handle, up.handle, down.handle, C.c_void_p(x.data_ptr()),
-                                       C.c_void_p(y.data_ptr()), _stream_at(x)))
+                                       C.c_void_p(y.data_ptr()), _stream_at(_any_fp8(gate, up, down), x)))
     return y
 
 

@@ -98,3 +98,33 @@ def test_expert_layer_over_the_largest_activations(fa, batch):
     y = fa.ffn_swiglu(_resident(fa, codes[:1], scales[:1]), _resident(fa, codes[4:5], scales[:1]), _resident(fa, *(p[:1] for p in parts[2])), to_dev(x[0]))
     want, room = _plain_layer([(codes[:1], scales[:1]), (codes[4:5], scales[:1]), tuple(p[:1] for p in parts[2])], x[:1], [[0]], [[1.0]])
     assert (np.abs(y.cpu().numpy() - want[0]) <= room[0] * 1.01).all()
+
+
+class _On:
+    """A tensor that says it is on a device `step` further on, which this machine need not have."""
+
+    def __init__(self, t, step=1):
+        self.t, self.step = t, step
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return self.t.get_device() + self.step
+
+
+@pytest.mark.gpu
+def test_the_other_kinds_take_a_peers_memory(fa):
+    """As they did before there were FP8_BLOCK matrices."""
+    import torch
+    n = 256
+    q = fa.Weights.from_host(fo.Q8_0, make_weights(fo.Q8_0, n, n, seed=1), n, n)
+    gate, down = (fa.Weights.from_host(fo.Q4_K, make_weights(fo.Q4_K, 2 * n, n, seed=s), 2 * n, n) for s in (2, 3))
+    rng = np.random.default_rng(3)
+    x = to_dev(rng.standard_normal((2, n)).astype(np.float32))
+    ids, weights = to_dev(np.array([[0], [1]], np.int32)), torch.ones((2, 1), device="cuda")
+    off = to_dev(np.array([0, 1, 2], np.int32))
+    for call in (lambda t: q.gemm(t(x)), lambda t: q.gemv(t(x[0])), lambda t: q.gemm_noalloc(t(x), torch.zeros_like(x)), lambda t: fa.gemm_pair(gate, down, t(x))[1],
+                 lambda t: fa.gemv_multi([q, q], t(x[0]))[1], lambda t: fa.ffn_swiglu(q, q, q, t(x[0])), lambda t: fa.gemm_grouped(gate, 2, t(off), t(x)),
+                 lambda t: fa.moe_ffn(gate, gate, down, 2, t(x), t(ids), t(weights)), lambda t: q.get_rows(t(ids[:, 0].contiguous()))):
+        assert torch.equal(call(lambda t: t), call(_On))
