@@ -172,7 +172,7 @@ def _stream():
 
 def _stream_at(fp8, *tensors):
     """_stream() for a call over tensors (or None).  fp8: with FP8_BLOCK weights, whose calls refuse tensors of another device than the
-    current one.  The other kinds' take a peer's memory as they always did."""
+    current one.  The other kinds' take a peer's memory as they always did; no kernel reads host memory that is not page-locked."""
     import torch
     try:
         here = torch._C._cuda_getDevice()
@@ -182,7 +182,7 @@ def _stream_at(fp8, *tensors):
     for t in tensors:
         if t is not None:
             at = t.get_device()
-            if fp8 and at != here:
+            if at != here and (fp8 or at < 0 and not t.is_pinned()):
                 raise ValueError("the tensor is on device %d, the current device is %d" % (at, here))
     return stream
 
@@ -273,7 +273,7 @@ class Weights:
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.numel() == self.cols
         y = out if out is not None else torch.empty(self.rows, dtype=torch.float32, device=x.device)
         check(lib().frk_hip_gemv_dev(self.handle, C.c_void_p(x.data_ptr()), C.c_void_p(y.data_ptr()), act_mode,
-                                     _stream_at(self.kind == FP8_BLOCK, x)))
+                                     _stream_at(self.kind == FP8_BLOCK, x, out)))
         return y
 
     def gemv_q8k(self, acts, out=None):
@@ -300,7 +300,7 @@ class Weights:
         batch = x.numel() // self.cols
         # (a small product waits for its call: like its input 0.3 us ahead of torch.empty)
         y = out if out is not None else x.new_empty((batch, self.rows))
-        check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), _stream_at(self.kind == FP8_BLOCK, x)))
+        check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), _stream_at(self.kind == FP8_BLOCK, x, out)))
         return y
 
     def gemm_acts(self, acts, out=None):
@@ -317,7 +317,7 @@ class Weights:
         batch = x.numel() // self.cols
         assert out.dtype == torch.float32 and out.is_cuda and out.is_contiguous() and out.numel() == batch * self.rows
         check(lib().frk_hip_gemm_noalloc_dev(self.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(out.data_ptr()),
-                                             _stream_at(self.kind == FP8_BLOCK, x)))
+                                             _stream_at(self.kind == FP8_BLOCK, x, out)))
         return out
 
     def dequant(self):
@@ -356,7 +356,7 @@ def _get_rows_dev(self, ids):
     assert ids.dtype == torch.int32 and ids.is_cuda and ids.is_contiguous()
     out = torch.empty((ids.numel(), self.cols), dtype=torch.float32, device=ids.device)
     check(lib().frk_hip_get_rows_dev(self.handle, C.c_void_p(ids.data_ptr()), ids.numel(), C.c_void_p(out.data_ptr()),
-                                     _stream()))
+                                     _stream_at(self.kind == FP8_BLOCK, ids)))
     return out
 
 
@@ -380,7 +380,7 @@ def gemm_pair(w0, w1, x, outs=None):
     batch = x.numel() // w0.cols
     y0, y1 = outs if outs is not None else (torch.empty((batch, w.rows), dtype=torch.float32, device=x.device) for w in (w0, w1))
     check(lib().frk_hip_gemm_pair_dev(w0.handle, w1.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(y0.data_ptr()),
-                                      C.c_void_p(y1.data_ptr()), _stream_at(_any_fp8(w0, w1), x)))
+                                      C.c_void_p(y1.data_ptr()), _stream_at(_any_fp8(w0, w1), x, y0, y1)))
     return y0, y1
 
 
@@ -449,7 +449,7 @@ def moe_ffn(gate, up, down, n_experts, x, ids, weights, out=None):
     batch, k = ids.shape
     y = out if out is not None else x.new_empty((batch, down.rows // n_experts))
     check(lib().frk_hip_moe_ffn_dev(gate.handle, up.handle, down.handle, n_experts, x.data_ptr(), batch, ids.data_ptr(), weights.data_ptr(), k,
-                                    y.data_ptr(), _stream_at(_any_fp8(gate, up, down), x)))
+                                    y.data_ptr(), _stream_at(_any_fp8(gate, up, down), x, ids, weights, out)))
     return y
 
 
@@ -467,7 +467,7 @@ def gemm_grouped(stacked, n_groups, group_off, x, gather=None, out=None):
         pairs = x_rows
     y = out if out is not None else x.new_empty((pairs, stacked.rows // n_groups))
     check(lib().frk_hip_gemm_grouped_dev(stacked.handle, n_groups, group_off.data_ptr(), gather.data_ptr() if gather is not None else None,
-                                         x.data_ptr(), x_rows, pairs, y.data_ptr(), _stream_at(stacked.kind == FP8_BLOCK, x)))
+                                         x.data_ptr(), x_rows, pairs, y.data_ptr(), _stream_at(stacked.kind == FP8_BLOCK, x, group_off, gather, out)))
     return y
 
 
@@ -497,7 +497,7 @@ def gemv_multi(ws, x, outs=None):
     ys = outs if outs is not None else [torch.empty(w.rows, dtype=torch.float32, device=x.device) for w in ws]
     hs = (C.c_void_p * n)(*[w.handle for w in ws])
     ps = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
-    check(lib().frk_hip_gemv_multi_dev(hs, n, C.c_void_p(x.data_ptr()), ps, _stream_at(_any_fp8(*ws), x)))
+    check(lib().frk_hip_gemv_multi_dev(hs, n, C.c_void_p(x.data_ptr()), ps, _stream_at(_any_fp8(*ws), x, *ys)))
     return ys
 
 
@@ -506,7 +506,7 @@ def ffn_swiglu(gate, up, down, x, out=None):
     import torch
     y = out if out is not None else torch.empty(down.rows, dtype=torch.float32, device=x.device)
     check(lib().frk_hip_ffn_swiglu_dev(gate.handle, up.handle, down.handle, C.c_void_p(x.data_ptr()),
-                                       C.c_void_p(y.data_ptr()), _stream_at(_any_fp8(gate, up, down), x)))
+                                       C.c_void_p(y.data_ptr()), _stream_at(_any_fp8(gate, up, down), x, y)))
     return y
 
 

@@ -114,8 +114,30 @@ class _On:
 
 
 @pytest.mark.gpu
+def test_every_tensor_of_a_call_is_on_the_current_device(fa):
+    import torch
+    rng = np.random.default_rng(2)
+    w = _resident(fa, *plain.random_matrix(rng, 128, 128))
+    x, y = torch.zeros((1, 128), device="cuda"), torch.zeros((1, 128), device="cuda")
+    ids, weights = torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.ones((1, 1), device="cuda")
+    off = to_dev(np.array([0, 1], np.int32))
+    calls = [lambda t: w.gemm(x, out=t(y)), lambda t: w.gemv(x, out=t(y)), lambda t: w.gemm_noalloc(x, t(y)), lambda t: fa.gemm_pair(w, w, x, outs=(y, t(y))),
+             lambda t: fa.gemv_multi([w, w], x, outs=[t(y), y]), lambda t: fa.ffn_swiglu(w, w, w, t(x)), lambda t: fa.ffn_swiglu(w, w, w, x, out=t(y)),
+             lambda t: fa.moe_ffn(w, w, w, 1, x, t(ids), weights), lambda t: fa.moe_ffn(w, w, w, 1, x, ids, t(weights)),
+             lambda t: fa.moe_ffn(w, w, w, 1, x, ids, weights, out=t(y)), lambda t: fa.gemm_grouped(w, 1, t(off), x),
+             lambda t: fa.gemm_grouped(w, 1, off, x, gather=t(ids)), lambda t: fa.gemm_grouped(w, 1, off, x, out=t(y)), lambda t: w.get_rows(t(ids))]
+    for call in calls:
+        call(lambda t: t)
+        with pytest.raises(ValueError, match="current device"):
+            call(_On)
+    for call in calls[7:10]:  # (host memory)
+        with pytest.raises(ValueError, match="device -1"):
+            call(lambda t: t.cpu())
+
+
+@pytest.mark.gpu
 def test_the_other_kinds_take_a_peers_memory(fa):
-    """As they did before there were FP8_BLOCK matrices."""
+    """As they did before there were FP8_BLOCK matrices; host memory has to be page-locked."""
     import torch
     n = 256
     q = fa.Weights.from_host(fo.Q8_0, make_weights(fo.Q8_0, n, n, seed=1), n, n)
@@ -128,3 +150,9 @@ def test_the_other_kinds_take_a_peers_memory(fa):
                  lambda t: fa.gemv_multi([q, q], t(x[0]))[1], lambda t: fa.ffn_swiglu(q, q, q, t(x[0])), lambda t: fa.gemm_grouped(gate, 2, t(off), t(x)),
                  lambda t: fa.moe_ffn(gate, gate, down, 2, t(x), t(ids), t(weights)), lambda t: q.get_rows(t(ids[:, 0].contiguous()))):
         assert torch.equal(call(lambda t: t), call(_On))
+    want = fa.moe_ffn(gate, gate, down, 2, x, ids, weights)
+    assert torch.equal(fa.moe_ffn(gate, gate, down, 2, x, ids.cpu().pin_memory(), weights.cpu().pin_memory()), want)
+    for call in (lambda: fa.moe_ffn(gate, gate, down, 2, x, ids.cpu(), weights), lambda: fa.moe_ffn(gate, gate, down, 2, x, ids, weights.cpu()),
+                 lambda: fa.gemv_multi([q], x[0].cpu()), lambda: fa.ffn_swiglu(q, q, q, x[0].cpu())):
+        with pytest.raises(ValueError, match="device -1"):
+            call()
