@@ -170,9 +170,18 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _stream_at(fp8, *tensors):
-    """_stream() for a call over tensors (or None).  fp8: with FP8_BLOCK weights, whose calls refuse tensors of another device than the
-    current one.  The other kinds' take a peer's memory as they always did; no kernel reads host memory that is not page-locked."""
+def _stream_raw():
+    """_stream() for a call over tensors on a GPU, as a number."""
+    import torch
+    try:
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    except AttributeError:
+        return torch.cuda.current_stream().cuda_stream
+
+
+def _fp8_stream(*tensors):
+    """_stream_raw() for a call with FP8_BLOCK weights, or routing by a rule, which refuses tensors (or None) of another device than the current one.  The
+    older kinds' calls take a peer's memory as they always did."""
     import torch
     try:
         here = torch._C._cuda_getDevice()
@@ -180,15 +189,29 @@ def _stream_at(fp8, *tensors):
     except AttributeError:
         here, stream = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
     for t in tensors:
-        if t is not None:
-            at = t.get_device()
-            if at != here and (fp8 or at < 0 and not t.is_pinned()):
-                raise ValueError("the tensor is on device %d, the current device is %d" % (at, here))
+        if t is not None and t.get_device() != here:
+            raise ValueError("the tensor is on device %d, the current device is %d" % (t.get_device(), here))
     return stream
 
 
+def _fp8_floats(t, n):
+    """An operand of a call with FP8_BLOCK weights that the call has n floats of.  (The older kinds' take any: a look at a tensor is 0.04 us
+    of calls that the host bounds.)"""
+    import torch
+    if t.numel() < n or t.dtype is not torch.float32 or not t.is_contiguous():
+        raise ValueError("%d values of %s: the call has %d contiguous floats" % (t.numel(), t.dtype, n))
+    return t
+
+
 def _any_fp8(*ws):
-    return any(w.kind == FP8_BLOCK for w in ws)
+    for w in ws:
+        if w.kind == FP8_BLOCK:
+            return True
+    return False
+
+
+def _on_a_gpu(t):  # (or page-locked: memory that a kernel can read)
+    return t.is_cuda or t.is_pinned()
 
 
 def _np_ptr(a):
@@ -246,7 +269,7 @@ class Weights:
         cls._check_fp8(codes.numel(), scales.numel(), rows, cols, matrices)
         h = C.c_void_p()
         check(lib().frk_hip_weights_from_device_fp8(C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), rows, cols,
-                                                    matrices, _stream_at(True, codes), C.byref(h)))
+                                                    matrices, _fp8_stream(codes), C.byref(h)))
         return cls(h, FP8_BLOCK, rows, cols)
 
     def keep_decoded(self):
@@ -272,8 +295,11 @@ class Weights:
         import torch
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.numel() == self.cols
         y = out if out is not None else torch.empty(self.rows, dtype=torch.float32, device=x.device)
-        check(lib().frk_hip_gemv_dev(self.handle, C.c_void_p(x.data_ptr()), C.c_void_p(y.data_ptr()), act_mode,
-                                     _stream_at(self.kind == FP8_BLOCK, x, out)))
+        if self.kind == FP8_BLOCK:
+            stream = _fp8_stream(x) if out is None else _fp8_stream(x, _fp8_floats(out, self.rows))
+        else:
+            stream = _stream_raw()
+        check(lib().frk_hip_gemv_dev(self.handle, C.c_void_p(x.data_ptr()), C.c_void_p(y.data_ptr()), act_mode, stream))
         return y
 
     def gemv_q8k(self, acts, out=None):
@@ -300,7 +326,11 @@ class Weights:
         batch = x.numel() // self.cols
         # (a small product waits for its call: like its input 0.3 us ahead of torch.empty)
         y = out if out is not None else x.new_empty((batch, self.rows))
-        check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), _stream_at(self.kind == FP8_BLOCK, x, out)))
+        if self.kind == FP8_BLOCK:
+            stream = _fp8_stream(x) if out is None else _fp8_stream(x, _fp8_floats(out, batch * self.rows))
+        else:
+            stream = _stream_raw()
+        check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), stream))
         return y
 
     def gemm_acts(self, acts, out=None):
@@ -316,8 +346,8 @@ class Weights:
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.shape[-1] == self.cols
         batch = x.numel() // self.cols
         assert out.dtype == torch.float32 and out.is_cuda and out.is_contiguous() and out.numel() == batch * self.rows
-        check(lib().frk_hip_gemm_noalloc_dev(self.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(out.data_ptr()),
-                                             _stream_at(self.kind == FP8_BLOCK, x, out)))
+        stream = _fp8_stream(x, out) if self.kind == FP8_BLOCK else _stream_raw()
+        check(lib().frk_hip_gemm_noalloc_dev(self.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(out.data_ptr()), stream))
         return out
 
     def dequant(self):
@@ -356,7 +386,7 @@ def _get_rows_dev(self, ids):
     assert ids.dtype == torch.int32 and ids.is_cuda and ids.is_contiguous()
     out = torch.empty((ids.numel(), self.cols), dtype=torch.float32, device=ids.device)
     check(lib().frk_hip_get_rows_dev(self.handle, C.c_void_p(ids.data_ptr()), ids.numel(), C.c_void_p(out.data_ptr()),
-                                     _stream_at(self.kind == FP8_BLOCK, ids)))
+                                     _fp8_stream(ids) if self.kind == FP8_BLOCK else _stream()))
     return out
 
 
@@ -379,8 +409,12 @@ def gemm_pair(w0, w1, x, outs=None):
     assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.shape[-1] == w0.cols == w1.cols
     batch = x.numel() // w0.cols
     y0, y1 = outs if outs is not None else (torch.empty((batch, w.rows), dtype=torch.float32, device=x.device) for w in (w0, w1))
+    if w0.kind == FP8_BLOCK or w1.kind == FP8_BLOCK:
+        stream = _fp8_stream(x) if outs is None else _fp8_stream(x, _fp8_floats(y0, batch * w0.rows), _fp8_floats(y1, batch * w1.rows))
+    else:
+        stream = _stream_raw()
     check(lib().frk_hip_gemm_pair_dev(w0.handle, w1.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(y0.data_ptr()),
-                                      C.c_void_p(y1.data_ptr()), _stream_at(_any_fp8(w0, w1), x, y0, y1)))
+                                      C.c_void_p(y1.data_ptr()), stream))
     return y0, y1
 
 
@@ -436,7 +470,7 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_b
         raise ValueError("score %r: one of %s" % (score, ", ".join(SCORES)))
     rule = RouteRule(SCORES[score], int(bool(norm)), groups, top_groups, group_best, scale, None if bias is None else bias.data_ptr())
     ids, w = logits.new_empty((batch, k), dtype=torch.int32), logits.new_empty((batch, k))
-    check(lib().frk_hip_route_dev(logits.data_ptr(), batch, n_experts, k, C.byref(rule), ids.data_ptr(), w.data_ptr(), _stream_at(True, logits)))
+    check(lib().frk_hip_route_dev(logits.data_ptr(), batch, n_experts, k, C.byref(rule), ids.data_ptr(), w.data_ptr(), _fp8_stream(logits)))
     return ids, w
 
 
@@ -448,8 +482,17 @@ def moe_ffn(gate, up, down, n_experts, x, ids, weights, out=None):
     assert ids.dtype == torch.int32 and ids.is_contiguous() and weights.dtype == torch.float32 and weights.is_contiguous()
     batch, k = ids.shape
     y = out if out is not None else x.new_empty((batch, down.rows // n_experts))
+    if _any_fp8(gate, up, down):
+        if x.numel() < batch * gate.cols or weights.numel() < batch * k:
+            raise ValueError("%d x %d ids over %d activations and %d weights" % (batch, k, x.numel(), weights.numel()))
+        if out is not None:
+            _fp8_floats(out, batch * (down.rows // n_experts))
+        stream = _fp8_stream(x, ids, weights, out)
+    else:
+        assert _on_a_gpu(ids) and _on_a_gpu(weights)
+        stream = _stream_raw()
     check(lib().frk_hip_moe_ffn_dev(gate.handle, up.handle, down.handle, n_experts, x.data_ptr(), batch, ids.data_ptr(), weights.data_ptr(), k,
-                                    y.data_ptr(), _stream_at(_any_fp8(gate, up, down), x, ids, weights, out)))
+                                    y.data_ptr(), stream))
     return y
 
 
@@ -466,8 +509,14 @@ def gemm_grouped(stacked, n_groups, group_off, x, gather=None, out=None):
     else:
         pairs = x_rows
     y = out if out is not None else x.new_empty((pairs, stacked.rows // n_groups))
+    if stacked.kind == FP8_BLOCK:
+        if out is not None:
+            _fp8_floats(out, pairs * (stacked.rows // n_groups))
+        stream = _fp8_stream(x, group_off, gather, out)
+    else:
+        stream = _stream_raw()
     check(lib().frk_hip_gemm_grouped_dev(stacked.handle, n_groups, group_off.data_ptr(), gather.data_ptr() if gather is not None else None,
-                                         x.data_ptr(), x_rows, pairs, y.data_ptr(), _stream_at(stacked.kind == FP8_BLOCK, x, group_off, gather, out)))
+                                         x.data_ptr(), x_rows, pairs, y.data_ptr(), stream))
     return y
 
 
@@ -495,9 +544,16 @@ def gemv_multi(ws, x, outs=None):
     import torch
     n = len(ws)
     ys = outs if outs is not None else [torch.empty(w.rows, dtype=torch.float32, device=x.device) for w in ws]
+    if _any_fp8(*ws):
+        if len(ys) != n:
+            raise ValueError("%d matrices, %d outputs" % (n, len(ys)))
+        stream = _fp8_stream(_fp8_floats(x, ws[0].cols), *[_fp8_floats(y, w.rows) for w, y in zip(ws, outs or ())])
+    else:
+        assert _on_a_gpu(x)
+        stream = _stream_raw()
     hs = (C.c_void_p * n)(*[w.handle for w in ws])
     ps = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
-    check(lib().frk_hip_gemv_multi_dev(hs, n, C.c_void_p(x.data_ptr()), ps, _stream_at(_any_fp8(*ws), x, *ys)))
+    check(lib().frk_hip_gemv_multi_dev(hs, n, C.c_void_p(x.data_ptr()), ps, stream))
     return ys
 
 
@@ -505,8 +561,13 @@ def ffn_swiglu(gate, up, down, x, out=None):
     """down(silu(gate x) * up x), all on the device."""
     import torch
     y = out if out is not None else torch.empty(down.rows, dtype=torch.float32, device=x.device)
+    if _any_fp8(gate, up, down):
+        stream = _fp8_stream(_fp8_floats(x, gate.cols), None if out is None else _fp8_floats(out, down.rows))
+    else:
+        assert _on_a_gpu(x)
+        stream = _stream_raw()
     check(lib().frk_hip_ffn_swiglu_dev(gate.handle, up.handle, down.handle, C.c_void_p(x.data_ptr()),
-                                       C.c_void_p(y.data_ptr()), _stream_at(_any_fp8(gate, up, down), x, y)))
+                                       C.c_void_p(y.data_ptr()), stream))
     return y
 
 
