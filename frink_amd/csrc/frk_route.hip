@@ -320,7 +320,6 @@ int launch_route(const float *logits, size_t batch, int n_experts, int k, const 
     RouteArgs a;
     a.logits = logits;
     a.bias = rule.bias_dev;
-    a.batch = batch;
     a.n_experts = n_experts;
     a.k = k;
     a.sigmoid = rule.score == FRK_SCORE_SIGMOID;
@@ -338,16 +337,24 @@ int launch_route(const float *logits, size_t batch, int n_experts, int k, const 
     a.scale = rule.scale;
     a.ids = ids;
     a.weights = weights;
-#define FRK_GO(NR) hipLaunchKernelGGL(route_kernel<NR>, dim3((unsigned)((batch + ROUTE_WAVES - 1) / ROUTE_WAVES)), dim3(64 * ROUTE_WAVES), 0, s, a)
-    switch (nr) {
-    case 1: FRK_GO(1); break;
-    case 2: FRK_GO(2); break;
-    case 4: FRK_GO(4); break;
-    case 8: FRK_GO(8); break;
-    default: FRK_GO(16); break;
-    }
+    // (a grid holds fewer than 2^32 threads, 64 a token)
+    constexpr size_t TOKENS = (size_t)1 << 25;
+    for (size_t first = 0; first < batch; first += TOKENS) {
+        a.batch = std::min(TOKENS, batch - first);
+#define FRK_GO(NR) hipLaunchKernelGGL(route_kernel<NR>, dim3((unsigned)((a.batch + ROUTE_WAVES - 1) / ROUTE_WAVES)), dim3(64 * ROUTE_WAVES), 0, s, a)
+        switch (nr) {
+        case 1: FRK_GO(1); break;
+        case 2: FRK_GO(2); break;
+        case 4: FRK_GO(4); break;
+        case 8: FRK_GO(8); break;
+        default: FRK_GO(16); break;
+        }
 #undef FRK_GO
-    FRK_LAUNCH_CHECK("route");
+        FRK_LAUNCH_CHECK("route");
+        a.logits += TOKENS * (size_t)n_experts;
+        a.ids += TOKENS * (size_t)k;
+        a.weights += TOKENS * (size_t)k;
+    }
     return FRK_OK;
 }
 

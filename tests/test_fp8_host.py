@@ -34,6 +34,20 @@ int main() {  // a call a line; its status, the kernels it launched and its erro
                 fill(w[i], kind, i < 2 ? 64 : 32, name == "ffn" && i == 2 ? 64 : cols), ws[i] = &w[i];
             }
             tell(name == "ffn" ? frk_hip_ffn_swiglu_dev(ws[0], ws[1], ws[2], room, room, nullptr) : frk_hip_gemv_multi_dev(ws.data(), n, room, ys.data(), nullptr));
+        } else if (name == "route") {  // tokens, experts, k; the tokens that its grids hold, and the most threads of one
+            size_t batch, n, k;
+            if (scanf("%zu %zu %zu", &batch, &n, &k) != 3) return 1;
+            frk_route_rule rule{};
+            rule.groups = rule.top_groups = rule.group_best = 1;
+            const size_t before = HipStub::get().shapes.size();
+            const int rc = frk_hip_route_dev(room, batch, n, k, &rule, (int32_t *)room, room, nullptr);
+            size_t tokens = 0, most = 0;
+            for (size_t i = before; i < HipStub::get().shapes.size(); i++) {
+                const auto [grid, group] = HipStub::get().shapes[i];
+                tokens += (size_t)grid.x * (group.x / 64), most = std::max(most, (size_t)grid.x * group.x);
+            }
+            HipStub::get().take();
+            printf("%d %zu %zu | %s\n", rc, tokens, most, frk_hip_last_error());
         } else if (name == "elsewhere") {  // a matrix of device 1, device 0 the current one: every entry point that takes it
             static frk_weights w, q;
             fill(w, FRK_KIND_FP8_BLOCK, 256, 256, 2), fill(q, FRK_KIND_Q4_K, 256, 256);
@@ -102,3 +116,11 @@ def test_a_matrix_of_another_device_is_refused(said):
     assert here[0] == 0
     for call, (rc, names, error) in enumerate(elsewhere):
         assert rc == -4 and names == ["-"] and "device" in error, (call, rc, names, error)
+
+
+@pytest.mark.parametrize("batch", [1, 1 << 25, (1 << 25) + 1, (1 << 26) - 4, 1 << 26, (1 << 27) + 5, 1 << 30])
+@pytest.mark.parametrize("experts", [1, 70, 1000])
+def test_routes_of_any_batch_fit_their_grids(said, batch, experts):
+    (rc, (tokens, most), error), = said("route %d %d 1" % (batch, experts))
+    assert rc == 0, error
+    assert batch <= int(tokens) < batch + 4 * 32 and int(most) < 1 << 32
