@@ -387,8 +387,9 @@ int frk_hip_weights_from_device(int kind, const void *dev_bytes, size_t len, siz
 static int check_f8_shape(size_t rows, size_t cols, size_t matrices) {
     if (rows == 0 || cols == 0 || matrices == 0) return set_error(FRK_ERR_SHAPE, "empty shape: rows=%zu cols=%zu matrices=%zu", rows, cols, matrices);
     if (rows % matrices) return set_error(FRK_ERR_SHAPE, "%zu rows do not divide into %zu matrices", rows, matrices);
-    // (a tile's 128 rows of activations lie within 32 bits of each other)
+    // (a tile's 128 rows of activations lie within 32 bits of each other; a grid holds fewer than 2^32 threads, 512 a strip of sixteen weight rows)
     if (rows > 0x7fffff00u || cols > (1u << 23)) return set_error(FRK_ERR_SHAPE, "shape too large: rows=%zu cols=%zu", rows, cols);
+    if (rows / matrices > (1u << 27) - 16) return set_error(FRK_ERR_SHAPE, "shape too large: matrices of %zu rows (at most 2^27 - 16)", rows / matrices);
     if (matrices > 65535) return set_error(FRK_ERR_SHAPE, "%zu matrices (at most 65535)", matrices);
     return FRK_OK;
 }

@@ -127,7 +127,7 @@ int frk_hip_weights_from_device(int kind, const void *dev_bytes, size_t len, siz
  * last blocks may be partly used.  register takes host buffers (borrowed for the call; synchronous; unlike
  * frk_hip_weights_register it keeps no cache), from_device buffers on the current device (copied on `stream`; they may be
  * freed once the stream has passed the call).  A call over such a handle while another device is the current one returns FRK_ERR_ARG,
- * and so do register and frk_hip_get_rows on another device than the host-buffer calls' (the one that was current at the first).  The resident copy pads rows to 16 and columns to 128.  At most 2^23 columns and 65535
+ * and so do register and frk_hip_get_rows on another device than the host-buffer calls' (the one that was current at the first).  The resident copy pads rows to 16 and columns to 128.  At most 2^27 - 16 rows a matrix, 2^23 columns and 65535
  * matrices; a gathered product's activations, two bytes a value quantized, at most 4 GiB.
  *
  * What takes such a handle, f32 in and f32 out as for the other kinds: frk_hip_gemv_dev (FRK_ACT_F32 and FRK_ACT_INT8 are the

@@ -17,6 +17,7 @@ struct HipStub {
     std::vector<std::pair<dim3, dim3>> shapes;  // of all launches: grid, workgroup
     std::pair<dim3, dim3> next;
     int device = 0;          // the current one
+    bool memory = true;      // allocations have some (else an address)
     bool capturing = false;  // what hipStreamIsCapturing says
     static HipStub &get() {
         static HipStub stub;
@@ -56,7 +57,7 @@ hipError_t hipLaunchKernel(const void *f, dim3 grid, dim3 group, void **, size_t
     HipStub::get().launched.push_back(HipStub::get().names[f]);
     return HipStub::get().shapes.emplace_back(grid, group), hipSuccess;
 }
-hipError_t hipMalloc(void **p, size_t n) { return (*p = calloc(1, n)) ? hipSuccess : hipErrorOutOfMemory; }
+hipError_t hipMalloc(void **p, size_t n) { return (*p = calloc(1, HipStub::get().memory ? n : 1)) ? hipSuccess : hipErrorOutOfMemory; }
 hipError_t hipHostMalloc(void **p, size_t n, unsigned) { return hipMalloc(p, n); }
 hipError_t hipFree(void *p) { return free(p), hipSuccess; }
 hipError_t hipMemcpy(void *to, const void *from, size_t n, hipMemcpyKind) { return memcpy(to, from, n), hipSuccess; }

@@ -48,6 +48,23 @@ int main() {  // a call a line; its status, the kernels it launched and its erro
             }
             HipStub::get().take();
             printf("%d %zu %zu | %s\n", rc, tokens, most, frk_hip_last_error());
+        } else if (name == "rows") {  // the largest grid of a one-token product, or what registration says
+            size_t rows, matrices;
+            if (scanf("%zu %zu", &rows, &matrices) != 2) return 1;
+            frk_weights *handle = nullptr;
+            HipStub::get().memory = false;
+            int rc = frk_hip_weights_from_device_fp8((uint8_t *)room, room, rows, 1, matrices, nullptr, &handle);
+            size_t most = 0;
+            const std::string error = frk_hip_last_error();
+            if (!rc) {
+                const size_t before = HipStub::get().shapes.size();
+                rc = frk_hip_gemv_dev(handle, room, room, FRK_ACT_F32, nullptr);
+                for (size_t i = before; i < HipStub::get().shapes.size(); i++) most = std::max(most, (size_t)HipStub::get().shapes[i].first.x * HipStub::get().shapes[i].second.x);
+                frk_hip_weights_release(handle);
+            }
+            HipStub::get().memory = true;
+            HipStub::get().take();
+            printf("%d %zu | %s\n", rc, most, error.c_str());
         } else if (name == "elsewhere") {  // a matrix of device 1, device 0 the current one: every entry point that takes it
             static frk_weights w, q;
             fill(w, FRK_KIND_FP8_BLOCK, 256, 256, 2), fill(q, FRK_KIND_Q4_K, 256, 256);
@@ -124,3 +141,15 @@ def test_routes_of_any_batch_fit_their_grids(said, batch, experts):
     (rc, (tokens, most), error), = said("route %d %d 1" % (batch, experts))
     assert rc == 0, error
     assert batch <= int(tokens) < batch + 4 * 32 and int(most) < 1 << 32
+
+
+@pytest.mark.parametrize("rows,matrices", [(1 << 27, 1), ((1 << 27) - 15, 1), (1 << 29, 4), (0x7fffff00, 1)])
+def test_matrices_of_more_rows_than_a_grid_holds_are_refused(said, rows, matrices):
+    (rc, _, error), = said("rows %d %d" % (rows, matrices))
+    assert rc == -3 and "too large" in error
+
+
+@pytest.mark.parametrize("rows,matrices", [((1 << 27) - 16, 1), (4 * ((1 << 27) - 16), 4), (17, 1)])
+def test_the_most_rows_fit_a_grid(said, rows, matrices):
+    (rc, (most,), error), = said("rows %d %d" % (rows, matrices))
+    assert rc == 0 and 0 < int(most) < 1 << 32, error
