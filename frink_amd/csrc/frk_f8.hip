@@ -556,6 +556,11 @@ int launch_f8_slots(const frk_weights *w, const frk_weights *up, const int32_t *
     const size_t lds = (size_t)g.w.blocks * F8_BLOCK * 2;
     return up ? go_f8_rows<8, 1, 4, true, F8_SLOTS_GLU>(g, grid, lds, s) : go_f8_rows<8, 1, 4, true, F8_SLOTS>(g, grid, lds, s);
 }
+int f8_grouped_fits(const frk_weights *w, size_t x_rows, size_t pairs, bool gathered) {
+    if (f8_few_pairs(pairs, w->matrices)) return FRK_OK;
+    const int shape = f8_grouped_shape(pairs, w->matrices);
+    return f8_tiles_fit(w, shape, f8_max_tiles(pairs, w->matrices, F8_TILE_SIZE[shape].tokens), 1, gathered ? x_rows : 0);
+}
 size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs) {
     return f8_acts_bytes(x_rows, w->cols) + 256 + f8_max_tiles(pairs, w->matrices, 32) * 16;
 }

@@ -197,9 +197,12 @@ struct F8Gemm {
 // over tiles of a shape (weight rows x tokens); parts > 1 (dense): shares of the columns, each its own copy of y, part_stride floats apart
 enum { F8_TILE_256x128, F8_TILE_256x64, F8_TILE_128x32, F8_TILE_SHAPES };
 struct F8TileSize {
-    int rows, tokens;
+    int rows, tokens, threads;
 };
-constexpr F8TileSize F8_TILE_SIZE[F8_TILE_SHAPES] = {{256, 128}, {256, 64}, {128, 32}};
+constexpr F8TileSize F8_TILE_SIZE[F8_TILE_SHAPES] = {{256, 128, 512}, {256, 64, 256}, {128, 32, 128}};
+// A status: whether tok_tiles tiles of tokens fit a grid, in `sheets` (matrices times parts), and gathered rows of activations (0: a list's are in
+// order) their 32-bit offsets.  Asked before a call takes memory or launches anything.
+int f8_tiles_fit(const frk_weights *w, int shape, size_t tok_tiles, size_t sheets, size_t gathered);
 int launch_f8_tile(const F8Gemm &g, int shape, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s);
 // How a dense batch is multiplied: by the rows kernel (shape -1; `fused`: its own quantization), or over tiles in `parts` shares
 struct F8Plan {
@@ -215,6 +218,7 @@ Layout f8_layout(size_t rows, size_t cols, size_t matrices, size_t *bytes);
 int launch_f8_repack(const uint8_t *src, const float *scales, const frk_weights *w, hipStream_t s);
 // `quantized`: ws holds the batch from a call before, of a plan with the same layout (both of the rows kernel or both over tiles)
 int launch_f8_gemm(const frk_weights *w, const F8Plan &plan, const float *x, size_t batch, float *y, void *ws, bool quantized, void *parts, hipStream_t s);
+int f8_grouped_fits(const frk_weights *w, size_t x_rows, size_t pairs, bool gathered);  // a status, as f8_tiles_fit's
 size_t f8_grouped_workspace_bytes(const frk_weights *w, size_t x_rows, size_t pairs);
 int launch_f8_grouped(const frk_weights *w, const int32_t *group_off, const int32_t *gather, const float *x, size_t x_rows, size_t pairs,
                       float *y, void *ws, hipStream_t s);

@@ -19,6 +19,7 @@ typedef float f8_v4f __attribute__((ext_vector_type(4)));
 constexpr int F8_MR = 4;
 template <int RW, int TW, int MT>
 struct F8TileShape {
+    static constexpr int SHAPE = TW == 2 ? F8_TILE_256x128 : RW == 4 ? F8_TILE_256x64 : F8_TILE_128x32;
     static constexpr int WAVES = RW * TW, ROWS = RW * F8_MR * F8_STRIP, TOKENS = TW * MT * 16, STAGES = 3;
     static constexpr int STAGE = TOKENS * F8_BLOCK * 2, REQUESTS = STAGE / 1024 / WAVES;  // of tokens; requests of a wavefront
     static_assert(REQUESTS * WAVES * 1024 == STAGE, "whole requests");
@@ -33,6 +34,7 @@ template <int RW, int TW, int MT>
 __global__ __launch_bounds__(64 * RW * TW, 2) void f8_tile_kernel(F8Gemm g, int row_tiles, int tok_tiles, int matrices, int parts, size_t part_stride) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = F8TileShape<RW, TW, MT>;
+    static_assert(T::ROWS == F8_TILE_SIZE[T::SHAPE].rows && T::TOKENS == F8_TILE_SIZE[T::SHAPE].tokens && 64 * T::WAVES == F8_TILE_SIZE[T::SHAPE].threads, "the table");
     constexpr int MR = F8_MR, G = T::G, STEPS = T::STEPS, STAGES = T::STAGES;
     extern __shared__ __align__(16) uint8_t f8_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -234,11 +236,6 @@ template <int RW, int TW, int MT>
 static int go_f8_tile(const F8Gemm &g, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s) {
     using T = F8TileShape<RW, TW, MT>;
     const size_t row_tiles = ((size_t)g.w.rows + T::ROWS - 1) / T::ROWS, total = row_tiles * tok_tiles;
-    if (total > 0x7ffffff8u || matrices * parts > 65535) return set_error(FRK_ERR_SHAPE, "%zu x %zu tiles of %zu matrices: too many", row_tiles, tok_tiles, matrices);
-    if (total == 0) return FRK_OK;
-    // (a request's offset of a lane is 32 bits wide: a gathered row's from the first, others' from their tile's)
-    if (g.src && (size_t)g.a.rows * g.w.blocks * (F8_BLOCK * 2) > 0xffffffffu)
-        return set_error(FRK_ERR_SHAPE, "%d gathered rows of %d blocks: more than 4 GiB of quantized activations", g.a.rows, g.w.blocks);
     static bool sized = false;  // a benign race: every thread sets the same attribute
     if (!sized) {
         hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tile_kernel<RW, TW, MT>), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -249,6 +246,17 @@ static int go_f8_tile(const F8Gemm &g, size_t tok_tiles, size_t matrices, int pa
     hipLaunchKernelGGL((f8_tile_kernel<RW, TW, MT>), dim3((unsigned)((total + 7) / 8 * 8), (unsigned)(matrices * parts)), dim3(64 * T::WAVES), T::LDS, s,
                        g, (int)row_tiles, (int)tok_tiles, (int)matrices, parts, part_stride);
     FRK_LAUNCH_CHECK("f8_tile");
+    return FRK_OK;
+}
+int f8_tiles_fit(const frk_weights *w, int shape, size_t tok_tiles, size_t sheets, size_t gathered) {
+    const F8Mat m = f8_mat(w);
+    const F8TileSize t = F8_TILE_SIZE[shape];
+    const size_t row_tiles = ((size_t)m.rows + t.rows - 1) / t.rows;
+    if ((row_tiles * tok_tiles + 7) / 8 * 8 * t.threads > 0xffffffffu || sheets > 65535)
+        return set_error(FRK_ERR_SHAPE, "%zu x %zu tiles %zu times: more than a grid holds", row_tiles, tok_tiles, sheets);
+    // (a request's offset of a lane is 32 bits wide: a gathered row's from the first, others' from their tile's)
+    if (gathered * m.blocks * (F8_BLOCK * 2) > 0xffffffffu)
+        return set_error(FRK_ERR_SHAPE, "%zu gathered rows of %d blocks: more than 4 GiB of quantized activations", gathered, m.blocks);
     return FRK_OK;
 }
 int launch_f8_tile(const F8Gemm &g, int shape, size_t tok_tiles, size_t matrices, int parts, size_t part_stride, hipStream_t s) {

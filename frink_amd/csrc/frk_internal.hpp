@@ -358,6 +358,7 @@ int launch_moe_ffn(const frk_weights *gate, const frk_weights *up, const frk_wei
 int moe_copy_intermediates(void *ws, size_t batch, int k, int n_experts, int hidden, int ffn, float *gate_out,
                            float *up_out, int8_t *act_q, float *act_d, int32_t *pos_of, hipStream_t s);
 // experts in 8-bit floating point with a scale for each block
+int f8_moe_fits(const frk_weights *gate, const frk_weights *down, size_t batch, int k, int n_experts);  // a status
 size_t f8_moe_workspace_bytes(size_t batch, int k, int n_experts, size_t hidden, size_t ffn);
 int launch_moe_ffn_f8(const frk_weights *gate, const frk_weights *up, const frk_weights *down, int n_experts, const float *x, size_t batch,
                       const int32_t *ids, const float *weights, int k, float *out, void *ws, hipStream_t s);

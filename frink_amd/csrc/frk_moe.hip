@@ -1250,6 +1250,15 @@ static F8MoeScratch f8_moe_carve(void *base, size_t batch, int k, int n_experts,
     if (end) *end = (size_t)(p - (char *)base);
     return m;
 }
+int f8_moe_fits(const frk_weights *gate, const frk_weights *down, size_t batch, int k, int n_experts) {
+    if (batch >= (size_t)1 << 24) return set_error(FRK_ERR_SHAPE, "a batch of %zu tokens (at most 2^24 - 1: a grid of 256 threads each)", batch);
+    const size_t pairs = batch * (size_t)k;
+    if (f8_few_slots(pairs, n_experts, gate->cols, down->cols)) return FRK_OK;
+    const int shape = f8_grouped_shape(pairs, n_experts), tile = F8_TILE_SIZE[shape].tokens;
+    const size_t tiles = moe_max_rows(pairs, n_experts, tile) / tile;
+    const int rc = f8_tiles_fit(gate, shape, tiles, 1, batch);
+    return rc ? rc : f8_tiles_fit(down, shape, tiles, 1, 0);
+}
 size_t f8_moe_workspace_bytes(size_t batch, int k, int n_experts, size_t hidden, size_t ffn) {
     size_t end = 0;
     (void)f8_moe_carve(nullptr, batch, k, n_experts, hidden, ffn, &end);

@@ -644,11 +644,17 @@ static int gemv_units_int(const frk_weights *w, const float *x, float *y, hipStr
 }
 
 // FP8_BLOCK: a row is quantized alike in every batch; its sums' order, and so their last bits, is the plan's for the batch.
+static int f8_plan_fits(const frk_weights *w, const F8Plan &plan, size_t batch) {
+    if (plan.shape < 0) return FRK_OK;
+    const size_t tokens = (size_t)F8_TILE_SIZE[plan.shape].tokens;
+    return f8_tiles_fit(w, plan.shape, (batch + tokens - 1) / tokens, w->matrices * plan.parts, 0);
+}
 static int gemm_f8(const frk_weights *w, const float *x, size_t batch, float *y, hipStream_t s, Scratch &scratch) {
     if (batch > (size_t)1 << 30) return set_error(FRK_ERR_SHAPE, "a batch of %zu rows is too large", batch);
     void *ws = nullptr, *parts = nullptr;
     const F8Plan plan = f8_plan(w, batch);
     int rc = f8_on_current_device(w);
+    if (!rc) rc = f8_plan_fits(w, plan, batch);
     if (!rc && plan.acts_bytes) rc = scratch.get(plan.acts_bytes, plan.parts_bytes, s, &ws, &parts);
     if (rc) return rc;
     return launch_f8_gemm(w, plan, x, batch, y, ws, false, parts, s);
@@ -664,6 +670,8 @@ static int gemm_f8_pair(const frk_weights *w0, const frk_weights *w1, const floa
     void *ws = nullptr, *parts = nullptr;
     int rc = f8_on_current_device(w0);
     if (!rc) rc = f8_on_current_device(w1);
+    if (!rc) rc = f8_plan_fits(w0, plan0, batch);
+    if (!rc) rc = f8_plan_fits(w1, plan1, batch);
     if (!rc) rc = scratch.get(plan0.acts_bytes, std::max(plan0.parts_bytes, plan1.parts_bytes), s, &ws, &parts);
     if (!rc) rc = launch_f8_gemm(w0, plan0, x, batch, y0, ws, false, parts, s);
     if (!rc) rc = launch_f8_gemm(w1, plan1, x, batch, y1, ws, true, parts, s);  // (its parts behind the first one's sum)
@@ -1505,6 +1513,7 @@ int frk_hip_moe_ffn_dev(const frk_weights *gate, const frk_weights *up, const fr
         int rc = f8_on_current_device(gate);
         if (!rc) rc = f8_on_current_device(up);
         if (!rc) rc = f8_on_current_device(down);
+        if (!rc) rc = f8_moe_fits(gate, down, batch, (int)k, (int)n_experts);
         if (!rc) rc = workspace(f8_moe_workspace_bytes(batch, (int)k, (int)n_experts, hidden, ffn), (hipStream_t)stream, lease);
         if (rc) return rc;
         return launch_moe_ffn_f8(gate, up, down, (int)n_experts, x, batch, ids, weights, (int)k, out, lease.ptr, (hipStream_t)stream);
@@ -1549,6 +1558,7 @@ int frk_hip_gemm_grouped_dev(const frk_weights *stacked, size_t n_groups, const 
         if (stacked->matrices != n_groups)
             return set_error(FRK_ERR_SHAPE, "the FP8_BLOCK stack holds %zu matrices, the call names %zu groups", stacked->matrices, n_groups);
         int rc = f8_on_current_device(stacked);
+        if (!rc) rc = f8_grouped_fits(stacked, x_rows, pairs, gather != nullptr);
         if (!rc) rc = workspace(f8_grouped_workspace_bytes(stacked, x_rows, pairs), (hipStream_t)stream, lease);
         if (rc) return rc;
         return launch_f8_grouped(stacked, group_off, gather, x, x_rows, pairs, y, lease.ptr, (hipStream_t)stream);

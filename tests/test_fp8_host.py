@@ -65,6 +65,23 @@ int main() {  // a call a line; its status, the kernels it launched and its erro
             HipStub::get().memory = true;
             HipStub::get().take();
             printf("%d %zu | %s\n", rc, most, error.c_str());
+        } else if (name == "gemm" || name == "grouped" || name == "moe") {  // rows, columns, matrices (experts), rows of x (tokens), pairs (top k)
+            size_t rows, cols, matrices, x_rows, n;
+            if (scanf("%zu %zu %zu %zu %zu", &rows, &cols, &matrices, &x_rows, &n) != 5) return 1;
+            frk_weights w, down;
+            fill(w, FRK_KIND_FP8_BLOCK, rows * matrices, cols, matrices), fill(down, FRK_KIND_FP8_BLOCK, cols * matrices, rows, matrices);
+            int32_t *const ids = (int32_t *)room;
+            HipStub::get().memory = false;
+            const size_t before = HipStub::get().shapes.size();
+            int rc;
+            if (name == "gemm") rc = frk_hip_gemm_dev(&w, room, x_rows, room, nullptr);
+            else if (name == "grouped") rc = frk_hip_gemm_grouped_dev(&w, matrices, ids, ids, room, x_rows, n, room, nullptr);
+            else rc = frk_hip_moe_ffn_dev(&w, &w, &down, matrices, room, x_rows, ids, room, n, room, nullptr);
+            HipStub::get().memory = true;
+            size_t most = 0;
+            for (size_t i = before; i < HipStub::get().shapes.size(); i++) most = std::max(most, (size_t)HipStub::get().shapes[i].first.x * HipStub::get().shapes[i].second.x);
+            HipStub::get().take();
+            printf("%d %zu %zu | %s\n", rc, HipStub::get().shapes.size() - before, most, frk_hip_last_error());
         } else if (name == "elsewhere") {  // a matrix of device 1, device 0 the current one: every entry point that takes it
             static frk_weights w, q;
             fill(w, FRK_KIND_FP8_BLOCK, 256, 256, 2), fill(q, FRK_KIND_Q4_K, 256, 256);
@@ -153,3 +170,20 @@ def test_matrices_of_more_rows_than_a_grid_holds_are_refused(said, rows, matrice
 def test_the_most_rows_fit_a_grid(said, rows, matrices):
     (rc, (most,), error), = said("rows %d %d" % (rows, matrices))
     assert rc == 0 and 0 < int(most) < 1 << 32, error
+
+
+@pytest.mark.parametrize("call,needle", [
+    ("grouped 1 64 1024 4 %d" % (1 << 30), "grid"), ("grouped 16 4096 8 %d 64" % (1 << 19), "4 GiB"), ("grouped 16 %d 8 %d 600" % (1 << 23, 500), "4 GiB"),
+    ("moe 8 4096 16 %d 4" % (1 << 19), "4 GiB"), ("moe 8 4 16 %d 4" % (1 << 24), "2.24 - 1"), ("moe 8 4 16 %d 64" % ((1 << 24) - 1), "top-k|experts"),
+    ("moe 300 4 1024 %d 64" % ((1 << 24) - 1), "grid|4 GiB"), ("gemm 1000 8 1 %d 0" % (1 << 30), "grid")])
+def test_what_no_launch_can_hold_is_refused_before_the_first(said, call, needle):
+    import re
+    (rc, (launches, _), error), = said(call)
+    assert rc == -3 and launches == "0" and re.search(needle, error), error
+
+
+@pytest.mark.parametrize("call", ["grouped 1 64 1024 4 %d" % (1 << 29), "grouped 16 4096 8 %d 64" % ((1 << 19) - 1), "grouped 16 4096 64 %d 20" % (1 << 20),
+                                  "moe 8 4096 16 %d 4" % ((1 << 19) - 1), "moe 8 4 16 %d 4" % ((1 << 24) - 1), "gemm 1000 8 1 %d 0" % (1 << 22)])
+def test_what_a_launch_just_holds_is_launched(said, call):
+    (rc, (launches, most), error), = said(call)
+    assert rc == 0 and int(launches) and int(most) < 1 << 32, error
