@@ -179,25 +179,26 @@ def _stream_raw():
         return torch.cuda.current_stream().cuda_stream
 
 
-def _fp8_stream(*tensors):
-    """_stream_raw() for a call with FP8_BLOCK weights, or routing by a rule, which refuses tensors (or None) of another device than the current one.  The
-    older kinds' calls take a peer's memory as they always did."""
+def _fp8_stream(x, others=()):
+    """_stream_raw() for a call with FP8_BLOCK weights, or routing by a rule, which refuses tensors of another device than the current one (others: or
+    None).  The older kinds' calls take a peer's memory as they always did."""
     import torch
     try:
         here = torch._C._cuda_getDevice()
         stream = torch._C._cuda_getCurrentRawStream(here)
     except AttributeError:
         here, stream = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
-    for t in tensors:
+    if x.get_device() != here:
+        raise ValueError("the tensor is on device %d, the current device is %d" % (x.get_device(), here))
+    for t in others:
         if t is not None and t.get_device() != here:
             raise ValueError("the tensor is on device %d, the current device is %d" % (t.get_device(), here))
     return stream
 
 
-def _fp8_floats(t, n):
+def _fp8_floats(torch, t, n):
     """An operand of a call with FP8_BLOCK weights that the call has n floats of.  (The older kinds' take any: a look at a tensor is 0.04 us
     of calls that the host bounds.)"""
-    import torch
     if t.numel() < n or t.dtype is not torch.float32 or not t.is_contiguous():
         raise ValueError("%d values of %s: the call has %d contiguous floats" % (t.numel(), t.dtype, n))
     return t
@@ -296,7 +297,7 @@ class Weights:
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.numel() == self.cols
         y = out if out is not None else torch.empty(self.rows, dtype=torch.float32, device=x.device)
         if self.kind == FP8_BLOCK:
-            stream = _fp8_stream(x) if out is None else _fp8_stream(x, _fp8_floats(out, self.rows))
+            stream = _fp8_stream(x) if out is None else _fp8_stream(x, (_fp8_floats(torch, out, self.rows),))
         else:
             stream = _stream_raw()
         check(lib().frk_hip_gemv_dev(self.handle, C.c_void_p(x.data_ptr()), C.c_void_p(y.data_ptr()), act_mode, stream))
@@ -327,7 +328,7 @@ class Weights:
         # (a small product waits for its call: like its input 0.3 us ahead of torch.empty)
         y = out if out is not None else x.new_empty((batch, self.rows))
         if self.kind == FP8_BLOCK:
-            stream = _fp8_stream(x) if out is None else _fp8_stream(x, _fp8_floats(out, batch * self.rows))
+            stream = _fp8_stream(x) if out is None else _fp8_stream(x, (_fp8_floats(torch, out, batch * self.rows),))
         else:
             stream = _stream_raw()
         check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), stream))
@@ -346,7 +347,7 @@ class Weights:
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.shape[-1] == self.cols
         batch = x.numel() // self.cols
         assert out.dtype == torch.float32 and out.is_cuda and out.is_contiguous() and out.numel() == batch * self.rows
-        stream = _fp8_stream(x, out) if self.kind == FP8_BLOCK else _stream_raw()
+        stream = _fp8_stream(x, (out,)) if self.kind == FP8_BLOCK else _stream_raw()
         check(lib().frk_hip_gemm_noalloc_dev(self.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(out.data_ptr()), stream))
         return out
 
@@ -410,7 +411,7 @@ def gemm_pair(w0, w1, x, outs=None):
     batch = x.numel() // w0.cols
     y0, y1 = outs if outs is not None else (torch.empty((batch, w.rows), dtype=torch.float32, device=x.device) for w in (w0, w1))
     if w0.kind == FP8_BLOCK or w1.kind == FP8_BLOCK:
-        stream = _fp8_stream(x) if outs is None else _fp8_stream(x, _fp8_floats(y0, batch * w0.rows), _fp8_floats(y1, batch * w1.rows))
+        stream = _fp8_stream(x) if outs is None else _fp8_stream(x, (_fp8_floats(torch, y0, batch * w0.rows), _fp8_floats(torch, y1, batch * w1.rows)))
     else:
         stream = _stream_raw()
     check(lib().frk_hip_gemm_pair_dev(w0.handle, w1.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(y0.data_ptr()),
@@ -486,8 +487,8 @@ def moe_ffn(gate, up, down, n_experts, x, ids, weights, out=None):
         if x.numel() < batch * gate.cols or weights.numel() < batch * k:
             raise ValueError("%d x %d ids over %d activations and %d weights" % (batch, k, x.numel(), weights.numel()))
         if out is not None:
-            _fp8_floats(out, batch * (down.rows // n_experts))
-        stream = _fp8_stream(x, ids, weights, out)
+            _fp8_floats(torch, out, batch * (down.rows // n_experts))
+        stream = _fp8_stream(x, (ids, weights, out))
     else:
         assert _on_a_gpu(ids) and _on_a_gpu(weights)
         stream = _stream_raw()
@@ -511,8 +512,8 @@ def gemm_grouped(stacked, n_groups, group_off, x, gather=None, out=None):
     y = out if out is not None else x.new_empty((pairs, stacked.rows // n_groups))
     if stacked.kind == FP8_BLOCK:
         if out is not None:
-            _fp8_floats(out, pairs * (stacked.rows // n_groups))
-        stream = _fp8_stream(x, group_off, gather, out)
+            _fp8_floats(torch, out, pairs * (stacked.rows // n_groups))
+        stream = _fp8_stream(x, (group_off, gather, out))
     else:
         stream = _stream_raw()
     check(lib().frk_hip_gemm_grouped_dev(stacked.handle, n_groups, group_off.data_ptr(), gather.data_ptr() if gather is not None else None,
@@ -547,7 +548,7 @@ def gemv_multi(ws, x, outs=None):
     if _any_fp8(*ws):
         if len(ys) != n:
             raise ValueError("%d matrices, %d outputs" % (n, len(ys)))
-        stream = _fp8_stream(_fp8_floats(x, ws[0].cols), *[_fp8_floats(y, w.rows) for w, y in zip(ws, outs or ())])
+        stream = _fp8_stream(_fp8_floats(torch, x, ws[0].cols), [_fp8_floats(torch, y, w.rows) for w, y in zip(ws, outs)] if outs is not None else ())
     else:
         assert _on_a_gpu(x)
         stream = _stream_raw()
@@ -562,7 +563,7 @@ def ffn_swiglu(gate, up, down, x, out=None):
     import torch
     y = out if out is not None else torch.empty(down.rows, dtype=torch.float32, device=x.device)
     if _any_fp8(gate, up, down):
-        stream = _fp8_stream(_fp8_floats(x, gate.cols), None if out is None else _fp8_floats(out, down.rows))
+        stream = _fp8_stream(_fp8_floats(torch, x, gate.cols), () if out is None else (_fp8_floats(torch, out, down.rows),))
     else:
         assert _on_a_gpu(x)
         stream = _stream_raw()
