@@ -2,8 +2,8 @@
 // experts, the top k, their weights.  The reference's counterparts live in crates/frink-moe; its plain softmax router with
 // its f32 arithmetic is route_top_k_softmax_kernel (frk_moe.hip).
 //
-// Scores are doubles: two experts whose scores differ by less than an f32 step are chosen as their logits say, and the same
-// whatever order a sum was added in.
+// Scores are doubles, so that experts whose scores differ by less than an f32 step are told apart; scores that are the same double go by
+// index (sigmoids of logits above 37 are all one).
 #include "frk_device.hpp"
 
 #include <algorithm>

@@ -317,14 +317,15 @@ int frk_hip_route_top_k_softmax_dev(const float *logits_dev, size_t batch, size_
  *            largest c; only experts of the `top_groups` groups of the largest values can be chosen.  1, 1, 1: no groups
  *   the k largest c are chosen, in descending order
  *   weights  the chosen experts' p, divided by their sum when norm != 0, times scale
- * Scores, their sums and comparisons are in 64 bits, so that no rounding of theirs decides between two experts; a weight is rounded to
- * f32 once.  Equal values go to the lower index, of groups too.  An expert whose logit is -inf or NaN has p = 0 and cannot be chosen
- * (a mask;
- * nor can one whose bias is -inf or NaN be chosen), nor counts in its group's value; a group of such experts only is chosen last.
- * Where fewer than k experts are left, the remaining slots get id -1 and weight 0, which frk_hip_moe_ffn_dev skips.  Logits of +inf share a softmax evenly.
+ * Scores, c, the groups' sums and all comparisons are in 64 bits; a weight is rounded to f32 once.  Values that are equal in 64 bits go to the
+ * lower index, of groups too, whatever their logits: a sigmoid is one from a logit of about 37 on and a half at all logits below 2^-53, a
+ * softmax term is zero from 746 below the largest logit on, and c is the bias where that is more than 2^53 times the score.
+ * An expert whose logit is -inf or NaN (a mask) has p = 0, cannot be chosen and does not count in its group's value; nor can one whose bias is -inf or
+ * NaN, nor does it count.  A group of such experts only is chosen last.  Where fewer than k experts are left, the remaining slots get id -1
+ * and weight 0, which frk_hip_moe_ffn_dev skips.  Logits of +inf share a softmax evenly.
  * The reference's routers with sigmoid scores, a bias and groups live in crates/frink-moe; the plain softmax one, whose f32
  * arithmetic a caller may depend on, is frk_hip_route_top_k_softmax_dev.
- * n_experts <= 1024, k <= 64, groups <= 64 and a divisor of n_experts, top_groups * (n_experts / groups) >= k. */
+ * n_experts <= 1024, k <= 64, groups <= 64 and a divisor of n_experts, top_groups * (n_experts / groups) >= k, at most 2^30 tokens. */
 enum { FRK_SCORE_SOFTMAX = 0, FRK_SCORE_SIGMOID = 1 };
 typedef struct {
     int32_t score;      /* FRK_SCORE_* */

@@ -16,3 +16,23 @@ def test_more_tokens_than_a_launch_holds(fa):
     want = 1 / (1 + torch.exp(-(logits[:, 0].double() - logits[:, 1].double()).abs()))
     # (rounded to f32 once, behind a handful of roundings in 64 bits)
     assert bool(((w[:, 0].double() - want).abs() <= want * (2.0 ** -24 + 2.0 ** -45)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rule,logits,bias,chosen", [
+    (dict(score="sigmoid"), {3: 40.0, 9: 60.0, 20: 50.0, 30: 20.0}, None, [3, 9, 20, 30]),          # all one but the last
+    (dict(score="sigmoid"), {i: -900.0 + i for i in range(40)}, None, [0, 1, 2, 3]),                # all zero
+    (dict(score="sigmoid"), {i: (i + 1) * 1e-25 for i in range(40)}, None, [0, 1, 2, 3]),           # all a half
+    (dict(score="softmax"), {i: -800.0 + i for i in range(39)} | {39: 0.0, 38: -1.0}, None, [39, 38, 0, 1]),
+    (dict(score="sigmoid"), {i: i / 8 for i in range(40)}, 2.0 ** 60, [0, 1, 2, 3]),                # the bias alone
+    (dict(score="sigmoid", groups=4, top_groups=2, group_best=2), {5: 40.0, 6: 41.0, 12: 90.0, 13: 90.0, 33: 50.0, 34: 50.0}, None, [5, 6, 12, 13])])
+def test_scores_that_are_equal_in_64_bits_go_by_index(fa, rule, logits, bias, chosen):
+    l = np.full((3, 40), -5.0, np.float32)
+    l[:, list(logits)] = list(logits.values())
+    b = None if bias is None else np.full(40, bias, np.float32)
+    ids, w = fa.route(to_dev(l), 4, bias=None if b is None else to_dev(b), **rule)
+    assert ids.cpu().numpy().tolist() == [chosen] * 3
+    with np.errstate(over="ignore"):
+        want_ids, want = plain.route(l, 4, bias=b, **rule)
+    assert np.array_equal(ids.cpu().numpy(), want_ids)
+    assert (np.abs(w.cpu().numpy() - want) <= want * (2.0 ** -24 + 2.0 ** -45) + 2.0 ** -150).all()
