@@ -138,7 +138,7 @@ int launch_f8_quantize(const float *x, const float *up, size_t rows, size_t cols
 // ---- A few tokens: the weights' bytes and the launch's own chain of steps bound it.  A workgroup of NW wavefronts has one strip of sixteen
 // weight rows and up to 16 TT tokens; its wavefronts share the columns, in order, straight from memory into registers, D blocks
 // ahead, and their sums meet in LDS.
-//   DENSE  strip blockIdx.x, matrix blockIdx.y, token tile blockIdx.z
+//   DENSE  strip blockIdx.x, matrix blockIdx.y, all tokens
 //   PAIRS  strip blockIdx.x, pair blockIdx.y of a grouped product: every sixteenth (FUSED: fourth) pair of its group takes the
 //          group's next sixteen (four), the others end at once.  No list is made in front of it: each wavefront looks the group up itself
 //   SLOTS  strip blockIdx.x, (token, slot) blockIdx.y of an expert layer: the matrix is the slot's expert (FUSED only).  With `up` the strip of
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
         matrix = g.ids ? g.ids[blockIdx.y] : 0, first = blockIdx.y, used = 1;
         if (matrix < 0 || matrix >= g.n_groups) return;  // (adds nothing to its token)
     } else {
-        matrix = blockIdx.y, first = (int)blockIdx.z * 16 * TT, used = min(16 * TT, g.M - first);
+        matrix = blockIdx.y, first = 0, used = min(16 * TT, g.M);
         y_col = (size_t)matrix * g.w.rows;
     }
     const int b0 = (int)((long long)blocks * wave / NW), b1 = (int)((long long)blocks * (wave + 1) / NW);
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
         auto fetch_x = [&](int u, int b) {
 #pragma unroll
             for (int t = 0; t < TT; t++) {
-                const size_t piece = PAIRS ? (size_t)row[t] * blocks + min(b, b1 - 1) : ((size_t)min((first >> 4) + t, (g.x_rows - 1) >> 4) * blocks + min(b, b1 - 1)) * F8_STRIP;
+                const size_t piece = PAIRS ? (size_t)row[t] * blocks + min(b, b1 - 1) : ((size_t)min(t, (g.x_rows - 1) >> 4) * blocks + min(b, b1 - 1)) * F8_STRIP;
                 const uint4 *const at = reinterpret_cast<const uint4 *>(g.a.v + piece * F8_BLOCK) + (PAIRS ? (lane >> 4) * 4 : token[t]);
 #pragma unroll
                 for (int k = 0; k < 4; k++) x[u][t][k] = at[PAIRS ? k : k * 64];
@@ -385,7 +385,8 @@ __global__ __launch_bounds__(64 * NW) void f8_rows_kernel(F8Rows g) {
 
 template <int NW, int TT, int D, bool FUSED, int MODE>
 static int go_f8_rows(const F8Rows &g, const dim3 &grid, size_t lds, hipStream_t s) {
-    if (f8_wide_rows(g.x, (size_t)g.cols)) hipLaunchKernelGGL((f8_rows_kernel<NW, TT, D, FUSED, MODE, true>), grid, dim3(64 * NW), lds, s, g);
+    // (WIDE: how a FUSED one reads x)
+    if (FUSED && f8_wide_rows(g.x, (size_t)g.cols)) hipLaunchKernelGGL((f8_rows_kernel<NW, TT, D, FUSED, MODE, FUSED>), grid, dim3(64 * NW), lds, s, g);
     else hipLaunchKernelGGL((f8_rows_kernel<NW, TT, D, FUSED, MODE, false>), grid, dim3(64 * NW), lds, s, g);
     FRK_LAUNCH_CHECK("f8_rows");
     return FRK_OK;

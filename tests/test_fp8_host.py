@@ -48,6 +48,32 @@ int main() {  // a call a line; its status, the kernels it launched and its erro
             }
             HipStub::get().take();
             printf("%d %zu %zu | %s\n", rc, tokens, most, frk_hip_last_error());
+        } else if (name == "kernels") {  // all there are of this kind, and those of its calls at two alignments of x
+            for (const auto &[handle, kernel] : HipStub::get().names)
+                if (kernel.compare(0, 3, "f8_") == 0 || kernel.find("_f8_") != std::string::npos) HipStub::get().launched.push_back(kernel);
+            tell(0);
+            std::string all;
+            HipStub::get().memory = false;
+            for (const float *x : {room, room + 1})
+                for (size_t cols : {256, 1028, 8192, 70000}) {
+                    frk_weights w, up, down, *fresh = nullptr;
+                    fill(w, FRK_KIND_FP8_BLOCK, 4 * 4096, cols, 4), fill(up, FRK_KIND_FP8_BLOCK, 4 * 4096, cols, 4), fill(down, FRK_KIND_FP8_BLOCK, 4 * cols, 4096, 4);
+                    for (size_t batch : {1, 3, 8, 16, 24, 40, 64, 100, 300, 4000}) {
+                        frk_hip_gemm_dev(&w, x, batch, room, nullptr);
+                        frk_hip_gemm_grouped_dev(&w, 4, (int32_t *)room, nullptr, x, batch, batch, room, nullptr);
+                        frk_hip_moe_ffn_dev(&w, &up, &down, 4, x, batch, (int32_t *)room, room, 2, room, nullptr);
+                    }
+                    frk_weights odd, back;
+                    fill(odd, FRK_KIND_FP8_BLOCK, 4 * 130, cols, 4), fill(back, FRK_KIND_FP8_BLOCK, 4 * cols, 130, 4);
+                    frk_hip_moe_ffn_dev(&odd, &odd, &back, 4, x, 1, (int32_t *)room, room, 2, room, nullptr);
+                    frk_weights one;
+                    fill(one, FRK_KIND_FP8_BLOCK, 64, cols);
+                    for (size_t batch : {20, 40, 64}) frk_hip_gemm_dev(&one, x, batch, room, nullptr);
+                    frk_hip_dequant_dev(&w, room, nullptr);
+                    frk_hip_weights_from_device_fp8((uint8_t *)room, room, 4, cols, 1, nullptr, &fresh);
+                }
+            HipStub::get().memory = true;
+            tell(0);
         } else if (name == "rows") {  // the largest grid of a one-token product, or what registration says
             size_t rows, matrices;
             if (scanf("%zu %zu", &rows, &matrices) != 2) return 1;
@@ -187,3 +213,11 @@ def test_what_no_launch_can_hold_is_refused_before_the_first(said, call, needle)
 def test_what_a_launch_just_holds_is_launched(said, call):
     (rc, (launches, most), error), = said(call)
     assert rc == 0 and int(launches) and int(most) < 1 << 32, error
+
+
+def test_no_kernel_is_built_that_no_call_reaches(said):
+    (_, built, _), (_, launched, _) = said("kernels", lines=2)
+    assert set(built) <= set(launched), set(built) - set(launched)
+    # <wavefronts, tiles of tokens, blocks ahead, quantizes itself, mode, how it then reads x>
+    rows = [n[len("f8_rows_kernel<"):-1].split(",") for n in built if n.startswith("f8_rows_kernel")]
+    assert rows and all(r[5] == "false" for r in rows if r[3] == "false")
