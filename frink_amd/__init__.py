@@ -170,19 +170,17 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _stream_raw():
+def _stream_raw(torch):
     """_stream() for a call over tensors on a GPU, as a number."""
-    import torch
     try:
         return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
     except AttributeError:
         return torch.cuda.current_stream().cuda_stream
 
 
-def _fp8_stream(x, others=()):
+def _fp8_stream(torch, x, others=()):
     """_stream_raw() for a call with FP8_BLOCK weights, or routing by a rule, which refuses tensors of another device than the current one (others: or
     None).  The older kinds' calls take a peer's memory as they always did."""
-    import torch
     try:
         here = torch._C._cuda_getDevice()
         stream = torch._C._cuda_getCurrentRawStream(here)
@@ -270,7 +268,7 @@ class Weights:
         cls._check_fp8(codes.numel(), scales.numel(), rows, cols, matrices)
         h = C.c_void_p()
         check(lib().frk_hip_weights_from_device_fp8(C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), rows, cols,
-                                                    matrices, _fp8_stream(codes), C.byref(h)))
+                                                    matrices, _fp8_stream(torch, codes), C.byref(h)))
         return cls(h, FP8_BLOCK, rows, cols)
 
     def keep_decoded(self):
@@ -297,9 +295,9 @@ class Weights:
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.numel() == self.cols
         y = out if out is not None else torch.empty(self.rows, dtype=torch.float32, device=x.device)
         if self.kind == FP8_BLOCK:
-            stream = _fp8_stream(x) if out is None else _fp8_stream(x, (_fp8_floats(torch, out, self.rows),))
+            stream = _fp8_stream(torch, x) if out is None else _fp8_stream(torch, x, (_fp8_floats(torch, out, self.rows),))
         else:
-            stream = _stream_raw()
+            stream = _stream_raw(torch)
         check(lib().frk_hip_gemv_dev(self.handle, C.c_void_p(x.data_ptr()), C.c_void_p(y.data_ptr()), act_mode, stream))
         return y
 
@@ -328,9 +326,9 @@ class Weights:
         # (a small product waits for its call: like its input 0.3 us ahead of torch.empty)
         y = out if out is not None else x.new_empty((batch, self.rows))
         if self.kind == FP8_BLOCK:
-            stream = _fp8_stream(x) if out is None else _fp8_stream(x, (_fp8_floats(torch, out, batch * self.rows),))
+            stream = _fp8_stream(torch, x) if out is None else _fp8_stream(torch, x, (_fp8_floats(torch, out, batch * self.rows),))
         else:
-            stream = _stream_raw()
+            stream = _stream_raw(torch)
         check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), stream))
         return y
 
@@ -347,7 +345,7 @@ class Weights:
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.shape[-1] == self.cols
         batch = x.numel() // self.cols
         assert out.dtype == torch.float32 and out.is_cuda and out.is_contiguous() and out.numel() == batch * self.rows
-        stream = _fp8_stream(x, (out,)) if self.kind == FP8_BLOCK else _stream_raw()
+        stream = _fp8_stream(torch, x, (out,)) if self.kind == FP8_BLOCK else _stream_raw(torch)
         check(lib().frk_hip_gemm_noalloc_dev(self.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(out.data_ptr()), stream))
         return out
 
@@ -387,7 +385,7 @@ def _get_rows_dev(self, ids):
     assert ids.dtype == torch.int32 and ids.is_cuda and ids.is_contiguous()
     out = torch.empty((ids.numel(), self.cols), dtype=torch.float32, device=ids.device)
     check(lib().frk_hip_get_rows_dev(self.handle, C.c_void_p(ids.data_ptr()), ids.numel(), C.c_void_p(out.data_ptr()),
-                                     _fp8_stream(ids) if self.kind == FP8_BLOCK else _stream()))
+                                     _fp8_stream(torch, ids) if self.kind == FP8_BLOCK else _stream()))
     return out
 
 
@@ -411,9 +409,9 @@ def gemm_pair(w0, w1, x, outs=None):
     batch = x.numel() // w0.cols
     y0, y1 = outs if outs is not None else (torch.empty((batch, w.rows), dtype=torch.float32, device=x.device) for w in (w0, w1))
     if w0.kind == FP8_BLOCK or w1.kind == FP8_BLOCK:
-        stream = _fp8_stream(x) if outs is None else _fp8_stream(x, (_fp8_floats(torch, y0, batch * w0.rows), _fp8_floats(torch, y1, batch * w1.rows)))
+        stream = _fp8_stream(torch, x) if outs is None else _fp8_stream(torch, x, (_fp8_floats(torch, y0, batch * w0.rows), _fp8_floats(torch, y1, batch * w1.rows)))
     else:
-        stream = _stream_raw()
+        stream = _stream_raw(torch)
     check(lib().frk_hip_gemm_pair_dev(w0.handle, w1.handle, C.c_void_p(x.data_ptr()), batch, C.c_void_p(y0.data_ptr()),
                                       C.c_void_p(y1.data_ptr()), stream))
     return y0, y1
@@ -471,7 +469,7 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_b
         raise ValueError("score %r: one of %s" % (score, ", ".join(SCORES)))
     rule = RouteRule(SCORES[score], int(bool(norm)), groups, top_groups, group_best, scale, None if bias is None else bias.data_ptr())
     ids, w = logits.new_empty((batch, k), dtype=torch.int32), logits.new_empty((batch, k))
-    check(lib().frk_hip_route_dev(logits.data_ptr(), batch, n_experts, k, C.byref(rule), ids.data_ptr(), w.data_ptr(), _fp8_stream(logits)))
+    check(lib().frk_hip_route_dev(logits.data_ptr(), batch, n_experts, k, C.byref(rule), ids.data_ptr(), w.data_ptr(), _fp8_stream(torch, logits)))
     return ids, w
 
 
@@ -488,10 +486,10 @@ def moe_ffn(gate, up, down, n_experts, x, ids, weights, out=None):
             raise ValueError("%d x %d ids over %d activations and %d weights" % (batch, k, x.numel(), weights.numel()))
         if out is not None:
             _fp8_floats(torch, out, batch * (down.rows // n_experts))
-        stream = _fp8_stream(x, (ids, weights, out))
+        stream = _fp8_stream(torch, x, (ids, weights, out))
     else:
         assert _on_a_gpu(ids) and _on_a_gpu(weights)
-        stream = _stream_raw()
+        stream = _stream_raw(torch)
     check(lib().frk_hip_moe_ffn_dev(gate.handle, up.handle, down.handle, n_experts, x.data_ptr(), batch, ids.data_ptr(), weights.data_ptr(), k,
                                     y.data_ptr(), stream))
     return y
@@ -513,9 +511,9 @@ def gemm_grouped(stacked, n_groups, group_off, x, gather=None, out=None):
     if stacked.kind == FP8_BLOCK:
         if out is not None:
             _fp8_floats(torch, out, pairs * (stacked.rows // n_groups))
-        stream = _fp8_stream(x, (group_off, gather, out))
+        stream = _fp8_stream(torch, x, (group_off, gather, out))
     else:
-        stream = _stream_raw()
+        stream = _stream_raw(torch)
     check(lib().frk_hip_gemm_grouped_dev(stacked.handle, n_groups, group_off.data_ptr(), gather.data_ptr() if gather is not None else None,
                                          x.data_ptr(), x_rows, pairs, y.data_ptr(), stream))
     return y
@@ -548,10 +546,10 @@ def gemv_multi(ws, x, outs=None):
     if _any_fp8(*ws):
         if len(ys) != n:
             raise ValueError("%d matrices, %d outputs" % (n, len(ys)))
-        stream = _fp8_stream(_fp8_floats(torch, x, ws[0].cols), [_fp8_floats(torch, y, w.rows) for w, y in zip(ws, outs)] if outs is not None else ())
+        stream = _fp8_stream(torch, _fp8_floats(torch, x, ws[0].cols), [_fp8_floats(torch, y, w.rows) for w, y in zip(ws, outs)] if outs is not None else ())
     else:
         assert _on_a_gpu(x)
-        stream = _stream_raw()
+        stream = _stream_raw(torch)
     hs = (C.c_void_p * n)(*[w.handle for w in ws])
     ps = (C.c_void_p * n)(*[y.data_ptr() for y in ys])
     check(lib().frk_hip_gemv_multi_dev(hs, n, C.c_void_p(x.data_ptr()), ps, stream))
@@ -563,10 +561,10 @@ def ffn_swiglu(gate, up, down, x, out=None):
     import torch
     y = out if out is not None else torch.empty(down.rows, dtype=torch.float32, device=x.device)
     if _any_fp8(gate, up, down):
-        stream = _fp8_stream(_fp8_floats(torch, x, gate.cols), () if out is None else (_fp8_floats(torch, out, down.rows),))
+        stream = _fp8_stream(torch, _fp8_floats(torch, x, gate.cols), () if out is None else (_fp8_floats(torch, out, down.rows),))
     else:
         assert _on_a_gpu(x)
-        stream = _stream_raw()
+        stream = _stream_raw(torch)
     check(lib().frk_hip_ffn_swiglu_dev(gate.handle, up.handle, down.handle, C.c_void_p(x.data_ptr()),
                                        C.c_void_p(y.data_ptr()), stream))
     return y
