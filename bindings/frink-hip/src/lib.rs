@@ -290,7 +290,7 @@ impl Weights {
     /// E4M3 codes `[rows][cols]` with an f32 scale for every block of 128 x 128, `matrices` of them stacked.
     pub fn register_fp8(codes: &[u8], scales: &[f32], rows: usize, cols: usize, matrices: usize) -> Result<Self, HipError> {
         let blocks = |n: usize| (n + 127) / 128;
-        if matrices == 0 || codes.len() != rows * cols || scales.len() != matrices * blocks(rows / matrices) * blocks(cols) {
+        if matrices == 0 || rows.checked_mul(cols) != Some(codes.len()) || scales.len() != matrices * blocks(rows / matrices) * blocks(cols) {
             return Err(HipError { status: ERR_SHAPE, message: format!("{} codes, {} scales for {rows} x {cols} in {matrices} matrices", codes.len(), scales.len()) });
         }
         let mut w = std::ptr::null_mut();

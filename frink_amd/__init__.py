@@ -252,8 +252,15 @@ class Weights:
 
     @classmethod
     def from_host_fp8(cls, codes, scales, rows, cols, matrices=1):
-        """E4M3 codes [rows][cols] (numpy uint8) with f32 scales [matrices][ceil(rows / matrices / 128)][ceil(cols / 128)]."""
-        codes, scales = np.ascontiguousarray(codes, np.uint8), np.ascontiguousarray(scales, np.float32)
+        """E4M3 codes [rows][cols] (numpy uint8, or another type of one byte) with f32 scales
+        [matrices][ceil(rows / matrices / 128)][ceil(cols / 128)]."""
+        codes, scales = np.ascontiguousarray(codes), np.ascontiguousarray(scales, np.float32)
+        if codes.dtype.itemsize == 1:  # (as they lie: a conversion of E4M3 numbers would be one of their values)
+            codes = codes.view(np.uint8)
+        elif codes.dtype.kind not in "iu" or codes.size and not 0 <= codes.min() <= codes.max() <= 255:
+            raise ValueError("codes of %s: E4M3 codes are bytes" % codes.dtype)
+        else:
+            codes = codes.astype(np.uint8)
         cls._check_fp8(codes.size, scales.size, rows, cols, matrices)
         h = C.c_void_p()
         check(lib().frk_hip_weights_register_fp8(_np_ptr(codes), _np_ptr(scales), rows, cols, matrices, C.byref(h)))

@@ -183,3 +183,20 @@ def test_operands_without_room_are_refused(fa):
                 call()
     with pytest.raises(ValueError, match="outputs"):
         fa.gemv_multi([w, w], x[0], outs=[y[0]])
+
+
+def test_host_codes_are_bytes():
+    import frink_amd
+    for codes in (np.full((2, 6), 1.5, np.float32), np.full((2, 6), 300), np.full((2, 6), -1)):
+        with pytest.raises(ValueError, match="bytes"):
+            frink_amd.Weights.from_host_fp8(codes, np.ones(1, np.float32), 2, 6)
+
+
+@pytest.mark.gpu
+def test_host_codes_of_any_byte_type(fa):
+    """One byte a code, taken as it lies; whole numbers that are bytes."""
+    codes = np.random.default_rng(1).permutation(256).astype(np.uint8).reshape(4, 64)
+    codes[(codes & 0x7f) == 0x7f] = 0
+    for c in (codes, codes.view(np.int8), codes.astype(np.int64), codes.view(np.dtype("V1"))):
+        got = fa.Weights.from_host_fp8(c, np.full(1, 2.0), 4, 64).dequant().cpu().numpy()
+        assert np.array_equal(got, plain.VALUES[codes].astype(np.float32) * 2)
