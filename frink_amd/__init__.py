@@ -474,6 +474,8 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_b
         assert bias.dtype == torch.float32 and bias.device == logits.device and bias.is_contiguous() and bias.numel() == n_experts
     if score not in SCORES:
         raise ValueError("score %r: one of %s" % (score, ", ".join(SCORES)))
+    if (groups | top_groups | group_best) >> 31:  # (the structure would take their lower 32 bits)
+        raise ValueError("%d groups, %d of them by their %d best" % (groups, top_groups, group_best))
     rule = RouteRule(SCORES[score], int(bool(norm)), groups, top_groups, group_best, scale, None if bias is None else bias.data_ptr())
     ids, w = logits.new_empty((batch, k), dtype=torch.int32), logits.new_empty((batch, k))
     check(lib().frk_hip_route_dev(logits.data_ptr(), batch, n_experts, k, C.byref(rule), ids.data_ptr(), w.data_ptr(), _fp8_stream(torch, logits)))

@@ -36,3 +36,18 @@ def test_scores_that_are_equal_in_64_bits_go_by_index(fa, rule, logits, bias, ch
         want_ids, want = plain.route(l, 4, bias=b, **rule)
     assert np.array_equal(ids.cpu().numpy(), want_ids)
     assert (np.abs(w.cpu().numpy() - want) <= want * (2.0 ** -24 + 2.0 ** -45) + 2.0 ** -150).all()
+
+
+@pytest.mark.parametrize("rule", [dict(groups=2 ** 32 + 1), dict(groups=2, top_groups=2 ** 32 + 2), dict(group_best=2 ** 35 + 1), dict(groups=1 - 2 ** 32)])
+def test_numbers_of_groups_past_32_bits(rule):
+    import types
+
+    import frink_amd
+    import torch
+
+    class Logits(types.SimpleNamespace):
+        def contiguous(self):
+            return self
+    logits = Logits(dtype=torch.float32, is_cuda=True, dim=lambda: 2, shape=(1, 8))
+    with pytest.raises(ValueError, match="groups"):
+        frink_amd.route(logits, 1, **rule)
