@@ -139,8 +139,8 @@ int frk_hip_weights_from_device(int kind, const void *dev_bytes, size_t len, siz
  * (magnitudes above 240 * 2^120, where the next code's value is no float, become that); an infinity or a NaN becomes a NaN and
  * takes no part in that: its output row is NaN.  So
  *   y[t][r] = sum over blocks b of scales[r / 128][b] * 2^e[t][b] * (sum over the block of code * quantized activation),
- * the products exact, the sums in f32, of 2^-16 of their value: the sum in the brackets overflows for no codes and activations.  (Results
- * below 2^-109 in magnitude are exact to some units of 2^-133.) */
+ * the products exact, the sums in f32.  The one in the brackets overflows for no codes and activations (what is summed is 2^-16 of the values:
+ * results below 2^-109 in magnitude are exact to some units of 2^-133). */
 int frk_hip_weights_register_fp8(const uint8_t *host_codes, const float *host_scales, size_t rows, size_t cols, size_t matrices,
                                  frk_weights **out);
 int frk_hip_weights_from_device_fp8(const uint8_t *dev_codes, const float *dev_scales, size_t rows, size_t cols, size_t matrices,

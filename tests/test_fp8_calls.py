@@ -200,3 +200,110 @@ def test_host_codes_of_any_byte_type(fa):
     for c in (codes, codes.view(np.int8), codes.astype(np.int64), codes.view(np.dtype("V1"))):
         got = fa.Weights.from_host_fp8(c, np.full(1, 2.0), 4, 64).dequant().cpu().numpy()
         assert np.array_equal(got, plain.VALUES[codes].astype(np.float32) * 2)
+
+
+@pytest.mark.gpu
+def test_matrices_past_32_bits(fa):
+    """4.8 GB of codes, as one matrix and as a stack: the first and the last rows."""
+    import torch
+    print("fp8, weights past 2^32 bytes", flush=True)
+    rows, cols, stack = 8 * (2 ** 18 + 128), 2304, 8
+    gen = torch.Generator("cuda").manual_seed(1)
+    codes = torch.randint(0, 127, (rows, cols), dtype=torch.uint8, device="cuda", generator=gen)
+    scales = torch.rand((rows // 128, cols // 128), device="cuda", generator=gen) * 2.0 ** -8
+    w = fa.Weights.from_device_fp8(codes, scales, rows, cols)
+    rng = np.random.default_rng(1)
+    x = _activations(rng, 100, cols)
+    picked = [slice(0, 128), slice(rows - 128, rows), slice(rows // 2, rows // 2 + 128)]
+    parts = [(codes[s].cpu().numpy(), scales[s.start // 128:s.start // 128 + 1].cpu().numpy()) for s in picked]
+    for batch in (1, 12, 40, 100):
+        y = w.gemm(to_dev(x[:batch]))
+        for s, p in zip(picked, parts):
+            want, room = plain.product(*p, x[:batch])
+            assert (np.abs(y[:, s].cpu().numpy() - want) <= room).all(), (batch, s)
+    assert np.array_equal(w.get_rows(to_dev(np.array([rows - 1], np.int32))).cpu().numpy()[0], plain.dequant(*parts[1])[-1].astype(np.float32))
+    w = fa.Weights.from_device_fp8(codes, scales, rows, cols, matrices=stack)
+    del codes
+    for pairs in (10, 100):
+        off = np.minimum(np.arange(stack + 1) * (pairs // stack), pairs).astype(np.int32)
+        off[-1] = pairs
+        y = fa.gemm_grouped(w, stack, to_dev(off), to_dev(x[:pairs]))
+        want, room = plain.product(*parts[1], x[off[-2]:pairs])
+        assert (np.abs(y[off[-2]:, -128:].cpu().numpy() - want) <= room).all(), pairs
+
+
+@pytest.mark.gpu
+def test_batches_past_32_bits(fa):
+    """8.9 GB of activations, 4.4 GB quantized, 2^31 results and more: the first and the last tokens."""
+    import torch
+    print("fp8, activations past 2^32 bytes", flush=True)
+    rows, cols, batch = 4160, 4224, 2 ** 19 + 5
+    rng = np.random.default_rng(2)
+    codes, scales = plain.random_matrix(rng, rows, cols)
+    w = _resident(fa, codes, scales)
+    x = torch.randn((batch, cols), device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    y = w.gemm(x)
+    assert y.numel() > 2 ** 31
+    for s in (slice(0, 3), slice(batch // 2, batch // 2 + 3), slice(batch - 7, batch)):
+        want, room = plain.product(codes[0], scales[0], x[s].cpu().numpy())
+        assert (np.abs(y[s].cpu().numpy() - want) <= room).all(), s
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pairs", [34, 300])
+def test_lists_that_point_outside_over_tiles(fa, pairs):
+    """As for a few pairs: offsets are clamped and made non-decreasing, gather entries clamped, rows of no group left as they were."""
+    import torch
+    rng = np.random.default_rng(pairs)
+    codes, scales = plain.random_matrix(rng, 150, 140, matrices=4)
+    x = _activations(rng, 6, 140)
+    w = _resident(fa, codes, scales)
+    gather = rng.integers(-3, 9, pairs).astype(np.int32)
+    gather[[0, 7]] = 2 ** 31 - 1, -2 ** 31
+    for off in ([2, 5, 3, 4, 8], [-7, 4, 100000, 2, 6], [3] * 5, [0, pairs, 0, pairs, 0], [9, 40, 31, 33, pairs - 1], [-2 ** 31, 20, 2 ** 31 - 1, 0, 0]):
+        y = torch.full((pairs, 150), 7.5, device="cuda")
+        fa.gemm_grouped(w, 4, to_dev(np.array(off, np.int32)), to_dev(x), gather=to_dev(gather), out=y)
+        got = y.cpu().numpy()
+        top = np.maximum.accumulate(np.clip(off, 0, pairs))
+        seen = np.zeros(pairs, bool)
+        for g in range(4):
+            s = slice(top[g], top[g + 1])
+            seen[s] = True
+            if top[g + 1] > top[g]:
+                want, room = plain.product(codes[g], scales[g], x[np.clip(gather[s], 0, 5)])
+                assert (np.abs(got[s] - want) <= room).all(), (off, g)
+        assert (got[~seen] == 7.5).all(), off
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,k", [(1, 6), (4, 6), (20, 6), (300, 3)])
+def test_expert_layer_over_any_ids(fa, batch, k):
+    """The same expert twice, ids that are no expert's, tokens without any: what is no expert adds nothing."""
+    from test_fp8_blocks import _layer, _plain_layer
+    rng = np.random.default_rng(batch)
+    experts, hidden, ffn = 8, 260, 132
+    parts, (gate, up, down) = _layer(fa, rng, experts, hidden, ffn)
+    x = _activations(rng, batch, hidden)
+    ids = rng.integers(-2, experts + 2, (batch, k)).astype(np.int32)
+    ids[0, 0], ids[0, 1] = 2 ** 31 - 1, -2 ** 31
+    ids[0, 2:4] = 5 if k > 3 else 1
+    ids[batch // 2] = ids[batch // 2] if batch < 3 else -1
+    weights = rng.standard_normal((batch, k)).astype(np.float32)
+    got = fa.moe_ffn(gate, up, down, experts, to_dev(x), to_dev(ids), to_dev(weights)).cpu().numpy()
+    want, room = _plain_layer(parts, x, ids, weights)
+    assert (np.abs(got - want) <= room * 1.01).all()
+    if batch > 2:
+        assert (got[batch // 2] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,batch", [(517, 4100, 70), (1000, 8192, 130), (999, 7000, 300)])
+def test_shares_of_the_columns_into_unaligned_outputs(fa, rows, cols, batch):
+    import torch
+    rng = np.random.default_rng(rows)
+    w = _resident(fa, *plain.random_matrix(rng, rows, cols))
+    x = to_dev(_activations(rng, batch, cols))
+    want = w.gemm(x)
+    y = torch.full((batch * rows + 2,), 3.0, device="cuda")
+    w.gemm(x, out=y[1:-1])
+    assert torch.equal(y[1:-1].view(batch, rows), want) and float(y[0]) == 3.0 and float(y[-1]) == 3.0
