@@ -534,6 +534,8 @@ __global__ __launch_bounds__(1024) void f8_tiles_quantize_kernel(F8TilesArgs a, 
 static size_t f8_max_tiles(size_t pairs, size_t groups, int tokens) { return pairs / (size_t)tokens + std::min(groups, pairs); }
 // Measured in us with tiles of 256x128 / 256x64 / 128x32 (weight rows x pairs): 32 groups of 2880 x 2880 and 256 pairs each on average 188 / 180 / 243, 64
 // 95 / 98 / 96, 32 88 / 68 / 75, 16 85 / 64 / 60; 128 of 768 x 2048 and 128 pairs 108 / 85 / 105, 32 68 / 54 / 59, 16 64 / 50 / 46, 4 63 / 47 / 42.
+// Large groups, 256x128 / 256x64: 32 of 2880 x 2880 and 1024 pairs 612 / 590, 8 of 1792 x 4096 and 512 105 / 68, 1024 123 / 121, 8 of 14336 x 4096 and 512 483 / 475,
+// 1024 889 / 896, 4 of 4096 x 4096 and 2048 269 / 247.
 int f8_grouped_shape(size_t pairs, size_t groups) { return pairs >= 24 * groups ? F8_TILE_256x64 : F8_TILE_128x32; }
 // A few pairs: a launch that looks the groups up itself.  In us, so / by tiles, a token's pairs over different groups: 128 groups of 768 x 2048, 16 pairs 8.0 /
 // 16.5, 32 14.5 / 16.9, 48 19.6 / 20.3, 64 24.2 / 23.0; 32 of 2880 x 2880, 16 pairs 25.0 / 33.2, 32 40.1 / 39.8, 48 53.4 / 49.8; 8 of 1792 x 4096, 16 15.0 / 26.0.
