@@ -128,7 +128,8 @@ int frk_hip_weights_from_device(int kind, const void *dev_bytes, size_t len, siz
  * frk_hip_weights_register it keeps no cache), from_device buffers on the current device (copied on `stream`; they may be
  * freed once the stream has passed the call).  A call over such a handle while another device is the current one returns FRK_ERR_ARG,
  * and so do register and frk_hip_get_rows on another device than the host-buffer calls' (the one that was current at the first).  The resident copy pads rows to 16 and columns to 128.  At most 2^27 - 16 rows a matrix, 2^23 columns and 65535
- * matrices; a gathered product's activations, two bytes a value quantized, at most 4 GiB.
+ * matrices; a gathered product's activations, two bytes a value quantized, at most 4 GiB; an expert layer's batch
+ * at most 2^24 - 1 tokens.  (What no launch can hold is FRK_ERR_SHAPE before the first.)
  *
  * What takes such a handle, f32 in and f32 out as for the other kinds: frk_hip_gemv_dev (FRK_ACT_F32 and FRK_ACT_INT8 are the
  * same here), frk_hip_gemv_multi_dev, frk_hip_ffn_swiglu_dev, frk_hip_gemm_dev, frk_hip_gemm_pair_dev,
