@@ -19,6 +19,7 @@ Q5_0, IQ4_XS, MXFP4 = 6, 23, 39
 # 8-bit floating point (OCP E4M3) with an f32 scale for every block of 128 x 128: no GGUF kind (Weights.from_device_fp8)
 FP8_BLOCK = 256
 SCORES = {"softmax": 0, "sigmoid": 1}
+ACTS_FORMS = {"q8_k": 0, "fp8": 1, "mxfp4": 2}  # how a BatchActs holds its rows
 KIND_NAME = {Q4_0: "Q4_0", Q8_0: "Q8_0", Q4_K: "Q4_K", Q5_K: "Q5_K", Q6_K: "Q6_K", Q5_0: "Q5_0", IQ4_XS: "IQ4_XS", MXFP4: "MXFP4"}
 BLOCK = {Q4_0: (18, 32), Q8_0: (34, 32), Q4_K: (144, 256), Q5_K: (176, 256), Q6_K: (210, 256),
          Q5_0: (22, 32), IQ4_XS: (136, 256), MXFP4: (17, 32)}  # (block_bytes, block_elems)
@@ -40,6 +41,8 @@ EXPORTS = [
     "frk_hip_get_rows_dev", "frk_hip_get_rows",
     "frk_hip_copy_dev", "frk_hip_read_dev", "frk_hip_issue_probe", "frk_hip_read_shape_dev", "frk_hip_gemm_grouped_dev",
     "frk_hip_weights_register_fp8", "frk_hip_weights_from_device_fp8", "frk_hip_route_dev",
+    "frk_hip_batch_acts_create_form", "frk_hip_batch_acts_values_dev", "frk_hip_rms_norm_dev", "frk_hip_quantize_mxfp4_dev",
+    "frk_hip_dequantize_mxfp4_dev", "frk_hip_gemm_mxfp4_dev",
 ]
 
 
@@ -123,6 +126,12 @@ def lib():
             "frk_hip_weights_register_fp8": (i, [vp, vp, sz, sz, sz, C.POINTER(vp)]),
             "frk_hip_weights_from_device_fp8": (i, [vp, vp, sz, sz, sz, vp, C.POINTER(vp)]),
             "frk_hip_route_dev": (i, [vp, sz, sz, sz, C.POINTER(RouteRule), vp, vp, vp]),
+            "frk_hip_batch_acts_create_form": (i, [sz, sz, i, C.POINTER(vp)]),
+            "frk_hip_batch_acts_values_dev": (i, [vp, vp, vp]),
+            "frk_hip_rms_norm_dev": (i, [i, vp, vp, i, vp, C.c_double, sz, sz, vp, vp, vp, vp]),
+            "frk_hip_quantize_mxfp4_dev": (i, [i, vp, sz, vp, vp]),
+            "frk_hip_dequantize_mxfp4_dev": (i, [vp, sz, vp, vp]),
+            "frk_hip_gemm_mxfp4_dev": (i, [vp, vp, sz, vp, vp]),
             "frk_hip_read_shape_dev": (i, [vp, sz, vp, i, i, i, i, vp]),
         }
         for name, (res, args) in sig.items():
@@ -339,9 +348,23 @@ class Weights:
         check(lib().frk_hip_gemm_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), stream))
         return y
 
+    def gemm_mxfp4(self, x, out=None):
+        """An MXFP4 matrix over x[batch][cols] f32 quantized to MXFP4 within the call (frk_hip_gemm_mxfp4_dev)."""
+        import torch
+        _float_type(torch, x, "f32")
+        if x.dim() == 0 or x.shape[-1] != self.cols:
+            raise ValueError("activations %s: the matrix has %d columns" % (tuple(x.shape), self.cols))
+        batch = x.numel() // self.cols
+        y = out if out is not None else x.new_empty((batch, self.rows))
+        stream = _fp8_stream(torch, x) if out is None else _fp8_stream(torch, x, (_fp8_floats(torch, out, batch * self.rows),))
+        check(lib().frk_hip_gemm_mxfp4_dev(self.handle, x.data_ptr(), batch, y.data_ptr(), stream))
+        return y
+
     def gemm_acts(self, acts, out=None):
         """apply_batch_with_acts: this matrix over a batch that a BatchActs holds quantized."""
         import torch
+        if acts.form != "q8_k" and out is not None:
+            _fp8_floats(torch, out, acts.batch * self.rows)
         y = out if out is not None else torch.empty((acts.batch, self.rows), dtype=torch.float32, device="cuda")
         check(lib().frk_hip_gemm_acts_dev(self.handle, acts.handle, C.c_void_p(y.data_ptr()), _stream()))
         return y
@@ -365,25 +388,126 @@ class Weights:
 
 class BatchActs:
     """A batch's activations quantized once for any number of matrices (the reference's BatchActs::Q8K):
-    frk_hip_batch_acts_create / frk_hip_quantize_batch_acts_dev / frk_hip_batch_acts_release."""
+    frk_hip_batch_acts_create_form / frk_hip_quantize_batch_acts_dev / frk_hip_batch_acts_release.  form: "q8_k" for the K-quants,
+    "fp8" for FP8_BLOCK, "mxfp4" for MXFP4 matrices."""
 
-    def __init__(self, max_batch, cols):
+    def __init__(self, max_batch, cols, form="q8_k"):
+        self.handle = None
+        if form not in ACTS_FORMS:
+            raise ValueError("form %r: one of %s" % (form, ", ".join(ACTS_FORMS)))
         h = C.c_void_p()
-        check(lib().frk_hip_batch_acts_create(max_batch, cols, C.byref(h)))
-        self.handle, self.max_batch, self.cols, self.batch = h, max_batch, cols, 0
+        check(lib().frk_hip_batch_acts_create_form(max_batch, cols, ACTS_FORMS[form], C.byref(h)))
+        self.handle, self.max_batch, self.cols, self.form, self.batch = h, max_batch, cols, form, 0
 
     def quantize(self, x):
         import torch
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.shape[-1] == self.cols
         batch = x.numel() // self.cols
-        check(lib().frk_hip_quantize_batch_acts_dev(self.handle, C.c_void_p(x.data_ptr()), batch, _stream()))
+        stream = _stream() if self.form == "q8_k" else _fp8_stream(torch, x)
+        check(lib().frk_hip_quantize_batch_acts_dev(self.handle, C.c_void_p(x.data_ptr()), batch, stream))
         self.batch = batch
         return self
+
+    def values(self, out=None):
+        """The numbers that the quantized batch stands for, [batch][cols] f32."""
+        import torch
+        if out is not None:
+            _fp8_floats(torch, out, self.batch * self.cols)
+        y = out if out is not None else torch.empty((self.batch, self.cols), dtype=torch.float32, device="cuda")
+        check(lib().frk_hip_batch_acts_values_dev(self.handle, y.data_ptr(), _fp8_stream(torch, y)))
+        return y
 
     def release(self):
         if self.handle:
             check(lib().frk_hip_batch_acts_release(self.handle))
             self.handle = None
+
+    def __del__(self):  # (not "q8_k": a graph captured over such an object may live longer, and always could)
+        try:
+            if self.handle and _lib is not None and self.form != "q8_k":
+                _lib.frk_hip_batch_acts_release(self.handle)
+                self.handle = None
+        except Exception:
+            pass
+
+
+def _float_types(torch):
+    global _FLOAT_TYPES
+    if _FLOAT_TYPES is None:
+        _FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    return _FLOAT_TYPES
+
+
+_FLOAT_TYPES = None  # torch's types -> FRK_TYPE_*
+
+
+def _float_type(torch, t, which="f32, bf16 or f16"):
+    """FRK_TYPE_* of a contiguous tensor on a GPU."""
+    kind = _float_types(torch).get(t.dtype)
+    if kind is None or (which == "f32" and kind) or not t.is_cuda or not t.is_contiguous():
+        raise ValueError("%s of %s on %s: contiguous %s on a GPU" % (tuple(t.shape), t.dtype, t.device, which))
+    return kind
+
+
+def rms_norm(x, weight=None, eps=1e-5, residual=None, out=None, sum_out=None, acts=None):
+    """frk_hip_rms_norm_dev: (y, h) with h = x + residual (x itself without one) and y = h / sqrt(mean(h^2) + eps) * weight over the
+    last dimension of x (f32, bf16 or f16; weight of any of them).  h goes to `sum_out` (which may be x or residual), y to `out`, both of x's
+    type and shape; with `acts` y is quantized into that BatchActs, which is returned in y's place (and y written only where `out` is given)."""
+    import torch
+    kind = _float_type(torch, x)
+    cols = x.shape[-1] if x.dim() else 0
+    if cols == 0 or x.numel() == 0:
+        raise ValueError("activations %s" % (tuple(x.shape),))
+    batch = x.numel() // cols
+    weight_kind = 0
+    if weight is not None:
+        weight_kind = _float_type(torch, weight)
+        if weight.numel() != cols:
+            raise ValueError("%d weights for rows of %d columns" % (weight.numel(), cols))
+    if residual is not None and sum_out is None:
+        sum_out = torch.empty_like(x)
+    if out is None and acts is None:
+        out = torch.empty_like(x)
+    for t in (residual, sum_out, out):
+        if t is not None and (t.dtype is not x.dtype or t.numel() != x.numel() or not t.is_contiguous()):
+            raise ValueError("%s of %s beside activations %s of %s" % (tuple(t.shape), t.dtype, tuple(x.shape), x.dtype))
+    stream = _fp8_stream(torch, x, (weight, residual, sum_out, out))
+    if acts is not None:
+        acts.batch = 0
+    check(lib().frk_hip_rms_norm_dev(kind, x.data_ptr(), None if residual is None else residual.data_ptr(), weight_kind,
+                                     None if weight is None else weight.data_ptr(), eps, batch, cols, None if sum_out is None else sum_out.data_ptr(),
+                                     None if out is None else out.data_ptr(), None if acts is None else acts.handle, stream))
+    if acts is not None:
+        acts.batch = batch
+    return out if acts is None else acts, x if sum_out is None else sum_out
+
+
+def quantize_mxfp4(x, out=None):
+    """frk_hip_quantize_mxfp4_dev: x[..., cols] (f32, bf16 or f16; cols a multiple of 32) as GGUF's MXFP4 blocks, uint8 [..., cols / 32 * 17]:
+    what Weights.from_device(MXFP4, ...) and a GGUF file take."""
+    import torch
+    kind = _float_type(torch, x)
+    if x.dim() == 0 or x.numel() == 0 or x.shape[-1] % 32:
+        raise ValueError("activations %s: a multiple of 32 columns" % (tuple(x.shape),))
+    shape = tuple(x.shape[:-1]) + (x.shape[-1] // 32 * 17,)
+    if out is not None and (out.dtype is not torch.uint8 or out.numel() != x.numel() // 32 * 17 or not out.is_contiguous()):
+        raise ValueError("%s of %s for %d blocks of 17 bytes" % (tuple(out.shape), out.dtype, x.numel() // 32))
+    blocks = out if out is not None else x.new_empty(shape, dtype=torch.uint8)
+    check(lib().frk_hip_quantize_mxfp4_dev(kind, x.data_ptr(), x.numel(), blocks.data_ptr(), _fp8_stream(torch, x, (blocks,))))
+    return blocks
+
+
+def dequantize_mxfp4(blocks, cols):
+    """frk_hip_dequantize_mxfp4_dev: the values of GGUF MXFP4 blocks (uint8), f32 [rows][cols]."""
+    import torch
+    if blocks.dtype is not torch.uint8 or not blocks.is_cuda or not blocks.is_contiguous():
+        raise ValueError("%s of %s on %s: contiguous bytes on a GPU" % (tuple(blocks.shape), blocks.dtype, blocks.device))
+    if cols <= 0 or cols % 32 or blocks.numel() == 0 or blocks.numel() % (cols // 32 * 17):
+        raise ValueError("%d bytes do not make rows of %d columns" % (blocks.numel(), cols))
+    rows = blocks.numel() // (cols // 32 * 17)
+    out = blocks.new_empty((rows, cols), dtype=torch.float32)
+    check(lib().frk_hip_dequantize_mxfp4_dev(blocks.data_ptr(), rows * cols, out.data_ptr(), _fp8_stream(torch, blocks)))
+    return out
 
 
 def _get_rows_dev(self, ids):

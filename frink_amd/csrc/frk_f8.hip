@@ -392,7 +392,6 @@ static int go_f8_rows(const F8Rows &g, const dim3 &grid, size_t lds, hipStream_t
     return FRK_OK;
 }
 
-constexpr size_t F8_ROWS_TOKENS = 64;  // most of the rows kernel
 static bool f8_fused_fits(size_t tokens, size_t cols) { return tokens * f8_blocks(cols) * F8_BLOCK * 2 <= F8_FUSED_LDS; }
 // Of a dense batch: up to four tokens; up to eight where the strips are one round of the chip and a token's quantization, which every workgroup
 // does, is short.  In us, so / with a launch for it (rows x columns): 4096 x 4096 one token 5.6 / 8.7, four 7.6 / 9.1, six 9.0 / 9.2; 2880 x 2880 four 6.6 / 8.4, six
@@ -407,9 +406,9 @@ static bool f8_fused(size_t tokens, const frk_weights *w, const F8Mat &m) {
 // columns cost a second launch, 3.3 us, and the traffic of the parts.  Every kernel, tile and number of shares timed at 35 sizes (24 to 4096
 // tokens, 576 x 7168 to 14336 x 4096): the choice is within 4 % of the fastest but for 512 tokens of 4096 x 14336 (74 against 71 us), 1500 of 2048 x 2048 (27.7
 // against 26.1) and 384 of 4096 x 4096 (32.2 against 28.8).
-F8Plan f8_plan(const frk_weights *w, size_t batch) {
+F8Plan f8_plan(const frk_weights *w, size_t batch, bool quantized) {
     const F8Mat m = f8_mat(w);
-    F8Plan best{-1, 1, f8_fused(batch, w, m), 0, 0};
+    F8Plan best{-1, 1, !quantized && f8_fused(batch, w, m), 0, 0};
     if (best.fused) return best;
     best.acts_bytes = f8_acts_bytes(batch, w->cols);
     if (batch <= 16) return best;  // (the tiles hold 32 tokens and more)

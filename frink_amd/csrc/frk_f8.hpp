@@ -68,6 +68,11 @@ static inline F8Acts f8_acts_carve(void *base, size_t rows, bool strips = false)
     return a;
 }
 
+// where column `in` of block b of a row lies in strips
+__device__ __forceinline__ size_t f8_strip_at(size_t row, int b, int in, int blocks) {
+    return ((row >> 4) * blocks + b) * (F8_STRIP * F8_BLOCK) + (size_t)((in >> 3 & 3) * 512 + ((in >> 5) * 16 + (row & 15)) * 8 + (in & 7));
+}
+
 // ---- quantization: 32 lanes a block, four neighbouring values each (whole lines a load, and a store of eight bytes a lane) ----
 __device__ __forceinline__ uint32_t f8_half_max(uint32_t v) {  // over 32 lanes
     v = max(v, (uint32_t)dpp_i<DPP_QUAD_XOR1>((int)v));
@@ -176,7 +181,7 @@ __device__ __forceinline__ void f8_quantize_blocks(const float *__restrict__ x, 
         float scale;
         const uint32_t codes = f8_quantize4(v[i], scale);
         const int b = first + 2 * i + (lane >> 5), in = (lane & 31) * 4;
-        const size_t at = out.strips ? ((row >> 4) * blocks + b) * (F8_STRIP * F8_BLOCK) + (size_t)((in >> 3 & 3) * 512 + ((in >> 5) * 16 + (row & 15)) * 8 + (in & 7))
+        const size_t at = out.strips ? f8_strip_at(row, b, in, blocks)
                                      : (row * blocks + b) * F8_BLOCK + in;
         if (b < blocks) *reinterpret_cast<uint2 *>(out.v + at) = f8_to_bf16(codes, scale);
     }
@@ -210,7 +215,8 @@ struct F8Plan {
     bool fused;
     size_t acts_bytes, parts_bytes;  // of scratch memory
 };
-F8Plan f8_plan(const frk_weights *w, size_t batch);
+constexpr size_t F8_ROWS_TOKENS = 64;  // most of the rows kernel
+F8Plan f8_plan(const frk_weights *w, size_t batch, bool quantized = false);  // quantized: never `fused`
 
 // ---- entry points for the runtime and the expert layers ----
 int f8_on_current_device(const frk_weights *w);  // a status: what every entry point refuses before it launches anything

@@ -1,0 +1,355 @@
+// MXFP4 (frk_mx4.hpp has the mathematics): quantization to rows and to GGUF blocks, the values back, and the products of a few tokens
+// over MXFP4 matrices as they are stored.
+#include "frk_mx4.hpp"
+
+#include <algorithm>
+
+namespace frk {
+
+typedef int mx4_v4i __attribute__((ext_vector_type(4)));
+typedef int mx4_v8i __attribute__((ext_vector_type(8)));
+typedef float mx4_v4f __attribute__((ext_vector_type(4)));
+
+#define FRK_LAUNCH_CHECK(what)                                                                          \
+    do {                                                                                                \
+        hipError_t e_ = hipGetLastError();                                                              \
+        if (e_ != hipSuccess) return set_error(FRK_ERR_HIP, what " launch: %s", hipGetErrorString(e_)); \
+    } while (0)
+
+// ---- a batch's rows: a wavefront four chunks of 256 columns at a time ----
+constexpr int MX4_CHUNKS = 4;
+template <bool WIDE>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(const float *__restrict__ x, size_t jobs, int jobs_a_row, int cols, Mx4Acts out) {
+    const int lane = threadIdx.x & 63, chunks = out.blocks / 8;
+    for (size_t j = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); j < jobs; j += (size_t)gridDim.x * 4) {
+        const size_t row = j / jobs_a_row;
+        const int first = (int)(j % jobs_a_row) * MX4_CHUNKS;
+        float v[MX4_CHUNKS][4];
+#pragma unroll
+        for (int i = 0; i < MX4_CHUNKS; i++) floats_load4<FLOATS_F32, WIDE>(x + row * (size_t)cols, (first + i) * 256 + lane * 4, cols, v[i]);
+#pragma unroll
+        for (int i = 0; i < MX4_CHUNKS; i++)
+            if (first + i < chunks) mx4_store_chunk(out, row, first + i, lane, v[i]);  // (uniform)
+    }
+}
+int launch_mx4_quantize(const float *x, size_t rows, size_t cols, const Mx4Acts &out, hipStream_t s) {
+    const int jobs_a_row = (out.blocks / 8 + MX4_CHUNKS - 1) / MX4_CHUNKS;
+    const size_t jobs = rows * jobs_a_row;
+    if (jobs == 0) return FRK_OK;
+    const dim3 grid((unsigned)std::min<size_t>((jobs + 3) / 4, 1 << 16));
+    if (floats_wide(x, cols, FLOATS_F32)) hipLaunchKernelGGL(mx4_quantize_kernel<true>, grid, dim3(256), 0, s, x, jobs, jobs_a_row, (int)cols, out);
+    else hipLaunchKernelGGL(mx4_quantize_kernel<false>, grid, dim3(256), 0, s, x, jobs, jobs_a_row, (int)cols, out);
+    FRK_LAUNCH_CHECK("mx4_quantize");
+    return FRK_OK;
+}
+
+// out[row][k]: what the quantized rows stand for
+__global__ __launch_bounds__(256) void mx4_values_kernel(Mx4Acts a, int cols, size_t n, float *__restrict__ out) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const size_t row = i / cols;
+        const int k = (int)(i % cols), in = k % MX4_BLOCK;
+        const size_t block = row * a.blocks + k / MX4_BLOCK;
+        out[i] = mx4_value(a.codes[block * 16 + (in & 15)] >> (in & 16 ? 4 : 0) & 15u, a.scales[block]);
+    }
+}
+int launch_mx4_values(const Mx4Acts &a, size_t cols, float *out, hipStream_t s) {
+    const size_t n = (size_t)a.rows * cols;
+    hipLaunchKernelGGL(mx4_values_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1 << 16)), dim3(256), 0, s, a, (int)cols, n, out);
+    FRK_LAUNCH_CHECK("mx4_values");
+    return FRK_OK;
+}
+
+// ---- GGUF blocks: the scale byte, then sixteen bytes of codes.  128 of them are 2176 bytes, 136 pieces of sixteen: a workgroup puts them
+// together in LDS. ----
+constexpr int GGUF_BLOCKS = 128;
+template <int TYPE, bool WIDE>
+__global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const typename Floats<TYPE>::type *__restrict__ x, size_t blocks, uint8_t *__restrict__ out, bool whole) {
+    __shared__ __align__(16) uint8_t lds[GGUF_BLOCKS * MXFP4_BYTES];
+    const int part = threadIdx.x & 3;
+    for (size_t first = (size_t)blockIdx.x * GGUF_BLOCKS; first < blocks; first += (size_t)gridDim.x * GGUF_BLOCKS) {
+        float lo[2][4], hi[2][4];  // four lanes a block, elements 4 part .. and 16 + 4 part ..
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const size_t b = first + i * 64 + (threadIdx.x >> 2);
+            const int left = b < blocks ? MX4_BLOCK : 0;
+            floats_load4<TYPE, WIDE>(x + b * MX4_BLOCK, 4 * part, left, lo[i]);
+            floats_load4<TYPE, WIDE>(x + b * MX4_BLOCK, 16 + 4 * part, left, hi[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            uint32_t top = max(mx4_top4(lo[i]), mx4_top4(hi[i]));
+            top = max(top, (uint32_t)dpp_i<DPP_QUAD_XOR1>((int)top));
+            top = max(top, (uint32_t)dpp_i<DPP_QUAD_XOR2>((int)top));
+            const uint32_t by = mx4_scale_byte(top);
+            const uint32_t codes = mx4_codes4(lo[i], by) | mx4_codes4(hi[i], by) << 4;
+            uint8_t *const to = lds + (i * 64 + (threadIdx.x >> 2)) * MXFP4_BYTES;
+            if (part == 0) to[0] = (uint8_t)by;
+#pragma unroll
+            for (int j = 0; j < 4; j++) to[1 + 4 * part + j] = (uint8_t)(codes >> (8 * j));
+        }
+        __syncthreads();
+        const size_t bytes = (blocks - first < GGUF_BLOCKS ? blocks - first : GGUF_BLOCKS) * MXFP4_BYTES;
+        uint8_t *const to = out + first * MXFP4_BYTES;
+        if (whole && bytes == sizeof lds) {
+            if (threadIdx.x < sizeof lds / 16) reinterpret_cast<uint4 *>(to)[threadIdx.x] = reinterpret_cast<const uint4 *>(lds)[threadIdx.x];
+        } else {
+            for (size_t i = threadIdx.x; i < bytes; i += 256) to[i] = lds[i];
+        }
+        __syncthreads();
+    }
+}
+template <int TYPE>
+static int go_quantize_mxfp4(const void *x, size_t blocks, uint8_t *out, hipStream_t s) {
+    typedef typename Floats<TYPE>::type T;
+    const dim3 grid((unsigned)std::min<size_t>((blocks + GGUF_BLOCKS - 1) / GGUF_BLOCKS, 1 << 16));
+    const bool whole = (uintptr_t)out % 16 == 0;
+    if (floats_wide(x, MX4_BLOCK, TYPE)) hipLaunchKernelGGL((quantize_mxfp4_kernel<TYPE, true>), grid, dim3(256), 0, s, (const T *)x, blocks, out, whole);
+    else hipLaunchKernelGGL((quantize_mxfp4_kernel<TYPE, false>), grid, dim3(256), 0, s, (const T *)x, blocks, out, whole);
+    FRK_LAUNCH_CHECK("quantize_mxfp4");
+    return FRK_OK;
+}
+int launch_quantize_mxfp4(int type, const void *x, size_t n, uint8_t *blocks, hipStream_t s) {
+    switch (type) {
+    case FLOATS_F32: return go_quantize_mxfp4<FLOATS_F32>(x, n / MX4_BLOCK, blocks, s);
+    case FLOATS_BF16: return go_quantize_mxfp4<FLOATS_BF16>(x, n / MX4_BLOCK, blocks, s);
+    default: return go_quantize_mxfp4<FLOATS_F16>(x, n / MX4_BLOCK, blocks, s);
+    }
+}
+__global__ __launch_bounds__(256) void dequantize_mxfp4_kernel(const uint8_t *__restrict__ in, size_t blocks, float *__restrict__ out, bool whole, bool wide) {
+    __shared__ __align__(16) uint8_t lds[GGUF_BLOCKS * MXFP4_BYTES];
+    for (size_t first = (size_t)blockIdx.x * GGUF_BLOCKS; first < blocks; first += (size_t)gridDim.x * GGUF_BLOCKS) {
+        const int n = (int)(blocks - first < GGUF_BLOCKS ? blocks - first : GGUF_BLOCKS);
+        const uint8_t *const from = in + first * MXFP4_BYTES;
+        if (whole && n == GGUF_BLOCKS) {
+            if (threadIdx.x < sizeof lds / 16) reinterpret_cast<uint4 *>(lds)[threadIdx.x] = reinterpret_cast<const uint4 *>(from)[threadIdx.x];
+        } else {
+            for (int i = threadIdx.x; i < n * MXFP4_BYTES; i += 256) lds[i] = from[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < GGUF_BLOCKS * 8 / 256; i++) {
+            const int four = i * 256 + (int)threadIdx.x, b = four >> 3, in4 = four & 3;  // four elements: 4 in4 .., of the upper half if (four & 4)
+            if (b >= n) break;
+            const uint8_t *const block = lds + b * MXFP4_BYTES;
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = mx4_value(block[1 + 4 * in4 + j] >> (four & 4) & 15u, block[0]);
+            float *const to = out + first * MX4_BLOCK + (size_t)four * 4;
+            if (wide) *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+            else to[0] = v[0], to[1] = v[1], to[2] = v[2], to[3] = v[3];
+        }
+        __syncthreads();
+    }
+}
+int launch_dequantize_mxfp4(const uint8_t *blocks, size_t n, float *out, hipStream_t s) {
+    const size_t nb = n / MX4_BLOCK;
+    hipLaunchKernelGGL(dequantize_mxfp4_kernel, dim3((unsigned)std::min<size_t>((nb + GGUF_BLOCKS - 1) / GGUF_BLOCKS, 1 << 16)), dim3(256), 0, s, blocks, nb, out,
+                       (uintptr_t)blocks % 16 == 0, (uintptr_t)out % 16 == 0);
+    FRK_LAUNCH_CHECK("dequantize_mxfp4");
+    return FRK_OK;
+}
+
+// ---- A few tokens: the weights' bytes bound it.  A workgroup of NW wavefronts has sixteen weight rows and up to 16 TT tokens; its
+// wavefronts share the columns, 512 at a time (a unit: sixteen blocks of a row, 64 bytes a lane in one piece, and a dword of scale bytes), and
+// their sums meet in LDS.  Lane l has weight row l % 16 and blocks 4 (l / 16) .. + 3 of a unit; product k of four takes block k of each lane.
+// FUSED: up to four tokens are quantized by the workgroup itself, a wavefront its own columns'. ----
+struct Mx4Rows {
+    Mx4Gemm g;
+    const float *x;  // FUSED
+    int cols;
+};
+constexpr int MX4_UNIT = 16, MX4_FUSED = 4;           // blocks; tokens
+constexpr int MX4_FUSED_UNIT = MX4_UNIT * 16 + MX4_UNIT;  // bytes of LDS a token and unit
+constexpr size_t MX4_FUSED_LDS = 40 * 1024;
+
+template <int NW, int TT, bool FUSED, bool WIDE>
+__global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int E2M1 = 4, D = TT >= 4 ? 1 : 2;  // units ahead
+    extern __shared__ __align__(16) uint8_t mx4_rows_lds[];  // FUSED: [units][tokens][MX4_FUSED_UNIT]
+    __shared__ float4 sums[NW][TT][64];
+    const Mx4Gemm &g = r.g;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int li = lane & 15, lg = lane >> 4;
+    const int units = (g.blocks + MX4_UNIT - 1) / MX4_UNIT, strip = blockIdx.x;
+    const int u0 = units * wave / NW, u1 = units * (wave + 1) / NW;
+    const uint8_t *const row = g.W + (size_t)min(strip * 16 + li, g.rows - 1) * g.row_stride;
+    const uint8_t *const row_scales = row + (size_t)g.blocks * 16;
+    mx4_v4f acc[TT];
+#pragma unroll
+    for (int t = 0; t < TT; t++) acc[t] = mx4_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (u0 < u1) {
+        uint4 w[D][4], x[FUSED ? 1 : D][TT][4];
+        uint32_t ws[D], xs[FUSED ? 1 : D][TT];
+        auto fetch_w = [&](int d, int u) {
+            u = min(u, u1 - 1);
+            // (blocks past the row's last: the last one's codes, which meet zeros)
+#pragma unroll
+            for (int k = 0; k < 4; k++) w[d][k] = stream_load16(row + (size_t)min(u * MX4_UNIT + 4 * lg + k, g.blocks - 1) * 16);
+            const int live = g.blocks - (u * MX4_UNIT + 4 * lg);
+            const uint32_t four = *reinterpret_cast<const uint32_t *>(row_scales + (live > 0 ? u * MX4_UNIT + 4 * lg : 0));
+            ws[d] = live >= 4 ? four : live > 0 ? four & (0xffffffffu >> (32 - 8 * live)) : 0u;
+        };
+        auto fetch_x = [&](int d, int u) {
+            u = min(u, u1 - 1);
+#pragma unroll
+            for (int t = 0; t < TT; t++) {
+                const size_t at = (size_t)min(16 * t + li, g.M - 1) * g.a.blocks + u * MX4_UNIT + 4 * lg;
+#pragma unroll
+                for (int k = 0; k < 4; k++) x[d][t][k] = reinterpret_cast<const uint4 *>(g.a.codes)[at + k];
+                xs[d][t] = *reinterpret_cast<const uint32_t *>(g.a.scales + at);
+            }
+        };
+        uint8_t *const own = mx4_rows_lds + (size_t)u0 * g.M * MX4_FUSED_UNIT;  // FUSED: this wavefront's units
+        if (FUSED) {
+            float v[2][4];
+            auto load = [&](int t, int u) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) floats_load4<FLOATS_F32, WIDE>(r.x + (size_t)t * r.cols, u * 512 + i * 256 + lane * 4, r.cols, v[i]);
+            };
+            auto store = [&](int t, int u) {
+                uint8_t *const to = own + ((size_t)(u - u0) * g.M + t) * MX4_FUSED_UNIT;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    uint32_t by;
+                    const uint32_t codes = mx4_quantize4(v[i], by);
+                    const int b = 8 * i + (lane >> 3);
+                    if ((lane & 4) == 0) *reinterpret_cast<uint32_t *>(to + b * 16 + (lane & 3) * 4) = codes;
+                    if ((lane & 7) == 0) to[MX4_UNIT * 16 + b] = (uint8_t)by;
+                }
+            };
+            load(0, u0);
+#pragma unroll
+            for (int d = 0; d < D; d++) fetch_w(d, u0 + d);
+            store(0, u0);
+            for (int u = u0, t = 1; u < u1; u++, t = 0)
+                for (; t < g.M; t++) {
+                    load(t, u);
+                    store(t, u);
+                }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wavefront reads its own stores only)
+        } else {
+#pragma unroll
+            for (int d = 0; d < D; d++) fetch_w(d, u0 + d), fetch_x(d, u0 + d);
+        }
+        auto consume = [&](int d, int u) {
+            if (FUSED) {
+                const uint8_t *const from = own + ((size_t)(u - u0) * g.M + min(li, g.M - 1)) * MX4_FUSED_UNIT;
+#pragma unroll
+                for (int k = 0; k < 4; k++) x[0][0][k] = *reinterpret_cast<const uint4 *>(from + (4 * lg + k) * 16);
+                xs[0][0] = *reinterpret_cast<const uint32_t *>(from + MX4_UNIT * 16 + 4 * lg);
+            }
+            const int e = FUSED ? 0 : d;
+#define FRK_MX4_PRODUCT(K)                                                                                                                    \
+    {                                                                                                                                         \
+        const mx4_v8i a = {(int)w[d][K].x, (int)w[d][K].y, (int)w[d][K].z, (int)w[d][K].w, 0, 0, 0, 0};                                       \
+        const mx4_v8i b = {(int)x[e][t][K].x, (int)x[e][t][K].y, (int)x[e][t][K].z, (int)x[e][t][K].w, 0, 0, 0, 0};                           \
+        acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], E2M1, E2M1, K, (int)ws[d], K, (int)xs[e][t]);                 \
+    }
+#pragma unroll
+            for (int t = 0; t < TT; t++) {
+                FRK_MX4_PRODUCT(0)
+                FRK_MX4_PRODUCT(1)
+                FRK_MX4_PRODUCT(2)
+                FRK_MX4_PRODUCT(3)
+            }
+#undef FRK_MX4_PRODUCT
+        };
+        for (int u = u0; u < u1; u += D)
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+                if (u + d >= u1) break;  // (uniform)
+                consume(d, u + d);
+                if (u + d + D < u1) {
+                    fetch_w(d, u + d + D);
+                    if (!FUSED) fetch_x(d, u + d + D);
+                }
+            }
+    }
+    // (the compiler does not count a product's wait states, eighteen at most, across the branches between it and the reads of its sum)
+#pragma unroll
+    for (int t = 0; t < TT; t++) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(acc[t]));
+#pragma unroll
+    for (int t = 0; t < TT; t++) sums[wave][t][lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+    __syncthreads();
+    if (wave >= TT) return;  // a wavefront a tile of tokens
+    const int tok = 16 * wave + li, r0 = strip * 16 + 4 * lg;
+    float4 v = sums[0][wave][lane];
+#pragma unroll
+    for (int k = 1; k < NW; k++) {
+        const float4 o = sums[k][wave][lane];
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+    }
+    if (tok >= g.M) return;
+    float *const dst = g.y + (size_t)tok * g.ldy + r0;
+    const float out[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (r0 + i < g.rows) dst[i] = out[i];
+#endif
+}
+template <int NW, int TT, bool FUSED>
+static int go_mx4_rows(const Mx4Rows &r, size_t lds, hipStream_t s) {
+    const dim3 grid((unsigned)((r.g.rows + 15) / 16));
+    if (FUSED && floats_wide(r.x, (size_t)r.cols, FLOATS_F32)) hipLaunchKernelGGL((mx4_rows_kernel<NW, TT, FUSED, FUSED>), grid, dim3(64 * NW), lds, s, r);
+    else hipLaunchKernelGGL((mx4_rows_kernel<NW, TT, FUSED, false>), grid, dim3(64 * NW), lds, s, r);
+    FRK_LAUNCH_CHECK("mx4_rows");
+    return FRK_OK;
+}
+
+constexpr size_t MX4_ROWS_TOKENS = 64;  // most of the rows kernel
+Mx4Plan mx4_plan(const frk_weights *w, size_t batch, bool quantized) {
+    const size_t units = (w->cols / MX4_BLOCK + MX4_UNIT - 1) / MX4_UNIT;
+    Mx4Plan p{-1, 1, !quantized && batch <= MX4_FUSED && batch * units * MX4_FUSED_UNIT <= MX4_FUSED_LDS, 0, 0};
+    if (p.fused) return p;
+    if (!quantized) p.acts_bytes = mx4_acts_bytes(batch, w->cols);
+    if (batch <= MX4_ROWS_TOKENS) return p;
+    p.shape = batch >= 512 ? MX4_TILE_256x256 : MX4_TILE_128x128;
+    return p;
+}
+int mx4_gemm_fits(const frk_weights *w, const Mx4Plan &plan, size_t batch) {
+    if (w->kind != FRK_KIND_MXFP4) return set_error(FRK_ERR_UNSUPPORTED, "MXFP4 activations feed MXFP4 weights only (kind %d)", w->kind);
+    int dev = -1;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipGetDevice: %s", hipGetErrorString(e));
+    if (dev != w->device) return set_error(FRK_ERR_ARG, "the matrix is on device %d, the current device is %d", w->device, dev);
+    // (lane offsets within a tile are 32 bits wide, columns of a fused row an int)
+    if (w->cols > (1u << 23)) return set_error(FRK_ERR_SHAPE, "shape too large: %zu columns (at most 2^23)", w->cols);
+    if (batch > (size_t)1 << 30) return set_error(FRK_ERR_SHAPE, "a batch of %zu rows is too large", batch);
+    if ((w->rows + 15) / 16 * 512 > 0xffffffffu) return set_error(FRK_ERR_SHAPE, "shape too large: %zu rows", w->rows);
+    return plan.shape < 0 ? FRK_OK : mx4_tiles_fit(w, plan.shape, batch);
+}
+int launch_mx4_gemm(const frk_weights *w, const Mx4Plan &plan, const float *x, const Mx4Acts *acts, size_t batch, float *y, void *ws, void *parts,
+                    hipStream_t s) {
+    Mx4Rows r{};
+    Mx4Gemm &g = r.g;
+    g.W = w->dev;
+    g.row_stride = w->layout.row_stride;
+    g.rows = (int)w->rows;
+    g.blocks = (int)(w->cols / MX4_BLOCK);
+    g.M = (int)batch;
+    g.ldy = w->rows;
+    if (acts) {
+        g.a = *acts;
+    } else if (!plan.fused) {
+        g.a = mx4_acts_carve(ws, batch, w->cols);
+        int rc = launch_mx4_quantize(x, batch, w->cols, g.a, s);
+        if (rc) return rc;
+    }
+    if (plan.shape >= 0) {
+        const size_t n = batch * w->rows;
+        g.y = plan.parts > 1 ? (float *)parts : y;
+        int rc = launch_mx4_tile(g, plan.shape, plan.parts, n, s);
+        if (rc || plan.parts == 1) return rc;
+        return launch_sum_parts((const float *)parts, plan.parts, n, y, s);
+    }
+    g.y = y;
+    r.x = x;
+    r.cols = (int)w->cols;
+    if (plan.fused) return go_mx4_rows<8, 1, true>(r, batch * ((g.blocks + MX4_UNIT - 1) / MX4_UNIT) * MX4_FUSED_UNIT, s);
+    if (batch <= 16) return go_mx4_rows<8, 1, false>(r, 0, s);
+    if (batch <= 32) return go_mx4_rows<8, 2, false>(r, 0, s);
+    return go_mx4_rows<8, 4, false>(r, 0, s);
+}
+
+}  // namespace frk

@@ -1,0 +1,185 @@
+// Products of MXFP4 matrices and MXFP4 activations (frk_mx4.hpp) over large tiles on the block-scaled matrix cores
+// (v_mfma_scale_f32_32x32x64_f8f6f4): sixteen bytes of E2M1 codes are a lane's operand, its block's E8M0 byte the scale.
+#include "frk_mx4.hpp"
+
+#include <algorithm>
+
+namespace frk {
+
+typedef int mx4_v4i __attribute__((ext_vector_type(4)));
+typedef int mx4_v8i __attribute__((ext_vector_type(8)));
+typedef float mx4_v16f __attribute__((ext_vector_type(16)));
+
+#define FRK_LAUNCH_CHECK(what)                                                                          \
+    do {                                                                                                \
+        hipError_t e_ = hipGetLastError();                                                              \
+        if (e_ != hipSuccess) return set_error(FRK_ERR_HIP, what " launch: %s", hipGetErrorString(e_)); \
+    } while (0)
+
+// RW x TW wavefronts of MR groups of 32 weight rows x MT groups of 32 tokens each.  A stage is eight blocks (256 columns) of every row:
+// 128 bytes of codes, eight lanes a row in one piece.
+template <int RW, int TW, int MR, int MT>
+struct Mx4TileShape {
+    static constexpr int WAVES = RW * TW, ROWS = RW * MR * 32, TOKENS = TW * MT * 32, ALL = ROWS + TOKENS;
+    static constexpr int STAGES = 2, STAGE = ALL * 128, SCALES = ALL * 16;  // scales: sixteen blocks, of two stages; two slots
+    static constexpr int W_REQUESTS = ROWS / 8 / WAVES, X_REQUESTS = TOKENS / 8 / WAVES, S_REQUESTS = (ALL / 64 + WAVES - 1) / WAVES;
+    static_assert(W_REQUESTS * 8 * WAVES == ROWS && X_REQUESTS * 8 * WAVES == TOKENS && ROWS % 64 == 0 && TOKENS % 64 == 0, "whole requests");
+    static constexpr size_t LDS = STAGES * STAGE + 2 * SCALES;
+    static_assert(LDS <= 160 * 1024, "LDS of a CU");
+};
+
+template <int RW, int TW, int MR, int MT>
+__global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, int row_tiles, int tok_tiles, int parts, size_t part_stride) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using T = Mx4TileShape<RW, TW, MR, MT>;
+    constexpr int E2M1 = 4;
+    extern __shared__ __align__(16) uint8_t mx4_lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int li = lane & 31, lh = lane >> 5;
+    const int rw = wave % RW, tw = wave / RW;
+    // An XCD (workgroup id mod 8) takes a run of the list, which goes through panels of eight token tiles row tile by row tile: its CUs
+    // then work on tiles that share their blocks in its L2.
+    const int total = row_tiles * tok_tiles, per_xcd = (total + 7) / 8;
+    const int index = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
+    if (((int)blockIdx.x >> 3) >= per_xcd || index >= total) return;
+    const int panel = index / (8 * row_tiles), wide_panel = min(8, tok_tiles - 8 * panel), in_panel = index - panel * 8 * row_tiles;
+    const int row0 = in_panel / wide_panel * T::ROWS, tok0 = (8 * panel + in_panel % wide_panel) * T::TOKENS;
+    // this part's stages
+    const int part = (int)blockIdx.y, stages = (g.blocks + 7) / 8;
+    const int from = (int)((long long)stages * part / parts), until = (int)((long long)stages * (part + 1) / parts);
+    const uint32_t lds0 = lds_address(mx4_lds);
+
+    // ---- requests: place p of row r of a stage holds piece p ^ (r / 2) % 8, so that the sixteen rows that LDS serves together touch all banks
+    uint32_t w_off[T::W_REQUESTS], x_off[T::X_REQUESTS], s_off[T::S_REQUESTS];
+    const uint8_t *const w_base = g.W + (size_t)row0 * g.row_stride;
+    const uint8_t *const x_base = g.a.codes + (size_t)tok0 * g.a.blocks * 16;
+    const uint8_t *const xs_base = g.a.scales + (size_t)tok0 * g.a.blocks;
+    const uint8_t *const ws_base = w_base + (size_t)g.blocks * 16;
+#pragma unroll
+    for (int c = 0; c < T::W_REQUESTS; c++) {
+        const int r = (c * T::WAVES + wave) * 8 + (lane >> 3);
+        w_off[c] = (uint32_t)min(r, g.rows - 1 - row0) * (uint32_t)g.row_stride + (uint32_t)((lane & 7) ^ ((r >> 1) & 7)) * 16;
+    }
+#pragma unroll
+    for (int c = 0; c < T::X_REQUESTS; c++) {
+        const int r = (c * T::WAVES + wave) * 8 + (lane >> 3);
+        x_off[c] = (uint32_t)min(r, g.M - 1 - tok0) * (uint32_t)(g.a.blocks * 16) + (uint32_t)((lane & 7) ^ ((r >> 1) & 7)) * 16;
+    }
+#pragma unroll
+    for (int c = 0; c < T::S_REQUESTS; c++) {  // 64 rows a request, weight rows first
+        const int q = c * T::WAVES + wave, r = q * 64 + lane;
+        s_off[c] = q * 64 < T::ROWS ? (uint32_t)min(r, g.rows - 1 - row0) * (uint32_t)g.row_stride
+                                    : (uint32_t)min(r - T::ROWS, g.M - 1 - tok0) * (uint32_t)g.a.blocks;
+    }
+    auto request = [&](int i) {
+        const uint32_t to = lds0 + (uint32_t)(i & 1) * T::STAGE;
+#pragma unroll
+        for (int c = 0; c < T::W_REQUESTS; c++) dma16(to + (uint32_t)(c * T::WAVES + wave) * 1024, w_base + (size_t)i * 128, w_off[c]);
+#pragma unroll
+        for (int c = 0; c < T::X_REQUESTS; c++) dma16(to + T::ROWS * 128 + (uint32_t)(c * T::WAVES + wave) * 1024, x_base + (size_t)i * 128, x_off[c]);
+        if ((i & 1) == 0 || i == from) {
+            const uint32_t scales = lds0 + T::STAGES * T::STAGE + (uint32_t)((i >> 1) & 1) * T::SCALES;
+#pragma unroll
+            for (int c = 0; c < T::S_REQUESTS; c++) {
+                const int q = c * T::WAVES + wave;
+                if (q * 64 < T::ALL) dma16(scales + (uint32_t)q * 1024, (q * 64 < T::ROWS ? ws_base : xs_base) + (size_t)(i >> 1) * 16, s_off[c]);
+            }
+        }
+    };
+    mx4_v16f acc[MT][MR];
+#pragma unroll
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int r = 0; r < MR; r++) acc[t][r] = mx4_v16f{0.0f};
+    // where this lane's blocks 4 lh + k of its row lie in a group of 32 rows: 16 k flipped
+    const uint32_t piece_at = (uint32_t)(li * 128 + ((4 * lh) ^ ((li >> 1) & 7)) * 16);
+    const uint32_t w_lane = (uint32_t)(rw * MR * 32) * 128, x_lane = (uint32_t)(T::ROWS + tw * MT * 32) * 128;
+
+    if (from < until) request(from);
+    for (int i = from; i < until; i++) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();  // the stage has landed, and everybody has read the one before
+        if (i + 1 < until) request(i + 1);
+        const uint8_t *const st = mx4_lds + (size_t)(i & 1) * T::STAGE;
+        const uint8_t *const sc = mx4_lds + T::STAGES * T::STAGE + (size_t)((i >> 1) & 1) * T::SCALES + (i & 1) * 8 + lh * 4 + li * 16;
+        // (a row's last stage may reach past its blocks: the codes there meet zeros, but a byte 255 would make them NaN)
+        const int live = g.blocks - (i * 8 + 4 * lh);
+        const uint32_t mask = live >= 4 ? 0xffffffffu : live > 0 ? 0xffffffffu >> (32 - 8 * live) : 0u;
+        int ws[MR], xs[MT];
+#pragma unroll
+        for (int r = 0; r < MR; r++) ws[r] = (int)(*reinterpret_cast<const uint32_t *>(sc + (rw * MR + r) * 512) & mask);
+#pragma unroll
+        for (int t = 0; t < MT; t++) xs[t] = (int)*reinterpret_cast<const uint32_t *>(sc + T::ROWS * 16 + (tw * MT + t) * 512);
+#define FRK_MX4_STEP(K)                                                                                                                        \
+    {                                                                                                                                          \
+        mx4_v8i w[MR], x[MT];                                                                                                                  \
+        _Pragma("unroll") for (int r = 0; r < MR; r++) {                                                                                       \
+            const mx4_v4i v = *reinterpret_cast<const mx4_v4i *>(st + w_lane + r * 4096 + (piece_at ^ (K * 16)));                              \
+            w[r] = mx4_v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0};                                                                                \
+        }                                                                                                                                      \
+        _Pragma("unroll") for (int t = 0; t < MT; t++) {                                                                                       \
+            const mx4_v4i v = *reinterpret_cast<const mx4_v4i *>(st + x_lane + t * 4096 + (piece_at ^ (K * 16)));                              \
+            x[t] = mx4_v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0};                                                                                \
+        }                                                                                                                                      \
+        _Pragma("unroll") for (int t = 0; t < MT; t++) _Pragma("unroll") for (int r = 0; r < MR; r++)                                          \
+            acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x[t], w[r], acc[t][r], E2M1, E2M1, K, xs[t], K, ws[r]);                \
+    }
+        FRK_MX4_STEP(0)
+        FRK_MX4_STEP(1)
+        FRK_MX4_STEP(2)
+        FRK_MX4_STEP(3)
+#undef FRK_MX4_STEP
+    }
+    // (the compiler does not count a product's wait states, eighteen at most, across the branches between it and the reads of its sum)
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    // register i of a lane: token 8 (i / 4) + 4 (lane / 32) + i % 4 of a group, weight row lane % 32
+#pragma unroll
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int tok = tok0 + (tw * MT + t) * 32 + 8 * (i >> 2) + 4 * lh + (i & 3);
+            if (tok >= g.M) continue;
+            float *const dst = g.y + part * part_stride + (size_t)tok * g.ldy;
+#pragma unroll
+            for (int r = 0; r < MR; r++) {
+                const int row = row0 + (rw * MR + r) * 32 + li;
+                if (row < g.rows) dst[row] = acc[t][r][i];
+            }
+        }
+#endif
+}
+
+template <int RW, int TW, int MR, int MT>
+static int go_mx4_tile(const Mx4Gemm &g, int parts, size_t part_stride, hipStream_t s) {
+    using T = Mx4TileShape<RW, TW, MR, MT>;
+    const size_t row_tiles = ((size_t)g.rows + T::ROWS - 1) / T::ROWS, tok_tiles = ((size_t)g.M + T::TOKENS - 1) / T::TOKENS, total = row_tiles * tok_tiles;
+    static bool sized = false;  // a benign race: every thread sets the same attribute
+    if (!sized) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_tile_kernel<RW, TW, MR, MT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)T::LDS);
+        if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFuncSetAttribute(mx4_tile): %s", hipGetErrorString(e));
+        sized = true;
+    }
+    hipLaunchKernelGGL((mx4_tile_kernel<RW, TW, MR, MT>), dim3((unsigned)((total + 7) / 8 * 8), (unsigned)parts), dim3(64 * T::WAVES), T::LDS, s, g,
+                       (int)row_tiles, (int)tok_tiles, parts, part_stride);
+    FRK_LAUNCH_CHECK("mx4_tile");
+    return FRK_OK;
+}
+int mx4_tiles_fit(const frk_weights *w, int shape, size_t batch) {
+    const Mx4TileSize t = MX4_TILE_SIZE[shape];
+    const size_t row_tiles = (w->rows + t.rows - 1) / t.rows, tok_tiles = (batch + t.tokens - 1) / t.tokens;
+    if ((row_tiles * tok_tiles + 7) / 8 * 8 * t.threads > 0xffffffffu)
+        return set_error(FRK_ERR_SHAPE, "%zu x %zu tiles: more than a grid holds", row_tiles, tok_tiles);
+    return FRK_OK;
+}
+int launch_mx4_tile(const Mx4Gemm &g, int shape, int parts, size_t part_stride, hipStream_t s) {
+    switch (shape) {
+    case MX4_TILE_256x256: return go_mx4_tile<2, 2, 4, 4>(g, parts, part_stride, s);
+    case MX4_TILE_128x128: return go_mx4_tile<2, 2, 2, 2>(g, parts, part_stride, s);
+    default: return go_mx4_tile<4, 1, 1, 2>(g, parts, part_stride, s);
+    }
+}
+
+}  // namespace frk

@@ -2,6 +2,7 @@
 // weight cache, the per-device workspace and the extern "C" entry points.
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <iterator>
@@ -14,6 +15,7 @@
 
 #include "frk_internal.hpp"
 #include "frk_f8.hpp"
+#include "frk_norm.hpp"
 #include "frk_stage.hpp"
 
 namespace frk {
@@ -649,6 +651,14 @@ static int f8_plan_fits(const frk_weights *w, const F8Plan &plan, size_t batch) 
     const size_t tokens = (size_t)F8_TILE_SIZE[plan.shape].tokens;
     return f8_tiles_fit(w, plan.shape, (batch + tokens - 1) / tokens, w->matrices * plan.parts, 0);
 }
+static int gemm_mx4(const frk_weights *w, const float *x, const Mx4Acts *acts, size_t batch, float *y, hipStream_t s, Scratch &scratch) {
+    void *ws = nullptr, *parts = nullptr;
+    const Mx4Plan plan = mx4_plan(w, batch, acts != nullptr);
+    int rc = mx4_gemm_fits(w, plan, batch);
+    if (!rc && plan.acts_bytes + plan.parts_bytes) rc = scratch.get(plan.acts_bytes, plan.parts_bytes, s, &ws, &parts);
+    if (rc) return rc;
+    return launch_mx4_gemm(w, plan, x, acts, batch, y, ws, parts, s);
+}
 static int gemm_f8(const frk_weights *w, const float *x, size_t batch, float *y, hipStream_t s, Scratch &scratch) {
     if (batch > (size_t)1 << 30) return set_error(FRK_ERR_SHAPE, "a batch of %zu rows is too large", batch);
     void *ws = nullptr, *parts = nullptr;
@@ -1183,37 +1193,79 @@ int frk_hip_gemm_pair_dev(const frk_weights *w0, const frk_weights *w1, const fl
 constexpr size_t ACTS_PLAIN_MAX_BATCH = 64, ACTS_TILED_MIN_BATCH = 2;
 }  // extern "C"
 struct frk_batch_acts {
+    int form = FRK_ACTS_Q8_K, device = 0;
     size_t max_batch = 0, cols = 0;
-    void *base = nullptr;       // one allocation: plain rows, then the tiled form
-    size_t tiled_off = 0;
+    void *base = nullptr;       // one allocation: Q8_K plain rows, then the tiled form; FP8 rows, then strips; MXFP4 rows
+    size_t tiled_off = 0;       // of the second
     size_t batch = 0;           // rows of the last quantization (0: none yet)
     frk::Q8KActs plain{nullptr, nullptr, nullptr};
 };
+// Which of FP8's two layouts a batch is wanted in: f8_plan multiplies up to sixteen rows from strips, more than F8_ROWS_TOKENS from rows
+static bool f8_acts_strips(size_t batch) { return batch <= F8_ROWS_TOKENS; }
+static bool f8_acts_rows(size_t batch) { return batch > 16; }
+static F8Acts f8_acts_of(const frk_batch_acts *a, size_t batch, bool strips) {
+    return f8_acts_carve((char *)a->base + (strips ? a->tiled_off : 0), batch, strips);
+}
+// where a batch of Q8_K goes: plain rows and tiles, or one of the two
+static Q8KActsOut q8k_plain_of(const frk_batch_acts *a, size_t batch) {
+    Q8KActsOut plain;
+    if (batch <= ACTS_PLAIN_MAX_BATCH) {
+        const size_t n = batch * a->cols;
+        plain.q = (int8_t *)a->base;
+        plain.d = (float *)((char *)a->base + round_up(n, 256));
+        plain.bsums = (int16_t *)((char *)a->base + round_up(n, 256) + round_up(n / QK_K * 4, 256));
+    }
+    return plain;
+}
+static int acts_on_current_device(const frk_batch_acts *a) {
+    int dev = -1;
+    FRK_HIP_TRY(hipGetDevice(&dev));
+    if (dev != a->device) return set_error(FRK_ERR_ARG, "the activations are on device %d, the current device is %d", a->device, dev);
+    return FRK_OK;
+}
 extern "C" {
 
-int frk_hip_batch_acts_create(size_t max_batch, size_t cols, frk_batch_acts **out) {
+int frk_hip_batch_acts_create_form(size_t max_batch, size_t cols, int form, frk_batch_acts **out) {
     clear_error();
     if (!out) return set_error(FRK_ERR_ARG, "frk_hip_batch_acts_create: null argument");
     *out = nullptr;
-    if (max_batch == 0 || cols == 0 || cols % QK_K != 0)
-        return set_error(FRK_ERR_SHAPE, "batch activations: %zu rows of %zu columns (whole 256-column blocks, at least one row)", max_batch, cols);
+    const size_t block = form == FRK_ACTS_Q8_K ? QK_K : form == FRK_ACTS_FP8 ? 1 : form == FRK_ACTS_MXFP4 ? MX4_BLOCK : 0;
+    if (!block) return set_error(FRK_ERR_UNSUPPORTED, "batch activations: no form %d", form);
+    if (max_batch == 0 || cols == 0 || cols % block != 0)
+        return set_error(FRK_ERR_SHAPE, "batch activations: %zu rows of %zu columns (whole %zu-column blocks, at least one row)", max_batch, cols, block);
+    if (form != FRK_ACTS_Q8_K && (cols > (1u << 23) || max_batch > (size_t)1 << 30))
+        return set_error(FRK_ERR_SHAPE, "batch activations: %zu rows of %zu columns (at most 2^30 of 2^23)", max_batch, cols);
     {
         std::lock_guard<std::mutex> lk(g_dev.mu);
         int rc = ensure_device_locked();
         if (rc) return rc;
     }
-    frk_batch_acts *a = new frk_batch_acts();
+    frk_batch_acts *a = new (std::nothrow) frk_batch_acts();
+    if (!a) return set_error(FRK_ERR_OOM, "no host memory for batch activations");
+    a->form = form;
     a->max_batch = max_batch;
     a->cols = cols;
-    a->tiled_off = round_up(acts_plain_bytes(std::min(max_batch, ACTS_PLAIN_MAX_BATCH), cols), 256);
-    const size_t bytes = a->tiled_off + (max_batch >= ACTS_TILED_MIN_BATCH ? round_up(q8k_tiled_bytes(max_batch, cols), 256) : 0);
-    hipError_t e = hipMalloc(&a->base, bytes);
+    size_t bytes;
+    if (form == FRK_ACTS_FP8) {
+        a->tiled_off = max_batch > 16 ? f8_acts_bytes(max_batch, cols) : 0;
+        bytes = a->tiled_off + f8_acts_bytes(std::min(max_batch, F8_ROWS_TOKENS), cols);
+    } else if (form == FRK_ACTS_MXFP4) {
+        bytes = mx4_acts_bytes(max_batch, cols);
+    } else {
+        a->tiled_off = round_up(acts_plain_bytes(std::min(max_batch, ACTS_PLAIN_MAX_BATCH), cols), 256);
+        bytes = a->tiled_off + (max_batch >= ACTS_TILED_MIN_BATCH ? round_up(q8k_tiled_bytes(max_batch, cols), 256) : 0);
+    }
+    hipError_t e = hipGetDevice(&a->device);
+    if (e == hipSuccess) e = hipMalloc(&a->base, bytes);
     if (e != hipSuccess) {
         delete a;
-        return set_error(FRK_ERR_HIP, "hipMalloc(%zu) for batch activations: %s", bytes, hipGetErrorString(e));
+        return set_error(e == hipErrorOutOfMemory && form != FRK_ACTS_Q8_K ? FRK_ERR_OOM : FRK_ERR_HIP, "hipMalloc(%zu) for batch activations: %s", bytes, hipGetErrorString(e));
     }
     *out = a;
     return FRK_OK;
+}
+int frk_hip_batch_acts_create(size_t max_batch, size_t cols, frk_batch_acts **out) {
+    return frk_hip_batch_acts_create_form(max_batch, cols, FRK_ACTS_Q8_K, out);
 }
 
 int frk_hip_batch_acts_release(frk_batch_acts *a) {
@@ -1231,16 +1283,24 @@ int frk_hip_quantize_batch_acts_dev(frk_batch_acts *a, const float *x, size_t ba
     if (batch == 0 || batch > a->max_batch)
         return set_error(FRK_ERR_SHAPE, "a batch of %zu rows in an object made for at most %zu", batch, a->max_batch);
     hipStream_t s = (hipStream_t)stream;
+    if (a->form != FRK_ACTS_Q8_K) {
+        int rc = acts_on_current_device(a);
+        if (rc) return rc;
+        a->batch = 0;
+        if (a->form == FRK_ACTS_MXFP4) {
+            rc = launch_mx4_quantize(x, batch, a->cols, mx4_acts_carve(a->base, batch, a->cols), s);
+        } else {
+            if (f8_acts_rows(batch)) rc = launch_f8_quantize(x, nullptr, batch, a->cols, nullptr, f8_acts_of(a, batch, false), s);
+            if (!rc && f8_acts_strips(batch)) rc = launch_f8_quantize(x, nullptr, batch, a->cols, nullptr, f8_acts_of(a, batch, true), s);
+        }
+        if (rc) return rc;
+        a->batch = batch;
+        return FRK_OK;
+    }
     a->batch = 0;
     const bool tiled = batch >= ACTS_TILED_MIN_BATCH;
-    Q8KActsOut plain;
-    if (batch <= ACTS_PLAIN_MAX_BATCH) {
-        const size_t n = batch * a->cols;
-        plain.q = (int8_t *)a->base;
-        plain.d = (float *)((char *)a->base + round_up(n, 256));
-        plain.bsums = (int16_t *)((char *)a->base + round_up(n, 256) + round_up(n / QK_K * 4, 256));
-        a->plain = Q8KActs{plain.q, plain.d, plain.bsums};
-    }
+    const Q8KActsOut plain = q8k_plain_of(a, batch);
+    if (plain.q) a->plain = Q8KActs{plain.q, plain.d, plain.bsums};
     const Q8KTiled tiles = q8k_tiled_carve((char *)a->base + a->tiled_off, batch, a->cols);
     const int rc = tiled ? (batch < tiled_from(a->cols) ? launch_quantize_q8_k_one_tile(x, batch, a->cols, tiles, s, plain)
                                                         : launch_quantize_q8_k_tiled(x, batch, a->cols, tiles, s, plain))
@@ -1250,12 +1310,32 @@ int frk_hip_quantize_batch_acts_dev(frk_batch_acts *a, const float *x, size_t ba
     return FRK_OK;
 }
 
+static int gemm_f8_acts(const frk_weights *w, const frk_batch_acts *a, float *y, hipStream_t s, Scratch &scratch) {
+    const F8Plan plan = f8_plan(w, a->batch, true);
+    void *parts = nullptr;
+    int rc = f8_on_current_device(w);
+    if (!rc) rc = f8_plan_fits(w, plan, a->batch);
+    if (!rc && plan.parts_bytes) rc = scratch.get(plan.parts_bytes, s, &parts);
+    if (rc) return rc;
+    return launch_f8_gemm(w, plan, nullptr, a->batch, y, f8_acts_of(a, a->batch, plan.shape < 0).v, true, parts, s);
+}
+
 int frk_hip_gemm_acts_dev(const frk_weights *w, const frk_batch_acts *a, float *y, void *stream) {
     clear_error();
     if (!w || !a || !y) return set_error(FRK_ERR_ARG, "frk_hip_gemm_acts_dev: null argument");
     if (a->batch == 0) return set_error(FRK_ERR_ARG, "frk_hip_gemm_acts_dev: the activations hold no quantized batch");
     if (w->cols != a->cols)
         return set_error(FRK_ERR_SHAPE, "the matrix has %zu columns, the quantized activations %zu", w->cols, a->cols);
+    if (a->form != FRK_ACTS_Q8_K) {
+        const int kind = a->form == FRK_ACTS_FP8 ? FRK_KIND_FP8_BLOCK : FRK_KIND_MXFP4;
+        if (w->kind != kind) return set_error(FRK_ERR_UNSUPPORTED, "activations of form %d feed weights of kind %d only (kind %d)", a->form, kind, w->kind);
+        int rc = acts_on_current_device(a);
+        if (rc) return rc;
+        Scratch scratch;
+        if (a->form == FRK_ACTS_FP8) return gemm_f8_acts(w, a, y, (hipStream_t)stream, scratch);
+        const Mx4Acts acts = mx4_acts_carve(a->base, a->batch, a->cols);
+        return gemm_mx4(w, nullptr, &acts, a->batch, y, (hipStream_t)stream, scratch);
+    }
     const bool k_quant = w->kind == FRK_KIND_Q4_K || w->kind == FRK_KIND_Q5_K || w->kind == FRK_KIND_Q6_K;
     if (!k_quant)
         return set_error(FRK_ERR_UNSUPPORTED, "Q8_K activations feed Q4_K, Q5_K and Q6_K weights only (kind %d): frk_hip_gemm_dev", w->kind);
@@ -1284,6 +1364,92 @@ int frk_hip_gemm_acts_dev(const frk_weights *w, const frk_batch_acts *a, float *
         if (rc) return rc;
     }
     return FRK_OK;
+}
+
+int frk_hip_batch_acts_values_dev(const frk_batch_acts *a, float *out, void *stream) {
+    clear_error();
+    if (!a || !out) return set_error(FRK_ERR_ARG, "frk_hip_batch_acts_values_dev: null argument");
+    if (a->batch == 0) return set_error(FRK_ERR_ARG, "frk_hip_batch_acts_values_dev: the activations hold no quantized batch");
+    int rc = acts_on_current_device(a);
+    if (rc) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    if (a->form == FRK_ACTS_MXFP4) return launch_mx4_values(mx4_acts_carve(a->base, a->batch, a->cols), a->cols, out, s);
+    if (a->form == FRK_ACTS_FP8) return launch_f8_values(f8_acts_of(a, a->batch, !f8_acts_rows(a->batch)), a->cols, out, s);
+    const Q8KActsOut plain = q8k_plain_of(a, a->batch);
+    return launch_q8_k_values(Q8KActs{plain.q, plain.d, plain.bsums}, q8k_tiled_carve((char *)a->base + a->tiled_off, a->batch, a->cols), a->batch, a->cols, out, s);
+}
+
+static bool is_float_type(int type) { return type == FRK_TYPE_F32 || type == FRK_TYPE_BF16 || type == FRK_TYPE_F16; }
+
+int frk_hip_rms_norm_dev(int type, const void *x, const void *residual, int weight_type, const void *weight, double eps, size_t batch, size_t cols, void *sum,
+                         void *y, frk_batch_acts *acts, void *stream) {
+    clear_error();
+    if (!x) return set_error(FRK_ERR_ARG, "frk_hip_rms_norm_dev: null argument");
+    if (!sum && !y && !acts) return set_error(FRK_ERR_ARG, "frk_hip_rms_norm_dev: no output");
+    if (!is_float_type(type) || (weight && !is_float_type(weight_type))) return set_error(FRK_ERR_UNSUPPORTED, "no numbers of type %d, weights of type %d", type, weight_type);
+    if (!(eps >= 0.0) || std::isinf(eps)) return set_error(FRK_ERR_ARG, "eps %g: a finite number, zero or more", eps);
+    if (batch == 0 || cols == 0) return set_error(FRK_ERR_SHAPE, "empty shape: batch=%zu cols=%zu", batch, cols);
+    if (batch > (size_t)1 << 30 || cols > (size_t)1 << 23) return set_error(FRK_ERR_SHAPE, "shape too large: batch=%zu cols=%zu (at most 2^30 rows of 2^23)", batch, cols);
+    if (y && (y == sum || (y == residual && acts))) return set_error(FRK_ERR_ARG, "frk_hip_rms_norm_dev: y and the sum are two outputs");
+    NormArgs a{};
+    a.x = x;
+    a.residual = residual;
+    a.weight = weight;
+    a.weight_type = weight_type;
+    a.eps = eps;
+    a.batch = a.rows = batch;
+    a.cols = (int)cols;
+    a.sum = sum;
+    a.y = y;
+    NormOut out{};
+    if (acts) {
+        if (batch > acts->max_batch) return set_error(FRK_ERR_SHAPE, "a batch of %zu rows in an object made for at most %zu", batch, acts->max_batch);
+        if (cols != acts->cols) return set_error(FRK_ERR_SHAPE, "rows of %zu columns in an object of %zu", cols, acts->cols);
+        int rc = acts_on_current_device(acts);
+        if (rc) return rc;
+        acts->batch = 0;
+        if (acts->form == FRK_ACTS_FP8) {
+            if (f8_acts_rows(batch)) out.f8 = f8_acts_of(acts, batch, false);
+            if (f8_acts_strips(batch)) out.f8_strips = f8_acts_of(acts, batch, true);
+            out.f8_blocks = (int)f8_blocks(cols);
+        } else if (acts->form == FRK_ACTS_MXFP4) {
+            out.mx4 = mx4_acts_carve(acts->base, batch, cols);
+        } else {
+            out.plain = q8k_plain_of(acts, batch);
+            if (out.plain.q) acts->plain = Q8KActs{out.plain.q, out.plain.d, out.plain.bsums};
+            out.q8k_blocks = (int)(cols / QK_K);
+            if (batch >= ACTS_TILED_MIN_BATCH) {
+                out.tiled = q8k_tiled_carve((char *)acts->base + acts->tiled_off, batch, cols);
+                if (batch >= tiled_from(cols)) a.rows = round_up(batch, 32);  // (as the quantizations do: the kernels of larger batches want zeros there)
+            }
+        }
+    }
+    int rc = launch_rms_norm(type, a, acts ? acts->form : (int)ACTS_NONE, out, (hipStream_t)stream);
+    if (rc) return rc;
+    if (acts) acts->batch = batch;
+    return FRK_OK;
+}
+
+int frk_hip_quantize_mxfp4_dev(int type, const void *x, size_t n, uint8_t *blocks, void *stream) {
+    clear_error();
+    if (!x || !blocks) return set_error(FRK_ERR_ARG, "frk_hip_quantize_mxfp4_dev: null argument");
+    if (!is_float_type(type)) return set_error(FRK_ERR_UNSUPPORTED, "no numbers of type %d", type);
+    if (n == 0 || n % MX4_BLOCK) return set_error(FRK_ERR_SHAPE, "%zu values: a multiple of %d, not zero", n, MX4_BLOCK);
+    return launch_quantize_mxfp4(type, x, n, blocks, (hipStream_t)stream);
+}
+int frk_hip_dequantize_mxfp4_dev(const uint8_t *blocks, size_t n, float *out, void *stream) {
+    clear_error();
+    if (!blocks || !out) return set_error(FRK_ERR_ARG, "frk_hip_dequantize_mxfp4_dev: null argument");
+    if (n == 0 || n % MX4_BLOCK) return set_error(FRK_ERR_SHAPE, "%zu values: a multiple of %d, not zero", n, MX4_BLOCK);
+    return launch_dequantize_mxfp4(blocks, n, out, (hipStream_t)stream);
+}
+
+int frk_hip_gemm_mxfp4_dev(const frk_weights *w, const float *x, size_t batch, float *y, void *stream) {
+    clear_error();
+    if (!w || !x || !y) return set_error(FRK_ERR_ARG, "frk_hip_gemm_mxfp4_dev: null argument");
+    if (batch == 0) return set_error(FRK_ERR_SHAPE, "empty shape: batch=0");
+    Scratch scratch;
+    return gemm_mx4(w, x, nullptr, batch, y, (hipStream_t)stream, scratch);
 }
 
 // ---- the entry point that allocates nothing ----

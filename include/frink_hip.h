@@ -310,6 +310,46 @@ int frk_hip_gemm_noalloc_dev(const frk_weights *w, const float *x_dev, size_t ba
 int frk_hip_route_top_k_softmax_dev(const float *logits_dev, size_t batch, size_t n_experts, size_t k,
                                     int norm, int32_t *ids_dev, float *weights_dev, void *stream);
 
+/* The same in two more forms, for the matrices of those kinds: FRK_ACTS_FP8 for FRK_KIND_FP8_BLOCK (any number of columns) and
+ * FRK_ACTS_MXFP4 for FRK_KIND_MXFP4 (whole blocks of 32), at most 2^30 rows of 2^23 columns.  _create is _create_form with FRK_ACTS_Q8_K.
+ * An object belongs to the device that was current when it was made; a call over one of these forms, or of the three functions
+ * below, while another is current returns FRK_ERR_ARG.
+ *   FP8    as frk_hip_gemm_dev quantizes a batch for such a matrix; y is bit for bit its result from nine rows on (fewer may be the same
+ *          products added in another order)
+ *   MXFP4  as frk_hip_gemm_mxfp4_dev does; y is bit for bit its result from five rows on
+ * The reference has no counterpart of either.  _values writes the numbers that the last quantization stands for, [batch][cols] f32. */
+enum { FRK_ACTS_Q8_K = 0, FRK_ACTS_FP8 = 1, FRK_ACTS_MXFP4 = 2 };
+int frk_hip_batch_acts_create_form(size_t max_batch, size_t cols, int form, frk_batch_acts **out);
+int frk_hip_batch_acts_values_dev(const frk_batch_acts *acts, float *out_dev, void *stream);
+
+/* Types of numbers that the functions below take. */
+enum { FRK_TYPE_F32 = 0, FRK_TYPE_BF16 = 1, FRK_TYPE_F16 = 2 };
+/* The norm in front of a group of projections, for rows x[batch][cols] of `type`:
+ *   h = x + residual, rounded to `type` (h = x where residual_dev is null)
+ *   r = 1 / sqrt(mean(h^2) + eps): the sum, the root and the quotient in 64 bits, rounded to f32 once
+ *   y = (h * r) * weight, two products rounded to f32 each (one where weight_dev is null); weight[cols] of weight_type
+ * and up to three outputs (null: not wanted; at least one): h into sum_dev, y rounded to `type` into y_dev, y in f32 quantized into `acts`,
+ * bit for bit as frk_hip_quantize_batch_acts_dev would, with which frk_hip_gemm_acts_dev then multiplies.
+ * sum_dev may be x_dev or residual_dev, y_dev may be x_dev, or residual_dev unless h or `acts` is wanted too; otherwise no two
+ * operands overlap.  A row with an infinity or a NaN has the NaN that the formula gives.  eps is a finite number, zero or more (a row of zeros has y = NaN with eps = 0).  At most 2^30 rows
+ * of 2^23 columns; rows need be aligned to their type only.  The order of the reference's norms (RMSNorm in crates/frink-core). */
+int frk_hip_rms_norm_dev(int type, const void *x_dev, const void *residual_dev, int weight_type, const void *weight_dev, double eps,
+                         size_t batch, size_t cols, void *sum_dev, void *y_dev, frk_batch_acts *acts, void *stream);
+
+/* n values (a multiple of 32) as MXFP4 blocks in GGUF's form, 17 bytes for every 32 -- what frk_hip_weights_from_device takes as
+ * FRK_KIND_MXFP4 -- and back.  A block's scale is 2^(floor(log2(amax)) - 2) (the byte is that exponent plus 127, 0 at the least); its
+ * values become the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 times the scale, halves the even code, larger ones 6 times it.  A block with
+ * an infinity or a NaN gets the byte 255 and zero codes; frk_hip_dequantize_mxfp4_dev makes NaN of such blocks (OCP's reading of that byte;
+ * frk_hip_dequant_dev over a resident matrix reads it as 2^128, as GGUF's dequantizer does). */
+int frk_hip_quantize_mxfp4_dev(int type, const void *x_dev, size_t n, uint8_t *blocks_dev, void *stream);
+int frk_hip_dequantize_mxfp4_dev(const uint8_t *blocks_dev, size_t n, float *out_dev, void *stream);
+/* y[batch][rows] = x[batch][cols] W^T with an FRK_KIND_MXFP4 matrix and x quantized within the call to MXFP4, every 32 columns as
+ * frk_hip_quantize_mxfp4_dev does.  Products of codes are exact and so are their sums within a block; blocks add up in f32 (results and parts of sums below
+ * 2^-126 may be zero).  Four bits an activation: frk_hip_gemm_dev multiplies the same matrix by activations of eight.
+ * A scale byte of 255 makes NaN of its weight row or activation row.  Scratch memory and graphs as with frk_hip_gemm_dev; at most 2^23 columns and 2^30 rows of x.
+ * FRK_ERR_ARG while another device than the matrix's is the current one. */
+int frk_hip_gemm_mxfp4_dev(const frk_weights *w, const float *x_dev, size_t batch, float *y_dev, void *stream);
+
 /* Routing by a rule, for a batch of tokens: logits[batch][n_experts] -> ids[batch][k], weights[batch][k].
  *   score    p = softmax(l) over a token's experts, or sigmoid(l) each
  *   bias     f32 [n_experts] on the device, or null: c = p + bias decides which experts are chosen (a bias for balance);
