@@ -43,55 +43,95 @@ int launch_mx4_quantize(const float *x, size_t rows, size_t cols, const Mx4Acts 
     return FRK_OK;
 }
 
-// out[row][k]: what the quantized rows stand for
-__global__ __launch_bounds__(256) void mx4_values_kernel(Mx4Acts a, int cols, size_t n, float *__restrict__ out) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const size_t row = i / cols;
-        const int k = (int)(i % cols), in = k % MX4_BLOCK;
-        const size_t block = row * a.blocks + k / MX4_BLOCK;
-        out[i] = mx4_value(a.codes[block * 16 + (in & 15)] >> (in & 16 ? 4 : 0) & 15u, a.scales[block]);
+// two values of a byte of codes, low half first, without their scale
+__device__ __forceinline__ float2 mx4_two(uint32_t four, int which) {
+    float2 o = make_float2(0.0f, 0.0f);
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef float two_t __attribute__((ext_vector_type(2)));
+    const two_t v = which == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, 1.0f, 0)
+                    : which == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, 1.0f, 1)
+                    : which == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, 1.0f, 2)
+                                 : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(four, 1.0f, 3);
+    o = make_float2(v.x, v.y);
+#endif
+    return o;
+}
+// what the quantized rows stand for: a wavefront 256 values at a time
+template <bool WIDE>
+__global__ __launch_bounds__(256) void mx4_values_kernel(Mx4Acts a, size_t jobs, int jobs_a_row, int cols, float *__restrict__ out) {
+    const int lane = threadIdx.x & 63;
+    for (size_t j = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); j < jobs; j += (size_t)gridDim.x * 4) {
+        const size_t row = j / jobs_a_row;
+        const int c = (int)(j % jobs_a_row);
+        const size_t block = row * a.blocks + (size_t)c * 8 + (lane >> 3);
+        const uint32_t codes = *reinterpret_cast<const uint32_t *>(a.codes + block * 16 + (lane & 3) * 4) >> (lane & 4);
+        const float scale = mx4_scale(a.scales[block]);
+        const float v[4] = {mx4_two(codes, 0).x * scale, mx4_two(codes, 1).x * scale, mx4_two(codes, 2).x * scale, mx4_two(codes, 3).x * scale};
+        floats_store4<FLOATS_F32, WIDE>(out + row * (size_t)cols, c * 256 + lane * 4, cols, v);
     }
 }
 int launch_mx4_values(const Mx4Acts &a, size_t cols, float *out, hipStream_t s) {
-    const size_t n = (size_t)a.rows * cols;
-    hipLaunchKernelGGL(mx4_values_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1 << 16)), dim3(256), 0, s, a, (int)cols, n, out);
+    const size_t jobs_a_row = (cols + 255) / 256, jobs = (size_t)a.rows * jobs_a_row;
+    const dim3 grid((unsigned)std::min<size_t>((jobs + 3) / 4, 1 << 16));
+    if (floats_wide(out, cols, FLOATS_F32)) hipLaunchKernelGGL(mx4_values_kernel<true>, grid, dim3(256), 0, s, a, jobs, (int)jobs_a_row, (int)cols, out);
+    else hipLaunchKernelGGL(mx4_values_kernel<false>, grid, dim3(256), 0, s, a, jobs, (int)jobs_a_row, (int)cols, out);
     FRK_LAUNCH_CHECK("mx4_values");
     return FRK_OK;
 }
 
-// ---- GGUF blocks: the scale byte, then sixteen bytes of codes.  128 of them are 2176 bytes, 136 pieces of sixteen: a workgroup puts them
-// together in LDS. ----
-constexpr int GGUF_BLOCKS = 128;
+// ---- GGUF blocks: the scale byte, then sixteen bytes of codes.  256 of them are 4352 bytes, 272 pieces of sixteen: a workgroup puts them
+// together in LDS.  Four lanes a block: of floats, a lane elements 4 l .. and 16 + 4 l .., whose codes share bytes; of two-byte numbers, eight
+// neighbours (sixteen bytes a load), whose codes meet those of the lane two further on. ----
+constexpr int GGUF_BLOCKS = 256;
+__device__ __forceinline__ void lds_put32(uint8_t *to, uint32_t v) { __builtin_memcpy(to, &v, 4); }  // (of any alignment)
 template <int TYPE, bool WIDE>
 __global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const typename Floats<TYPE>::type *__restrict__ x, size_t blocks, uint8_t *__restrict__ out, bool whole) {
+    typedef typename Floats<TYPE>::type T;
+    constexpr bool TWO_BYTES = sizeof(T) == 2;
+    constexpr int N = GGUF_BLOCKS / 64;
     __shared__ __align__(16) uint8_t lds[GGUF_BLOCKS * MXFP4_BYTES];
-    const int part = threadIdx.x & 3;
+    const int part = threadIdx.x & 3, low = TWO_BYTES ? 8 * part : 4 * part, high = TWO_BYTES ? 8 * part + 4 : 16 + 4 * part;
     for (size_t first = (size_t)blockIdx.x * GGUF_BLOCKS; first < blocks; first += (size_t)gridDim.x * GGUF_BLOCKS) {
-        float lo[2][4], hi[2][4];  // four lanes a block, elements 4 part .. and 16 + 4 part ..
+        float a[N][4], b[N][4];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const size_t b = first + i * 64 + (threadIdx.x >> 2);
-            const int left = b < blocks ? MX4_BLOCK : 0;
-            floats_load4<TYPE, WIDE>(x + b * MX4_BLOCK, 4 * part, left, lo[i]);
-            floats_load4<TYPE, WIDE>(x + b * MX4_BLOCK, 16 + 4 * part, left, hi[i]);
+        for (int i = 0; i < N; i++) {
+            const size_t block = first + i * 64 + (threadIdx.x >> 2);
+            const int left = block < blocks ? MX4_BLOCK : 0;
+            const T *const from = x + block * MX4_BLOCK;
+            if (TWO_BYTES && WIDE) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (left) v = *reinterpret_cast<const uint4 *>(from + low);
+                const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    a[i][j] = Floats<TYPE>::get((T)(d[j >> 1] >> (16 * (j & 1))));
+                    b[i][j] = Floats<TYPE>::get((T)(d[2 + (j >> 1)] >> (16 * (j & 1))));
+                }
+            } else {
+                floats_load4<TYPE, WIDE>(from, low, left, a[i]);
+                floats_load4<TYPE, WIDE>(from, high, left, b[i]);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            uint32_t top = max(mx4_top4(lo[i]), mx4_top4(hi[i]));
+        for (int i = 0; i < N; i++) {
+            uint32_t top = max(mx4_top4(a[i]), mx4_top4(b[i]));
             top = max(top, (uint32_t)dpp_i<DPP_QUAD_XOR1>((int)top));
             top = max(top, (uint32_t)dpp_i<DPP_QUAD_XOR2>((int)top));
-            const uint32_t by = mx4_scale_byte(top);
-            const uint32_t codes = mx4_codes4(lo[i], by) | mx4_codes4(hi[i], by) << 4;
+            const uint32_t by = mx4_scale_byte(top), ca = mx4_codes4(a[i], by), cb = mx4_codes4(b[i], by);
             uint8_t *const to = lds + (i * 64 + (threadIdx.x >> 2)) * MXFP4_BYTES;
             if (part == 0) to[0] = (uint8_t)by;
-#pragma unroll
-            for (int j = 0; j < 4; j++) to[1 + 4 * part + j] = (uint8_t)(codes >> (8 * j));
+            if (TWO_BYTES) {
+                const uint32_t fa = (uint32_t)dpp_i<DPP_QUAD_XOR2>((int)ca), fb = (uint32_t)dpp_i<DPP_QUAD_XOR2>((int)cb);
+                if (part < 2) lds_put32(to + 1 + low, ca | fa << 4), lds_put32(to + 5 + low, cb | fb << 4);
+            } else {
+                lds_put32(to + 1 + low, ca | cb << 4);
+            }
         }
         __syncthreads();
         const size_t bytes = (blocks - first < GGUF_BLOCKS ? blocks - first : GGUF_BLOCKS) * MXFP4_BYTES;
         uint8_t *const to = out + first * MXFP4_BYTES;
         if (whole && bytes == sizeof lds) {
-            if (threadIdx.x < sizeof lds / 16) reinterpret_cast<uint4 *>(to)[threadIdx.x] = reinterpret_cast<const uint4 *>(lds)[threadIdx.x];
+            for (int i = threadIdx.x; i < (int)sizeof lds / 16; i += 256) reinterpret_cast<uint4 *>(to)[i] = reinterpret_cast<const uint4 *>(lds)[i];
         } else {
             for (size_t i = threadIdx.x; i < bytes; i += 256) to[i] = lds[i];
         }
@@ -103,7 +143,7 @@ static int go_quantize_mxfp4(const void *x, size_t blocks, uint8_t *out, hipStre
     typedef typename Floats<TYPE>::type T;
     const dim3 grid((unsigned)std::min<size_t>((blocks + GGUF_BLOCKS - 1) / GGUF_BLOCKS, 1 << 16));
     const bool whole = (uintptr_t)out % 16 == 0;
-    if (floats_wide(x, MX4_BLOCK, TYPE)) hipLaunchKernelGGL((quantize_mxfp4_kernel<TYPE, true>), grid, dim3(256), 0, s, (const T *)x, blocks, out, whole);
+    if ((uintptr_t)x % 16 == 0) hipLaunchKernelGGL((quantize_mxfp4_kernel<TYPE, true>), grid, dim3(256), 0, s, (const T *)x, blocks, out, whole);
     else hipLaunchKernelGGL((quantize_mxfp4_kernel<TYPE, false>), grid, dim3(256), 0, s, (const T *)x, blocks, out, whole);
     FRK_LAUNCH_CHECK("quantize_mxfp4");
     return FRK_OK;
@@ -121,19 +161,21 @@ __global__ __launch_bounds__(256) void dequantize_mxfp4_kernel(const uint8_t *__
         const int n = (int)(blocks - first < GGUF_BLOCKS ? blocks - first : GGUF_BLOCKS);
         const uint8_t *const from = in + first * MXFP4_BYTES;
         if (whole && n == GGUF_BLOCKS) {
-            if (threadIdx.x < sizeof lds / 16) reinterpret_cast<uint4 *>(lds)[threadIdx.x] = reinterpret_cast<const uint4 *>(from)[threadIdx.x];
+            for (int i = threadIdx.x; i < (int)sizeof lds / 16; i += 256) reinterpret_cast<uint4 *>(lds)[i] = reinterpret_cast<const uint4 *>(from)[i];
         } else {
             for (int i = threadIdx.x; i < n * MXFP4_BYTES; i += 256) lds[i] = from[i];
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < GGUF_BLOCKS * 8 / 256; i++) {
-            const int four = i * 256 + (int)threadIdx.x, b = four >> 3, in4 = four & 3;  // four elements: 4 in4 .., of the upper half if (four & 4)
+            const int four = i * 256 + (int)threadIdx.x, b = four >> 3;  // four elements: 4 (four % 4) .., of the upper half if (four & 4)
             if (b >= n) break;
             const uint8_t *const block = lds + b * MXFP4_BYTES;
-            float v[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = mx4_value(block[1 + 4 * in4 + j] >> (four & 4) & 15u, block[0]);
+            uint32_t codes;
+            __builtin_memcpy(&codes, block + 1 + 4 * (four & 3), 4);
+            codes = codes >> (four & 4);  // (the low halves of the bytes are this thread's)
+            const float scale = mx4_scale(block[0]);
+            const float v[4] = {mx4_two(codes, 0).x * scale, mx4_two(codes, 1).x * scale, mx4_two(codes, 2).x * scale, mx4_two(codes, 3).x * scale};
             float *const to = out + first * MX4_BLOCK + (size_t)four * 4;
             if (wide) *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
             else to[0] = v[0], to[1] = v[1], to[2] = v[2], to[3] = v[3];
@@ -150,8 +192,8 @@ int launch_dequantize_mxfp4(const uint8_t *blocks, size_t n, float *out, hipStre
 }
 
 // ---- A few tokens: the weights' bytes bound it.  A workgroup of NW wavefronts has sixteen weight rows and up to 16 TT tokens; its
-// wavefronts share the columns, 512 at a time (a unit: sixteen blocks of a row, 64 bytes a lane in one piece, and a dword of scale bytes), and
-// their sums meet in LDS.  Lane l has weight row l % 16 and blocks 4 (l / 16) .. + 3 of a unit; product k of four takes block k of each lane.
+// wavefronts share the columns, 512 at a time (a unit: sixteen blocks of a row), and their sums meet in LDS.  Lane l has weight row l % 16 and,
+// in product k of a unit's four, block 4 k + l / 16, so that a load brings 64 bytes of each row in one piece.
 // FUSED: up to four tokens are quantized by the workgroup itself, a wavefront its own columns'. ----
 struct Mx4Rows {
     Mx4Gemm g;
@@ -162,10 +204,10 @@ constexpr int MX4_UNIT = 16, MX4_FUSED = 4;           // blocks; tokens
 constexpr int MX4_FUSED_UNIT = MX4_UNIT * 16 + MX4_UNIT;  // bytes of LDS a token and unit
 constexpr size_t MX4_FUSED_LDS = 40 * 1024;
 
-template <int NW, int TT, bool FUSED, bool WIDE>
+template <int NW, int TT, int D, bool FUSED, bool WIDE>
 __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int E2M1 = 4, D = TT >= 4 ? 1 : 2;  // units ahead
+    constexpr int E2M1 = 4;
     extern __shared__ __align__(16) uint8_t mx4_rows_lds[];  // FUSED: [units][tokens][MX4_FUSED_UNIT]
     __shared__ float4 sums[NW][TT][64];
     const Mx4Gemm &g = r.g;
@@ -179,25 +221,23 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
 #pragma unroll
     for (int t = 0; t < TT; t++) acc[t] = mx4_v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (u0 < u1) {
-        uint4 w[D][4], x[FUSED ? 1 : D][TT][4];
-        uint32_t ws[D], xs[FUSED ? 1 : D][TT];
+        // D units ahead; the scales: a row's sixteen bytes, of which product k takes byte l / 16 of dword k
+        uint4 w[D][4], ws[D], x[FUSED ? 1 : D][TT][4], xs[FUSED ? 1 : D][TT];
         auto fetch_w = [&](int d, int u) {
             u = min(u, u1 - 1);
             // (blocks past the row's last: the last one's codes, which meet zeros)
 #pragma unroll
-            for (int k = 0; k < 4; k++) w[d][k] = stream_load16(row + (size_t)min(u * MX4_UNIT + 4 * lg + k, g.blocks - 1) * 16);
-            const int live = g.blocks - (u * MX4_UNIT + 4 * lg);
-            const uint32_t four = *reinterpret_cast<const uint32_t *>(row_scales + (live > 0 ? u * MX4_UNIT + 4 * lg : 0));
-            ws[d] = live >= 4 ? four : live > 0 ? four & (0xffffffffu >> (32 - 8 * live)) : 0u;
+            for (int k = 0; k < 4; k++) w[d][k] = stream_load16(row + (size_t)min(u * MX4_UNIT + 4 * k + lg, g.blocks - 1) * 16);
+            ws[d] = stream_load16(row_scales + u * MX4_UNIT);
         };
         auto fetch_x = [&](int d, int u) {
             u = min(u, u1 - 1);
 #pragma unroll
             for (int t = 0; t < TT; t++) {
-                const size_t at = (size_t)min(16 * t + li, g.M - 1) * g.a.blocks + u * MX4_UNIT + 4 * lg;
+                const size_t at = (size_t)min(16 * t + li, g.M - 1) * g.a.blocks + u * MX4_UNIT;
 #pragma unroll
-                for (int k = 0; k < 4; k++) x[d][t][k] = reinterpret_cast<const uint4 *>(g.a.codes)[at + k];
-                xs[d][t] = *reinterpret_cast<const uint32_t *>(g.a.scales + at);
+                for (int k = 0; k < 4; k++) x[d][t][k] = reinterpret_cast<const uint4 *>(g.a.codes)[at + 4 * k + lg];
+                xs[d][t] = *reinterpret_cast<const uint4 *>(g.a.scales + at);
             }
         };
         uint8_t *const own = mx4_rows_lds + (size_t)u0 * g.M * MX4_FUSED_UNIT;  // FUSED: this wavefront's units
@@ -236,24 +276,23 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
             if (FUSED) {
                 const uint8_t *const from = own + ((size_t)(u - u0) * g.M + min(li, g.M - 1)) * MX4_FUSED_UNIT;
 #pragma unroll
-                for (int k = 0; k < 4; k++) x[0][0][k] = *reinterpret_cast<const uint4 *>(from + (4 * lg + k) * 16);
-                xs[0][0] = *reinterpret_cast<const uint32_t *>(from + MX4_UNIT * 16 + 4 * lg);
+                for (int k = 0; k < 4; k++) x[0][0][k] = *reinterpret_cast<const uint4 *>(from + (4 * k + lg) * 16);
+                xs[0][0] = *reinterpret_cast<const uint4 *>(from + MX4_UNIT * 16);
             }
             const int e = FUSED ? 0 : d;
-#define FRK_MX4_PRODUCT(K)                                                                                                                    \
-    {                                                                                                                                         \
-        const mx4_v8i a = {(int)w[d][K].x, (int)w[d][K].y, (int)w[d][K].z, (int)w[d][K].w, 0, 0, 0, 0};                                       \
-        const mx4_v8i b = {(int)x[e][t][K].x, (int)x[e][t][K].y, (int)x[e][t][K].z, (int)x[e][t][K].w, 0, 0, 0, 0};                           \
-        acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], E2M1, E2M1, K, (int)ws[d], K, (int)xs[e][t]);                 \
-    }
+            const uint32_t wb[4] = {ws[d].x, ws[d].y, ws[d].z, ws[d].w};
 #pragma unroll
-            for (int t = 0; t < TT; t++) {
-                FRK_MX4_PRODUCT(0)
-                FRK_MX4_PRODUCT(1)
-                FRK_MX4_PRODUCT(2)
-                FRK_MX4_PRODUCT(3)
+            for (int k = 0; k < 4; k++) {
+                // (past the row's last block whatever lies there: no byte of it may be a NaN)
+                const int ew = u * MX4_UNIT + 4 * k + lg < g.blocks ? (int)(wb[k] >> (8 * lg)) : 0;
+                const mx4_v8i a = {(int)w[d][k].x, (int)w[d][k].y, (int)w[d][k].z, (int)w[d][k].w, 0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < TT; t++) {
+                    const uint32_t xb[4] = {xs[e][t].x, xs[e][t].y, xs[e][t].z, xs[e][t].w};
+                    const mx4_v8i b = {(int)x[e][t][k].x, (int)x[e][t][k].y, (int)x[e][t][k].z, (int)x[e][t][k].w, 0, 0, 0, 0};
+                    acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], E2M1, E2M1, 0, ew, 0, (int)(xb[k] >> (8 * lg)));
+                }
             }
-#undef FRK_MX4_PRODUCT
         };
         for (int u = u0; u < u1; u += D)
 #pragma unroll
@@ -288,11 +327,11 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
         if (r0 + i < g.rows) dst[i] = out[i];
 #endif
 }
-template <int NW, int TT, bool FUSED>
+template <int NW, int TT, int D, bool FUSED>
 static int go_mx4_rows(const Mx4Rows &r, size_t lds, hipStream_t s) {
     const dim3 grid((unsigned)((r.g.rows + 15) / 16));
-    if (FUSED && floats_wide(r.x, (size_t)r.cols, FLOATS_F32)) hipLaunchKernelGGL((mx4_rows_kernel<NW, TT, FUSED, FUSED>), grid, dim3(64 * NW), lds, s, r);
-    else hipLaunchKernelGGL((mx4_rows_kernel<NW, TT, FUSED, false>), grid, dim3(64 * NW), lds, s, r);
+    if (FUSED && floats_wide(r.x, (size_t)r.cols, FLOATS_F32)) hipLaunchKernelGGL((mx4_rows_kernel<NW, TT, D, FUSED, FUSED>), grid, dim3(64 * NW), lds, s, r);
+    else hipLaunchKernelGGL((mx4_rows_kernel<NW, TT, D, FUSED, false>), grid, dim3(64 * NW), lds, s, r);
     FRK_LAUNCH_CHECK("mx4_rows");
     return FRK_OK;
 }
@@ -346,10 +385,12 @@ int launch_mx4_gemm(const frk_weights *w, const Mx4Plan &plan, const float *x, c
     g.y = y;
     r.x = x;
     r.cols = (int)w->cols;
-    if (plan.fused) return go_mx4_rows<8, 1, true>(r, batch * ((g.blocks + MX4_UNIT - 1) / MX4_UNIT) * MX4_FUSED_UNIT, s);
-    if (batch <= 16) return go_mx4_rows<8, 1, false>(r, 0, s);
-    if (batch <= 32) return go_mx4_rows<8, 2, false>(r, 0, s);
-    return go_mx4_rows<8, 4, false>(r, 0, s);
+    const size_t units = (g.blocks + MX4_UNIT - 1) / MX4_UNIT, lds = batch * units * MX4_FUSED_UNIT;
+    const bool one = units <= 8;  // a unit a wavefront at most
+    if (plan.fused) return one ? go_mx4_rows<8, 1, 1, true>(r, lds, s) : go_mx4_rows<8, 1, 2, true>(r, lds, s);
+    if (batch <= 16) return one ? go_mx4_rows<8, 1, 1, false>(r, 0, s) : go_mx4_rows<8, 1, 2, false>(r, 0, s);
+    if (batch <= 32) return one ? go_mx4_rows<8, 2, 1, false>(r, 0, s) : go_mx4_rows<8, 2, 2, false>(r, 0, s);
+    return go_mx4_rows<8, 4, 1, false>(r, 0, s);
 }
 
 }  // namespace frk

@@ -77,11 +77,8 @@ __device__ __forceinline__ void mx4_store_chunk(const Mx4Acts &out, size_t row, 
     if ((lane & 7) == 0) out.scales[block] = (uint8_t)by;
 }
 
-// E2M1 code (three bits of magnitude, a sign) times 2^(by - 127)
-__device__ __forceinline__ float mx4_value(uint32_t code, uint32_t by) {
-    const float scale = by == 255u ? __uint_as_float(0x7fc00000u) : by == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(by << 23);
-    const float half = (float)(0xc8643210u >> (4 * (code & 7)) & 15u) * 0.5f;  // 0, 1, 2, 3, 4, 6, 8, 12 halves
-    return (code & 8 ? -half : half) * scale;
+__device__ __forceinline__ float mx4_scale(uint32_t by) {
+    return by == 255u ? __uint_as_float(0x7fc00000u) : by == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(by << 23);
 }
 
 // ---- numbers of the types that norms and quantizations take ----

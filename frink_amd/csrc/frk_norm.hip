@@ -18,10 +18,36 @@ namespace frk {
         if (e_ != hipSuccess) return set_error(FRK_ERR_HIP, what " launch: %s", hipGetErrorString(e_)); \
     } while (0)
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+// v (op) lane-permuted v, the permutation given by a DPP control word
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)(uint32_t)dpp_i<CTRL>((int)b) | (uint64_t)(uint32_t)dpp_i<CTRL>((int)(b >> 32)) << 32));
+}
+__device__ __forceinline__ double row_sum64(double v) {  // over sixteen lanes
+    v += dpp_d<DPP_QUAD_XOR1>(v);
+    v += dpp_d<DPP_QUAD_XOR2>(v);
+    v += dpp_d<DPP_HALF_MIRROR>(v);
+    v += dpp_d<DPP_ROW_MIRROR>(v);
     return v;
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)b, lane) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32));
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+    v = row_sum64(v);
+    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+// 1 / sqrt(a) to a few units in the last place of 64 bits: the instruction's value and two of Newton's steps (a root and a quotient correct to the
+// last bit are 60 instructions more, and the f32 that it is rounded to differs once in 2^27)
+__device__ __forceinline__ double inverse_root(double a) {
+    double y = __builtin_amdgcn_rsq(a);
+    if (a > 0.0 && a < 1.0e300) {  // (zero and infinity: the instruction's)
+        y = fma(y, fma(-0.5 * a * y, y, 0.5), y);
+        y = fma(y, fma(-0.5 * a * y, y, 0.5), y);
+    }
+    return y;
 }
 
 // 256 values of a row (four a lane) in the form that the products read
@@ -93,9 +119,19 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a, NormOut out)
 #pragma unroll
             for (int i = 0; i < 4; i++) sum = fma((double)v[i], (double)v[i], sum);
         };
+        auto load_weight = [&](int c, float (&w)[4]) {
+            const int k = c * 256 + lane * 4;
+            if (!a.weight) return;
+            if (a.weight_type == FLOATS_F32) floats_load4<FLOATS_F32, WIDE>((const float *)a.weight, k, cols, w);
+            else if (a.weight_type == FLOATS_BF16) floats_load4<FLOATS_BF16, WIDE>((const uint16_t *)a.weight, k, cols, w);
+            else floats_load4<FLOATS_F16, WIDE>((const uint16_t *)a.weight, k, cols, w);
+        };
+        float w[N][4];
         if (CHUNKS) {
 #pragma unroll
             for (int i = 0; i < N; i++) load(mine + i * a.waves, h[i], a.sum != nullptr);
+#pragma unroll
+            for (int i = 0; i < N; i++) load_weight(mine + i * a.waves, w[i]);  // (here: not another trip to memory behind the sum)
 #pragma unroll
             for (int i = 0; i < N; i++) add(h[i]);
         } else {
@@ -108,20 +144,16 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a, NormOut out)
         if (a.waves > 1) {  // (uniform over the launch)
             if (lane == 0) sums[parity][wave] = sum;
             __syncthreads();
-            sum = sums[parity][slot];
-            for (int w = 1; w < a.waves; w++) sum += sums[parity][slot + w];
+            const double part = sums[parity][slot + (lane & 15 & (a.waves - 1))];
+            sum = row_sum64((lane & 15) < a.waves ? part : 0.0);
         }
-        const float r = (float)(1.0 / sqrt(sum / (double)cols + a.eps));
-        auto finish = [&](int c, const float (&v)[4]) {
+        const float r = (float)inverse_root(fma(sum, a.inverse_cols, a.eps));
+        auto finish = [&](int c, const float (&v)[4], const float (&w)[4]) {
             const int k = c * 256 + lane * 4;
             float y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) y[i] = v[i] * r;
             if (a.weight) {
-                float w[4];
-                if (a.weight_type == FLOATS_F32) floats_load4<FLOATS_F32, WIDE>((const float *)a.weight, k, cols, w);
-                else if (a.weight_type == FLOATS_BF16) floats_load4<FLOATS_BF16, WIDE>((const uint16_t *)a.weight, k, cols, w);
-                else floats_load4<FLOATS_F16, WIDE>((const uint16_t *)a.weight, k, cols, w);
 #pragma unroll
                 for (int i = 0; i < 4; i++) y[i] *= w[i];
             }
@@ -134,13 +166,14 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a, NormOut out)
         if (CHUNKS) {
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (mine + i * a.waves < chunks) finish(mine + i * a.waves, h[i]);
+                if (mine + i * a.waves < chunks) finish(mine + i * a.waves, h[i], w[i]);
         } else {
             // (the residual, where the sum may have taken its place or x's, is in the sum)
             for (int c = mine; c < chunks; c += a.waves) {
                 if (a.sum) floats_load4<TYPE, WIDE>(h_out, c * 256 + lane * 4, live ? cols : 0, h[0]);
                 else load(c, h[0], false);
-                finish(c, h[0]);
+                load_weight(c, w[0]);
+                finish(c, h[0], w[0]);
             }
         }
     }
@@ -181,6 +214,7 @@ static int go_rms_norm_type(const NormArgs &a, int form, const NormOut &out, hip
 }
 int launch_rms_norm(int type, NormArgs a, int form, const NormOut &out, hipStream_t s) {
     // a form's rows are padded with zeros to whole blocks, MXFP4's to sixteen
+    a.inverse_cols = 1.0 / a.cols;
     a.chunks = form == ACTS_MXFP4 ? out.mx4.blocks / 8 : (a.cols + 255) / 256;
     switch (type) {
     case FLOATS_F32: return go_rms_norm_type<FLOATS_F32>(a, form, out, s);
@@ -189,37 +223,45 @@ int launch_rms_norm(int type, NormArgs a, int form, const NormOut &out, hipStrea
     }
 }
 
-// ---- what quantized rows stand for ----
-__global__ __launch_bounds__(256) void q8_k_values_kernel(Q8KActs plain, Q8KTiled tiled, int nb, size_t n, float *__restrict__ out) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const size_t block = i / QK_K;
-        if (plain.q) {
-            out[i] = (float)plain.q[i] * plain.d[block];
+// ---- what quantized rows stand for: a wavefront 256 values at a time ----
+template <int FORM, bool WIDE>
+__global__ __launch_bounds__(256) void acts_values_kernel(NormOut in, size_t jobs, int jobs_a_row, int cols, float *__restrict__ out) {
+    const int lane = threadIdx.x & 63;
+    for (size_t j = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); j < jobs; j += (size_t)gridDim.x * 4) {
+        const size_t row = j / jobs_a_row;
+        const int c = (int)(j % jobs_a_row);
+        float v[4];
+        if (FORM == ACTS_FP8) {
+            const F8Acts &a = in.f8.v ? in.f8 : in.f8_strips;
+            const int b = min(2 * c + (lane >> 5), in.f8_blocks - 1), at = (lane & 31) * 4;
+            const uint2 two = *reinterpret_cast<const uint2 *>(a.v + (a.strips ? f8_strip_at(row, b, at, in.f8_blocks) : (row * in.f8_blocks + b) * F8_BLOCK + at));
+            const uint32_t d[2] = {two.x, two.y};
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = __uint_as_float(i & 1 ? d[i >> 1] & 0xffff0000u : d[i >> 1] << 16) * F8_UP;
         } else {
-            const int row = (int)(block / nb), kb = (int)(block % nb);
-            out[i] = (float)tiled.q[q8k_tiled_index(nb, row, kb, (int)(i % QK_K))] * tiled.d[((size_t)(row >> 5) * nb + kb) * 32 + (row & 31)];
+            const int nb = in.q8k_blocks;
+            const size_t rec = (row >> 5) * nb + c;
+            const uint32_t q = in.plain.q ? reinterpret_cast<const uint32_t *>(in.plain.q + (row * nb + c) * QK_K)[lane]
+                                          : *reinterpret_cast<const uint32_t *>(in.tiled.q + q8k_tiled_index(nb, (int)row, c, lane * 4));
+            const float d = in.plain.q ? in.plain.d[row * nb + c] : in.tiled.d[rec * 32 + (row & 31)];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = (float)(int8_t)(q >> (8 * i)) * d;
         }
+        floats_store4<FLOATS_F32, WIDE>(out + row * (size_t)cols, c * 256 + lane * 4, cols, v);
     }
 }
-int launch_q8_k_values(const Q8KActs &plain, const Q8KTiled &tiled, size_t rows, size_t cols, float *out, hipStream_t s) {
-    const size_t n = rows * cols;
-    hipLaunchKernelGGL(q8_k_values_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1 << 16)), dim3(256), 0, s, plain, tiled, (int)(cols / QK_K), n, out);
-    FRK_LAUNCH_CHECK("q8_k_values");
+template <int FORM>
+static int go_acts_values(const NormOut &in, size_t rows, size_t cols, float *out, hipStream_t s) {
+    const size_t jobs_a_row = (cols + 255) / 256, jobs = rows * jobs_a_row;
+    const dim3 grid((unsigned)std::min<size_t>((jobs + 3) / 4, 1 << 16));
+    if (floats_wide(out, cols, FLOATS_F32)) hipLaunchKernelGGL((acts_values_kernel<FORM, true>), grid, dim3(256), 0, s, in, jobs, (int)jobs_a_row, (int)cols, out);
+    else hipLaunchKernelGGL((acts_values_kernel<FORM, false>), grid, dim3(256), 0, s, in, jobs, (int)jobs_a_row, (int)cols, out);
+    FRK_LAUNCH_CHECK("acts_values");
     return FRK_OK;
 }
-__global__ __launch_bounds__(256) void acts_values_fp8_kernel(F8Acts a, int cols, int blocks, size_t n, float *__restrict__ out) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const size_t row = i / cols;
-        const int k = (int)(i % cols), b = k / F8_BLOCK, in = k % F8_BLOCK;
-        const size_t at = a.strips ? f8_strip_at(row, b, in, blocks) : (row * blocks + b) * F8_BLOCK + in;
-        out[i] = __uint_as_float((uint32_t)a.v[at] << 16) * F8_UP;
-    }
-}
-int launch_f8_values(const F8Acts &a, size_t cols, float *out, hipStream_t s) {
-    const size_t n = (size_t)a.rows * cols;
-    hipLaunchKernelGGL(acts_values_fp8_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1 << 16)), dim3(256), 0, s, a, (int)cols, (int)f8_blocks(cols), n, out);
-    FRK_LAUNCH_CHECK("f8_values");
-    return FRK_OK;
+int launch_acts_values(int form, const NormOut &in, size_t rows, size_t cols, float *out, hipStream_t s) {
+    if (form == ACTS_MXFP4) return launch_mx4_values(in.mx4, cols, out, s);
+    return form == ACTS_FP8 ? go_acts_values<ACTS_FP8>(in, rows, cols, out, s) : go_acts_values<ACTS_Q8_K>(in, rows, cols, out, s);
 }
 
 }  // namespace frk

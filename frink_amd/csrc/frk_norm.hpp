@@ -12,9 +12,9 @@ struct NormArgs {
     const void *x, *residual;  // [batch][cols] of one type; residual: or null
     const void *weight;        // [cols] of weight_type, or null: ones
     int weight_type;
-    double eps;
+    double eps, inverse_cols;
     size_t batch, rows;  // rows: the batch, or more of a form whose last tile's rows are to be zeros
-    int cols, chunks, waves;  // (chunks, waves: the launch's own)
+    int cols, chunks, waves;  // (chunks, waves, inverse_cols: the launch's own)
     void *sum, *y;       // of x's type; or null
 };
 struct NormOut {  // (of one form; null pointers: not wanted)
@@ -26,7 +26,7 @@ struct NormOut {  // (of one form; null pointers: not wanted)
     Mx4Acts mx4;
 };
 int launch_rms_norm(int type, NormArgs a, int form, const NormOut &out, hipStream_t s);
-int launch_q8_k_values(const Q8KActs &plain, const Q8KTiled &tiled, size_t rows, size_t cols, float *out, hipStream_t s);
-int launch_f8_values(const F8Acts &a, size_t cols, float *out, hipStream_t s);
+// the numbers that a batch in one form (its pointers set) stands for
+int launch_acts_values(int form, const NormOut &in, size_t rows, size_t cols, float *out, hipStream_t s);
 
 }  // namespace frk

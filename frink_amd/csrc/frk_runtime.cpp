@@ -1366,17 +1366,30 @@ int frk_hip_gemm_acts_dev(const frk_weights *w, const frk_batch_acts *a, float *
     return FRK_OK;
 }
 
+// where a batch lies in an object
+static NormOut acts_out(const frk_batch_acts *a, size_t batch) {
+    NormOut out{};
+    if (a->form == FRK_ACTS_FP8) {
+        if (f8_acts_rows(batch)) out.f8 = f8_acts_of(a, batch, false);
+        if (f8_acts_strips(batch)) out.f8_strips = f8_acts_of(a, batch, true);
+        out.f8_blocks = (int)f8_blocks(a->cols);
+    } else if (a->form == FRK_ACTS_MXFP4) {
+        out.mx4 = mx4_acts_carve(a->base, batch, a->cols);
+    } else {
+        out.plain = q8k_plain_of(a, batch);
+        if (batch >= ACTS_TILED_MIN_BATCH) out.tiled = q8k_tiled_carve((char *)a->base + a->tiled_off, batch, a->cols);
+        out.q8k_blocks = (int)(a->cols / QK_K);
+    }
+    return out;
+}
+
 int frk_hip_batch_acts_values_dev(const frk_batch_acts *a, float *out, void *stream) {
     clear_error();
     if (!a || !out) return set_error(FRK_ERR_ARG, "frk_hip_batch_acts_values_dev: null argument");
     if (a->batch == 0) return set_error(FRK_ERR_ARG, "frk_hip_batch_acts_values_dev: the activations hold no quantized batch");
     int rc = acts_on_current_device(a);
     if (rc) return rc;
-    hipStream_t s = (hipStream_t)stream;
-    if (a->form == FRK_ACTS_MXFP4) return launch_mx4_values(mx4_acts_carve(a->base, a->batch, a->cols), a->cols, out, s);
-    if (a->form == FRK_ACTS_FP8) return launch_f8_values(f8_acts_of(a, a->batch, !f8_acts_rows(a->batch)), a->cols, out, s);
-    const Q8KActsOut plain = q8k_plain_of(a, a->batch);
-    return launch_q8_k_values(Q8KActs{plain.q, plain.d, plain.bsums}, q8k_tiled_carve((char *)a->base + a->tiled_off, a->batch, a->cols), a->batch, a->cols, out, s);
+    return launch_acts_values(a->form, acts_out(a, a->batch), a->batch, a->cols, out, (hipStream_t)stream);
 }
 
 static bool is_float_type(int type) { return type == FRK_TYPE_F32 || type == FRK_TYPE_BF16 || type == FRK_TYPE_F16; }
@@ -1408,21 +1421,10 @@ int frk_hip_rms_norm_dev(int type, const void *x, const void *residual, int weig
         int rc = acts_on_current_device(acts);
         if (rc) return rc;
         acts->batch = 0;
-        if (acts->form == FRK_ACTS_FP8) {
-            if (f8_acts_rows(batch)) out.f8 = f8_acts_of(acts, batch, false);
-            if (f8_acts_strips(batch)) out.f8_strips = f8_acts_of(acts, batch, true);
-            out.f8_blocks = (int)f8_blocks(cols);
-        } else if (acts->form == FRK_ACTS_MXFP4) {
-            out.mx4 = mx4_acts_carve(acts->base, batch, cols);
-        } else {
-            out.plain = q8k_plain_of(acts, batch);
-            if (out.plain.q) acts->plain = Q8KActs{out.plain.q, out.plain.d, out.plain.bsums};
-            out.q8k_blocks = (int)(cols / QK_K);
-            if (batch >= ACTS_TILED_MIN_BATCH) {
-                out.tiled = q8k_tiled_carve((char *)acts->base + acts->tiled_off, batch, cols);
-                if (batch >= tiled_from(cols)) a.rows = round_up(batch, 32);  // (as the quantizations do: the kernels of larger batches want zeros there)
-            }
-        }
+        out = acts_out(acts, batch);
+        if (out.plain.q) acts->plain = Q8KActs{out.plain.q, out.plain.d, out.plain.bsums};
+        // (as the quantizations do: the kernels of larger batches want zeros in a last tile's other rows)
+        if (out.tiled.q && batch >= tiled_from(cols)) a.rows = round_up(batch, 32);
     }
     int rc = launch_rms_norm(type, a, acts ? acts->form : (int)ACTS_NONE, out, (hipStream_t)stream);
     if (rc) return rc;
