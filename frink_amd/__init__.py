@@ -351,7 +351,8 @@ class Weights:
     def gemm_mxfp4(self, x, out=None):
         """An MXFP4 matrix over x[batch][cols] f32 quantized to MXFP4 within the call (frk_hip_gemm_mxfp4_dev)."""
         import torch
-        _float_type(torch, x, "f32")
+        if _float_type(torch, x, "f32"):
+            raise ValueError("activations of %s: f32" % x.dtype)
         if x.dim() == 0 or x.shape[-1] != self.cols:
             raise ValueError("activations %s: the matrix has %d columns" % (tuple(x.shape), self.cols))
         batch = x.numel() // self.cols
@@ -431,22 +432,24 @@ class BatchActs:
             pass
 
 
-def _float_types(torch):
-    global _FLOAT_TYPES
-    if _FLOAT_TYPES is None:
-        _FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    return _FLOAT_TYPES
-
-
 _FLOAT_TYPES = None  # torch's types -> FRK_TYPE_*
 
 
 def _float_type(torch, t, which="f32, bf16 or f16"):
     """FRK_TYPE_* of a contiguous tensor on a GPU."""
-    kind = _float_types(torch).get(t.dtype)
-    if kind is None or (which == "f32" and kind) or not t.is_cuda or not t.is_contiguous():
+    global _FLOAT_TYPES
+    if _FLOAT_TYPES is None:
+        _FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    kind = _FLOAT_TYPES.get(t.dtype)
+    if kind is None or not t.is_cuda or not t.is_contiguous():
         raise ValueError("%s of %s on %s: contiguous %s on a GPU" % (tuple(t.shape), t.dtype, t.device, which))
     return kind
+
+
+def _like(t, x, n):
+    """A second operand of x's type and n values."""
+    if t.dtype is not x.dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError("%s of %s beside activations %s of %s" % (tuple(t.shape), t.dtype, tuple(x.shape), x.dtype))
 
 
 def rms_norm(x, weight=None, eps=1e-5, residual=None, out=None, sum_out=None, acts=None):
@@ -454,32 +457,38 @@ def rms_norm(x, weight=None, eps=1e-5, residual=None, out=None, sum_out=None, ac
     last dimension of x (f32, bf16 or f16; weight of any of them).  h goes to `sum_out` (which may be x or residual), y to `out`, both of x's
     type and shape; with `acts` y is quantized into that BatchActs, which is returned in y's place (and y written only where `out` is given)."""
     import torch
-    kind = _float_type(torch, x)
-    cols = x.shape[-1] if x.dim() else 0
-    if cols == 0 or x.numel() == 0:
+    kind, n = _float_type(torch, x), x.numel()
+    if n == 0 or x.dim() == 0:
         raise ValueError("activations %s" % (tuple(x.shape),))
-    batch = x.numel() // cols
-    weight_kind = 0
+    cols = x.shape[-1]
+    # (a call's host side, 2.2 us of it the launch, is what one token's norm waits for: nothing is looked at twice)
+    w_kind, w_ptr, r_ptr, s_ptr, y_ptr = 0, None, None, None, None
     if weight is not None:
-        weight_kind = _float_type(torch, weight)
+        w_kind, w_ptr = _float_type(torch, weight), weight.data_ptr()
         if weight.numel() != cols:
             raise ValueError("%d weights for rows of %d columns" % (weight.numel(), cols))
-    if residual is not None and sum_out is None:
-        sum_out = torch.empty_like(x)
-    if out is None and acts is None:
+    if residual is not None:
+        _like(residual, x, n)
+        r_ptr = residual.data_ptr()
+        if sum_out is None:
+            sum_out, s_ptr = (h := torch.empty_like(x)), h.data_ptr()
+    if sum_out is not None and s_ptr is None:
+        _like(sum_out, x, n)
+        s_ptr = sum_out.data_ptr()
+    if out is not None:
+        _like(out, x, n)
+        y_ptr = out.data_ptr()
+    elif acts is None:
         out = torch.empty_like(x)
-    for t in (residual, sum_out, out):
-        if t is not None and (t.dtype is not x.dtype or t.numel() != x.numel() or not t.is_contiguous()):
-            raise ValueError("%s of %s beside activations %s of %s" % (tuple(t.shape), t.dtype, tuple(x.shape), x.dtype))
+        y_ptr = out.data_ptr()
     stream = _fp8_stream(torch, x, (weight, residual, sum_out, out))
-    if acts is not None:
-        acts.batch = 0
-    check(lib().frk_hip_rms_norm_dev(kind, x.data_ptr(), None if residual is None else residual.data_ptr(), weight_kind,
-                                     None if weight is None else weight.data_ptr(), eps, batch, cols, None if sum_out is None else sum_out.data_ptr(),
-                                     None if out is None else out.data_ptr(), None if acts is None else acts.handle, stream))
-    if acts is not None:
-        acts.batch = batch
-    return out if acts is None else acts, x if sum_out is None else sum_out
+    if acts is None:
+        check(lib().frk_hip_rms_norm_dev(kind, x.data_ptr(), r_ptr, w_kind, w_ptr, eps, n // cols, cols, s_ptr, y_ptr, None, stream))
+        return out, x if sum_out is None else sum_out
+    acts.batch = 0
+    check(lib().frk_hip_rms_norm_dev(kind, x.data_ptr(), r_ptr, w_kind, w_ptr, eps, n // cols, cols, s_ptr, y_ptr, acts.handle, stream))
+    acts.batch = n // cols
+    return acts, x if sum_out is None else sum_out
 
 
 def quantize_mxfp4(x, out=None):

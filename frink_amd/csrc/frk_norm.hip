@@ -181,16 +181,17 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a, NormOut out)
 
 template <int TYPE, int FORM, bool WIDE>
 static int go_rms_norm(NormArgs a, const NormOut &out, hipStream_t s) {
-    // Few rows: as many wavefronts a row as it has chunks, up to sixteen.  Many rows: four chunks a wavefront.
-    const int chunks = a.chunks;
-    const bool few = a.rows <= 512;
+    // Two chunks a wavefront, four where the rows fill the chip.  us (a launch after the other, x and the residual of 4 batches in turn, f32 to FP8),
+    // chunks a wavefront 1 / 2 / 4 / 8: 4096 columns, 1 row 3.9 / 3.9 / 5.0 / 9.0, 512 rows 8.7 / 7.7 / 8.5 / 13.4, 2048 rows 30.4 / 27.7 / 29.0 /
+    // 31.0; of 8192 columns (sixteen wavefronts hold two) 2 / 4 / 8: 1 row 4.7 / 5.5 / 9.5, 128 rows 6.3 / 7.3 / 12.8, 512 rows 13.9 / 12.8 / 15.9.
+    const int chunks = a.chunks, most = a.rows > 256 ? 8 : 16;
     int waves = 1;
-    while (waves < 16 && waves * (few ? 1 : 4) < chunks) waves *= 2;
+    while ((waves < most && 2 * waves < chunks) || (waves < 16 && 4 * waves < chunks)) waves *= 2;
     a.waves = waves;
-    const int waves_wg = std::max(waves, few ? 1 : 4);
+    const int waves_wg = std::max(waves, a.rows > 512 ? 4 : 1);
     const size_t rows_wg = (size_t)(waves_wg / waves);
     const dim3 grid((unsigned)std::min<size_t>((a.rows + rows_wg - 1) / rows_wg, 1 << 16)), block(64 * waves_wg);
-    if (chunks <= waves) hipLaunchKernelGGL((rms_norm_kernel<TYPE, 1, FORM, WIDE>), grid, block, 0, s, a, out);
+    if (chunks <= 2 * waves) hipLaunchKernelGGL((rms_norm_kernel<TYPE, 2, FORM, WIDE>), grid, block, 0, s, a, out);
     else if (chunks <= 4 * waves) hipLaunchKernelGGL((rms_norm_kernel<TYPE, 4, FORM, WIDE>), grid, block, 0, s, a, out);
     else hipLaunchKernelGGL((rms_norm_kernel<TYPE, 0, FORM, WIDE>), grid, block, 0, s, a, out);
     FRK_LAUNCH_CHECK("rms_norm");
