@@ -3,6 +3,7 @@
 #include "frk_mx4.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace frk {
 
@@ -21,10 +22,13 @@ typedef float mx4_v16f __attribute__((ext_vector_type(16)));
 template <int RW, int TW, int MR, int MT>
 struct Mx4TileShape {
     static constexpr int WAVES = RW * TW, ROWS = RW * MR * 32, TOKENS = TW * MT * 32, ALL = ROWS + TOKENS;
-    static constexpr int STAGES = 2, STAGE = ALL * 128, SCALES = ALL * 16;  // scales: sixteen blocks, of two stages; two slots
-    static constexpr int W_REQUESTS = ROWS / 8 / WAVES, X_REQUESTS = TOKENS / 8 / WAVES, S_REQUESTS = (ALL / 64 + WAVES - 1) / WAVES;
+    static constexpr int STAGES = 2, STAGE = ALL * 128, SCALES = ALL * 16;  // scales: sixteen blocks, of two stages; two places
+    static constexpr int W_REQUESTS = ROWS / 8 / WAVES, X_REQUESTS = TOKENS / 8 / WAVES, REQUESTS = W_REQUESTS + X_REQUESTS;
+    static constexpr int S_REQUESTS = (ALL / 64 + WAVES - 1) / WAVES;
     static_assert(W_REQUESTS * 8 * WAVES == ROWS && X_REQUESTS * 8 * WAVES == TOKENS && ROWS % 64 == 0 && TOKENS % 64 == 0, "whole requests");
+    static constexpr int PITCH = MR * 32 + 4;  // floats a token in the results' place in LDS: sixteen lanes' pieces in different banks
     static constexpr size_t LDS = STAGES * STAGE + 2 * SCALES;
+    static_assert((size_t)WAVES * 32 * PITCH * 4 <= LDS, "a group of tokens of every wavefront");
     static_assert(LDS <= 160 * 1024, "LDS of a CU");
 };
 
@@ -55,35 +59,33 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, in
     const uint8_t *const x_base = g.a.codes + (size_t)tok0 * g.a.blocks * 16;
     const uint8_t *const xs_base = g.a.scales + (size_t)tok0 * g.a.blocks;
     const uint8_t *const ws_base = w_base + (size_t)g.blocks * 16;
+    const int last_row = g.rows - 1 - row0, last_token = g.M - 1 - tok0;
 #pragma unroll
     for (int c = 0; c < T::W_REQUESTS; c++) {
         const int r = (c * T::WAVES + wave) * 8 + (lane >> 3);
-        w_off[c] = (uint32_t)min(r, g.rows - 1 - row0) * (uint32_t)g.row_stride + (uint32_t)((lane & 7) ^ ((r >> 1) & 7)) * 16;
+        w_off[c] = (uint32_t)min(r, last_row) * (uint32_t)g.row_stride + (uint32_t)((lane & 7) ^ ((r >> 1) & 7)) * 16;
     }
 #pragma unroll
     for (int c = 0; c < T::X_REQUESTS; c++) {
         const int r = (c * T::WAVES + wave) * 8 + (lane >> 3);
-        x_off[c] = (uint32_t)min(r, g.M - 1 - tok0) * (uint32_t)(g.a.blocks * 16) + (uint32_t)((lane & 7) ^ ((r >> 1) & 7)) * 16;
+        x_off[c] = (uint32_t)min(r, last_token) * (uint32_t)(g.a.blocks * 16) + (uint32_t)((lane & 7) ^ ((r >> 1) & 7)) * 16;
     }
 #pragma unroll
     for (int c = 0; c < T::S_REQUESTS; c++) {  // 64 rows a request, weight rows first
-        const int q = c * T::WAVES + wave, r = q * 64 + lane;
-        s_off[c] = q * 64 < T::ROWS ? (uint32_t)min(r, g.rows - 1 - row0) * (uint32_t)g.row_stride
-                                    : (uint32_t)min(r - T::ROWS, g.M - 1 - tok0) * (uint32_t)g.a.blocks;
+        const int q = min(c * T::WAVES + wave, T::ALL / 64 - 1), r = q * 64 + lane;
+        s_off[c] = q * 64 < T::ROWS ? (uint32_t)min(r, last_row) * (uint32_t)g.row_stride : (uint32_t)min(r - T::ROWS, last_token) * (uint32_t)g.a.blocks;
     }
-    auto request = [&](int i) {
+    auto request_codes = [&](int i, int c) {  // request c of stage i
         const uint32_t to = lds0 + (uint32_t)(i & 1) * T::STAGE;
+        if (c < T::W_REQUESTS) dma16(to + (uint32_t)(c * T::WAVES + wave) * 1024, w_base + (size_t)i * 128, w_off[c]);
+        else dma16(to + T::ROWS * 128 + (uint32_t)((c - T::W_REQUESTS) * T::WAVES + wave) * 1024, x_base + (size_t)i * 128, x_off[c - T::W_REQUESTS]);
+    };
+    auto request_scales = [&](int i) {  // of the two stages that i is one of
+        const uint32_t to = lds0 + T::STAGES * T::STAGE + (uint32_t)((i >> 1) & 1) * T::SCALES;
 #pragma unroll
-        for (int c = 0; c < T::W_REQUESTS; c++) dma16(to + (uint32_t)(c * T::WAVES + wave) * 1024, w_base + (size_t)i * 128, w_off[c]);
-#pragma unroll
-        for (int c = 0; c < T::X_REQUESTS; c++) dma16(to + T::ROWS * 128 + (uint32_t)(c * T::WAVES + wave) * 1024, x_base + (size_t)i * 128, x_off[c]);
-        if ((i & 1) == 0 || i == from) {
-            const uint32_t scales = lds0 + T::STAGES * T::STAGE + (uint32_t)((i >> 1) & 1) * T::SCALES;
-#pragma unroll
-            for (int c = 0; c < T::S_REQUESTS; c++) {
-                const int q = c * T::WAVES + wave;
-                if (q * 64 < T::ALL) dma16(scales + (uint32_t)q * 1024, (q * 64 < T::ROWS ? ws_base : xs_base) + (size_t)(i >> 1) * 16, s_off[c]);
-            }
+        for (int c = 0; c < T::S_REQUESTS; c++) {
+            const int q = min(c * T::WAVES + wave, T::ALL / 64 - 1);
+            dma16(to + (uint32_t)q * 1024, (q * 64 < T::ROWS ? ws_base : xs_base) + (size_t)(i >> 1) * 16, s_off[c]);
         }
     };
     mx4_v16f acc[MT][MR];
@@ -95,59 +97,124 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, in
     const uint32_t piece_at = (uint32_t)(li * 128 + ((4 * lh) ^ ((li >> 1) & 7)) * 16);
     const uint32_t w_lane = (uint32_t)(rw * MR * 32) * 128, x_lane = (uint32_t)(T::ROWS + tw * MT * 32) * 128;
 
-    if (from < until) request(from);
-    for (int i = from; i < until; i++) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        lds_barrier();  // the stage has landed, and everybody has read the one before
-        if (i + 1 < until) request(i + 1);
-        const uint8_t *const st = mx4_lds + (size_t)(i & 1) * T::STAGE;
+    // A stage is four steps of MR x MT products, a step one block of every lane.  Beside a step's products the wavefront reads the next step's
+    // operands.  In front of a stage's last step it waits for the next stage and for everybody to have read the present one, whose place
+    // is then asked for again: a third of the requests beside each of the next three steps.
+    mx4_v4i w[2][MR], x[2][MT];
+    int ws[MR], xs[MT], next_ws[MR], next_xs[MT];
+    auto read_scales = [&](int i) {
         const uint8_t *const sc = mx4_lds + T::STAGES * T::STAGE + (size_t)((i >> 1) & 1) * T::SCALES + (i & 1) * 8 + lh * 4 + li * 16;
-        // (a row's last stage may reach past its blocks: the codes there meet zeros, but a byte 255 would make them NaN)
-        const int live = g.blocks - (i * 8 + 4 * lh);
-        const uint32_t mask = live >= 4 ? 0xffffffffu : live > 0 ? 0xffffffffu >> (32 - 8 * live) : 0u;
-        int ws[MR], xs[MT];
 #pragma unroll
-        for (int r = 0; r < MR; r++) ws[r] = (int)(*reinterpret_cast<const uint32_t *>(sc + (rw * MR + r) * 512) & mask);
+        for (int r = 0; r < MR; r++) next_ws[r] = *reinterpret_cast<const int *>(sc + (rw * MR + r) * 512);
 #pragma unroll
-        for (int t = 0; t < MT; t++) xs[t] = (int)*reinterpret_cast<const uint32_t *>(sc + T::ROWS * 16 + (tw * MT + t) * 512);
-#define FRK_MX4_STEP(K)                                                                                                                        \
-    {                                                                                                                                          \
-        mx4_v8i w[MR], x[MT];                                                                                                                  \
-        _Pragma("unroll") for (int r = 0; r < MR; r++) {                                                                                       \
-            const mx4_v4i v = *reinterpret_cast<const mx4_v4i *>(st + w_lane + r * 4096 + (piece_at ^ (K * 16)));                              \
-            w[r] = mx4_v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0};                                                                                \
+        for (int t = 0; t < MT; t++) next_xs[t] = *reinterpret_cast<const int *>(sc + T::ROWS * 16 + (tw * MT + t) * 512);
+    };
+    auto read = [&](int i, int k, int n) {  // operand n of step k of stage i
+        const uint8_t *const st = mx4_lds + (size_t)(i & 1) * T::STAGE + (piece_at ^ (uint32_t)(k * 16));
+        if (n < MR) w[k & 1][n] = *reinterpret_cast<const mx4_v4i *>(st + w_lane + n * 4096);
+        else x[k & 1][n - MR] = *reinterpret_cast<const mx4_v4i *>(st + x_lane + (n - MR) * 4096);
+    };
+    // (the reads beside the first half of the products, so that they have come when the others are done)
+    constexpr int PRODUCTS = MR * MT, READS = MR + MT, READS_EACH = (2 * READS + PRODUCTS - 1) / PRODUCTS, FIRST = (T::REQUESTS + 2) / 3, SECOND = (2 * T::REQUESTS + 1) / 3;
+    // step K's products and what goes beside them: operands of the next step (stage I), requests BEGIN .. END - 1 of stage A
+#define FRK_MX4_STEP(K, I, ASK, A, BEGIN, END)                                                                                                \
+    _Pragma("unroll") for (int t = 0; t < MT; t++) _Pragma("unroll") for (int r = 0; r < MR; r++) {                                            \
+        const mx4_v4i &xv = x[K & 1][t], &wv = w[K & 1][r];                                                                                    \
+        const int at = t * MR + r;                                                                                                             \
+        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_v8i{wv[0], wv[1], wv[2], wv[3], 0, 0, 0, 0},                           \
+                                                                    mx4_v8i{xv[0], xv[1], xv[2], xv[3], 0, 0, 0, 0}, acc[t][r], E2M1, E2M1, K, \
+                                                                    ws[r], K, xs[t]);                                                          \
+        if (K == 3 && at == 0) read_scales(I);                                                                                                 \
+        _Pragma("unroll") for (int n = at * READS_EACH; n < min((at + 1) * READS_EACH, READS); n++) read(I, (K + 1) & 3, n);                   \
+        if (ASK) {                                                                                                                             \
+            constexpr int COUNT = (END) - (BEGIN);                                                                                            \
+            _Pragma("unroll") for (int c = (BEGIN) + at * COUNT / PRODUCTS; c < (BEGIN) + (at + 1) * COUNT / PRODUCTS; c++) request_codes(A, c); \
         }                                                                                                                                      \
-        _Pragma("unroll") for (int t = 0; t < MT; t++) {                                                                                       \
-            const mx4_v4i v = *reinterpret_cast<const mx4_v4i *>(st + x_lane + t * 4096 + (piece_at ^ (K * 16)));                              \
-            x[t] = mx4_v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0};                                                                                \
-        }                                                                                                                                      \
-        _Pragma("unroll") for (int t = 0; t < MT; t++) _Pragma("unroll") for (int r = 0; r < MR; r++)                                          \
-            acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x[t], w[r], acc[t][r], E2M1, E2M1, K, xs[t], K, ws[r]);                \
+        __builtin_amdgcn_sched_barrier(0);                                                                                                     \
     }
-        FRK_MX4_STEP(0)
-        FRK_MX4_STEP(1)
-        FRK_MX4_STEP(2)
-        FRK_MX4_STEP(3)
+    // LEFT: how many stages behind the present one there are (two: or more)
+    auto stage = [&](int i, auto left) {
+        constexpr int LEFT = decltype(left)::value;
+        // (a row's last stage may reach past its blocks: the codes there meet zeros, but a byte 255 would make them NaN.  Only there, and only here:
+        // behind the reads themselves it is a wait for them)
+        int mask = -1;
+        if (LEFT == 0) {
+            const int live = g.blocks - (i * 8 + 4 * lh);
+            mask = live >= 4 ? -1 : live > 0 ? (int)(0xffffffffu >> (32 - 8 * live)) : 0;
+        }
+#pragma unroll
+        for (int r = 0; r < MR; r++) ws[r] = next_ws[r] & mask;
+#pragma unroll
+        for (int t = 0; t < MT; t++) xs[t] = next_xs[t];
+        FRK_MX4_STEP(0, i, LEFT >= 1, i + 1, FIRST, SECOND)
+        if (LEFT >= 1 && (i & 1)) request_scales(i + 1);
+        FRK_MX4_STEP(1, i, LEFT >= 1, i + 1, SECOND, T::REQUESTS)
+        FRK_MX4_STEP(2, i, false, 0, 0, 0)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();
+        // (behind the last stage whatever lies there, which nobody multiplies)
+        FRK_MX4_STEP(3, i + 1, LEFT >= 2, i + 2, 0, FIRST)
+    };
+    if (from < until) {
+        request_scales(from);
+#pragma unroll
+        for (int c = 0; c < T::REQUESTS; c++) request_codes(from, c);
+        if (from + 1 < until) {
+#pragma unroll
+            for (int c = 0; c < FIRST; c++) request_codes(from + 1, c);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(FIRST) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        lds_barrier();
+        read_scales(from);
+#pragma unroll
+        for (int n = 0; n < READS; n++) read(from, 0, n);
+    }
+    int i = from;
+    for (; i + 2 < until; i++) stage(i, std::integral_constant<int, 2>());
+    if (i + 1 < until) stage(i++, std::integral_constant<int, 1>());
+    if (i < until) stage(i, std::integral_constant<int, 0>());
 #undef FRK_MX4_STEP
-    }
     // (the compiler does not count a product's wait states, eighteen at most, across the branches between it and the reads of its sum)
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    // register i of a lane: token 8 (i / 4) + 4 (lane / 32) + i % 4 of a group, weight row lane % 32
+    // ---- register i of a lane: weight row 8 (i / 4) + 4 (lane / 32) + i % 4 of a group, token lane % 32.  Through LDS, a group of tokens at a time and
+    // each wavefront in a place of its own, so that a store writes whole lines, sixteen bytes a lane (a dword a lane, whichever way round: 17000
+    // of the 76000 cycles of a tile of 4096 columns).
+    lds_barrier();  // (the last reads)
+    constexpr int LANES = MR * 8, TOKENS_EACH = 64 / LANES;  // of a token, tokens a store
+    float *const own = reinterpret_cast<float *>(mx4_lds) + wave * 32 * T::PITCH;
+    const int row_first = row0 + rw * MR * 32 + (lane % LANES) * 4;
+    float *const y = g.y + part * part_stride + row_first;
+    const bool wide = g.ldy % 4 == 0 && part_stride % 4 == 0 && (g.rows & 3) == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
 #pragma unroll
-    for (int t = 0; t < MT; t++)
+    for (int t = 0; t < MT; t++) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int tok = tok0 + (tw * MT + t) * 32 + 8 * (i >> 2) + 4 * lh + (i & 3);
+        for (int r = 0; r < MR; r++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                *reinterpret_cast<float4 *>(own + li * T::PITCH + r * 32 + q * 8 + lh * 4) =
+                    make_float4(acc[t][r][4 * q], acc[t][r][4 * q + 1], acc[t][r][4 * q + 2], acc[t][r][4 * q + 3]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wavefront reads its own stores only)
+#pragma unroll
+        for (int j = 0; j < 32 / TOKENS_EACH; j++) {
+            const int in = j * TOKENS_EACH + lane / LANES, tok = tok0 + (tw * MT + t) * 32 + in;
+            const float4 v = *reinterpret_cast<const float4 *>(own + in * T::PITCH + (lane % LANES) * 4);
             if (tok >= g.M) continue;
-            float *const dst = g.y + part * part_stride + (size_t)tok * g.ldy;
+            float *const dst = y + (size_t)tok * g.ldy;
+            if (wide) {
+                if (row_first < g.rows) *reinterpret_cast<float4 *>(dst) = v;
+            } else {
+                const float out[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int r = 0; r < MR; r++) {
-                const int row = row0 + (rw * MR + r) * 32 + li;
-                if (row < g.rows) dst[row] = acc[t][r][i];
+                for (int n = 0; n < 4; n++)
+                    if (row_first + n < g.rows) dst[n] = out[n];
             }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
 #endif
 }
 
