@@ -205,40 +205,44 @@ constexpr int MX4_UNIT = 16, MX4_FUSED = 4;           // blocks; tokens
 constexpr int MX4_FUSED_UNIT = MX4_UNIT * 16 + MX4_UNIT;  // bytes of LDS a token and unit
 constexpr size_t MX4_FUSED_LDS = 40 * 1024;
 
-template <int NW, int TT, int D, bool FUSED, bool WIDE>
+template <int NW, int SR, int TT, bool FUSED, bool WIDE>
 __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int E2M1 = 4;
     extern __shared__ __align__(16) uint8_t mx4_rows_lds[];  // FUSED: [units][tokens][MX4_FUSED_UNIT]
-    __shared__ float4 sums[NW][TT][64];
+    __shared__ float4 sums[NW][SR * TT][64];
     const Mx4Gemm &g = r.g;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int li = lane & 15, lg = lane >> 4;
-    const int units = (g.blocks + MX4_UNIT - 1) / MX4_UNIT, strip = blockIdx.x;
+    const int units = (g.blocks + MX4_UNIT - 1) / MX4_UNIT, strip = blockIdx.x * SR;
     const int u0 = units * wave / NW, u1 = units * (wave + 1) / NW;
-    const uint8_t *const row = g.W + (size_t)min(strip * 16 + li, g.rows - 1) * g.row_stride;
-    const uint8_t *const row_scales = row + (size_t)g.blocks * 16;
-    mx4_v4f acc[TT];
+    const uint8_t *row[SR];
 #pragma unroll
-    for (int t = 0; t < TT; t++) acc[t] = mx4_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r = 0; r < SR; r++) row[r] = g.W + (size_t)min((strip + r) * 16 + li, g.rows - 1) * g.row_stride;
+    mx4_v4f acc[SR][TT];
+#pragma unroll
+    for (int r = 0; r < SR; r++)
+#pragma unroll
+        for (int t = 0; t < TT; t++) acc[r][t] = mx4_v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (u0 < u1) {
-        // D units ahead; the scales: a row's sixteen bytes, of which product k takes byte l / 16 of dword k
-        uint4 w[D][4], ws[D], x[FUSED ? 1 : D][TT][4], xs[FUSED ? 1 : D][TT];
-        auto fetch_w = [&](int d, int u) {
-            u = min(u, u1 - 1);
+        // the scales: a row's sixteen bytes, of which product k takes byte l / 16 of dword k
+        uint4 w[SR][4], ws[SR], x[TT][4], xs[TT];
+        auto fetch_w = [&](int u) {
             // (blocks past the row's last: the last one's codes, which meet zeros)
 #pragma unroll
-            for (int k = 0; k < 4; k++) w[d][k] = stream_load16(row + (size_t)min(u * MX4_UNIT + 4 * k + lg, g.blocks - 1) * 16);
-            ws[d] = stream_load16(row_scales + u * MX4_UNIT);
+            for (int r = 0; r < SR; r++) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) w[r][k] = stream_load16(row[r] + (size_t)min(u * MX4_UNIT + 4 * k + lg, g.blocks - 1) * 16);
+                ws[r] = stream_load16(row[r] + (size_t)g.blocks * 16 + u * MX4_UNIT);
+            }
         };
-        auto fetch_x = [&](int d, int u) {
-            u = min(u, u1 - 1);
+        auto fetch_x = [&](int u) {
 #pragma unroll
             for (int t = 0; t < TT; t++) {
                 const size_t at = (size_t)min(16 * t + li, g.M - 1) * g.a.blocks + u * MX4_UNIT;
 #pragma unroll
-                for (int k = 0; k < 4; k++) x[d][t][k] = reinterpret_cast<const uint4 *>(g.a.codes)[at + 4 * k + lg];
-                xs[d][t] = *reinterpret_cast<const uint4 *>(g.a.scales + at);
+                for (int k = 0; k < 4; k++) x[t][k] = reinterpret_cast<const uint4 *>(g.a.codes)[at + 4 * k + lg];
+                xs[t] = *reinterpret_cast<const uint4 *>(g.a.scales + at);
             }
         };
         uint8_t *const own = mx4_rows_lds + (size_t)u0 * g.M * MX4_FUSED_UNIT;  // FUSED: this wavefront's units
@@ -260,8 +264,7 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
                 }
             };
             load(0, u0);
-#pragma unroll
-            for (int d = 0; d < D; d++) fetch_w(d, u0 + d);
+            fetch_w(u0);
             store(0, u0);
             for (int u = u0, t = 1; u < u1; u++, t = 0)
                 for (; t < g.M; t++) {
@@ -270,50 +273,58 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
                 }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wavefront reads its own stores only)
         } else {
-#pragma unroll
-            for (int d = 0; d < D; d++) fetch_w(d, u0 + d), fetch_x(d, u0 + d);
+            fetch_w(u0), fetch_x(u0);
         }
-        auto consume = [&](int d, int u) {
+        auto consume = [&](int u) {
             if (FUSED) {
                 const uint8_t *const from = own + ((size_t)(u - u0) * g.M + min(li, g.M - 1)) * MX4_FUSED_UNIT;
 #pragma unroll
-                for (int k = 0; k < 4; k++) x[0][0][k] = *reinterpret_cast<const uint4 *>(from + (4 * k + lg) * 16);
-                xs[0][0] = *reinterpret_cast<const uint4 *>(from + MX4_UNIT * 16);
+                for (int k = 0; k < 4; k++) x[0][k] = *reinterpret_cast<const uint4 *>(from + (4 * k + lg) * 16);
+                xs[0] = *reinterpret_cast<const uint4 *>(from + MX4_UNIT * 16);
             }
-            const int e = FUSED ? 0 : d;
-            const uint32_t wb[4] = {ws[d].x, ws[d].y, ws[d].z, ws[d].w};
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                // (past the row's last block whatever lies there: no byte of it may be a NaN)
-                const int ew = u * MX4_UNIT + 4 * k + lg < g.blocks ? (int)(wb[k] >> (8 * lg)) : 0;
-                const mx4_v8i a = {(int)w[d][k].x, (int)w[d][k].y, (int)w[d][k].z, (int)w[d][k].w, 0, 0, 0, 0};
+                mx4_v8i a[SR];
+                int ew[SR];
+#pragma unroll
+                for (int r = 0; r < SR; r++) {
+                    const uint4 &v = w[r][k];
+                    const uint32_t wb[4] = {ws[r].x, ws[r].y, ws[r].z, ws[r].w};
+                    a[r] = mx4_v8i{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+                    // (past the row's last block whatever lies there: no byte of it may be a NaN)
+                    ew[r] = u * MX4_UNIT + 4 * k + lg < g.blocks ? (int)(wb[k] >> (8 * lg)) : 0;
+                }
 #pragma unroll
                 for (int t = 0; t < TT; t++) {
-                    const uint32_t xb[4] = {xs[e][t].x, xs[e][t].y, xs[e][t].z, xs[e][t].w};
-                    const mx4_v8i b = {(int)x[e][t][k].x, (int)x[e][t][k].y, (int)x[e][t][k].z, (int)x[e][t][k].w, 0, 0, 0, 0};
-                    acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], E2M1, E2M1, 0, ew, 0, (int)(xb[k] >> (8 * lg)));
+                    const uint32_t xb[4] = {xs[t].x, xs[t].y, xs[t].z, xs[t].w};
+                    const mx4_v8i b = {(int)x[t][k].x, (int)x[t][k].y, (int)x[t][k].z, (int)x[t][k].w, 0, 0, 0, 0};
+#pragma unroll
+                    for (int r = 0; r < SR; r++)
+                        acc[r][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[r], b, acc[r][t], E2M1, E2M1, 0, ew[r], 0, (int)(xb[k] >> (8 * lg)));
                 }
             }
         };
-        for (int u = u0; u < u1; u += D)
-#pragma unroll
-            for (int d = 0; d < D; d++) {
-                if (u + d >= u1) break;  // (uniform)
-                consume(d, u + d);
-                if (u + d + D < u1) {
-                    fetch_w(d, u + d + D);
-                    if (!FUSED) fetch_x(d, u + d + D);
-                }
+        for (int u = u0; u < u1; u++) {
+            consume(u);
+            if (u + 1 < u1) {
+                fetch_w(u + 1);
+                if (!FUSED) fetch_x(u + 1);
             }
+        }
     }
     // (the compiler does not count a product's wait states, eighteen at most, across the branches between it and the reads of its sum)
 #pragma unroll
-    for (int t = 0; t < TT; t++) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(acc[t]));
+    for (int r = 0; r < SR; r++)
 #pragma unroll
-    for (int t = 0; t < TT; t++) sums[wave][t][lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+        for (int t = 0; t < TT; t++) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(acc[r][t]));
+#pragma unroll
+    for (int r = 0; r < SR; r++)
+#pragma unroll
+        for (int t = 0; t < TT; t++) sums[wave][r * TT + t][lane] = make_float4(acc[r][t][0], acc[r][t][1], acc[r][t][2], acc[r][t][3]);
     __syncthreads();
-    if (wave >= TT) return;  // a wavefront a tile of tokens
-    const int tok = 16 * wave + li, r0 = strip * 16 + 4 * lg;
+    static_assert(SR * TT <= NW, "a wavefront a strip and tile of tokens");
+    if (wave >= SR * TT) return;
+    const int tok = 16 * (wave % TT) + li, r0 = (strip + wave / TT) * 16 + 4 * lg;
     float4 v = sums[0][wave][lane];
 #pragma unroll
     for (int k = 1; k < NW; k++) {
@@ -328,23 +339,51 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
         if (r0 + i < g.rows) dst[i] = out[i];
 #endif
 }
-template <int NW, int TT, int D, bool FUSED>
+template <int NW, int SR, int TT, bool FUSED>
 static int go_mx4_rows(const Mx4Rows &r, size_t lds, hipStream_t s) {
-    const dim3 grid((unsigned)((r.g.rows + 15) / 16));
-    if (FUSED && floats_wide(r.x, (size_t)r.cols, FLOATS_F32)) hipLaunchKernelGGL((mx4_rows_kernel<NW, TT, D, FUSED, FUSED>), grid, dim3(64 * NW), lds, s, r);
-    else hipLaunchKernelGGL((mx4_rows_kernel<NW, TT, D, FUSED, false>), grid, dim3(64 * NW), lds, s, r);
+    const dim3 grid((unsigned)((r.g.rows + 16 * SR - 1) / (16 * SR)));
+    if (FUSED && floats_wide(r.x, (size_t)r.cols, FLOATS_F32)) hipLaunchKernelGGL((mx4_rows_kernel<NW, SR, TT, FUSED, FUSED>), grid, dim3(64 * NW), lds, s, r);
+    else hipLaunchKernelGGL((mx4_rows_kernel<NW, SR, TT, FUSED, false>), grid, dim3(64 * NW), lds, s, r);
     FRK_LAUNCH_CHECK("mx4_rows");
     return FRK_OK;
 }
 
 constexpr size_t MX4_ROWS_TOKENS = 64;  // most of the rows kernel
+// By estimated time, in us: a stage of 256 columns takes a tile's workgroups `alone` while each has a CU to itself, `shared` times the workgroups a CU from
+// there on (up to what a CU holds; more are another round), a round besides `ends` + `ends_shared` times those.  Shares of the
+// columns cost a second launch and the traffic of the parts.  Every kernel, tile and number of shares timed at 48 sizes (32 to 4096 tokens, 1024 x
+// 4096 to 14336 x 4096, 4096 x 14336): the choice is within 2 % of the fastest on average; 20 % off at 4096 tokens of 8192 x 1024, whose results are what is to be
+// written (48.5 against 41.4 us).
 Mx4Plan mx4_plan(const frk_weights *w, size_t batch, bool quantized) {
-    const size_t units = (w->cols / MX4_BLOCK + MX4_UNIT - 1) / MX4_UNIT;
+    const size_t units = (w->cols / MX4_BLOCK + MX4_UNIT - 1) / MX4_UNIT, stages = (w->cols + 255) / 256, n = batch * w->rows;
     Mx4Plan p{-1, 1, !quantized && batch <= MX4_FUSED && batch * units * MX4_FUSED_UNIT <= MX4_FUSED_LDS, 0, 0};
     if (p.fused) return p;
     if (!quantized) p.acts_bytes = mx4_acts_bytes(batch, w->cols);
-    if (batch <= MX4_ROWS_TOKENS) return p;
-    p.shape = batch >= 512 ? MX4_TILE_256x256 : MX4_TILE_128x128;
+    if (batch <= 16) return p;
+    double least = 1e300;
+    if (batch <= MX4_ROWS_TOKENS) {
+        const bool few = batch <= 32;
+        least = 2.0 + std::max(1.0, units / 8.0) * (few ? 4.2 : 6.5) * std::max(1.0, w->rows / 16.0 / (few ? 340.0 : 320.0));
+    }
+    static constexpr struct {
+        double alone, shared, ends, ends_shared, held;  // workgroups that a CU holds
+    } COST[MX4_TILE_SHAPES] = {{1.36, 1.84, 6.0, 4.5, 1}, {0.84, 0.64, 2.5, 1.3, 2}, {0.70, 0.42, 1.8, 0.9, 2}, {0.61, 0.28, 0.6, 0.6, 4}};
+    for (int shape = 0; shape < MX4_TILE_SHAPES; shape++)
+        for (int parts = 1; parts <= 8; parts *= 2) {
+            if (parts > 1 && (2 * (size_t)parts > stages || parts * n * 4 > SPLIT_PARTS_BYTES)) break;
+            const Mx4TileSize t = MX4_TILE_SIZE[shape];
+            const auto &c = COST[shape];
+            const double fill = (double)((w->rows + t.rows - 1) / t.rows) * (double)((batch + t.tokens - 1) / t.tokens) * parts / 256.0;
+            const double rounds = std::floor(fill / c.held + 1e-9), rest = fill - rounds * c.held, chain = (double)((stages + parts - 1) / parts);
+            auto round = [&](double f) { return chain * std::max(c.alone, c.shared * f) + c.ends + c.ends_shared * f; };
+            double us = 2.0 + rounds * round(c.held) + (rest > 1e-9 ? round(rest) : 0.0);
+            if (parts > 1) {
+                const double mb = 4e-6 * (double)n * parts;
+                us += 2.0 + 0.6 * std::min(mb, 10.0) + 0.15 * std::max(mb - 10.0, 0.0);
+            }
+            if (us < least) least = us, p.shape = shape, p.parts = parts;
+        }
+    if (p.parts > 1) p.parts_bytes = p.parts * n * 4;
     return p;
 }
 int mx4_gemm_fits(const frk_weights *w, const Mx4Plan &plan, size_t batch) {
@@ -386,12 +425,30 @@ int launch_mx4_gemm(const frk_weights *w, const Mx4Plan &plan, const float *x, c
     g.y = y;
     r.x = x;
     r.cols = (int)w->cols;
-    const size_t units = (g.blocks + MX4_UNIT - 1) / MX4_UNIT, lds = batch * units * MX4_FUSED_UNIT;
-    const bool one = units <= 8;  // a unit a wavefront at most
-    if (plan.fused) return one ? go_mx4_rows<8, 1, 1, true>(r, lds, s) : go_mx4_rows<8, 1, 2, true>(r, lds, s);
-    if (batch <= 16) return one ? go_mx4_rows<8, 1, 1, false>(r, 0, s) : go_mx4_rows<8, 1, 2, false>(r, 0, s);
-    if (batch <= 32) return one ? go_mx4_rows<8, 2, 1, false>(r, 0, s) : go_mx4_rows<8, 2, 2, false>(r, 0, s);
-    return go_mx4_rows<8, 4, 1, false>(r, 0, s);
+    // Strips a workgroup, and its wavefronts, by the number of strips: us, the quantization included, 8 wavefronts a strip / two / four: 4096 x 4096 1
+    // token 4.2 / 6.0 / 9.3, 16 tokens 7.9 / 9.5 / 12.9; 14336 x 4096 1 token 10.5 / 10.1 / 10.3, 4 14.8 / 12.4 / 12.0, 16 16.1 / 14.5 / 13.9, 32
+    // 21.9 / 18.3 / 15.8; 32000 x 4096 1 token 20.1 / 17.9 / 19.3, 32 39.6 / 30.3 / 28.0.  Sixteen wavefronts a strip for long rows of up to four tokens: 4096 x
+    // 14336 1 token 10.5 against 10.8, 4 14.6 against 16.8.
+    const size_t units = (g.blocks + MX4_UNIT - 1) / MX4_UNIT, lds = batch * units * MX4_FUSED_UNIT, strips = (w->rows + 15) / 16;
+    const int most = strips < 448 ? 1 : strips < 800 || batch == 1 || batch > 32 ? 2 : 4;
+#define FRK_MX4_ROWS(TT, FUSED, LDS)                                         \
+    if (most == 1) return go_mx4_rows<8, 1, TT, FUSED>(r, LDS, s);           \
+    if (most == 2) return go_mx4_rows<8, 2, TT, FUSED>(r, LDS, s);
+    if (plan.fused) {
+        if (most == 1 && units >= 16) return go_mx4_rows<16, 1, 1, true>(r, lds, s);
+        FRK_MX4_ROWS(1, true, lds)
+        return go_mx4_rows<8, 4, 1, true>(r, lds, s);
+    }
+    if (batch <= 16) {
+        FRK_MX4_ROWS(1, false, 0)
+        return go_mx4_rows<8, 4, 1, false>(r, 0, s);
+    }
+    if (batch <= 32) {
+        FRK_MX4_ROWS(2, false, 0)
+        return go_mx4_rows<8, 4, 2, false>(r, 0, s);
+    }
+    return most == 1 ? go_mx4_rows<8, 1, 4, false>(r, 0, s) : go_mx4_rows<8, 2, 4, false>(r, 0, s);
+#undef FRK_MX4_ROWS
 }
 
 }  // namespace frk

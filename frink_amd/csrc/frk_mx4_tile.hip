@@ -245,7 +245,8 @@ int launch_mx4_tile(const Mx4Gemm &g, int shape, int parts, size_t part_stride, 
     switch (shape) {
     case MX4_TILE_256x256: return go_mx4_tile<2, 2, 4, 4>(g, parts, part_stride, s);
     case MX4_TILE_128x128: return go_mx4_tile<2, 2, 2, 2>(g, parts, part_stride, s);
-    default: return go_mx4_tile<4, 1, 1, 2>(g, parts, part_stride, s);
+    case MX4_TILE_64x128: return go_mx4_tile<1, 4, 2, 1>(g, parts, part_stride, s);
+    default: return go_mx4_tile<2, 2, 1, 1>(g, parts, part_stride, s);
     }
 }
 
