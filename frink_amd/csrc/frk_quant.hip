@@ -75,29 +75,30 @@ __global__ __launch_bounds__(256) void quantize_q8_0_kernel(const float *__restr
 __global__ __launch_bounds__(256) void repack_kernel(int kind, const uint8_t *__restrict__ src,
                                                      uint8_t *__restrict__ dst, size_t rows, size_t src_row_bytes,
                                                      Layout l) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * src_row_bytes) return;
-    const size_t r = i / src_row_bytes, o = i % src_row_bytes;
-    size_t to;
-    if (kind == FRK_KIND_Q6_K) {
-        const size_t blk = o / Q6_K_BYTES, w = o % Q6_K_BYTES;
-        if (w < 128) to = blk * 128 + w;
-        else if (w < 192) to = l.off_a + blk * 64 + (w - 128);
-        else if (w < 208) to = l.off_b + blk * 16 + (w - 192);
-        else to = l.off_c + blk * 2 + (w - 208);
-    } else if (kind == FRK_KIND_Q8_0) {
-        const size_t blk = o / Q8_0_BYTES, w = o % Q8_0_BYTES;
-        to = w < 2 ? l.off_a + blk * 2 + w : blk * 32 + (w - 2);
-    } else if (kind == FRK_KIND_Q4_0) {
-        const size_t blk = o / Q4_0_BYTES, w = o % Q4_0_BYTES;
-        to = w < 2 ? l.off_a + blk * 2 + w : blk * 16 + (w - 2);
-    } else if (kind == FRK_KIND_MXFP4) {
-        const size_t blk = o / MXFP4_BYTES, w = o % MXFP4_BYTES;
-        to = w < 1 ? l.off_a + blk : blk * 16 + (w - 1);
-    } else {
-        to = o;
+    // (a grid holds fewer than 2^32 threads)
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < rows * src_row_bytes; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / src_row_bytes, o = i % src_row_bytes;
+        size_t to;
+        if (kind == FRK_KIND_Q6_K) {
+            const size_t blk = o / Q6_K_BYTES, w = o % Q6_K_BYTES;
+            if (w < 128) to = blk * 128 + w;
+            else if (w < 192) to = l.off_a + blk * 64 + (w - 128);
+            else if (w < 208) to = l.off_b + blk * 16 + (w - 192);
+            else to = l.off_c + blk * 2 + (w - 208);
+        } else if (kind == FRK_KIND_Q8_0) {
+            const size_t blk = o / Q8_0_BYTES, w = o % Q8_0_BYTES;
+            to = w < 2 ? l.off_a + blk * 2 + w : blk * 32 + (w - 2);
+        } else if (kind == FRK_KIND_Q4_0) {
+            const size_t blk = o / Q4_0_BYTES, w = o % Q4_0_BYTES;
+            to = w < 2 ? l.off_a + blk * 2 + w : blk * 16 + (w - 2);
+        } else if (kind == FRK_KIND_MXFP4) {
+            const size_t blk = o / MXFP4_BYTES, w = o % MXFP4_BYTES;
+            to = w < 1 ? l.off_a + blk : blk * 16 + (w - 1);
+        } else {
+            to = o;
+        }
+        dst[r * l.row_stride + to] = src[i];
     }
-    dst[r * l.row_stride + to] = src[i];
 }
 
 // ---- dequantizers, one thread per element, reading the resident layout ----
@@ -304,7 +305,7 @@ int launch_repack(int kind, const uint8_t *src, uint8_t *dst, size_t rows, size_
         hipError_t e = hipMemsetAsync(dst, 0, rows * l.row_stride, s);
         if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipMemsetAsync: %s", hipGetErrorString(e));
     }
-    hipLaunchKernelGGL(repack_kernel, dim3(blocks_for(rows * src_row_bytes, 256)), dim3(256), 0, s, kind, src, dst,
+    hipLaunchKernelGGL(repack_kernel, dim3((unsigned)std::min<size_t>((rows * src_row_bytes + 255) / 256, 1 << 23)), dim3(256), 0, s, kind, src, dst,
                        rows, src_row_bytes, l);
     FRK_LAUNCH_CHECK("repack");
     return FRK_OK;
