@@ -119,7 +119,15 @@ extern "C" {
     fn frk_hip_gemm_noalloc_dev(w: *const FrkWeights, x: *const f32, batch: usize, y: *mut f32,
                                 stream: *mut c_void) -> c_int;
     fn frk_hip_batch_acts_create(max_batch: usize, cols: usize, out: *mut *mut FrkBatchActs) -> c_int;
+    fn frk_hip_batch_acts_create_form(max_batch: usize, cols: usize, form: c_int, out: *mut *mut FrkBatchActs) -> c_int;
     fn frk_hip_batch_acts_release(acts: *mut FrkBatchActs) -> c_int;
+    fn frk_hip_batch_acts_values_dev(acts: *const FrkBatchActs, out: *mut f32, stream: *mut c_void) -> c_int;
+    fn frk_hip_rms_norm_dev(kind: c_int, x: *const c_void, residual: *const c_void, weight_kind: c_int, weight: *const c_void, eps: f64,
+                            batch: usize, cols: usize, sum: *mut c_void, y: *mut c_void, acts: *mut FrkBatchActs,
+                            stream: *mut c_void) -> c_int;
+    fn frk_hip_quantize_mxfp4_dev(kind: c_int, x: *const c_void, n: usize, blocks: *mut u8, stream: *mut c_void) -> c_int;
+    fn frk_hip_dequantize_mxfp4_dev(blocks: *const u8, n: usize, out: *mut f32, stream: *mut c_void) -> c_int;
+    fn frk_hip_gemm_mxfp4_dev(w: *const FrkWeights, x: *const f32, batch: usize, y: *mut f32, stream: *mut c_void) -> c_int;
     fn frk_hip_quantize_batch_acts_dev(acts: *mut FrkBatchActs, x: *const f32, batch: usize, stream: *mut c_void) -> c_int;
     fn frk_hip_gemm_acts_dev(w: *const FrkWeights, acts: *const FrkBatchActs, y: *mut f32, stream: *mut c_void) -> c_int;
     fn frk_hip_gemm_grouped_dev(stacked: *const FrkWeights, n_groups: usize, group_off: *const i32, gather: *const i32,
@@ -403,6 +411,18 @@ pub mod dev {
             check(unsafe { frk_hip_batch_acts_create(max_batch, cols, &mut p) })?;
             Ok(BatchActs(p))
         }
+        /// The same for `FP8_BLOCK` (form 1) or `MXFP4` (form 2) matrices; no counterpart in the reference.
+        pub fn new_form(max_batch: usize, cols: usize, form: c_int) -> Result<Self, HipError> {
+            let mut p = std::ptr::null_mut();
+            check(unsafe { frk_hip_batch_acts_create_form(max_batch, cols, form, &mut p) })?;
+            Ok(BatchActs(p))
+        }
+        /// The numbers that the last quantization stands for.
+        /// # Safety
+        /// `out` has room for the batch times the columns.
+        pub unsafe fn values(&self, out: *mut f32, stream: *mut c_void) -> Result<(), HipError> {
+            check(frk_hip_batch_acts_values_dev(self.0, out, stream))
+        }
         /// `quantize_batch_acts` (weight_matrix.rs:2348-2426).
         /// # Safety
         /// `x` holds `batch * cols` floats on the device.
@@ -420,6 +440,33 @@ pub mod dev {
     /// `y` has room for the quantized batch times `w.rows()` floats.
     pub unsafe fn gemm_acts(w: &Weights, acts: &BatchActs, y: *mut f32, stream: *mut c_void) -> Result<(), HipError> {
         check(frk_hip_gemm_acts_dev(w.0, acts.0, y, stream))
+    }
+    /// Root-mean-square norm of f32 rows with the residual's addition: `sum` gets `x + residual`, `y` and / or `acts` the normalized
+    /// rows (the order of the reference's RMSNorm); null pointers where there is none.
+    /// # Safety
+    /// `x[batch][cols]`, `residual`, `sum`, `y` alike and `weight[cols]` on the device.
+    pub unsafe fn rms_norm(x: *const f32, residual: *const f32, weight: *const f32, eps: f64, batch: usize, cols: usize, sum: *mut f32,
+                           y: *mut f32, acts: Option<&mut BatchActs>, stream: *mut c_void) -> Result<(), HipError> {
+        let acts = acts.map_or(std::ptr::null_mut(), |a| a.0);
+        check(frk_hip_rms_norm_dev(0, x as *const c_void, residual as *const c_void, 0, weight as *const c_void, eps, batch, cols,
+                                   sum as *mut c_void, y as *mut c_void, acts, stream))
+    }
+    /// `n` f32 values (a multiple of 32) as GGUF's MXFP4 blocks, 17 bytes each.
+    /// # Safety
+    /// `x[n]` and `blocks[n / 32 * 17]` on the device.
+    pub unsafe fn quantize_mxfp4(x: *const f32, n: usize, blocks: *mut u8, stream: *mut c_void) -> Result<(), HipError> {
+        check(frk_hip_quantize_mxfp4_dev(0, x as *const c_void, n, blocks, stream))
+    }
+    /// # Safety
+    /// `blocks[n / 32 * 17]` and `out[n]` on the device.
+    pub unsafe fn dequantize_mxfp4(blocks: *const u8, n: usize, out: *mut f32, stream: *mut c_void) -> Result<(), HipError> {
+        check(frk_hip_dequantize_mxfp4_dev(blocks, n, out, stream))
+    }
+    /// `gemm` of an MXFP4 matrix with the activations quantized to MXFP4 within the call.
+    /// # Safety
+    /// as `gemm`.
+    pub unsafe fn gemm_mxfp4(w: &Weights, x: *const f32, batch: usize, y: *mut f32, stream: *mut c_void) -> Result<(), HipError> {
+        check(frk_hip_gemm_mxfp4_dev(w.0, x, batch, y, stream))
     }
     /// The grouped GEMM (`enqueue_mul_mm_grouped_dev`, crates/frink-cuda/src/mul_mm_launch.rs:391-470): group `g` is
     /// rows `[g*R, (g+1)*R)` of `stacked`; pair `p` of group `g` reads row `gather[p]` of `x` (row `p` when `gather`

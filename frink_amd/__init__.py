@@ -364,10 +364,9 @@ class Weights:
     def gemm_acts(self, acts, out=None):
         """apply_batch_with_acts: this matrix over a batch that a BatchActs holds quantized."""
         import torch
-        if acts.form != "q8_k" and out is not None:
-            _fp8_floats(torch, out, acts.batch * self.rows)
         y = out if out is not None else torch.empty((acts.batch, self.rows), dtype=torch.float32, device="cuda")
-        check(lib().frk_hip_gemm_acts_dev(self.handle, acts.handle, C.c_void_p(y.data_ptr()), _stream()))
+        stream = _stream() if acts.form == "q8_k" or out is None else _fp8_stream(torch, _fp8_floats(torch, out, acts.batch * self.rows))
+        check(lib().frk_hip_gemm_acts_dev(self.handle, acts.handle, C.c_void_p(y.data_ptr()), stream))
         return y
 
     def gemm_noalloc(self, x, out):

@@ -3,6 +3,7 @@
 #include "frk_mx4.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace frk {
@@ -222,13 +223,14 @@ template <int RW, int TW, int MR, int MT>
 static int go_mx4_tile(const Mx4Gemm &g, int parts, size_t part_stride, hipStream_t s) {
     using T = Mx4TileShape<RW, TW, MR, MT>;
     const size_t row_tiles = ((size_t)g.rows + T::ROWS - 1) / T::ROWS, tok_tiles = ((size_t)g.M + T::TOKENS - 1) / T::TOKENS, total = row_tiles * tok_tiles;
-    static bool sized = false;  // a benign race: every thread sets the same attribute
-    if (!sized) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_tile_kernel<RW, TW, MR, MT>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)T::LDS);
-        if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFuncSetAttribute(mx4_tile): %s", hipGetErrorString(e));
-        sized = true;
+    static std::atomic<uint64_t> sized{0};  // a bit a device (two threads may set the same attribute)
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && (dev >= 64 || !(sized.load(std::memory_order_relaxed) >> dev & 1))) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_tile_kernel<RW, TW, MR, MT>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::LDS);
+        if (e == hipSuccess && dev < 64) sized.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
     }
+    if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFuncSetAttribute(mx4_tile): %s", hipGetErrorString(e));
     hipLaunchKernelGGL((mx4_tile_kernel<RW, TW, MR, MT>), dim3((unsigned)((total + 7) / 8 * 8), (unsigned)parts), dim3(64 * T::WAVES), T::LDS, s, g,
                        (int)row_tiles, (int)tok_tiles, parts, part_stride);
     FRK_LAUNCH_CHECK("mx4_tile");

@@ -1403,7 +1403,7 @@ int frk_hip_rms_norm_dev(int type, const void *x, const void *residual, int weig
     if (!(eps >= 0.0) || std::isinf(eps)) return set_error(FRK_ERR_ARG, "eps %g: a finite number, zero or more", eps);
     if (batch == 0 || cols == 0) return set_error(FRK_ERR_SHAPE, "empty shape: batch=%zu cols=%zu", batch, cols);
     if (batch > (size_t)1 << 30 || cols > (size_t)1 << 23) return set_error(FRK_ERR_SHAPE, "shape too large: batch=%zu cols=%zu (at most 2^30 rows of 2^23)", batch, cols);
-    if (y && (y == sum || (y == residual && acts))) return set_error(FRK_ERR_ARG, "frk_hip_rms_norm_dev: y and the sum are two outputs");
+    if (y && y == sum) return set_error(FRK_ERR_ARG, "frk_hip_rms_norm_dev: y and the sum are two outputs");
     NormArgs a{};
     a.x = x;
     a.residual = residual;

@@ -225,8 +225,12 @@ class WeightMatrix {
 class BatchActs {
   public:
     static Result<BatchActs> with_room_for(size_t max_batch, size_t cols) {
+        return with_room_for(max_batch, cols, FRK_ACTS_Q8_K);
+    }
+    // FRK_ACTS_FP8 and FRK_ACTS_MXFP4, which the reference has no counterpart of: for matrices of those kinds
+    static Result<BatchActs> with_room_for(size_t max_batch, size_t cols, int form) {
         frk_batch_acts *h = nullptr;
-        int rc = frk_hip_batch_acts_create(max_batch, cols, &h);
+        int rc = frk_hip_batch_acts_create_form(max_batch, cols, form, &h);
         if (rc != FRK_OK) return last_error(rc);
         return BatchActs(h);
     }
@@ -247,6 +251,19 @@ class BatchActs {
     }
     Result<bool> quantize_dev(const float *x_dev, size_t batch, void *stream) {
         int rc = frk_hip_quantize_batch_acts_dev(h_, x_dev, batch, stream);
+        if (rc != FRK_OK) return last_error(rc);
+        return true;
+    }
+    // a norm's result quantized (frk_hip_rms_norm_dev over f32 rows; weight, residual and sum: or null)
+    Result<bool> rms_norm_dev(const float *x_dev, const float *residual_dev, const float *weight_dev, double eps, size_t batch, size_t cols,
+                              float *sum_dev, void *stream) {
+        int rc = frk_hip_rms_norm_dev(FRK_TYPE_F32, x_dev, residual_dev, FRK_TYPE_F32, weight_dev, eps, batch, cols, sum_dev, nullptr, h_, stream);
+        if (rc != FRK_OK) return last_error(rc);
+        return true;
+    }
+    // the numbers that the last quantization stands for, [batch][cols]
+    Result<bool> values_dev(float *out_dev, void *stream) const {
+        int rc = frk_hip_batch_acts_values_dev(h_, out_dev, stream);
         if (rc != FRK_OK) return last_error(rc);
         return true;
     }

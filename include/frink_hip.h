@@ -330,8 +330,7 @@ enum { FRK_TYPE_F32 = 0, FRK_TYPE_BF16 = 1, FRK_TYPE_F16 = 2 };
  *   y = (h * r) * weight, two products rounded to f32 each (one where weight_dev is null); weight[cols] of weight_type
  * and up to three outputs (null: not wanted; at least one): h into sum_dev, y rounded to `type` into y_dev, y in f32 quantized into `acts`,
  * bit for bit as frk_hip_quantize_batch_acts_dev would, with which frk_hip_gemm_acts_dev then multiplies.
- * sum_dev may be x_dev or residual_dev, y_dev may be x_dev, or residual_dev unless h or `acts` is wanted too; otherwise no two
- * operands overlap.  A row with an infinity or a NaN has the NaN that the formula gives.  eps is a finite number, zero or more (a row of zeros has y = NaN with eps = 0).  At most 2^30 rows
+ * sum_dev and y_dev may each be x_dev or residual_dev, but are two outputs; otherwise no two operands overlap.  A row with an infinity or a NaN has the NaN that the formula gives.  eps is a finite number, zero or more (a row of zeros has y = NaN with eps = 0).  At most 2^30 rows
  * of 2^23 columns; rows need be aligned to their type only.  The order of the reference's norms (RMSNorm in crates/frink-core). */
 int frk_hip_rms_norm_dev(int type, const void *x_dev, const void *residual_dev, int weight_type, const void *weight_dev, double eps,
                          size_t batch, size_t cols, void *sum_dev, void *y_dev, frk_batch_acts *acts, void *stream);
