@@ -428,9 +428,9 @@ int launch_mx4_gemm(const frk_weights *w, const Mx4Plan &plan, const float *x, c
     // Strips a workgroup, and its wavefronts, by the number of strips: us, the quantization included, 8 wavefronts a strip / two / four: 4096 x 4096 1
     // token 4.2 / 6.0 / 9.3, 16 tokens 7.9 / 9.5 / 12.9; 14336 x 4096 1 token 10.5 / 10.1 / 10.3, 4 14.8 / 12.4 / 12.0, 16 16.1 / 14.5 / 13.9, 32
     // 21.9 / 18.3 / 15.8; 32000 x 4096 1 token 20.1 / 17.9 / 19.3, 32 39.6 / 30.3 / 28.0.  Sixteen wavefronts a strip for long rows of up to four tokens: 4096 x
-    // 14336 1 token 10.5 against 10.8, 4 14.6 against 16.8.
+    // 14336 1 token 10.5 against 10.8, 4 14.6 against 16.8.  More than 16 tokens of so many rows that four strips would pay are the tiles' (mx4_plan).
     const size_t units = (g.blocks + MX4_UNIT - 1) / MX4_UNIT, lds = batch * units * MX4_FUSED_UNIT, strips = (w->rows + 15) / 16;
-    const int most = strips < 448 ? 1 : strips < 800 || batch == 1 || batch > 32 ? 2 : 4;
+    const int most = strips < 448 ? 1 : strips < 800 || batch == 1 || batch > 16 ? 2 : 4;
 #define FRK_MX4_ROWS(TT, FUSED, LDS)                                         \
     if (most == 1) return go_mx4_rows<8, 1, TT, FUSED>(r, LDS, s);           \
     if (most == 2) return go_mx4_rows<8, 2, TT, FUSED>(r, LDS, s);
@@ -443,10 +443,7 @@ int launch_mx4_gemm(const frk_weights *w, const Mx4Plan &plan, const float *x, c
         FRK_MX4_ROWS(1, false, 0)
         return go_mx4_rows<8, 4, 1, false>(r, 0, s);
     }
-    if (batch <= 32) {
-        FRK_MX4_ROWS(2, false, 0)
-        return go_mx4_rows<8, 4, 2, false>(r, 0, s);
-    }
+    if (batch <= 32) return most == 1 ? go_mx4_rows<8, 1, 2, false>(r, 0, s) : go_mx4_rows<8, 2, 2, false>(r, 0, s);
     return most == 1 ? go_mx4_rows<8, 1, 4, false>(r, 0, s) : go_mx4_rows<8, 2, 4, false>(r, 0, s);
 #undef FRK_MX4_ROWS
 }

@@ -149,7 +149,8 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a, NormOut out)
         }
         const float r = (float)inverse_root(fma(sum, a.inverse_cols, a.eps));
         auto finish = [&](int c, const float (&v)[4], const float (&w)[4]) {
-            const int k = c * 256 + lane * 4;
+            int k = c * 256 + lane * 4;
+            if (!WIDE) asm("" : "+v"(k));  // (the addresses made anew: kept from the loads they spilled)
             float y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) y[i] = v[i] * r;

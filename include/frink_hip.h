@@ -345,7 +345,8 @@ int frk_hip_dequantize_mxfp4_dev(const uint8_t *blocks_dev, size_t n, float *out
 /* y[batch][rows] = x[batch][cols] W^T with an FRK_KIND_MXFP4 matrix and x quantized within the call to MXFP4, every 32 columns as
  * frk_hip_quantize_mxfp4_dev does.  Products of codes are exact and so are their sums within a block; blocks add up in f32 (results and parts of sums below
  * 2^-126 may be zero).  Four bits an activation: frk_hip_gemm_dev multiplies the same matrix by activations of eight.
- * A scale byte of 255 makes NaN of its weight row or activation row.  Scratch memory and graphs as with frk_hip_gemm_dev; at most 2^23 columns and 2^30 rows of x.
+ * A scale byte of 255 makes NaN of its weight row or activation row.  Scratch memory and graphs as with frk_hip_gemm_dev; at most 2^23 columns and 2^30 rows of x, and no
+ * more tiles of results than a grid holds (FRK_ERR_SHAPE, before any launch).
  * FRK_ERR_ARG while another device than the matrix's is the current one. */
 int frk_hip_gemm_mxfp4_dev(const frk_weights *w, const float *x_dev, size_t batch, float *y_dev, void *stream);
 
