@@ -484,7 +484,9 @@ def rms_norm(x, weight=None, eps=1e-5, residual=None, out=None, sum_out=None, ac
     if acts is None:
         check(lib().frk_hip_rms_norm_dev(kind, x.data_ptr(), r_ptr, w_kind, w_ptr, eps, n // cols, cols, s_ptr, y_ptr, None, stream))
         return out, x if sum_out is None else sum_out
-    acts.batch = 0
+    if not acts.handle:
+        raise ValueError("the activations are released")
+    # (a refusal leaves the object's batch as it was, there as here: its outputs are sized by it)
     check(lib().frk_hip_rms_norm_dev(kind, x.data_ptr(), r_ptr, w_kind, w_ptr, eps, n // cols, cols, s_ptr, y_ptr, acts.handle, stream))
     acts.batch = n // cols
     return acts, x if sum_out is None else sum_out

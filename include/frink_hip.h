@@ -317,6 +317,8 @@ int frk_hip_route_top_k_softmax_dev(const float *logits_dev, size_t batch, size_
  *   FP8    as frk_hip_gemm_dev quantizes a batch for such a matrix; y is bit for bit its result from nine rows on (fewer may be the same
  *          products added in another order)
  *   MXFP4  as frk_hip_gemm_mxfp4_dev does; y is bit for bit its result from five rows on
+ * Where a batch lies in an object depends on its number of rows: a captured product or _values reads what was last quantized with the
+ * number that the object held at the capture, and the object outlives the graph.
  * The reference has no counterpart of either.  _values writes the numbers that the last quantization stands for, [batch][cols] f32. */
 enum { FRK_ACTS_Q8_K = 0, FRK_ACTS_FP8 = 1, FRK_ACTS_MXFP4 = 2 };
 int frk_hip_batch_acts_create_form(size_t max_batch, size_t cols, int form, frk_batch_acts **out);
@@ -330,8 +332,9 @@ enum { FRK_TYPE_F32 = 0, FRK_TYPE_BF16 = 1, FRK_TYPE_F16 = 2 };
  *   y = (h * r) * weight, two products rounded to f32 each (one where weight_dev is null); weight[cols] of weight_type
  * and up to three outputs (null: not wanted; at least one): h into sum_dev, y rounded to `type` into y_dev, y in f32 quantized into `acts`,
  * bit for bit as frk_hip_quantize_batch_acts_dev would, with which frk_hip_gemm_acts_dev then multiplies.
- * sum_dev and y_dev may each be x_dev or residual_dev, but are two outputs; otherwise no two operands overlap.  A row with an infinity or a NaN has the NaN that the formula gives.  eps is a finite number, zero or more (a row of zeros has y = NaN with eps = 0).  At most 2^30 rows
- * of 2^23 columns; rows need be aligned to their type only.  The order of the reference's norms (RMSNorm in crates/frink-core). */
+ * sum_dev and y_dev may each be x_dev or residual_dev, but are two outputs; otherwise no two operands overlap.  A row with an infinity or a
+ * NaN has the NaN that the formula gives.  eps is a finite number, zero or more (a row of zeros has y = NaN with eps = 0).  At most 2^30
+ * rows of 2^23 columns; rows need be aligned to their type only.  A refused call leaves `acts` as it was.  The order of the reference's norms (RMSNorm in crates/frink-core). */
 int frk_hip_rms_norm_dev(int type, const void *x_dev, const void *residual_dev, int weight_type, const void *weight_dev, double eps,
                          size_t batch, size_t cols, void *sum_dev, void *y_dev, frk_batch_acts *acts, void *stream);
 
@@ -343,11 +346,10 @@ int frk_hip_rms_norm_dev(int type, const void *x_dev, const void *residual_dev, 
 int frk_hip_quantize_mxfp4_dev(int type, const void *x_dev, size_t n, uint8_t *blocks_dev, void *stream);
 int frk_hip_dequantize_mxfp4_dev(const uint8_t *blocks_dev, size_t n, float *out_dev, void *stream);
 /* y[batch][rows] = x[batch][cols] W^T with an FRK_KIND_MXFP4 matrix and x quantized within the call to MXFP4, every 32 columns as
- * frk_hip_quantize_mxfp4_dev does.  Products of codes are exact and so are their sums within a block; blocks add up in f32 (results and parts of sums below
- * 2^-126 may be zero).  Four bits an activation: frk_hip_gemm_dev multiplies the same matrix by activations of eight.
- * A scale byte of 255 makes NaN of its weight row or activation row.  Scratch memory and graphs as with frk_hip_gemm_dev; at most 2^23 columns and 2^30 rows of x, and no
- * more tiles of results than a grid holds (FRK_ERR_SHAPE, before any launch).
- * FRK_ERR_ARG while another device than the matrix's is the current one. */
+ * frk_hip_quantize_mxfp4_dev does.  Products of codes are exact and so are their sums within a block; blocks add up in f32 (results and
+ * parts of sums below 2^-126 may be zero).  Four bits an activation: frk_hip_gemm_dev multiplies the same matrix by activations of eight.
+ * A scale byte of 255 makes NaN of its weight row or activation row.  Scratch memory and graphs as with frk_hip_gemm_dev; at most 2^23
+ * columns and 2^30 rows of x, and no more tiles of results than a grid holds (FRK_ERR_SHAPE, before any launch).  FRK_ERR_ARG while another device than the matrix's is the current one. */
 int frk_hip_gemm_mxfp4_dev(const frk_weights *w, const float *x_dev, size_t batch, float *y_dev, void *stream);
 
 /* Routing by a rule, for a batch of tokens: logits[batch][n_experts] -> ids[batch][k], weights[batch][k].

@@ -260,3 +260,25 @@ def test_operands_that_do_not_fit_are_refused(fa):
         with pytest.raises(fa.BackendError) as e:
             fa.rms_norm(bad, None, acts=acts)
         assert e.value.code == fa.ERR_SHAPE and acts.batch == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", list(FORMS))
+def test_a_refused_norm_leaves_the_batch_as_it_was(fa, form):
+    """The outputs of values() and gemm_acts are sized by what the object holds, also behind a refusal."""
+    import torch
+    x = torch.randn((3, 256), device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    acts = fa.BatchActs(3, 256, form).quantize(x)
+    want = acts.values()
+    for bad in (torch.ones((4, 256), device="cuda"), x[:, :128].contiguous()):
+        with pytest.raises(fa.BackendError):
+            fa.rms_norm(bad, acts=acts)
+        assert acts.batch == 3 and torch.equal(acts.values(), want)
+    with pytest.raises(ValueError):
+        fa.rms_norm(x, acts=acts, out=torch.empty((2, 256), device="cuda"))
+    assert acts.batch == 3 and torch.equal(acts.values(torch.empty((3, 256), device="cuda")), want)
+    with pytest.raises(ValueError):
+        acts.values(torch.empty((2, 256), device="cuda"))
+    acts.release()
+    with pytest.raises(ValueError):
+        fa.rms_norm(x, acts=acts, sum_out=torch.empty_like(x))
