@@ -3,6 +3,7 @@
 #include "frk_mx4.hpp"
 
 #include <algorithm>
+#include <atomic>
 
 namespace frk {
 
@@ -194,7 +195,9 @@ int launch_dequantize_mxfp4(const uint8_t *blocks, size_t n, float *out, hipStre
 
 // ---- A few tokens: the weights' bytes bound it.  A workgroup of NW wavefronts has sixteen weight rows and up to 16 TT tokens; its
 // wavefronts share the columns, 512 at a time (a unit: sixteen blocks of a row), and their sums meet in LDS.  Lane l has weight row l % 16 and,
-// in product k of a unit's four, block 4 k + l / 16, so that a load brings 64 bytes of each row in one piece.
+// in product k of a unit's four (v_mfma_scale_f32_16x16x128_f8f6f4), block 4 k + l / 16.  The weights come through LDS, 256 bytes of a row in one
+// piece: loaded as operands, sixteen bytes of sixteen rows side by side, one token of 14336 x 4096 took 10.3 us, not 8.3 (31 MB, 3.8 TB/s from launch to
+// end; 32000 x 4096 14.7 us, 4.7 TB/s).
 // FUSED: up to four tokens are quantized by the workgroup itself, a wavefront its own columns'. ----
 struct Mx4Rows {
     Mx4Gemm g;
@@ -203,14 +206,15 @@ struct Mx4Rows {
 };
 constexpr int MX4_UNIT = 16, MX4_FUSED = 4;           // blocks; tokens
 constexpr int MX4_FUSED_UNIT = MX4_UNIT * 16 + MX4_UNIT;  // bytes of LDS a token and unit
-constexpr size_t MX4_FUSED_LDS = 40 * 1024;
+constexpr int MX4_STRIP_UNIT = 16 * 256;  // bytes of codes of sixteen rows' unit
+constexpr size_t MX4_FUSED_LDS = 32 * 1024;
 
 template <int NW, int SR, int TT, bool FUSED, bool WIDE>
 __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int E2M1 = 4;
-    extern __shared__ __align__(16) uint8_t mx4_rows_lds[];  // FUSED: [units][tokens][MX4_FUSED_UNIT]
-    __shared__ float4 sums[NW][SR * TT][64];
+    extern __shared__ __align__(16) uint8_t mx4_rows_lds[];  // [wavefronts][strips][MX4_STRIP_UNIT], then (FUSED) [units][tokens][MX4_FUSED_UNIT]
+    static_assert(TT * 1024 <= MX4_STRIP_UNIT, "a wavefront's sums lie where its weights did");
     const Mx4Gemm &g = r.g;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int li = lane & 15, lg = lane >> 4;
@@ -219,6 +223,16 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
     const uint8_t *row[SR];
 #pragma unroll
     for (int r = 0; r < SR; r++) row[r] = g.W + (size_t)min((strip + r) * 16 + li, g.rows - 1) * g.row_stride;
+    // A request brings a unit of four rows, sixteen lanes a row in one piece; place p of row r holds block p ^ r % 16, so that the sixteen rows' reads
+    // touch all banks.
+    uint8_t *const staged = mx4_rows_lds + wave * SR * MX4_STRIP_UNIT;
+    const uint32_t staged_at = lds_address(staged);
+    const uint8_t *const first = g.W + (size_t)strip * 16 * g.row_stride;
+    uint32_t row_off[SR][4];
+#pragma unroll
+    for (int r = 0; r < SR; r++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) row_off[r][q] = (uint32_t)min(r * 16 + 4 * q + lg, g.rows - 1 - strip * 16) * (uint32_t)g.row_stride;
     mx4_v4f acc[SR][TT];
 #pragma unroll
     for (int r = 0; r < SR; r++)
@@ -226,14 +240,24 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
         for (int t = 0; t < TT; t++) acc[r][t] = mx4_v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (u0 < u1) {
         // the scales: a row's sixteen bytes, of which product k takes byte l / 16 of dword k
-        uint4 w[SR][4], ws[SR], x[TT][4], xs[TT];
+        uint4 w[SR][4], ws[SR], next_ws[SR], x[TT][4], xs[TT];
+        auto w_off = [&](int u, int r, int q) { return row_off[r][q] + (uint32_t)min(u * MX4_UNIT + (li ^ (4 * q + lg)), g.blocks - 1) * 16; };
         auto fetch_w = [&](int u) {
             // (blocks past the row's last: the last one's codes, which meet zeros)
 #pragma unroll
             for (int r = 0; r < SR; r++) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) w[r][k] = stream_load16(row[r] + (size_t)min(u * MX4_UNIT + 4 * k + lg, g.blocks - 1) * 16);
-                ws[r] = stream_load16(row[r] + (size_t)g.blocks * 16 + u * MX4_UNIT);
+                for (int q = 0; q < 4; q++) dma16_nt(staged_at + r * MX4_STRIP_UNIT + q * 1024, first, w_off(u, r, q));
+                next_ws[r] = stream_load16(row[r] + (size_t)g.blocks * 16 + u * MX4_UNIT);
+            }
+        };
+        auto take_w = [&]() {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int r = 0; r < SR; r++) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) w[r][k] = *reinterpret_cast<const uint4 *>(staged + r * MX4_STRIP_UNIT + li * 256 + ((4 * k + lg) ^ li) * 16);
+                ws[r] = next_ws[r];
             }
         };
         auto fetch_x = [&](int u) {
@@ -245,35 +269,34 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
                 xs[t] = *reinterpret_cast<const uint4 *>(g.a.scales + at);
             }
         };
-        uint8_t *const own = mx4_rows_lds + (size_t)u0 * g.M * MX4_FUSED_UNIT;  // FUSED: this wavefront's units
+        uint8_t *const own = mx4_rows_lds + NW * SR * MX4_STRIP_UNIT + (size_t)u0 * g.M * MX4_FUSED_UNIT;  // FUSED: this wavefront's units
         if (FUSED) {
-            float v[2][4];
-            auto load = [&](int t, int u) {
+            float v[MX4_FUSED][2][4];
+            for (int u = u0; u < u1; u++) {  // (all tokens' values asked for at once, the first unit's in front of the weights)
 #pragma unroll
-                for (int i = 0; i < 2; i++) floats_load4<FLOATS_F32, WIDE>(r.x + (size_t)t * r.cols, u * 512 + i * 256 + lane * 4, r.cols, v[i]);
-            };
-            auto store = [&](int t, int u) {
-                uint8_t *const to = own + ((size_t)(u - u0) * g.M + t) * MX4_FUSED_UNIT;
+                for (int t = 0; t < MX4_FUSED; t++)
+                    if (t < g.M) {
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    uint32_t by;
-                    const uint32_t codes = mx4_quantize4(v[i], by);
-                    const int b = 8 * i + (lane >> 3);
-                    if ((lane & 4) == 0) *reinterpret_cast<uint32_t *>(to + b * 16 + (lane & 3) * 4) = codes;
-                    if ((lane & 7) == 0) to[MX4_UNIT * 16 + b] = (uint8_t)by;
-                }
-            };
-            load(0, u0);
-            fetch_w(u0);
-            store(0, u0);
-            for (int u = u0, t = 1; u < u1; u++, t = 0)
-                for (; t < g.M; t++) {
-                    load(t, u);
-                    store(t, u);
-                }
+                        for (int i = 0; i < 2; i++) floats_load4<FLOATS_F32, WIDE>(r.x + (size_t)t * r.cols, u * 512 + i * 256 + lane * 4, r.cols, v[t][i]);
+                    }
+                if (u == u0) fetch_w(u0);
+#pragma unroll
+                for (int t = 0; t < MX4_FUSED; t++)
+                    if (t < g.M) {
+                        uint8_t *const to = own + ((size_t)(u - u0) * g.M + t) * MX4_FUSED_UNIT;
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            uint32_t by;
+                            const uint32_t codes = mx4_quantize4(v[t][i], by);
+                            const int b = 8 * i + (lane >> 3);
+                            if ((lane & 4) == 0) *reinterpret_cast<uint32_t *>(to + b * 16 + (lane & 3) * 4) = codes;
+                            if ((lane & 7) == 0) to[MX4_UNIT * 16 + b] = (uint8_t)by;
+                        }
+                    }
+            }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (a wavefront reads its own stores only)
         } else {
-            fetch_w(u0), fetch_x(u0);
+            fetch_w(u0);
         }
         auto consume = [&](int u) {
             if (FUSED) {
@@ -305,11 +328,13 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
             }
         };
         for (int u = u0; u < u1; u++) {
-            consume(u);
+            if (!FUSED) fetch_x(u);
+            take_w();
             if (u + 1 < u1) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the place is read)
                 fetch_w(u + 1);
-                if (!FUSED) fetch_x(u + 1);
             }
+            consume(u);
         }
     }
     // (the compiler does not count a product's wait states, eighteen at most, across the branches between it and the reads of its sum)
@@ -320,15 +345,17 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
 #pragma unroll
     for (int r = 0; r < SR; r++)
 #pragma unroll
-        for (int t = 0; t < TT; t++) sums[wave][r * TT + t][lane] = make_float4(acc[r][t][0], acc[r][t][1], acc[r][t][2], acc[r][t][3]);
+        for (int t = 0; t < TT; t++)
+            reinterpret_cast<float4 *>(staged)[(r * TT + t) * 64 + lane] = make_float4(acc[r][t][0], acc[r][t][1], acc[r][t][2], acc[r][t][3]);
     __syncthreads();
     static_assert(SR * TT <= NW, "a wavefront a strip and tile of tokens");
     if (wave >= SR * TT) return;
     const int tok = 16 * (wave % TT) + li, r0 = (strip + wave / TT) * 16 + 4 * lg;
-    float4 v = sums[0][wave][lane];
+    const float4 *const sums = reinterpret_cast<const float4 *>(mx4_rows_lds) + wave * 64 + lane;
+    float4 v = sums[0];
 #pragma unroll
     for (int k = 1; k < NW; k++) {
-        const float4 o = sums[k][wave][lane];
+        const float4 o = sums[k * (SR * MX4_STRIP_UNIT / 16)];
         v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
     }
     if (tok >= g.M) return;
@@ -340,35 +367,48 @@ __global__ __launch_bounds__(64 * NW) void mx4_rows_kernel(Mx4Rows r) {
 #endif
 }
 template <int NW, int SR, int TT, bool FUSED>
-static int go_mx4_rows(const Mx4Rows &r, size_t lds, hipStream_t s) {
+static int go_mx4_rows(const Mx4Rows &r, size_t fused_lds, hipStream_t s) {
     const dim3 grid((unsigned)((r.g.rows + 16 * SR - 1) / (16 * SR)));
-    if (FUSED && floats_wide(r.x, (size_t)r.cols, FLOATS_F32)) hipLaunchKernelGGL((mx4_rows_kernel<NW, SR, TT, FUSED, FUSED>), grid, dim3(64 * NW), lds, s, r);
+    const bool wide = FUSED && floats_wide(r.x, (size_t)r.cols, FLOATS_F32);
+    const size_t lds = NW * SR * MX4_STRIP_UNIT + fused_lds;
+    static std::atomic<uint64_t> sized{0};  // a bit a device (two threads may set the same attributes)
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && (dev >= 64 || !(sized.load(std::memory_order_relaxed) >> dev & 1))) {
+        const int most = (int)(NW * SR * MX4_STRIP_UNIT + (FUSED ? MX4_FUSED_LDS : 0));
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_rows_kernel<NW, SR, TT, FUSED, FUSED>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (FUSED && e == hipSuccess)
+            e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_rows_kernel<NW, SR, TT, FUSED, false>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e == hipSuccess && dev < 64) sized.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+    }
+    if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFuncSetAttribute(mx4_rows): %s", hipGetErrorString(e));
+    if (wide) hipLaunchKernelGGL((mx4_rows_kernel<NW, SR, TT, FUSED, FUSED>), grid, dim3(64 * NW), lds, s, r);
     else hipLaunchKernelGGL((mx4_rows_kernel<NW, SR, TT, FUSED, false>), grid, dim3(64 * NW), lds, s, r);
     FRK_LAUNCH_CHECK("mx4_rows");
     return FRK_OK;
 }
 
-constexpr size_t MX4_ROWS_TOKENS = 64;  // most of the rows kernel
-// By estimated time, in us: a stage of 256 columns takes a tile's workgroups `alone` while each has a CU to itself, `shared` times the workgroups a CU from
-// there on (up to what a CU holds; more are another round), a round besides `ends` + `ends_shared` times those.  Shares of the
-// columns cost a second launch and the traffic of the parts.  Every kernel, tile and number of shares timed at 48 sizes (32 to 4096 tokens, 1024 x
-// 4096 to 14336 x 4096, 4096 x 14336): the choice is within 2 % of the fastest on average; 20 % off at 4096 tokens of 8192 x 1024, whose results are what is to be
-// written (48.5 against 41.4 us).
+constexpr size_t MX4_ROWS_TOKENS = 32;  // most of the rows kernel
+// By estimated time, in us: the rows kernel by what it reads (a strip's unit 0.95 ns with one tile of tokens, 1.4 with two); a stage of 256 columns takes a
+// tile's workgroups `alone` while each has a CU to itself, `shared` times the workgroups a CU from there on (up to what a CU holds; more are another
+// round), a round besides `ends` + `ends_shared` times those.  Shares of the columns cost a second launch and the traffic of the parts.  Every tile
+// and number of shares timed at 104 sizes (17 to 4096 tokens, 1024 x 4096 to 32000 x 4096, 4096 x 14336): the choice is within 1 % of the fastest on
+// average, 14 % off at 64 tokens of 4096 x 4096.
 Mx4Plan mx4_plan(const frk_weights *w, size_t batch, bool quantized) {
     const size_t units = (w->cols / MX4_BLOCK + MX4_UNIT - 1) / MX4_UNIT, stages = (w->cols + 255) / 256, n = batch * w->rows;
     Mx4Plan p{-1, 1, !quantized && batch <= MX4_FUSED && batch * units * MX4_FUSED_UNIT <= MX4_FUSED_LDS, 0, 0};
     if (p.fused) return p;
     if (!quantized) p.acts_bytes = mx4_acts_bytes(batch, w->cols);
-    if (batch <= 16) return p;
     double least = 1e300;
     if (batch <= MX4_ROWS_TOKENS) {
-        const bool few = batch <= 32;
-        least = 2.0 + std::max(1.0, units / 8.0) * (few ? 4.2 : 6.5) * std::max(1.0, w->rows / 16.0 / (few ? 340.0 : 320.0));
+        const double read = (double)((w->rows + 15) / 16) * (double)units;
+        least = 2.0 + (batch <= 16 ? 0.8 + 0.95e-3 * read : 1.0 + 1.4e-3 * read);
     }
     static constexpr struct {
         double alone, shared, ends, ends_shared, held;  // workgroups that a CU holds
-    } COST[MX4_TILE_SHAPES] = {{1.36, 1.84, 6.0, 4.5, 1}, {0.84, 0.64, 2.5, 1.3, 2}, {0.70, 0.42, 1.8, 0.9, 2}, {0.61, 0.28, 0.6, 0.6, 4}};
-    for (int shape = 0; shape < MX4_TILE_SHAPES; shape++)
+    } COST[MX4_TILE_SHAPES] = {{1.36, 1.81, 6.6, 8.0, 1}, {0.86, 1.12, 1.0, 7.4, 1}, {0.49, 0.73, 1.35, 2.0, 1}, {0.34, 0.45, 1.0, 0.7, 2}, {0.28, 0.35, 1.0, 0.0, 2}};
+    for (int shape = 0; shape < MX4_TILE_SHAPES; shape++) {
+        if (!mx4_tiles_fit(w, shape, batch)) continue;
         for (int parts = 1; parts <= 8; parts *= 2) {
             if (parts > 1 && (2 * (size_t)parts > stages || parts * n * 4 > SPLIT_PARTS_BYTES)) break;
             const Mx4TileSize t = MX4_TILE_SIZE[shape];
@@ -379,10 +419,11 @@ Mx4Plan mx4_plan(const frk_weights *w, size_t batch, bool quantized) {
             double us = 2.0 + rounds * round(c.held) + (rest > 1e-9 ? round(rest) : 0.0);
             if (parts > 1) {
                 const double mb = 4e-6 * (double)n * parts;
-                us += 2.0 + 0.6 * std::min(mb, 10.0) + 0.15 * std::max(mb - 10.0, 0.0);
+                us += 1.7 + 0.43 * std::min(mb, 10.0) + 0.08 * std::max(mb - 10.0, 0.0);
             }
             if (us < least) least = us, p.shape = shape, p.parts = parts;
         }
+    }
     if (p.parts > 1) p.parts_bytes = p.parts * n * 4;
     return p;
 }
@@ -396,7 +437,8 @@ int mx4_gemm_fits(const frk_weights *w, const Mx4Plan &plan, size_t batch) {
     if (w->cols > (1u << 23)) return set_error(FRK_ERR_SHAPE, "shape too large: %zu columns (at most 2^23)", w->cols);
     if (batch > (size_t)1 << 30) return set_error(FRK_ERR_SHAPE, "a batch of %zu rows is too large", batch);
     if ((w->rows + 15) / 16 * 512 > 0xffffffffu) return set_error(FRK_ERR_SHAPE, "shape too large: %zu rows", w->rows);
-    return plan.shape < 0 ? FRK_OK : mx4_tiles_fit(w, plan.shape, batch);
+    if (plan.shape < 0 && batch > MX4_ROWS_TOKENS) return set_error(FRK_ERR_SHAPE, "%zu rows times %zu: more tiles than a grid holds", w->rows, batch);
+    return FRK_OK;
 }
 int launch_mx4_gemm(const frk_weights *w, const Mx4Plan &plan, const float *x, const Mx4Acts *acts, size_t batch, float *y, void *ws, void *parts,
                     hipStream_t s) {
@@ -425,27 +467,18 @@ int launch_mx4_gemm(const frk_weights *w, const Mx4Plan &plan, const float *x, c
     g.y = y;
     r.x = x;
     r.cols = (int)w->cols;
-    // Strips a workgroup, and its wavefronts, by the number of strips: us, the quantization included, 8 wavefronts a strip / two / four: 4096 x 4096 1
-    // token 4.2 / 6.0 / 9.3, 16 tokens 7.9 / 9.5 / 12.9; 14336 x 4096 1 token 10.5 / 10.1 / 10.3, 4 14.8 / 12.4 / 12.0, 16 16.1 / 14.5 / 13.9, 32
-    // 21.9 / 18.3 / 15.8; 32000 x 4096 1 token 20.1 / 17.9 / 19.3, 32 39.6 / 30.3 / 28.0.  Sixteen wavefronts a strip for long rows of up to four tokens: 4096 x
-    // 14336 1 token 10.5 against 10.8, 4 14.6 against 16.8.  More than 16 tokens of so many rows that four strips would pay are the tiles' (mx4_plan).
+    // Strips a workgroup, and its wavefronts.  us, the quantization included, eight wavefronts of one strip / two / four: 4096 x 4096 1 token 4.2 / 5.3 /
+    // 7.4, 16 tokens 7.4 / 8.5 / 10.8; 14336 x 4096 1 token 8.5 / 8.6 / 8.5, 4 11.1 / 10.0 / 9.3, 16 13.6 / 12.6 / 12.0; 32000 x 4096 1 token 15.3 / 14.8 /
+    // 16.2, 16 23.6 / 19.9 / 20.5 (four strips: one workgroup a CU, so 1024 strips at a time).  Sixteen wavefronts a strip for long rows of up to four
+    // tokens: 4096 x 14336 1 token 9.0 against 10.2, 4 12.9 against 15.8.
     const size_t units = (g.blocks + MX4_UNIT - 1) / MX4_UNIT, lds = batch * units * MX4_FUSED_UNIT, strips = (w->rows + 15) / 16;
-    const int most = strips < 448 ? 1 : strips < 800 || batch == 1 || batch > 16 ? 2 : 4;
-#define FRK_MX4_ROWS(TT, FUSED, LDS)                                         \
-    if (most == 1) return go_mx4_rows<8, 1, TT, FUSED>(r, LDS, s);           \
-    if (most == 2) return go_mx4_rows<8, 2, TT, FUSED>(r, LDS, s);
     if (plan.fused) {
-        if (most == 1 && units >= 16) return go_mx4_rows<16, 1, 1, true>(r, lds, s);
-        FRK_MX4_ROWS(1, true, lds)
-        return go_mx4_rows<8, 4, 1, true>(r, lds, s);
+        if (strips < 448) return units >= 16 ? go_mx4_rows<16, 1, 1, true>(r, lds, s) : go_mx4_rows<8, 1, 1, true>(r, lds, s);
+        return strips < 512 || strips > 1024 || batch == 1 ? go_mx4_rows<8, 2, 1, true>(r, lds, s) : go_mx4_rows<8, 4, 1, true>(r, lds, s);
     }
-    if (batch <= 16) {
-        FRK_MX4_ROWS(1, false, 0)
-        return go_mx4_rows<8, 4, 1, false>(r, 0, s);
-    }
-    if (batch <= 32) return most == 1 ? go_mx4_rows<8, 1, 2, false>(r, 0, s) : go_mx4_rows<8, 2, 2, false>(r, 0, s);
-    return most == 1 ? go_mx4_rows<8, 1, 4, false>(r, 0, s) : go_mx4_rows<8, 2, 4, false>(r, 0, s);
-#undef FRK_MX4_ROWS
+    // (more tokens of so many rows that more strips would pay are the tiles' but for a few sizes)
+    if (batch > 16) return go_mx4_rows<8, 1, 2, false>(r, 0, s);
+    return strips < 448 ? go_mx4_rows<8, 1, 1, false>(r, 0, s) : go_mx4_rows<8, 2, 1, false>(r, 0, s);
 }
 
 }  // namespace frk

@@ -156,12 +156,12 @@ struct Mx4Gemm {
     size_t ldy;
 };
 // over tiles: weight rows x tokens, `parts` shares of the columns, each its own copy of y, part_stride floats apart
-enum { MX4_TILE_256x256, MX4_TILE_128x128, MX4_TILE_64x128, MX4_TILE_64x64, MX4_TILE_SHAPES };
+enum { MX4_TILE_256x256, MX4_TILE_256x128, MX4_TILE_128x128, MX4_TILE_64x128, MX4_TILE_64x64, MX4_TILE_SHAPES };
 struct Mx4TileSize {
     int rows, tokens, threads;
 };
-constexpr Mx4TileSize MX4_TILE_SIZE[MX4_TILE_SHAPES] = {{256, 256, 256}, {128, 128, 256}, {64, 128, 256}, {64, 64, 256}};
-int mx4_tiles_fit(const frk_weights *w, int shape, size_t batch);  // a status: whether a grid holds them
+constexpr Mx4TileSize MX4_TILE_SIZE[MX4_TILE_SHAPES] = {{256, 256, 256}, {256, 128, 512}, {128, 128, 256}, {64, 128, 256}, {64, 64, 256}};
+bool mx4_tiles_fit(const frk_weights *w, int shape, size_t batch);  // whether a grid holds them
 int launch_mx4_tile(const Mx4Gemm &g, int shape, int parts, size_t part_stride, hipStream_t s);
 // How a batch is multiplied: by the rows kernel (shape -1; `fused`: its own quantization), or over tiles in `parts` shares
 struct Mx4Plan {

@@ -1,5 +1,11 @@
 // Products of MXFP4 matrices and MXFP4 activations (frk_mx4.hpp) over large tiles on the block-scaled matrix cores
 // (v_mfma_scale_f32_32x32x64_f8f6f4): sixteen bytes of E2M1 codes are a lane's operand, its block's E8M0 byte the scale.
+//   y[t][r] = sum over blocks b of 2^(sw[r][b] + sx[t][b] - 254) * sum over the 32 of b of w x
+// Products of codes and a block's sum are exact, blocks add up in f32.
+// What bounds it: a full chip of 256 x 256 tiles its power (4096 tokens of 4096 x 14336: 114 us, 4.2 PFLOP/s; the clock falls to 1.44 GHz; the products
+// alone 86 us, with the operands' reads 110); fewer workgroups the time from a request to its bytes, which is why smaller tiles have three or four
+// stages (64 tokens of 14336 x 4096, two stages / three / four of 64 x 64: 13.7 / 9.4 / 8.8 us; 512 of 4096 x 14336, two / three of 64 x 128:
+// 43.2 / 28.6).
 #include "frk_mx4.hpp"
 
 #include <algorithm>
@@ -19,24 +25,25 @@ typedef float mx4_v16f __attribute__((ext_vector_type(16)));
     } while (0)
 
 // RW x TW wavefronts of MR groups of 32 weight rows x MT groups of 32 tokens each.  A stage is eight blocks (256 columns) of every row:
-// 128 bytes of codes, eight lanes a row in one piece.
-template <int RW, int TW, int MR, int MT>
+// 128 bytes of codes, eight lanes a row in one piece.  STAGES of them are in LDS or on their way there.
+template <int RW, int TW, int MR, int MT, int DEPTH>
 struct Mx4TileShape {
     static constexpr int WAVES = RW * TW, ROWS = RW * MR * 32, TOKENS = TW * MT * 32, ALL = ROWS + TOKENS;
-    static constexpr int STAGES = 2, STAGE = ALL * 128, SCALES = ALL * 16;  // scales: sixteen blocks, of two stages; two places
+    static constexpr int STAGES = DEPTH, STAGE = ALL * 128, SCALES = ALL * 16;  // scales: sixteen blocks, of two stages
     static constexpr int W_REQUESTS = ROWS / 8 / WAVES, X_REQUESTS = TOKENS / 8 / WAVES, REQUESTS = W_REQUESTS + X_REQUESTS;
     static constexpr int S_REQUESTS = (ALL / 64 + WAVES - 1) / WAVES;
     static_assert(W_REQUESTS * 8 * WAVES == ROWS && X_REQUESTS * 8 * WAVES == TOKENS && ROWS % 64 == 0 && TOKENS % 64 == 0, "whole requests");
     static constexpr int PITCH = MR * 32 + 4;  // floats a token in the results' place in LDS: sixteen lanes' pieces in different banks
-    static constexpr size_t LDS = STAGES * STAGE + 2 * SCALES;
+    static constexpr int SCALE_PLACES = STAGES > 3 ? 4 : 2;  // (a power of two: STAGES / 2 + 1 pairs of stages are on their way)
+    static constexpr size_t LDS = STAGES * STAGE + SCALE_PLACES * SCALES;
     static_assert((size_t)WAVES * 32 * PITCH * 4 <= LDS, "a group of tokens of every wavefront");
     static_assert(LDS <= 160 * 1024, "LDS of a CU");
 };
 
-template <int RW, int TW, int MR, int MT>
+template <int RW, int TW, int MR, int MT, int DEPTH>
 __global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, int row_tiles, int tok_tiles, int parts, size_t part_stride) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    using T = Mx4TileShape<RW, TW, MR, MT>;
+    using T = Mx4TileShape<RW, TW, MR, MT, DEPTH>;
     constexpr int E2M1 = 4;
     extern __shared__ __align__(16) uint8_t mx4_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -76,13 +83,15 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, in
         const int q = min(c * T::WAVES + wave, T::ALL / 64 - 1), r = q * 64 + lane;
         s_off[c] = q * 64 < T::ROWS ? (uint32_t)min(r, last_row) * (uint32_t)g.row_stride : (uint32_t)min(r - T::ROWS, last_token) * (uint32_t)g.a.blocks;
     }
-    auto request_codes = [&](int i, int c) {  // request c of stage i
-        const uint32_t to = lds0 + (uint32_t)(i & 1) * T::STAGE;
+    // the places of the stages in front of the present one (which STAGES - 1 behind it takes), of the present one and of the next
+    uint32_t before = (T::STAGES - 1) * T::STAGE, here = 0, next = T::STAGE;
+    auto request_codes = [&](int i, uint32_t place, int c) {  // request c of stage i
+        const uint32_t to = lds0 + place;
         if (c < T::W_REQUESTS) dma16(to + (uint32_t)(c * T::WAVES + wave) * 1024, w_base + (size_t)i * 128, w_off[c]);
         else dma16(to + T::ROWS * 128 + (uint32_t)((c - T::W_REQUESTS) * T::WAVES + wave) * 1024, x_base + (size_t)i * 128, x_off[c - T::W_REQUESTS]);
     };
     auto request_scales = [&](int i) {  // of the two stages that i is one of
-        const uint32_t to = lds0 + T::STAGES * T::STAGE + (uint32_t)((i >> 1) & 1) * T::SCALES;
+        const uint32_t to = lds0 + T::STAGES * T::STAGE + (uint32_t)((i >> 1) & (T::SCALE_PLACES - 1)) * T::SCALES;
 #pragma unroll
         for (int c = 0; c < T::S_REQUESTS; c++) {
             const int q = min(c * T::WAVES + wave, T::ALL / 64 - 1);
@@ -100,40 +109,40 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, in
 
     // A stage is four steps of MR x MT products, a step one block of every lane.  Beside a step's products the wavefront reads the next step's
     // operands.  In front of a stage's last step it waits for the next stage and for everybody to have read the present one, whose place
-    // is then asked for again: a third of the requests beside each of the next three steps.
+    // is then asked for again, STAGES stages on: a third of the requests beside each of the next three steps.
     mx4_v4i w[2][MR], x[2][MT];
     int ws[MR], xs[MT], next_ws[MR], next_xs[MT];
     auto read_scales = [&](int i) {
-        const uint8_t *const sc = mx4_lds + T::STAGES * T::STAGE + (size_t)((i >> 1) & 1) * T::SCALES + (i & 1) * 8 + lh * 4 + li * 16;
+        const uint8_t *const sc = mx4_lds + T::STAGES * T::STAGE + (size_t)((i >> 1) & (T::SCALE_PLACES - 1)) * T::SCALES + (i & 1) * 8 + lh * 4 + li * 16;
 #pragma unroll
         for (int r = 0; r < MR; r++) next_ws[r] = *reinterpret_cast<const int *>(sc + (rw * MR + r) * 512);
 #pragma unroll
         for (int t = 0; t < MT; t++) next_xs[t] = *reinterpret_cast<const int *>(sc + T::ROWS * 16 + (tw * MT + t) * 512);
     };
-    auto read = [&](int i, int k, int n) {  // operand n of step k of stage i
-        const uint8_t *const st = mx4_lds + (size_t)(i & 1) * T::STAGE + (piece_at ^ (uint32_t)(k * 16));
+    auto read = [&](uint32_t place, int k, int n) {  // operand n of step k of the stage there
+        const uint8_t *const st = mx4_lds + place + (piece_at ^ (uint32_t)(k * 16));
         if (n < MR) w[k & 1][n] = *reinterpret_cast<const mx4_v4i *>(st + w_lane + n * 4096);
         else x[k & 1][n - MR] = *reinterpret_cast<const mx4_v4i *>(st + x_lane + (n - MR) * 4096);
     };
     // (the reads beside the first half of the products, so that they have come when the others are done)
     constexpr int PRODUCTS = MR * MT, READS = MR + MT, READS_EACH = (2 * READS + PRODUCTS - 1) / PRODUCTS, FIRST = (T::REQUESTS + 2) / 3, SECOND = (2 * T::REQUESTS + 1) / 3;
     // step K's products and what goes beside them: operands of the next step (stage I), requests BEGIN .. END - 1 of stage A
-#define FRK_MX4_STEP(K, I, ASK, A, BEGIN, END)                                                                                                \
+#define FRK_MX4_STEP(K, FROM, ASK, A, TO, BEGIN, END)                                                                                           \
     _Pragma("unroll") for (int t = 0; t < MT; t++) _Pragma("unroll") for (int r = 0; r < MR; r++) {                                            \
         const mx4_v4i &xv = x[K & 1][t], &wv = w[K & 1][r];                                                                                    \
         const int at = t * MR + r;                                                                                                             \
         acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_v8i{wv[0], wv[1], wv[2], wv[3], 0, 0, 0, 0},                           \
                                                                     mx4_v8i{xv[0], xv[1], xv[2], xv[3], 0, 0, 0, 0}, acc[t][r], E2M1, E2M1, K, \
                                                                     ws[r], K, xs[t]);                                                          \
-        if (K == 3 && at == 0) read_scales(I);                                                                                                 \
-        _Pragma("unroll") for (int n = at * READS_EACH; n < min((at + 1) * READS_EACH, READS); n++) read(I, (K + 1) & 3, n);                   \
+        if (K == 3 && at == 0) read_scales(i + 1);                                                                                               \
+        _Pragma("unroll") for (int n = at * READS_EACH; n < min((at + 1) * READS_EACH, READS); n++) read(FROM, (K + 1) & 3, n);                \
         if (ASK) {                                                                                                                             \
             constexpr int COUNT = (END) - (BEGIN);                                                                                            \
-            _Pragma("unroll") for (int c = (BEGIN) + at * COUNT / PRODUCTS; c < (BEGIN) + (at + 1) * COUNT / PRODUCTS; c++) request_codes(A, c); \
+            _Pragma("unroll") for (int c = (BEGIN) + at * COUNT / PRODUCTS; c < (BEGIN) + (at + 1) * COUNT / PRODUCTS; c++) request_codes(A, TO, c); \
         }                                                                                                                                      \
         __builtin_amdgcn_sched_barrier(0);                                                                                                     \
     }
-    // LEFT: how many stages behind the present one there are (two: or more)
+    // LEFT: how many stages behind the present one there are (STAGES: or more)
     auto stage = [&](int i, auto left) {
         constexpr int LEFT = decltype(left)::value;
         // (a row's last stage may reach past its blocks: the codes there meet zeros, but a byte 255 would make them NaN.  Only there, and only here:
@@ -147,33 +156,44 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, in
         for (int r = 0; r < MR; r++) ws[r] = next_ws[r] & mask;
 #pragma unroll
         for (int t = 0; t < MT; t++) xs[t] = next_xs[t];
-        FRK_MX4_STEP(0, i, LEFT >= 1, i + 1, FIRST, SECOND)
-        if (LEFT >= 1 && (i & 1)) request_scales(i + 1);
-        FRK_MX4_STEP(1, i, LEFT >= 1, i + 1, SECOND, T::REQUESTS)
-        FRK_MX4_STEP(2, i, false, 0, 0, 0)
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        FRK_MX4_STEP(0, here, LEFT >= T::STAGES - 1, i + T::STAGES - 1, before, FIRST, SECOND)
+        if (LEFT >= T::STAGES - 1 && !((i + T::STAGES - 1) & 1)) request_scales(i + T::STAGES - 1);
+        FRK_MX4_STEP(1, here, LEFT >= T::STAGES - 1, i + T::STAGES - 1, before, SECOND, T::REQUESTS)
+        FRK_MX4_STEP(2, here, false, 0, 0, 0, 0)
+        // (all but the requests of the stages behind the next one)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((LEFT < 2 ? 0 : LEFT < T::STAGES ? LEFT - 1 : T::STAGES - 2) * T::REQUESTS) : "memory");
         lds_barrier();
         // (behind the last stage whatever lies there, which nobody multiplies)
-        FRK_MX4_STEP(3, i + 1, LEFT >= 2, i + 2, 0, FIRST)
+        FRK_MX4_STEP(3, next, LEFT >= T::STAGES, i + T::STAGES, here, 0, FIRST)
+        before = here, here = next, next = next == (T::STAGES - 1) * T::STAGE ? 0 : next + T::STAGE;
     };
     if (from < until) {
         request_scales(from);
 #pragma unroll
-        for (int c = 0; c < T::REQUESTS; c++) request_codes(from, c);
-        if (from + 1 < until) {
+        for (int n = 1; n < T::STAGES - 1; n++)
+            if (!((from + n) & 1) && from + n < until) request_scales(from + n);
 #pragma unroll
-            for (int c = 0; c < FIRST; c++) request_codes(from + 1, c);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(FIRST) : "memory");
+        for (int n = 0; n < T::STAGES - 1; n++)
+            if (from + n < until) {
+#pragma unroll
+                for (int c = 0; c < T::REQUESTS; c++) request_codes(from + n, n * T::STAGE, c);
+            }
+        if (from + T::STAGES - 1 < until) {
+#pragma unroll
+            for (int c = 0; c < FIRST; c++) request_codes(from + T::STAGES - 1, (T::STAGES - 1) * T::STAGE, c);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((T::STAGES - 2) * T::REQUESTS + FIRST) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         lds_barrier();
         read_scales(from);
 #pragma unroll
-        for (int n = 0; n < READS; n++) read(from, 0, n);
+        for (int n = 0; n < READS; n++) read(0, 0, n);
     }
     int i = from;
-    for (; i + 2 < until; i++) stage(i, std::integral_constant<int, 2>());
+    for (; i + T::STAGES < until; i++) stage(i, std::integral_constant<int, T::STAGES>());
+    if (T::STAGES > 3 && i + 3 < until) stage(i++, std::integral_constant<int, 3>());
+    if (T::STAGES > 2 && i + 2 < until) stage(i++, std::integral_constant<int, 2>());
     if (i + 1 < until) stage(i++, std::integral_constant<int, 1>());
     if (i < until) stage(i, std::integral_constant<int, 0>());
 #undef FRK_MX4_STEP
@@ -219,36 +239,35 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, in
 #endif
 }
 
-template <int RW, int TW, int MR, int MT>
+template <int RW, int TW, int MR, int MT, int DEPTH>
 static int go_mx4_tile(const Mx4Gemm &g, int parts, size_t part_stride, hipStream_t s) {
-    using T = Mx4TileShape<RW, TW, MR, MT>;
+    using T = Mx4TileShape<RW, TW, MR, MT, DEPTH>;
     const size_t row_tiles = ((size_t)g.rows + T::ROWS - 1) / T::ROWS, tok_tiles = ((size_t)g.M + T::TOKENS - 1) / T::TOKENS, total = row_tiles * tok_tiles;
     static std::atomic<uint64_t> sized{0};  // a bit a device (two threads may set the same attribute)
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
     if (e == hipSuccess && (dev >= 64 || !(sized.load(std::memory_order_relaxed) >> dev & 1))) {
-        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_tile_kernel<RW, TW, MR, MT>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::LDS);
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&mx4_tile_kernel<RW, TW, MR, MT, DEPTH>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::LDS);
         if (e == hipSuccess && dev < 64) sized.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
     }
     if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFuncSetAttribute(mx4_tile): %s", hipGetErrorString(e));
-    hipLaunchKernelGGL((mx4_tile_kernel<RW, TW, MR, MT>), dim3((unsigned)((total + 7) / 8 * 8), (unsigned)parts), dim3(64 * T::WAVES), T::LDS, s, g,
+    hipLaunchKernelGGL((mx4_tile_kernel<RW, TW, MR, MT, DEPTH>), dim3((unsigned)((total + 7) / 8 * 8), (unsigned)parts), dim3(64 * T::WAVES), T::LDS, s, g,
                        (int)row_tiles, (int)tok_tiles, parts, part_stride);
     FRK_LAUNCH_CHECK("mx4_tile");
     return FRK_OK;
 }
-int mx4_tiles_fit(const frk_weights *w, int shape, size_t batch) {
+bool mx4_tiles_fit(const frk_weights *w, int shape, size_t batch) {
     const Mx4TileSize t = MX4_TILE_SIZE[shape];
     const size_t row_tiles = (w->rows + t.rows - 1) / t.rows, tok_tiles = (batch + t.tokens - 1) / t.tokens;
-    if ((row_tiles * tok_tiles + 7) / 8 * 8 * t.threads > 0xffffffffu)
-        return set_error(FRK_ERR_SHAPE, "%zu x %zu tiles: more than a grid holds", row_tiles, tok_tiles);
-    return FRK_OK;
+    return (row_tiles * tok_tiles + 7) / 8 * 8 * t.threads <= 0xffffffffu;
 }
 int launch_mx4_tile(const Mx4Gemm &g, int shape, int parts, size_t part_stride, hipStream_t s) {
     switch (shape) {
-    case MX4_TILE_256x256: return go_mx4_tile<2, 2, 4, 4>(g, parts, part_stride, s);
-    case MX4_TILE_128x128: return go_mx4_tile<2, 2, 2, 2>(g, parts, part_stride, s);
-    case MX4_TILE_64x128: return go_mx4_tile<1, 4, 2, 1>(g, parts, part_stride, s);
-    default: return go_mx4_tile<2, 2, 1, 1>(g, parts, part_stride, s);
+    case MX4_TILE_256x256: return go_mx4_tile<2, 2, 4, 4, 2>(g, parts, part_stride, s);
+    case MX4_TILE_256x128: return go_mx4_tile<4, 2, 2, 2, 3>(g, parts, part_stride, s);
+    case MX4_TILE_128x128: return go_mx4_tile<2, 2, 2, 2, 3>(g, parts, part_stride, s);
+    case MX4_TILE_64x128: return go_mx4_tile<1, 4, 2, 1, 3>(g, parts, part_stride, s);
+    default: return go_mx4_tile<2, 2, 1, 1, 4>(g, parts, part_stride, s);
     }
 }
 

@@ -99,7 +99,10 @@ SHAPES = [(1, 32, 1), (15, 64, 2), (16, 480, 1), (17, 512, 4), (129, 544, 5), (3
           (144, 14336, 5), (576, 2304, 9), (33, 1152, 200), (272, 384, 257), (512, 1152, 300), (31, 4096, 1), (7200, 160, 1), (7200, 160, 7), (7201, 96, 40),
           (12801, 96, 1), (12801, 128, 3), (13000, 64, 20), (12900, 96, 32), (12900, 96, 64), (40, 28672, 1), (33, 65536, 1), (33, 65536, 2), (20, 7168, 4), (20, 8192, 3),
           (100, 1024, 700), (4096, 128, 7), (2880, 160, 97), (300, 8192, 64), (200, 16384, 100), (70, 14336, 48), (513, 4128, 30), (1030, 512, 1100),
-          (65, 32, 65), (3001, 288, 513)]
+          (65, 32, 65), (3001, 288, 513),
+          # each tile and share of the columns, with rows, tokens and stages that end inside
+          (8200, 544, 1500), (2049, 1056, 2050), (14337, 1312, 257), (14337, 1568, 130), (8200, 1568, 257), (8200, 32, 200), (3001, 544, 700), (3001, 8224, 65),
+          (1537, 16416, 65), (8200, 8224, 6), (257, 2336, 33), (257, 3360, 97), (513, 800, 33), (300, 1056, 70)]
 
 
 @pytest.mark.gpu

@@ -142,14 +142,15 @@ def test_another_device_is_refused(said):
 
 
 @pytest.mark.parametrize("call", ["norm %d 64 -1" % (1 << 30), "norm 3 %d -1" % (1 << 23), "norm %d 256 0" % (1 << 25), "norm %d 4 1" % (1 << 28), "norm %d 32 2" % (1 << 30),
-                                  "gemm 64 32 %d" % (1 << 28), "gemm %d 32 1" % ((1 << 27) - 16), "gemm %d 32 16" % ((1 << 27) - 16), "gemm 64 %d 20" % (1 << 23), "gemm 64 %d 4" % (1 << 23), "acts 4096 4096 %d" % (1 << 22)])
+                                  "gemm 64 32 %d" % (1 << 28), "gemm %d 32 1" % ((1 << 27) - 16), "gemm %d 32 16" % ((1 << 27) - 16), "gemm 64 %d 20" % (1 << 23), "gemm 64 %d 4" % (1 << 23), "acts 4096 4096 %d" % (1 << 22),
+                                  "gemm 1 32 %d" % (1 << 30)])
 def test_what_grids_hold_is_launched(said, call):
     (rc, most, names, error), = said(call)
     assert rc == 0 and names != ["-"] and 0 < most < 1 << 32, (rc, most, error)
 
 
 @pytest.mark.parametrize("call", ["norm %d 64 -1" % ((1 << 30) + 1), "norm 1 %d -1" % ((1 << 23) + 1), "norm 4 300 0", "norm 4 48 2", "gemm 64 %d 1" % ((1 << 23) + 32),
-                                  "gemm 64 32 %d" % ((1 << 30) + 1), "gemm 1 32 %d" % (1 << 30), "gemm 2000000000 32 %d" % (1 << 29), "acts 2000000000 32 %d" % (1 << 29), "blocks 0", "blocks 48"])
+                                  "gemm 64 32 %d" % ((1 << 30) + 1), "gemm %d 32 %d" % ((1 << 27) - 16, 1 << 30), "acts %d 32 %d" % ((1 << 27) - 16, 1 << 30), "blocks 0", "blocks 48"])
 def test_what_no_launch_holds_is_refused_before_the_first(said, call):
     for rc, _, names, error in said(call):
         assert rc == -3 and not [n for n in names if "quantize" not in n and n != "-"] and error, (rc, names)
@@ -181,7 +182,7 @@ def test_compiled_kernels(tmp_path, name):
     assert r.returncode == 0, r.stderr[-2000:]
     asm = out.read_text()
     assert ("v_mfma" in asm) == ("mx4" in name) and isa_mfma_lint.violations(asm) == []
-    for k in isa_wait_lint.kernels(asm):
+    for k in isa_wait_lint.kernels(asm) if "mx4" in name else ():  # (the norms ask for nothing by hand)
         assert isa_wait_lint.violations(asm, k) == [], k
     scratch = re.findall(r"\.private_segment_fixed_size: (\d+)", asm)
     assert len(scratch) > 3 and set(scratch) == {"0"}, scratch
