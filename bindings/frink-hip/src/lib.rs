@@ -442,7 +442,7 @@ pub mod dev {
         check(frk_hip_gemm_acts_dev(w.0, acts.0, y, stream))
     }
     /// Root-mean-square norm of f32 rows with the residual's addition: `sum` gets `x + residual`, `y` and / or `acts` the normalized
-    /// rows (the order of the reference's RMSNorm); null pointers where there is none.
+    /// rows (`rms_norm`, crates/frink-core/src/matmul.rs, on the device); null pointers where there is none.
     /// # Safety
     /// `x[batch][cols]`, `residual`, `sum`, `y` alike and `weight[cols]` on the device.
     pub unsafe fn rms_norm(x: *const f32, residual: *const f32, weight: *const f32, eps: f64, batch: usize, cols: usize, sum: *mut f32,

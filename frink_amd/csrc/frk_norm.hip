@@ -6,6 +6,8 @@
 //
 // Memory bounds it: x and the residual are read once, h and the result written once.  A row is up to sixteen wavefronts', a lane four
 // neighbouring values of every 256 -- what the quantizations' blocks are dealt by, too -- in registers between the sum and the products.
+// 16384 x 4096 of f32 with a residual 191 us, 1.07 GB (5.6 TB/s, part of it from the caches); 1 x 4096 to FP8 4.1, of which a launch that does
+// nothing is 2.
 #include "frk_norm.hpp"
 
 #include <algorithm>

@@ -134,8 +134,8 @@ int frk_hip_weights_from_device(int kind, const void *dev_bytes, size_t len, siz
  * What takes such a handle, f32 in and f32 out as for the other kinds: frk_hip_gemv_dev (FRK_ACT_F32 and FRK_ACT_INT8 are the
  * same here), frk_hip_gemv_multi_dev, frk_hip_ffn_swiglu_dev, frk_hip_gemm_dev, frk_hip_gemm_pair_dev,
  * frk_hip_gemm_noalloc_dev, frk_hip_gemm_grouped_dev and frk_hip_moe_ffn_dev (n_groups, n_experts = matrices; three such stacks
- * and a hidden size that is a multiple of four), frk_hip_dequant_dev, frk_hip_get_rows(_dev); the others return
- * FRK_ERR_UNSUPPORTED.  Every 128 columns of an activation row are quantized within the call to E4M3, to the nearest and
+ * and a hidden size that is a multiple of four), frk_hip_dequant_dev, frk_hip_get_rows(_dev), frk_hip_gemm_acts_dev over activations in
+ * FRK_ACTS_FP8; the others return FRK_ERR_UNSUPPORTED.  Every 128 columns of an activation row are quantized within the call to E4M3, to the nearest and
  * halves to even, under 2^e, e the least exponent of -100 or more that brings the largest finite magnitude to 448 or less
  * (magnitudes above 240 * 2^120, where the next code's value is no float, become that); an infinity or a NaN becomes a NaN and
  * takes no part in that: its output row is NaN.  So
@@ -334,7 +334,8 @@ enum { FRK_TYPE_F32 = 0, FRK_TYPE_BF16 = 1, FRK_TYPE_F16 = 2 };
  * bit for bit as frk_hip_quantize_batch_acts_dev would, with which frk_hip_gemm_acts_dev then multiplies.
  * sum_dev and y_dev may each be x_dev or residual_dev, but are two outputs; otherwise no two operands overlap.  A row with an infinity or a
  * NaN has the NaN that the formula gives.  eps is a finite number, zero or more (a row of zeros has y = NaN with eps = 0).  At most 2^30
- * rows of 2^23 columns; rows need be aligned to their type only.  A refused call leaves `acts` as it was.  The order of the reference's norms (RMSNorm in crates/frink-core). */
+ * rows of 2^23 columns; rows need be aligned to their type only.  A refused call leaves `acts` as it was.
+ * (The reference norms on the host, `rms_norm` in crates/frink-core/src/matmul.rs; the bits here are this definition's.) */
 int frk_hip_rms_norm_dev(int type, const void *x_dev, const void *residual_dev, int weight_type, const void *weight_dev, double eps,
                          size_t batch, size_t cols, void *sum_dev, void *y_dev, frk_batch_acts *acts, void *stream);
 
