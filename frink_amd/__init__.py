@@ -497,14 +497,18 @@ def quantize_mxfp4(x, out=None):
     what Weights.from_device(MXFP4, ...) and a GGUF file take."""
     import torch
     kind = _float_type(torch, x)
-    if x.dim() == 0 or x.numel() == 0 or x.shape[-1] % 32:
-        raise ValueError("activations %s: a multiple of 32 columns" % (tuple(x.shape),))
-    shape = tuple(x.shape[:-1]) + (x.shape[-1] // 32 * 17,)
-    if out is not None and (out.dtype is not torch.uint8 or out.numel() != x.numel() // 32 * 17 or not out.is_contiguous()):
-        raise ValueError("%s of %s for %d blocks of 17 bytes" % (tuple(out.shape), out.dtype, x.numel() // 32))
-    blocks = out if out is not None else x.new_empty(shape, dtype=torch.uint8)
-    check(lib().frk_hip_quantize_mxfp4_dev(kind, x.data_ptr(), x.numel(), blocks.data_ptr(), _fp8_stream(torch, x, (blocks,))))
-    return blocks
+    n, shape = x.numel(), list(x.shape)
+    if n == 0 or not shape or shape[-1] % 32:
+        raise ValueError("activations %s: a multiple of 32 columns" % (tuple(shape),))
+    if out is None:
+        shape[-1] = shape[-1] // 32 * 17
+        out, stream = x.new_empty(shape, dtype=torch.uint8), _fp8_stream(torch, x)
+    else:
+        if out.dtype is not torch.uint8 or out.numel() != n // 32 * 17 or not out.is_contiguous():
+            raise ValueError("%s of %s for %d blocks of 17 bytes" % (tuple(out.shape), out.dtype, n // 32))
+        stream = _fp8_stream(torch, x, (out,))
+    check(lib().frk_hip_quantize_mxfp4_dev(kind, x.data_ptr(), n, out.data_ptr(), stream))
+    return out
 
 
 def dequantize_mxfp4(blocks, cols):
@@ -512,9 +516,10 @@ def dequantize_mxfp4(blocks, cols):
     import torch
     if blocks.dtype is not torch.uint8 or not blocks.is_cuda or not blocks.is_contiguous():
         raise ValueError("%s of %s on %s: contiguous bytes on a GPU" % (tuple(blocks.shape), blocks.dtype, blocks.device))
-    if cols <= 0 or cols % 32 or blocks.numel() == 0 or blocks.numel() % (cols // 32 * 17):
-        raise ValueError("%d bytes do not make rows of %d columns" % (blocks.numel(), cols))
-    rows = blocks.numel() // (cols // 32 * 17)
+    n = blocks.numel()
+    if cols <= 0 or cols % 32 or n == 0 or n % (cols // 32 * 17):
+        raise ValueError("%d bytes do not make rows of %d columns" % (n, cols))
+    rows = n // (cols // 32 * 17)
     out = blocks.new_empty((rows, cols), dtype=torch.float32)
     check(lib().frk_hip_dequantize_mxfp4_dev(blocks.data_ptr(), rows * cols, out.data_ptr(), _fp8_stream(torch, blocks)))
     return out
