@@ -87,6 +87,10 @@ __device__ __forceinline__ void store_quantized(const NormOut &out, size_t row, 
     }
 }
 
+// A workgroup's place where an XCD (workgroup id mod 8) is to have eight neighbours at a time, in a grid of whole 64s: Q8_K's tiles have pieces of
+// eight rows in a line, which are then put together in one L2 (512 x 4096 8.8 -> 8.0 us, 16384 x 4096 202 -> 172).
+__device__ __forceinline__ unsigned in_eights(unsigned b) { return gridDim.x % 64 ? b : (b & ~63u) + (b & 7) * 8 + (b >> 3 & 7); }
+
 // `waves` wavefronts a row, the workgroup's others another row.  CHUNKS: of 256 values of a row that a wavefront holds; 0: any number, which
 // are read a second time behind the sum.
 template <int TYPE, int CHUNKS, int FORM, bool WIDE>
@@ -97,7 +101,7 @@ __global__ __launch_bounds__(1024) void rms_norm_kernel(NormArgs a, NormOut out)
     const int rows_wg = (int)(blockDim.x >> 6) / a.waves, mine = wave % a.waves, slot = wave - mine;
     const int cols = a.cols, chunks = a.chunks;
     int parity = 0;
-    for (size_t row0 = (size_t)blockIdx.x * rows_wg; row0 < a.rows; row0 += (size_t)gridDim.x * rows_wg, parity ^= 1) {
+    for (size_t row0 = (size_t)(FORM == ACTS_Q8_K ? in_eights(blockIdx.x) : blockIdx.x) * rows_wg; row0 < a.rows; row0 += (size_t)gridDim.x * rows_wg, parity ^= 1) {
         const size_t row = row0 + wave / a.waves;
         const bool live = row < a.batch, there = row < a.rows;  // (rows past the batch, of a last tile: zeros)
         const T *const x = (const T *)a.x + (live ? row * (size_t)cols : 0);
@@ -193,7 +197,9 @@ static int go_rms_norm(NormArgs a, const NormOut &out, hipStream_t s) {
     a.waves = waves;
     const int waves_wg = std::max(waves, a.rows > 512 ? 4 : 1);
     const size_t rows_wg = (size_t)(waves_wg / waves);
-    const dim3 grid((unsigned)std::min<size_t>((a.rows + rows_wg - 1) / rows_wg, 1 << 16)), block(64 * waves_wg);
+    size_t groups = std::min<size_t>((a.rows + rows_wg - 1) / rows_wg, 1 << 16);
+    if (FORM == ACTS_Q8_K && groups > 32) groups = (groups + 63) / 64 * 64;
+    const dim3 grid((unsigned)groups), block(64 * waves_wg);
     if (chunks <= 2 * waves) hipLaunchKernelGGL((rms_norm_kernel<TYPE, 2, FORM, WIDE>), grid, block, 0, s, a, out);
     else if (chunks <= 4 * waves) hipLaunchKernelGGL((rms_norm_kernel<TYPE, 4, FORM, WIDE>), grid, block, 0, s, a, out);
     else hipLaunchKernelGGL((rms_norm_kernel<TYPE, 0, FORM, WIDE>), grid, block, 0, s, a, out);
@@ -227,13 +233,16 @@ int launch_rms_norm(int type, NormArgs a, int form, const NormOut &out, hipStrea
     }
 }
 
-// ---- what quantized rows stand for: a wavefront 256 values at a time ----
+// ---- what quantized rows stand for: a wavefront 256 values at a time, a workgroup the same columns of eight rows (a line of Q8_K's tiles: in
+// rows' order 16384 x 4096 took 81.7 us, not 72.6) ----
 template <int FORM, bool WIDE>
-__global__ __launch_bounds__(256) void acts_values_kernel(NormOut in, size_t jobs, int jobs_a_row, int cols, float *__restrict__ out) {
+__global__ __launch_bounds__(512) void acts_values_kernel(NormOut in, size_t rows, int chunks, int cols, float *__restrict__ out) {
     const int lane = threadIdx.x & 63;
-    for (size_t j = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); j < jobs; j += (size_t)gridDim.x * 4) {
-        const size_t row = j / jobs_a_row;
-        const int c = (int)(j % jobs_a_row);
+    const size_t jobs = (rows + 7) / 8 * chunks;
+    for (size_t j = blockIdx.x; j < jobs; j += gridDim.x) {
+        const size_t row = j / chunks * 8 + (threadIdx.x >> 6);
+        const int c = (int)(j % chunks);
+        if (row >= rows) continue;
         float v[4];
         if (FORM == ACTS_FP8) {
             const F8Acts &a = in.f8.v ? in.f8 : in.f8_strips;
@@ -256,10 +265,10 @@ __global__ __launch_bounds__(256) void acts_values_kernel(NormOut in, size_t job
 }
 template <int FORM>
 static int go_acts_values(const NormOut &in, size_t rows, size_t cols, float *out, hipStream_t s) {
-    const size_t jobs_a_row = (cols + 255) / 256, jobs = rows * jobs_a_row;
-    const dim3 grid((unsigned)std::min<size_t>((jobs + 3) / 4, 1 << 16));
-    if (floats_wide(out, cols, FLOATS_F32)) hipLaunchKernelGGL((acts_values_kernel<FORM, true>), grid, dim3(256), 0, s, in, jobs, (int)jobs_a_row, (int)cols, out);
-    else hipLaunchKernelGGL((acts_values_kernel<FORM, false>), grid, dim3(256), 0, s, in, jobs, (int)jobs_a_row, (int)cols, out);
+    const size_t chunks = (cols + 255) / 256;
+    const dim3 grid((unsigned)std::min<size_t>((rows + 7) / 8 * chunks, 1 << 16));
+    if (floats_wide(out, cols, FLOATS_F32)) hipLaunchKernelGGL((acts_values_kernel<FORM, true>), grid, dim3(512), 0, s, in, rows, (int)chunks, (int)cols, out);
+    else hipLaunchKernelGGL((acts_values_kernel<FORM, false>), grid, dim3(512), 0, s, in, rows, (int)chunks, (int)cols, out);
     FRK_LAUNCH_CHECK("acts_values");
     return FRK_OK;
 }
