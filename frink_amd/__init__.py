@@ -364,10 +364,14 @@ class Weights:
     def gemm_acts(self, acts, out=None):
         """apply_batch_with_acts: this matrix over a batch that a BatchActs holds quantized."""
         import torch
-        y = out if out is not None else torch.empty((acts.batch, self.rows), dtype=torch.float32, device="cuda")
-        stream = _stream() if acts.form == "q8_k" or out is None else _fp8_stream(torch, _fp8_floats(torch, out, acts.batch * self.rows))
-        check(lib().frk_hip_gemm_acts_dev(self.handle, acts.handle, C.c_void_p(y.data_ptr()), stream))
-        return y
+        if out is None:
+            out, stream = torch.empty((acts.batch, self.rows), dtype=torch.float32, device="cuda"), _stream_raw(torch)
+        elif acts.form == "q8_k":
+            stream = _stream_raw(torch)
+        else:
+            stream = _fp8_stream(torch, _fp8_floats(torch, out, acts.batch * self.rows))
+        check(lib().frk_hip_gemm_acts_dev(self.handle, acts.handle, out.data_ptr(), stream))
+        return out
 
     def gemm_noalloc(self, x, out):
         """frk_hip_gemm_noalloc_dev: the caller brings the output; the call allocates nothing."""
@@ -411,11 +415,12 @@ class BatchActs:
     def values(self, out=None):
         """The numbers that the quantized batch stands for, [batch][cols] f32."""
         import torch
-        if out is not None:
-            _fp8_floats(torch, out, self.batch * self.cols)
-        y = out if out is not None else torch.empty((self.batch, self.cols), dtype=torch.float32, device="cuda")
-        check(lib().frk_hip_batch_acts_values_dev(self.handle, y.data_ptr(), _fp8_stream(torch, y)))
-        return y
+        if out is None:
+            out, stream = torch.empty((self.batch, self.cols), dtype=torch.float32, device="cuda"), _stream_raw(torch)
+        else:
+            stream = _fp8_stream(torch, _fp8_floats(torch, out, self.batch * self.cols))
+        check(lib().frk_hip_batch_acts_values_dev(self.handle, out.data_ptr(), stream))
+        return out
 
     def release(self):
         if self.handle:
