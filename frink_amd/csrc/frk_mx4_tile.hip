@@ -14,7 +14,6 @@
 
 namespace frk {
 
-typedef float mx4_v4f __attribute__((ext_vector_type(4)));
 typedef int mx4_v4i __attribute__((ext_vector_type(4)));
 typedef int mx4_v8i __attribute__((ext_vector_type(8)));
 typedef float mx4_v16f __attribute__((ext_vector_type(16)));
@@ -210,9 +209,6 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, in
     float *const own = reinterpret_cast<float *>(mx4_lds) + wave * 32 * T::PITCH;
     const int row_first = row0 + rw * MR * 32 + (lane % LANES) * 4;
     float *const y = g.y + part * part_stride + row_first;
-    // Results that the L2s would hold go past them, not out of them all at once when the kernel ends (17 MB: 512 tokens of 8192 x 1024 9.2 -> 7.5 us, 1024 of 4096 x 4096
-    // 17.0 -> 15.7).  More of them leave in time by themselves: 134 MB (4096 of 8192 x 1024) 46 us, past the caches 50; 59 MB the same either way.
-    const bool through = (size_t)g.M * g.ldy * parts <= (size_t)12 << 20;
     const bool wide = g.ldy % 4 == 0 && part_stride % 4 == 0 && (g.rows & 3) == 0 && (reinterpret_cast<uintptr_t>(g.y) & 15) == 0;
 #pragma unroll
     for (int t = 0; t < MT; t++) {
@@ -230,10 +226,7 @@ __global__ __launch_bounds__(64 * RW * TW, 1) void mx4_tile_kernel(Mx4Gemm g, in
             if (tok >= g.M) continue;
             float *const dst = y + (size_t)tok * g.ldy;
             if (wide) {
-                if (row_first < g.rows) {
-                    if (through) __builtin_nontemporal_store(mx4_v4f{v.x, v.y, v.z, v.w}, reinterpret_cast<mx4_v4f *>(dst));
-                    else *reinterpret_cast<float4 *>(dst) = v;
-                }
+                if (row_first < g.rows) *reinterpret_cast<float4 *>(dst) = v;
             } else {
                 const float out[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
