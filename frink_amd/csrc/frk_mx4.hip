@@ -394,7 +394,7 @@ constexpr size_t MX4_ROWS_TOKENS = 32;  // most of the rows kernel
 // tile's workgroups `alone` while each has a CU to itself, `shared` times the workgroups a CU from there on (up to what a CU holds; more are another
 // round), a round besides `ends` + `ends_shared` times those.  Shares of the columns cost a second launch and the traffic of the parts.  Every tile
 // and number of shares timed at 104 sizes (17 to 4096 tokens, 1024 x 4096 to 32000 x 4096, 4096 x 14336): the choice is within 1 % of the fastest on
-// average, 14 % off at 64 tokens of 4096 x 4096.
+// average, 13 % off at 4096 tokens of 8192 x 1024.
 Mx4Plan mx4_plan(const frk_weights *w, size_t batch, bool quantized) {
     const size_t units = (w->cols / MX4_BLOCK + MX4_UNIT - 1) / MX4_UNIT, stages = (w->cols + 255) / 256, n = batch * w->rows;
     Mx4Plan p{-1, 1, !quantized && batch <= MX4_FUSED && batch * units * MX4_FUSED_UNIT <= MX4_FUSED_LDS, 0, 0};
