@@ -1271,9 +1271,13 @@ int frk_hip_batch_acts_create(size_t max_batch, size_t cols, frk_batch_acts **ou
 int frk_hip_batch_acts_release(frk_batch_acts *a) {
     clear_error();
     if (!a) return FRK_OK;
-    hipError_t e = hipFree(a->base);
-    delete a;
+    // (a capture under way, of this thread's or another's, allows hipFree in relaxed mode only: in another one it ends the capture)
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    FRK_HIP_TRY(hipThreadExchangeStreamCaptureMode(&mode));
+    const hipError_t e = hipFree(a->base);
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
     if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFree: %s", hipGetErrorString(e));
+    delete a;
     return FRK_OK;
 }
 

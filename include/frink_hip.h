@@ -281,7 +281,8 @@ int frk_hip_gemm_pair_dev(const frk_weights *w0, const frk_weights *w1, const fl
  * to 19 and all of more than 64; for other lengths it may be the same integers added in another order).  K-quant matrices (Q4_K, Q5_K, Q6_K) of `cols`
  * columns; other kinds return FRK_ERR_UNSUPPORTED.  A quantization and the GEMMs that read it are ordered
  * by the stream they are enqueued on; the object is not to be re-quantized while a GEMM that reads it is
- * still in flight on another stream. */
+ * still in flight on another stream.  _release may be called while some other work is captured into a graph; one that fails
+ * leaves the object as it was. */
 typedef struct frk_batch_acts frk_batch_acts;
 int frk_hip_batch_acts_create(size_t max_batch, size_t cols, frk_batch_acts **out);
 int frk_hip_batch_acts_release(frk_batch_acts *acts);
