@@ -370,6 +370,7 @@ class Weights:
             stream = _stream_raw(torch)
         else:
             stream = _fp8_stream(torch, _fp8_floats(torch, out, acts.batch * self.rows))
+        acts._used_on(torch, stream)
         check(lib().frk_hip_gemm_acts_dev(self.handle, acts.handle, out.data_ptr(), stream))
         return out
 
@@ -393,21 +394,29 @@ class Weights:
 class BatchActs:
     """A batch's activations quantized once for any number of matrices (the reference's BatchActs::Q8K):
     frk_hip_batch_acts_create_form / frk_hip_quantize_batch_acts_dev / frk_hip_batch_acts_release.  form: "q8_k" for the K-quants,
-    "fp8" for FP8_BLOCK, "mxfp4" for MXFP4 matrices."""
+    "fp8" for FP8_BLOCK, "mxfp4" for MXFP4 matrices.
+
+    Its device memory is freed by release(), or when Python drops the object; but once a call over it has been captured into a graph,
+    which replays the memory's address for as long as it lives, by release() alone: after the last replay."""
 
     def __init__(self, max_batch, cols, form="q8_k"):
-        self.handle = None
+        self.handle, self.in_a_graph = None, False
         if form not in ACTS_FORMS:
             raise ValueError("form %r: one of %s" % (form, ", ".join(ACTS_FORMS)))
         h = C.c_void_p()
         check(lib().frk_hip_batch_acts_create_form(max_batch, cols, ACTS_FORMS[form], C.byref(h)))
         self.handle, self.max_batch, self.cols, self.form, self.batch = h, max_batch, cols, form, 0
 
+    def _used_on(self, torch, stream):  # (asking is 0.3 us; the default stream cannot be captured)
+        if stream and not self.in_a_graph and torch.cuda.is_current_stream_capturing():
+            self.in_a_graph = True
+
     def quantize(self, x):
         import torch
         assert x.dtype == torch.float32 and x.is_cuda and x.is_contiguous() and x.shape[-1] == self.cols
         batch = x.numel() // self.cols
-        stream = _stream() if self.form == "q8_k" else _fp8_stream(torch, x)
+        stream = _stream_raw(torch) if self.form == "q8_k" else _fp8_stream(torch, x)
+        self._used_on(torch, stream)
         check(lib().frk_hip_quantize_batch_acts_dev(self.handle, C.c_void_p(x.data_ptr()), batch, stream))
         self.batch = batch
         return self
@@ -419,6 +428,7 @@ class BatchActs:
             out, stream = torch.empty((self.batch, self.cols), dtype=torch.float32, device="cuda"), _stream_raw(torch)
         else:
             stream = _fp8_stream(torch, _fp8_floats(torch, out, self.batch * self.cols))
+        self._used_on(torch, stream)
         check(lib().frk_hip_batch_acts_values_dev(self.handle, out.data_ptr(), stream))
         return out
 
@@ -427,9 +437,9 @@ class BatchActs:
             check(lib().frk_hip_batch_acts_release(self.handle))
             self.handle = None
 
-    def __del__(self):  # (not "q8_k": a graph captured over such an object may live longer, and always could)
+    def __del__(self):
         try:
-            if self.handle and _lib is not None and self.form != "q8_k":
+            if self.handle and _lib is not None and not self.in_a_graph:
                 _lib.frk_hip_batch_acts_release(self.handle)
                 self.handle = None
         except Exception:
@@ -491,6 +501,7 @@ def rms_norm(x, weight=None, eps=1e-5, residual=None, out=None, sum_out=None, ac
         return out, x if sum_out is None else sum_out
     if not acts.handle:
         raise ValueError("the activations are released")
+    acts._used_on(torch, stream)
     # (a refusal leaves the object's batch as it was, there as here: its outputs are sized by it)
     check(lib().frk_hip_rms_norm_dev(kind, x.data_ptr(), r_ptr, w_kind, w_ptr, eps, n // cols, cols, s_ptr, y_ptr, acts.handle, stream))
     acts.batch = n // cols
