@@ -460,21 +460,22 @@ def _float_type(torch, t, which="f32, bf16 or f16"):
     return kind
 
 
-def _like(t, x, n):
-    """A second operand of x's type and n values."""
-    if t.dtype is not x.dtype or t.numel() != n or not t.is_contiguous():
+def _like(t, x, shape):
+    """A second operand of x's type and shape."""
+    if t.dtype is not x.dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError("%s of %s beside activations %s of %s" % (tuple(t.shape), t.dtype, tuple(x.shape), x.dtype))
 
 
 def rms_norm(x, weight=None, eps=1e-5, residual=None, out=None, sum_out=None, acts=None):
     """frk_hip_rms_norm_dev: (y, h) with h = x + residual (x itself without one) and y = h / sqrt(mean(h^2) + eps) * weight over the
     last dimension of x (f32, bf16 or f16; weight of any of them).  h goes to `sum_out` (which may be x or residual), y to `out`, both of x's
-    type and shape; with `acts` y is quantized into that BatchActs, which is returned in y's place (and y written only where `out` is given)."""
+    type and shape, as the residual is; with `acts` y is quantized into that BatchActs, which is returned in y's place (and y written only where `out` is given)."""
     import torch
     kind, n = _float_type(torch, x), x.numel()
     if n == 0 or x.dim() == 0:
         raise ValueError("activations %s" % (tuple(x.shape),))
-    cols = x.shape[-1]
+    shape = x.shape
+    cols = shape[-1]
     # (a call's host side, 2.2 us of it the launch, is what one token's norm waits for: nothing is looked at twice)
     w_kind, w_ptr, r_ptr, s_ptr, y_ptr = 0, None, None, None, None
     if weight is not None:
@@ -482,15 +483,15 @@ def rms_norm(x, weight=None, eps=1e-5, residual=None, out=None, sum_out=None, ac
         if weight.numel() != cols:
             raise ValueError("%d weights for rows of %d columns" % (weight.numel(), cols))
     if residual is not None:
-        _like(residual, x, n)
+        _like(residual, x, shape)
         r_ptr = residual.data_ptr()
         if sum_out is None:
             sum_out, s_ptr = (h := torch.empty_like(x)), h.data_ptr()
     if sum_out is not None and s_ptr is None:
-        _like(sum_out, x, n)
+        _like(sum_out, x, shape)
         s_ptr = sum_out.data_ptr()
     if out is not None:
-        _like(out, x, n)
+        _like(out, x, shape)
         y_ptr = out.data_ptr()
     elif acts is None:
         out = torch.empty_like(x)
