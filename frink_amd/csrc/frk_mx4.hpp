@@ -5,7 +5,7 @@
 // c: E2M1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives), e: E8M0 bytes.  A block of floats is quantized under
 // 2^(floor(log2(amax)) - 2), which leaves its largest magnitude between 4 and 8; each value becomes the nearest E2M1 number, halves
 // the even code, magnitudes above 6 the number 6.  A block with an infinity or a NaN gets the byte 255, E8M0's NaN, and zero codes.
-// Blocks of magnitudes below 2^-125 keep the byte 0.
+// Blocks of magnitudes below 2^-124 have the byte 0, whose scale is 2^-127.
 #pragma once
 
 #include "frk_device.hpp"

@@ -313,8 +313,8 @@ int frk_hip_route_top_k_softmax_dev(const float *logits_dev, size_t batch, size_
 
 /* The same in two more forms, for the matrices of those kinds: FRK_ACTS_FP8 for FRK_KIND_FP8_BLOCK (any number of columns) and
  * FRK_ACTS_MXFP4 for FRK_KIND_MXFP4 (whole blocks of 32), at most 2^30 rows of 2^23 columns.  _create is _create_form with FRK_ACTS_Q8_K.
- * An object belongs to the device that was current when it was made; a call over one of these forms, or of the three functions
- * below, while another is current returns FRK_ERR_ARG.
+ * An object belongs to the device that was current when it was made: while another one is current, a call over one of these forms, and
+ * _values and frk_hip_rms_norm_dev over an object of any form, return FRK_ERR_ARG.
  *   FP8    as frk_hip_gemm_dev quantizes a batch for such a matrix; y is bit for bit its result from nine rows on (fewer may be the same
  *          products added in another order)
  *   MXFP4  as frk_hip_gemm_mxfp4_dev does; y is bit for bit its result from five rows on
@@ -329,7 +329,8 @@ int frk_hip_batch_acts_values_dev(const frk_batch_acts *acts, float *out_dev, vo
 enum { FRK_TYPE_F32 = 0, FRK_TYPE_BF16 = 1, FRK_TYPE_F16 = 2 };
 /* The norm in front of a group of projections, for rows x[batch][cols] of `type`:
  *   h = x + residual, rounded to `type` (h = x where residual_dev is null)
- *   r = 1 / sqrt(mean(h^2) + eps): the sum, the root and the quotient in 64 bits, rounded to f32 once
+ *   r = 1 / sqrt(mean(h^2) + eps): the sum, the root and the quotient in 64 bits, rounded to f32 once (in about one row of 2^27 to the f32
+ *       number beside the nearest one; the order of the additions, and so which of the two, may depend on the number of rows)
  *   y = (h * r) * weight, two products rounded to f32 each (one where weight_dev is null); weight[cols] of weight_type
  * and up to three outputs (null: not wanted; at least one): h into sum_dev, y rounded to `type` into y_dev, y in f32 quantized into `acts`,
  * bit for bit as frk_hip_quantize_batch_acts_dev would, with which frk_hip_gemm_acts_dev then multiplies.
