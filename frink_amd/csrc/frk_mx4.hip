@@ -82,8 +82,9 @@ int launch_mx4_values(const Mx4Acts &a, size_t cols, float *out, hipStream_t s) 
 
 // ---- GGUF blocks: the scale byte, then sixteen bytes of codes.  256 of them are 4352 bytes, 272 pieces of sixteen: a workgroup puts them
 // together in LDS.  Four lanes a block: of floats, a lane elements 4 l .. and 16 + 4 l .., whose codes share bytes; of two-byte numbers, eight
-// neighbours (sixteen bytes a load), whose codes meet those of the lane two further on.  14336 x 4096 of bf16 28.7 us, of f32 49.5, back 40.5: 5.2, 5.4 and
-// 6.6 TB/s, what memory gives. ----
+// neighbours (sixteen bytes a load), whose codes meet those of the lane two further on.  14336 x 4096 of bf16 27.6 us, of f32 48, back 44, one matrix
+// after another: 5.4, 5.5 and 6.0 TB/s, what memory gives.  Behind a kernel that has just written 235 MB (the way back, a fill) the first takes 41 to 43: what that one
+// left in the caches goes out to memory beside it. ----
 constexpr int GGUF_BLOCKS = 256;
 __device__ __forceinline__ void lds_put32(uint8_t *to, uint32_t v) { __builtin_memcpy(to, &v, 4); }  // (of any alignment)
 template <int TYPE, bool WIDE>

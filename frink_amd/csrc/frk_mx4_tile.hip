@@ -2,8 +2,9 @@
 // (v_mfma_scale_f32_32x32x64_f8f6f4): sixteen bytes of E2M1 codes are a lane's operand, its block's E8M0 byte the scale.
 //   y[t][r] = sum over blocks b of 2^(sw[r][b] + sx[t][b] - 254) * sum over the 32 of b of w x
 // Products of codes and a block's sum are exact, blocks add up in f32.
-// What bounds it: a full chip of 256 x 256 tiles its power (4096 tokens of 4096 x 14336: 114 us, 4.2 PFLOP/s; the clock falls to 1.44 GHz; the products
-// alone 86 us, with the operands' reads 110); fewer workgroups the time from a request to its bytes, which is why smaller tiles have three or four
+// What bounds it: a full chip of 256 x 256 tiles (4096 tokens of 4096 x 14336) its 239 thousand cycles, of which the matrix cores are busy 48 %, and the
+// clock that its power leaves: 116 us behind the quantization in front of it (4.1 PFLOP/s, 2.1 GHz), 130 to 140 one product after the other (3.4 to
+// 3.7; 1.7 to 1.85 GHz; the products without anything else 86, with the operands' reads 110); fewer workgroups the time from a request to its bytes, which is why smaller tiles have three or four
 // stages (64 tokens of 14336 x 4096, two stages / three / four of 64 x 64: 13.7 / 9.4 / 8.8 us; 512 of 4096 x 14336, two / three of 64 x 128:
 // 43.2 / 28.6).
 #include "frk_mx4.hpp"

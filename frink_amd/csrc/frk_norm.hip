@@ -6,7 +6,7 @@
 //
 // Memory bounds it: x and the residual are read once, h and the result written once.  A row is up to sixteen wavefronts', a lane four
 // neighbouring values of every 256 -- what the quantizations' blocks are dealt by, too -- in registers between the sum and the products.
-// 16384 x 4096 of f32 with a residual 191 us, 1.07 GB (5.6 TB/s, part of it from the caches); 1 x 4096 to FP8 4.1, of which a launch that does
+// 16384 x 4096 of f32 with a residual 191 us, 1.07 GB (5.6 TB/s, part of it from the caches); 1 x 4096 to FP8 4.4, of which a launch that does
 // nothing is 2.
 #include "frk_norm.hpp"
 
@@ -88,7 +88,8 @@ __device__ __forceinline__ void store_quantized(const NormOut &out, size_t row, 
 }
 
 // A workgroup's place where an XCD (workgroup id mod 8) is to have eight neighbours at a time, in a grid of whole 64s: Q8_K's tiles have pieces of
-// eight rows in a line, which are then put together in one L2 (512 x 4096 8.8 -> 8.0 us, 16384 x 4096 202 -> 172).
+// eight rows in a line, which are then put together in one L2 (a norm after the other, 512 x 4096 8.8 -> 8.0 to 8.3 us, 16384 x 4096
+// 202 -> 172 to 180).
 __device__ __forceinline__ unsigned in_eights(unsigned b) { return gridDim.x % 64 ? b : (b & ~63u) + (b & 7) * 8 + (b >> 3 & 7); }
 
 // `waves` wavefronts a row, the workgroup's others another row.  CHUNKS: of 256 values of a row that a wavefront holds; 0: any number, which
