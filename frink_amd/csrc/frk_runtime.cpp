@@ -467,6 +467,16 @@ int frk_hip_weights_from_device_fp8(const uint8_t *dev_codes, const float *dev_s
     return make_f8_resident(dev_codes, dev_scales, rows, cols, matrices, (hipStream_t)stream, out);
 }
 
+// A capture under way, of this thread's or another's, allows hipFree in relaxed mode only: in another one it ends the capture.
+static hipError_t free_device(void *p) {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    hipError_t e = hipThreadExchangeStreamCaptureMode(&mode);
+    if (e != hipSuccess) return e;
+    e = hipFree(p);
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    return e;
+}
+
 int frk_hip_weights_release(frk_weights *w) {
     clear_error();
     if (!w) return FRK_OK;
@@ -476,9 +486,9 @@ int frk_hip_weights_release(frk_weights *w) {
         return FRK_OK;
     }
     if (w->cached) g_dev.cache.erase(std::make_pair(w->host_key, w->host_len));
-    hipError_t e = hipFree(w->dev);
+    hipError_t e = free_device(w->dev);
     if (uint8_t *kept = w->decoded.load(std::memory_order_acquire)) {
-        const hipError_t e2 = hipFree(kept);
+        const hipError_t e2 = free_device(kept);
         if (e == hipSuccess) e = e2;
     }
     delete w;
@@ -1271,11 +1281,7 @@ int frk_hip_batch_acts_create(size_t max_batch, size_t cols, frk_batch_acts **ou
 int frk_hip_batch_acts_release(frk_batch_acts *a) {
     clear_error();
     if (!a) return FRK_OK;
-    // (a capture under way, of this thread's or another's, allows hipFree in relaxed mode only: in another one it ends the capture)
-    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-    FRK_HIP_TRY(hipThreadExchangeStreamCaptureMode(&mode));
-    const hipError_t e = hipFree(a->base);
-    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    const hipError_t e = free_device(a->base);
     if (e != hipSuccess) return set_error(FRK_ERR_HIP, "hipFree: %s", hipGetErrorString(e));
     delete a;
     return FRK_OK;

@@ -42,6 +42,30 @@ def test_an_object_that_ends_during_a_capture_leaves_the_capture_alone(fa, form,
         assert torch.equal(y, want) and torch.equal(z, want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("decoded", [False, True])
+def test_a_matrix_dropped_during_a_capture_leaves_the_capture_alone(fa, decoded):
+    import torch
+    print("a matrix dropped during a capture", decoded, flush=True)
+    rng = np.random.default_rng(3)
+    x, weight = to_dev(rng.standard_normal((3, 256)).astype(np.float32)), to_dev(rng.uniform(0.5, 1.5, 256).astype(np.float32))
+    want = fa.rms_norm(x, weight)[0]
+    w = fa.Weights.from_device(fa.MXFP4, to_dev(plain.blocks(*plain.random_matrix(rng, 64, 256)).reshape(-1)), 64, 256)
+    if decoded:
+        w.keep_decoded()
+    y, stream, graph = torch.empty_like(x), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        del w
+        gc.collect()
+        fa.rms_norm(x, weight, out=y)
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
 class _Library:
     """The library's entry points, of which the calls are kept and nothing else."""
 
