@@ -30,7 +30,7 @@ def _operands(rows, cols, batch):
 
 # both sides of the longest rows that the workgroups quantize for themselves (one, two and four tokens); one and two strips a workgroup, two tiles of
 # tokens, tiles whole and in shares; rows that end inside a unit of sixteen blocks and inside a stage of eight
-CASES = [(33, 61440, 1), (33, 61472, 1), (33, 65536, 1), (33, 65536, 2), (47, 30720, 2), (47, 30752, 2), (33, 65536, 3), (33, 15360, 4), (33, 15392, 4), (33, 65568, 4),
+CASES = [(33, 61440, 1), (33, 61472, 1), (33, 65536, 1), (33, 65536, 2), (47, 30688, 2), (47, 30752, 2), (33, 65536, 3), (33, 15360, 4), (33, 15392, 4), (33, 65568, 4),
          (40, 28672, 1), (7201, 15360, 4), (7201, 15392, 4), (7201, 8224, 3), (49, 65568, 9), (33, 65536, 16), (33, 65536, 20), (33, 65568, 32), (33, 65568, 33), (65, 65536, 70),
          (300, 32800, 200), (257, 16416, 300), (2049, 4128, 1100)]
 
